@@ -247,6 +247,121 @@ model_status tie_head_argmax_noalloc(const float *x, int ldx, const float *w, in
                                      int vocab, int k, float *logits, int ldl, int32_t *next,
                                      void *stream);
 
+/* ---- the paged cache and beams, over device memory -----------------------
+ * No counterpart in the reference (one sequence, one contiguous cache:
+ * src/kv_cache.c:150-190, src/model.c:826-850). For a caller that schedules
+ * its own batches: pages are built, filled, attended to and reordered on the
+ * GPU, without a copy of the lengths to the host.
+ *
+ * A pool is two arrays (keys, values) of n_pages pages of KV_CACHE_PAGE_ROWS
+ * rows of n_kv_head * 64 elements, fp32 (TIE_KV_F32) or bf16 (TIE_KV_BF16),
+ * contiguous. A page table has pages_per_seq int32 entries per sequence; an
+ * entry outside [0, n_pages) is unmapped. A slot is page * KV_CACHE_PAGE_ROWS
+ * + row, or -1 for none. New tokens of a batch form rows: those of sequence s
+ * are row_start[s] .. row_start[s + 1] - 1, at positions ctx_lens[s], ...
+ *
+ * Pointers are DEVICE pointers of one device (made current for the call) and
+ * `stream` a cudaStream_t of it (NULL: the legacy default stream); work is
+ * enqueued and not waited for. Activations, pages and workspaces are 16-byte
+ * aligned, leading dimensions multiples of 4 floats. A workspace holds nothing
+ * from one call to the next, but two calls that overlap on the GPU (streams,
+ * replayed graphs) need one each. Nothing is allocated, and every call may be
+ * captured into a graph. MODEL_ERR_ARG for a null or misaligned pointer, a
+ * shape or format without meaning, or host memory; MODEL_ERR_CAPACITY for a
+ * workspace too small or a limit below; MODEL_ERR_DEVICE for a CUDA failure.
+ * Limits: 4096 sequences or requests, 2^27 pages, 16 beams. */
+enum { TIE_KV_F32 = 0, TIE_KV_BF16 = 1 };
+
+/* Page table entries, row starts and slot maps from request lengths. Sequence
+ * s has ctx_lens[s] positions cached and appends new_lens[s] (>= 0). Its
+ * entries for the pages that start among the new positions are assigned from
+ * the free list, a stack of max_free entries of which n_free[0] count: entry
+ * n_free - 1 first, in the order of sequences and positions, as the engine's
+ * own pool does. n_free_out[0] receives what is left (it may be n_free).
+ * Without a free list (free_pages, n_free, n_free_out NULL) the table is taken
+ * as complete.
+ * row_start[n_seq + 1] receives the row starts; seq_of, pos_of, slot_of
+ * [max_rows] each row's sequence, position and slot (-1 where that entry is
+ * unmapped), and -1 for rows behind the last sequence's.
+ * status[0] receives MODEL_OK; MODEL_ERR_CAPACITY for too few free pages, a
+ * sequence beyond pages_per_seq pages or more than max_rows rows; or
+ * MODEL_ERR_ARG for a negative length or an n_free outside 0..max_free. With
+ * either error nothing is assigned, row_start is 0 throughout and every row is
+ * -1, so what follows in the stream does nothing. */
+model_status tie_page_plan(const int32_t *ctx_lens, const int32_t *new_lens, int n_seq,
+                           int32_t *page_table, int pages_per_seq, int n_pages,
+                           const int32_t *free_pages, int max_free, const int32_t *n_free,
+                           int32_t *n_free_out, int32_t *row_start, int32_t *seq_of,
+                           int32_t *pos_of, int32_t *slot_of, int max_rows, int32_t *status,
+                           void *stream);
+
+/* Key and value rows into their slots: row r of k and v (n_kv_head * 64 floats,
+ * ld floats apart) to slot slots[r] of the pool, rounded to nearest even for
+ * bf16. A slot outside the pool stores nothing; of two rows with one slot
+ * either may stay. rows == 0 is allowed. */
+model_status tie_kv_store(const float *k, const float *v, int ld, const int32_t *slots, int rows,
+                          void *k_pages, void *v_pages, int kv_format, int n_pages, int n_kv_head,
+                          void *stream);
+
+/* Causal attention of new tokens over the cache that holds them: for row r of
+ * sequence s at position p and query head h (n_head of them, a multiple of
+ * n_kv_head; K/V head h / (n_head / n_kv_head)),
+ *   out[r][h] = sum_j softmax_j(scale * q[r][h] . k[j]) v[j],  0 <= j <= p,
+ * over the positions whose page is mapped; 0 where none is left. The new
+ * tokens' own keys and values are read from the pages (tie_kv_store first).
+ * q and out: `rows` rows of n_head * 64 floats, ldq and ldo apart, not
+ * overlapping. max_new bounds the new tokens per sequence. A sequence without
+ * new tokens, with more than max_new, with row_start outside 0..rows or beyond
+ * pages_per_seq pages is left out: its rows of out stay as they were, and so
+ * do rows behind the last sequence's. Sums and softmax statistics are fp32.
+ * A key or value that is not finite makes the rows that see it not finite and
+ * no others. The result of a row depends, in its rounding, on how the batch
+ * splits its keys, and is the same for the same call.
+ * status, if not NULL, receives MODEL_ERR_DEVICE when a bounded wait in the
+ * kernel expires (the output is then incomplete); it is not written otherwise. */
+size_t tie_attention_paged_workspace(void);
+model_status tie_attention_paged(const float *q, int ldq, int n_head, const void *k_pages,
+                                 const void *v_pages, int kv_format, int n_pages, int n_kv_head,
+                                 const int32_t *page_table, int pages_per_seq,
+                                 const int32_t *row_start, const int32_t *ctx_lens, int n_seq,
+                                 int max_new, int rows, float scale, float *out, int ldo,
+                                 void *workspace, size_t workspace_bytes, int32_t *status,
+                                 void *stream);
+
+/* One step of beam search. Row r * beams + b of logits (ldl floats apart) and
+ * scores belongs to beam b of request r. A candidate (b, v) has the total
+ *   scores[b] + logits[b][v] - logsumexp(logits[b]),
+ * formed in double; a finished beam (done != 0; done may be NULL) has the one
+ * candidate (b, eos_id) with its score unchanged. The `beams` largest totals
+ * are kept, the lowest b * vocab + v first among equal ones (within one beam
+ * logits are compared as they are). A NaN logit counts as -inf; a total that
+ * is NaN counts as -inf, as do all of a row whose largest logit is infinite.
+ * Places: a beam's best kept candidate stays in that beam's place; the others
+ * take the places left, lowest first, best first. So a beam that has children
+ * is its own first child, and tie_kv_reorder moves no row that others copy.
+ * Per place: next (token), parent (row index r * beams + b), scores_out (may
+ * be scores), done_out (may be done, may be NULL: parent finished, or token ==
+ * eos_id). eos_id < 0: none, then done and done_out must be NULL. */
+size_t tie_beam_select_workspace(int n_req, int beams, int vocab);
+model_status tie_beam_select(const float *logits, int ldl, const float *scores,
+                             const int32_t *done, int n_req, int beams, int vocab, int eos_id,
+                             int32_t *next, int32_t *parent, float *scores_out, int32_t *done_out,
+                             void *workspace, size_t workspace_bytes, void *stream);
+
+/* The cached rows follow the beams: for every layer (layer_stride elements
+ * apart in each of k_pages and v_pages) and every sequence s = r * beams + b
+ * whose parent[s] is another beam of request r, the rows of positions first[r]
+ * .. length[r] - 1 of s's pages become those of the parent's, as they were
+ * before the call (any permutation). Positions before first[r] are taken to be
+ * equal in all beams of the request (the prompt); pages that hold later ones
+ * belong to one beam each. A parent outside the request, an unmapped page and
+ * a page that both beams share move nothing. */
+model_status tie_kv_reorder(void *k_pages, void *v_pages, int kv_format, int n_layer,
+                            size_t layer_stride, int n_pages, int n_kv_head,
+                            const int32_t *page_table, int pages_per_seq, const int32_t *parent,
+                            const int32_t *first, const int32_t *length, int n_req, int beams,
+                            void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,6 +17,7 @@
 #include "../../include/tie_b200.h"
 #include "internal.h"
 #include "json_doc.h"
+#include "ops.h"
 #include "tc_gemm.h"
 
 #include <algorithm>
@@ -267,12 +268,21 @@ namespace {
 // and, with TIE_DEBUG set in the environment, one line per failure on stderr.
 thread_local char g_dev_err[256] = "";
 
-void note_cuda(cudaError_t e, const char* what, int line) {
-    std::snprintf(g_dev_err, sizeof g_dev_err, "%s (%s) at model.cu:%d: %s", cudaGetErrorName(e),
-                  cudaGetErrorString(e), line, what);
+}  // namespace
+
+namespace tie {
+void note_device_error(cudaError_t e, const char* what, const char* file, int line) {
+    const char* base = std::strrchr(file, '/');
+    std::snprintf(g_dev_err, sizeof g_dev_err, "%s (%s) at %s:%d: %s", cudaGetErrorName(e), cudaGetErrorString(e),
+                  base ? base + 1 : file, line, what);
     static const bool verbose = std::getenv("TIE_DEBUG") != nullptr;
     if (verbose) std::fprintf(stderr, "tie_b200: %s\n", g_dev_err);
 }
+}  // namespace tie
+
+namespace {
+
+void note_cuda(cudaError_t e, const char* what, int line) { note_device_error(e, what, "model.cu", line); }
 
 #define CU(expr)                                                   \
     do {                                                           \

@@ -1,0 +1,324 @@
+// ops_attn.cu -- causal attention of new tokens over a paged cache: the entry
+// point, the streaming kernel for sequences of few rows, and the join of split
+// sequences.
+//
+// The reference attends one new token of its one sequence (src/model.c:826-850)
+// or a whole prompt to itself (src/model.c:705-732); here any number of new
+// tokens per sequence attend to everything cached before them and to
+// themselves:
+//
+//   out = sum_j softmax_j(scale q . k_j) v_j,   j <= ctx + i,
+//
+// with an online softmax (running maximum and sum in fp32) over the keys, each
+// read once through the page table.
+#include "paged_attn.cuh"
+
+#include <cuda_bf16.h>
+
+#include <climits>
+#include <cmath>
+
+namespace tie {
+namespace {
+
+// ------------------------------------------------------- few rows: streaming --
+// Bound by the reading of K and V. A CTA of 8 warps per unit; warp w takes the
+// unit's pages w, w + 8, ... Its lanes load a page's 16 keys and values as 16
+// 16-byte loads each (lane = 16 half + dl: position 2 i + half, dims 4 dl ..
+// 4 dl + 3; 8-byte loads for bf16), all in flight before the first product.
+// The 8 partial dot products a lane holds per row are summed over the 16 lanes
+// of a half by exchanging halves of the set (8 shuffles, not 32), which leaves
+// one score per lane pair; each probability then goes back to the lanes of its
+// half by one shuffle per position. The warps' (max, sum, output) are joined
+// in shared memory.
+constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
+constexpr unsigned kAll = 0xffffffffu;
+
+template <bool BF16>
+__device__ __forceinline__ float4 load4(const void* base, size_t at) {
+    if constexpr (BF16) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(base) + at));
+        return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                           __uint_as_float(u.y & 0xffff0000u));
+    } else {
+        return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + at));
+    }
+}
+
+struct FewSmem {
+    float m[kFewWarps][kFewRows], l[kFewWarps][kFewRows];
+    float o[kFewWarps][kFewRows][kHeadDim];
+};
+
+// The pages [p0, p1) of sequence s for rows tile * kFewRows .. + R - 1 (n_rows
+// of them real) of K/V head g; leaves each warp's partial in `sm`.
+template <int R, bool BF16>
+__device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const SeqShape& q, int s, int tile, int g, int p0,
+                                         int p1, int n_rows, FewSmem* sm) {
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, half = lane >> 4, dl = lane & 15;
+    float qv[R][4], o[R][4], m[R], l[R];
+    int last[R];                       // the last position each row sees
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = min(tile * kFewRows + r, q.rows - 1), tok = i / a.group;
+        last[r] = q.ctx + tok;
+        const float4 x = __ldg(reinterpret_cast<const float4*>(a.q + (size_t)(q.row0 + tok) * a.ldq +
+                                                               (g * a.group + i % a.group) * kHeadDim + 4 * dl));
+        qv[r][0] = x.x * a.scale2; qv[r][1] = x.y * a.scale2; qv[r][2] = x.z * a.scale2; qv[r][3] = x.w * a.scale2;
+        o[r][0] = o[r][1] = o[r][2] = o[r][3] = 0.f;
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+    }
+    const size_t w = (size_t)a.n_kv_head * kHeadDim;
+    const int32_t* table = a.table + (size_t)s * a.width;
+    const int own = 2 * ((dl >> 3 & 1) * 4 + (dl >> 2 & 1) * 2 + (dl >> 1 & 1)) + half;   // this lane's position of a page
+    int page = p0 + warp < p1 ? __ldg(table + p0 + warp) : -1;
+    for (int p = p0 + warp; p < p1; p += kFewWarps) {
+        const int cur = page;
+        if (p + kFewWarps < p1) page = __ldg(table + p + kFewWarps);
+        if (cur < 0 || cur >= a.n_pages) continue;         // an unmapped page holds no positions
+        const size_t at = ((size_t)cur * kPageRows + half) * w + g * kHeadDim + 4 * dl;
+        float4 kk[8], vv[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) kk[i] = load4<BF16>(a.k, at + 2 * i * w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vv[i] = load4<BF16>(a.v, at + 2 * i * w);
+        const int pos0 = p * kPageRows;
+        const bool whole = pos0 + kPageRows - 1 <= last[0];   // rows are in token order: last[0] is the least
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float d[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                d[i] = fmaf(kk[i].w, qv[r][3], fmaf(kk[i].z, qv[r][2], fmaf(kk[i].y, qv[r][1], kk[i].x * qv[r][0])));
+            const bool b3 = dl & 8, b2 = dl & 4, b1 = dl & 2;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                d[i] = (b3 ? d[i + 4] : d[i]) + __shfl_xor_sync(kAll, b3 ? d[i] : d[i + 4], 8);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                d[i] = (b2 ? d[i + 2] : d[i]) + __shfl_xor_sync(kAll, b2 ? d[i] : d[i + 2], 4);
+            float sc = (b1 ? d[1] : d[0]) + __shfl_xor_sync(kAll, b1 ? d[0] : d[1], 2);
+            sc += __shfl_xor_sync(kAll, sc, 1);
+            if (!whole && pos0 + own > last[r]) sc = -INFINITY;
+            float mx = sc;
+#pragma unroll
+            for (int x = 2; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, x));
+            const float m_new = fmaxf(m[r], mx), base = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = ex2_ftz(m[r] - base), pr = ex2_ftz(sc - base);
+            m[r] = m_new;
+            l[r] = fmaf(l[r], alpha, pr);                  // two lanes hold each position: halved at the end
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[r][c] *= alpha;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float pi = __shfl_sync(kAll, pr, (lane & 16) | (i << 1));
+                // a position the row does not see may hold anything: its value is not multiplied
+                if (whole || pos0 + 2 * i + half <= last[r]) {
+                    o[r][0] = fmaf(pi, vv[i].x, o[r][0]);
+                    o[r][1] = fmaf(pi, vv[i].y, o[r][1]);
+                    o[r][2] = fmaf(pi, vv[i].z, o[r][2]);
+                    o[r][3] = fmaf(pi, vv[i].w, o[r][3]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) l[r] += __shfl_xor_sync(kAll, l[r], x);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[r][c] += __shfl_xor_sync(kAll, o[r][c], 16);
+        if (r < n_rows) {
+            if (lane == 0) { sm->m[warp][r] = m[r]; sm->l[warp][r] = 0.5f * l[r]; }
+            if (half == 0)
+                *reinterpret_cast<float4*>(&sm->o[warp][r][4 * dl]) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
+        }
+    }
+}
+
+template <int RMAX, bool BF16>
+__global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_rows_kernel(PagedAttnArgs a) {
+    pdl_trigger();
+    extern __shared__ int s_sched[];
+    __shared__ ScheduleScratch<kFewThreads> scratch;
+    __shared__ __align__(16) FewSmem sm;
+    const int t = threadIdx.x;
+    Schedule sch;
+    build_schedule<kFewThreads>(a, 0, s_sched, &scratch, t, &sch);
+    const int units = sch.unit[a.n_seq];
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+        const int s = owner_of(sch.unit, a.n_seq, u);
+        const SeqShape q = seq_shape(a, s);
+        const int sp = splits_of(q, sch.chunk), in = u - sch.unit[s];
+        const int g = in % a.n_kv_head, split = in / a.n_kv_head % sp, tile = in / a.n_kv_head / sp;
+        const int n_rows = min(kFewRows, q.rows - tile * kFewRows);
+        // the tile's last row bounds its keys
+        const int keys = q.ctx + (tile * kFewRows + n_rows - 1) / a.group + 1;
+        const int p0 = split * sch.chunk, p1 = min(p0 + sch.chunk, (keys + kPageRows - 1) / kPageRows);
+        if (RMAX == 1 || n_rows == 1) few_rows<1, BF16>(a, q, s, tile, g, p0, p1, n_rows, &sm);
+        else if (RMAX == 2 || n_rows == 2) few_rows<(RMAX < 2 ? RMAX : 2), BF16>(a, q, s, tile, g, p0, p1, n_rows, &sm);
+        else if (RMAX == 4 || n_rows <= 4) few_rows<(RMAX < 4 ? RMAX : 4), BF16>(a, q, s, tile, g, p0, p1, n_rows, &sm);
+        else few_rows<RMAX, BF16>(a, q, s, tile, g, p0, p1, n_rows, &sm);
+        __syncthreads();
+        for (int e = t; e < n_rows * kHeadDim; e += kFewThreads) {
+            const int r = e / kHeadDim, d = e % kHeadDim;
+            float mx = sm.m[0][r];
+#pragma unroll
+            for (int w = 1; w < kFewWarps; ++w) mx = fmaxf(mx, sm.m[w][r]);
+            const float base = mx == -INFINITY ? 0.f : mx;
+            float l = 0.f, o = 0.f;
+#pragma unroll
+            for (int w = 0; w < kFewWarps; ++w) {
+                const float f = ex2_ftz(sm.m[w][r] - base);
+                l = fmaf(sm.l[w][r], f, l);
+                if (f > 0.f) o = fmaf(sm.o[w][r][d], f, o);
+            }
+            if (sp == 1) {
+                const int i = tile * kFewRows + r;
+                a.out[(size_t)(q.row0 + i / a.group) * a.ldo + (g * a.group + i % a.group) * kHeadDim + d] =
+                    l == 0.f ? 0.f : o / l;
+            } else {
+                const size_t pu = (size_t)(sch.part[s] + in) * kFewRows + r;
+                a.part_o[0][pu * kHeadDim + d] = o;
+                if (d == 0) { a.part_ml[0][2 * pu] = mx; a.part_ml[0][2 * pu + 1] = l; }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------ the join --
+// Split sequences: a warp per (row, head) adds its splits in order, lane l dims
+// 2 l and 2 l + 1.
+constexpr int kJoinThreads = 256;
+
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(PagedAttnArgs a) {
+    extern __shared__ int s_sched[];
+    __shared__ ScheduleScratch<kJoinThreads> scratch;
+    const int t = threadIdx.x, lane = t & 31;
+    pdl_wait();
+    for (int kind = 0; kind < (a.only_few ? 1 : 2); ++kind) {
+        Schedule sch;
+        build_schedule<kJoinThreads>(a, kind, s_sched, &scratch, t, &sch);
+        const int tr = tile_rows_of(kind);
+        // units that left partials come in groups of `splits` per (tile, head);
+        // an item is one row of one group
+        const long long items = (long long)sch.part[a.n_seq] * tr;
+        for (long long x = (long long)blockIdx.x * (kJoinThreads / 32) + (t >> 5); x < items;
+             x += (long long)gridDim.x * (kJoinThreads / 32)) {
+            const int pu = (int)(x / tr), r = (int)(x % tr);
+            const int s = owner_of(sch.part, a.n_seq, pu);
+            const SeqShape q = seq_shape(a, s);
+            const int sp = splits_of(q, sch.chunk), in = pu - sch.part[s];
+            const int g = in % a.n_kv_head, split = in / a.n_kv_head % sp, tile = in / a.n_kv_head / sp;
+            const int i = tile * tr + r;
+            if (split || i >= q.rows) continue;
+            float mx = -INFINITY;
+            for (int k = lane; k < sp; k += 32)
+                mx = fmaxf(mx, a.part_ml[kind][2 * ((size_t)(pu + k * a.n_kv_head) * tr + r)]);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, o));
+            const float base = mx == -INFINITY ? 0.f : mx;
+            float l = 0.f, ox = 0.f, oy = 0.f;
+            for (int k = 0; k < sp; ++k) {
+                const size_t at = (size_t)(pu + k * a.n_kv_head) * tr + r;
+                const float2 ml = *reinterpret_cast<const float2*>(a.part_ml[kind] + 2 * at);
+                const float f = ex2_ftz(ml.x - base);
+                const float2 v = *reinterpret_cast<const float2*>(a.part_o[kind] + at * kHeadDim + 2 * lane);
+                l = fmaf(ml.y, f, l);
+                if (f > 0.f) { ox = fmaf(v.x, f, ox); oy = fmaf(v.y, f, oy); }
+            }
+            *reinterpret_cast<float2*>(a.out + (size_t)(q.row0 + i / a.group) * a.ldo +
+                                       (g * a.group + i % a.group) * kHeadDim + 2 * lane) =
+                l == 0.f ? make_float2(0.f, 0.f) : make_float2(ox / l, oy / l);
+        }
+        __syncthreads();
+    }
+}
+
+// Units aimed at when sequences are split: four per SM of the streaming kernel
+// (two resident CTAs), two of the tensor-core kernel (one resident).
+int target_of(int kind, int sms) { return (kind ? 2 : 4) * sms; }
+
+// A split sequence has more steps than a chunk, so its units number at most
+// twice its steps over the chunk: all partials fit 2 x target units.
+size_t part_rows(int kind, int sms) { return 2 * (size_t)target_of(kind, sms) * tile_rows_of(kind); }
+size_t scratch_bytes(int sms) { return (part_rows(0, sms) + part_rows(1, sms)) * (kHeadDim + 2) * sizeof(float); }
+
+}  // namespace
+}  // namespace tie
+
+using namespace tie;
+
+extern "C" size_t tie_attention_paged_workspace(void) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return 0; }
+    return scratch_bytes(sm_count(dev));
+}
+
+extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head, const void* k_pages,
+                                            const void* v_pages, int kv_format, int n_pages, int n_kv_head,
+                                            const int32_t* page_table, int pages_per_seq, const int32_t* row_start,
+                                            const int32_t* ctx_lens, int n_seq, int max_new, int rows, float scale,
+                                            float* out, int ldo, void* workspace, size_t workspace_bytes,
+                                            int32_t* status, void* stream) {
+    if (!q || !k_pages || !v_pages || !page_table || !row_start || !ctx_lens || !out || !workspace) return MODEL_ERR_ARG;
+    if (!pool_shape_ok(kv_format, n_pages, n_kv_head) || n_head <= 0 || n_head % n_kv_head || n_head > 8192)
+        return MODEL_ERR_ARG;
+    if (pages_per_seq <= 0 || n_seq <= 0 || max_new < 0 || rows < 0 || !std::isfinite(scale)) return MODEL_ERR_ARG;
+    const int w = n_head * kHeadDim;
+    if (ldq < w || ldo < w || (ldq & 3) || (ldo & 3)) return MODEL_ERR_ARG;
+    if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(workspace))
+        return MODEL_ERR_ARG;
+    if (n_seq > kOpsMaxSeqs || pages_per_seq > kOpsMaxPages - 1) return MODEL_ERR_CAPACITY;
+    // units are counted in int32: at most one per row and head, and one per
+    // sequence and K/V head, before any split
+    if ((long long)rows * n_head + (long long)n_seq * n_kv_head > INT_MAX / 2) return MODEL_ERR_CAPACITY;
+    if (rows == 0 || max_new == 0) return MODEL_OK;
+    OnDeviceOf dev(out);
+    if (dev.status() != MODEL_OK) return dev.status();
+    const int sms = sm_count(dev.device());
+    if (workspace_bytes < scratch_bytes(sms)) return MODEL_ERR_CAPACITY;
+    PagedAttnArgs a{};
+    a.q = q; a.ldq = ldq; a.n_head = n_head;
+    a.k = k_pages; a.v = v_pages;
+    a.n_pages = n_pages; a.n_kv_head = n_kv_head; a.group = n_head / n_kv_head;
+    a.table = page_table; a.width = pages_per_seq;
+    a.row_start = row_start; a.ctx = ctx_lens;
+    a.n_seq = n_seq; a.max_new = max_new; a.rows = rows;
+    a.scale2 = (float)((double)scale * 1.4426950408889634);
+    a.out = out; a.ldo = ldo;
+    float* f = static_cast<float*>(workspace);
+    for (int kind = 0; kind < 2; ++kind) {
+        a.target[kind] = target_of(kind, sms);
+        a.part_o[kind] = f;
+        f += part_rows(kind, sms) * kHeadDim;
+    }
+    for (int kind = 0; kind < 2; ++kind) {
+        a.part_ml[kind] = f;
+        f += part_rows(kind, sms) * 2;
+    }
+    a.status = status;
+    const bool bf16 = kv_format == TIE_KV_BF16;
+    const long long most = (long long)max_new * a.group;      // rows of one sequence and K/V head
+    a.only_few = 1;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const size_t smem = 2 * (size_t)(n_seq + 1) * sizeof(int);
+    {
+        const int rmax = most <= 1 ? 1 : most <= 2 ? 2 : most <= 4 ? 4 : kFewRows;
+        void (*kernel)(PagedAttnArgs) = nullptr;
+        if (bf16)
+            kernel = rmax == 1 ? few_rows_kernel<1, true> : rmax == 2 ? few_rows_kernel<2, true>
+                     : rmax == 4 ? few_rows_kernel<4, true> : few_rows_kernel<8, true>;
+        else
+            kernel = rmax == 1 ? few_rows_kernel<1, false> : rmax == 2 ? few_rows_kernel<2, false>
+                     : rmax == 4 ? few_rows_kernel<4, false> : few_rows_kernel<8, false>;
+        // the prefix sums of more than about 3,700 sequences pass the 48 KB a kernel has unasked
+        TIE_OP_CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        kernel<<<(unsigned)(sms * (rmax <= 2 ? 2 : 1)), kFewThreads, smem, st>>>(a);
+        TIE_OP_CU(cudaGetLastError());
+    }
+    TIE_OP_CU(launch_pdl(join_kernel, dim3((unsigned)sms * 2), dim3(kJoinThreads), smem, st, a));
+    return MODEL_OK;
+}

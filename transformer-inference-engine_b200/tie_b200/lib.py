@@ -21,6 +21,7 @@ for _i, _n in enumerate(MODEL_STATUS + KV_STATUS):
 MODEL_PATH_NOCACHE, MODEL_PATH_CACHE = 0, 1
 TIE_STEP_PERSISTENT, TIE_STEP_CHAINED, TIE_STEP_STREAM = 0, 1, 2
 TIE_WEIGHTS_F32, TIE_WEIGHTS_BF16, TIE_WEIGHTS_INT8 = 0, 1, 2
+TIE_KV_F32, TIE_KV_BF16 = 0, 1
 MODEL_CPROJ_AS_STORED, MODEL_CPROJ_TRANSPOSED = 0, 1
 
 _fp = C.POINTER(C.c_float)
@@ -132,6 +133,18 @@ def library():
         "tie_last_device_error": (C.c_char_p, []),
         "tie_head_argmax_noalloc": (C.c_int, [_vp, C.c_int, _vp, C.c_int, C.c_int, C.c_int, C.c_int,
                                               _vp, C.c_int, _vp, _vp]),
+        "tie_page_plan": (C.c_int, [_vp, _vp, C.c_int, _vp, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp, _vp, _vp,
+                                    _vp, _vp, C.c_int, _vp, _vp]),
+        "tie_kv_store": (C.c_int, [_vp, _vp, C.c_int, _vp, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp]),
+        "tie_attention_paged_workspace": (C.c_size_t, []),
+        "tie_attention_paged": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, C.c_int,
+                                          _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_float, _vp, C.c_int, _vp,
+                                          C.c_size_t, _vp, _vp]),
+        "tie_beam_select_workspace": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+        "tie_beam_select": (C.c_int, [_vp, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp,
+                                      _vp, C.c_size_t, _vp]),
+        "tie_kv_reorder": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_size_t, C.c_int, C.c_int, _vp, C.c_int, _vp,
+                                     _vp, _vp, C.c_int, C.c_int, _vp]),
         "kv_cache_footprint_for": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
         "kv_cache_create": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(_vp)]),
         "kv_cache_destroy": (None, [_vp]),
