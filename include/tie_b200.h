@@ -262,7 +262,7 @@ model_status tie_head_argmax_noalloc(const float *x, int ldx, const float *w, in
  *
  * Pointers are DEVICE pointers of one device (made current for the call) and
  * `stream` a cudaStream_t of it (NULL: the legacy default stream); work is
- * enqueued and not waited for. Activations, pages and workspaces are 16-byte
+ * enqueued and not waited for. Activations and workspaces are 16-byte, pages 32-byte
  * aligned, leading dimensions multiples of 4 floats. A workspace holds nothing
  * from one call to the next, but two calls that overlap on the GPU (streams,
  * replayed graphs) need one each. Nothing is allocated, and every call may be

@@ -31,7 +31,8 @@ void note_device_error(cudaError_t e, const char* what, const char* file, int li
         }                                                                  \
     } while (0)
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+inline bool aligned16(const void* p) { return aligned(p, 16); }
 
 // For the length of a call, makes the device that holds `p` the current one
 // (the caller's pointers need not be on it). status() is MODEL_ERR_ARG for

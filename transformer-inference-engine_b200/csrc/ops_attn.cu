@@ -269,7 +269,7 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
     if (pages_per_seq <= 0 || n_seq <= 0 || max_new < 0 || rows < 0 || !std::isfinite(scale)) return MODEL_ERR_ARG;
     const int w = n_head * kHeadDim;
     if (ldq < w || ldo < w || (ldq & 3) || (ldo & 3)) return MODEL_ERR_ARG;
-    if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(workspace))
+    if (!aligned16(q) || !aligned(k_pages, 32) || !aligned(v_pages, 32) || !aligned16(out) || !aligned16(workspace))
         return MODEL_ERR_ARG;
     if (n_seq > kOpsMaxSeqs || pages_per_seq > kOpsMaxPages - 1) return MODEL_ERR_CAPACITY;
     // units are counted in int32: at most one per row and head, and one per
@@ -302,10 +302,11 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
     a.status = status;
     const bool bf16 = kv_format == TIE_KV_BF16;
     const long long most = (long long)max_new * a.group;      // rows of one sequence and K/V head
-    a.only_few = 1;
+    a.only_few = most <= kFewRows;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const size_t smem = 2 * (size_t)(n_seq + 1) * sizeof(int);
-    {
+    if (!a.only_few) TIE_OP_CU(launch_paged_attn_tc(a, bf16, sms, st));
+    if (a.group <= kFewRows) {
         const int rmax = most <= 1 ? 1 : most <= 2 ? 2 : most <= 4 ? 4 : kFewRows;
         void (*kernel)(PagedAttnArgs) = nullptr;
         if (bf16)

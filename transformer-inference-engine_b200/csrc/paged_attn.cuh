@@ -165,4 +165,7 @@ __device__ __forceinline__ float ex2_ftz(float x) {
     return y;
 }
 
+// Tensor-core kernel (k_paged_tc.cu) for the sequences of kind 1.
+cudaError_t launch_paged_attn_tc(const PagedAttnArgs& a, bool bf16, int sms, cudaStream_t st);
+
 }  // namespace tie
