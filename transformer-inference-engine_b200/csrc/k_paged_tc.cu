@@ -89,26 +89,96 @@ constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kTileKeys >> 3) << 17) | ((
 constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) /* B is MN-major */ | ((uint32_t)(kHeadDim >> 3) << 17) |
                              ((uint32_t)(kTileRows >> 4) << 24);
 
-// D += A . B with A in tensor memory (two fp16 of consecutive k per 32-bit column)
+// D += A . B with A in tensor memory (two fp16 of consecutive k per 32-bit
+// column). Called by a whole, converged warp, of which one lane issues: with
+// one lane in a branch of its own every operand of every MMA would be moved to
+// a uniform register there and then, and the MMAs would wait for the moves.
 __device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, one;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+__device__ __forceinline__ void commit_elected(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred one;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(bar)
+        : "memory");
 }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float2 unpack2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
-// (a, b) as two packed fp16 terms each: hi, and lo in a float's bits
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, float& lo) {
+// two floats in one register pair, and the packed fp32 operations on them
+// (each lane rounds as the scalar operation does)
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// (a, b) as two fp16 terms each: hi and lo, packed. x - hi is exact in fp32.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     hi = pack2(a, b);
-    const float2 f = unpack2(hi);
-    lo = __uint_as_float(pack2(a - f.x, b - f.y));
+    float ra, rb;
+    asm("{\n\t.reg .b16 h0, h1, one;\n\t"
+        "mov.b32 {h0, h1}, %2;\n\t"
+        "mov.b16 one, 0xBC00;\n\t"              // -1
+        "fma.rn.f32.f16 %0, h0, one, %3;\n\t"
+        "fma.rn.f32.f16 %1, h1, one, %4;\n\t}"
+        : "=f"(ra), "=f"(rb)
+        : "r"(hi), "f"(a), "f"(b));
+    lo = pack2(ra, rb);
+}
+
+// 64 columns of the warp's 32 lanes, by two loads and one wait
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t* x = r + 32 * h;
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+            "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+            "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+            : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]),
+              "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]),
+              "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]), "=r"(x[21]), "=r"(x[22]), "=r"(x[23]),
+              "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]), "=r"(x[31])
+            : "r"(taddr + 32u * h));
+    }
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    // no use of a register is moved ahead of the wait
+#pragma unroll
+    for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(r[i]));
 }
 
 // the larger magnitude; NaN if either is
@@ -145,6 +215,14 @@ struct Row8<false> {
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = x[i];
     }
+    // zero for every element that is not finite; whether there was one
+    __device__ __forceinline__ bool clear_odd() {
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (!(fabsf(x[i]) < INFINITY)) { x[i] = 0.f; odd = true; }
+        return odd;
+    }
 };
 template <>
 struct Row8<true> {
@@ -162,30 +240,42 @@ struct Row8<true> {
             y[2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
         }
     }
+    __device__ __forceinline__ bool clear_odd() {
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if ((x[i] & 0x7f80u) == 0x7f80u) { x[i] &= 0xffff0000u; odd = true; }
+            if ((x[i] & 0x7f800000u) == 0x7f800000u) { x[i] &= 0xffffu; odd = true; }
+        }
+        return odd;
+    }
 };
 
-__device__ __forceinline__ float group8_max(float m) {
+// the largest of 8 lanes (a row's) or of the warp (a page's)
+__device__ __forceinline__ float lanes_max(float m, int lanes) {
 #pragma unroll
-    for (int o = 4; o; o >>= 1) m = max_abs(m, __shfl_xor_sync(kAll, m, o));
+    for (int o = 1; o < lanes; o <<= 1) m = max_abs(m, __shfl_xor_sync(kAll, m, o));
     return m;
 }
 
-// Scales 8 elements by 2^(268 - e - 127), splits them, and stores the terms at
-// the row's 16-byte chunk c of a 128-byte-swizzled operand.
+// Scales 8 elements, splits them, and stores the terms at the row's 16-byte
+// chunk `off` of a 128-byte-swizzled operand.
 template <bool BF16>
-__device__ __forceinline__ void store_terms(uint8_t* hi, uint32_t off, float (&y)[8], float scale) {
+__device__ __forceinline__ void store_terms(uint8_t* hi, uint32_t off, const float (&y)[8], float scale) {
     uint32_t h[4], l[4];
+    const f32x2 sc = pair(scale, scale);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float a = y[2 * i] * scale, b = y[2 * i + 1] * scale;
-        h[i] = pack2(a, b);
-        if constexpr (!BF16) {
-            const float2 f = unpack2(h[i]);
-            l[i] = pack2(a - f.x, b - f.y);
-        }
+        const float2 v = unpair(mul2(pair(y[2 * i], y[2 * i + 1]), sc));
+        if constexpr (BF16) h[i] = pack2(v.x, v.y);
+        else split2(v.x, v.y, h[i], l[i]);
     }
     *reinterpret_cast<uint4*>(hi + off) = make_uint4(h[0], h[1], h[2], h[3]);
     if constexpr (!BF16) *reinterpret_cast<uint4*>(hi + kTermBytes + off) = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+__device__ __forceinline__ float max_abs8(const float (&y)[8]) {
+    return max_abs(max_abs(max_abs(y[0], y[1]), max_abs(y[2], y[3])), max_abs(max_abs(y[4], y[5]), max_abs(y[6], y[7])));
 }
 
 template <bool BF16>
@@ -254,6 +344,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
         return false;
     };
 
+    auto wait_all = [&](const uint64_t* bar, uint32_t parity) -> bool { return __all_sync(kAll, wait(bar, parity)); };
+
     const int units = sch.unit[a.n_seq];
     const size_t w = (size_t)a.n_kv_head * kHeadDim;
 
@@ -263,6 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
     struct Unit {
         SeqShape q;
         int s, in, sp, g, row0, n_rows, key0, key1, steps;
+        int first_last;   // the least last visible position of the rows
         const int32_t* table;
     };
     auto unit_of = [&](int u) {
@@ -281,6 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
         x.key1 = (int)min((long long)seen, (long long)x.key0 + (long long)sch.chunk * kTileKeys);
         x.steps = x.key1 > x.key0 ? (x.key1 - x.key0 + kTileKeys - 1) / kTileKeys : 0;
         x.table = a.table + (size_t)x.s * a.width;
+        x.first_last = x.q.ctx + x.row0 / a.group;
         return x;
     };
     // the end of a unit, for all threads: nothing of it is in flight; false ends the loop
@@ -304,7 +398,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
             // failed wait clears `ok` and the n.steps run on, storing nothing.
             const int qq = warp & 3, hf = warp >> 2, r = qq * 32 + lane;
             const int i = min(n.row0 + r, n.q.rows - 1), last = n.q.ctx + i / a.group;
-            const int first_last = n.q.ctx + n.row0 / a.group;   // the least last visible position of the tile
             auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + qq) : "memory"); };
             float m = -INFINITY, l = 0.f;
             bool ok = true;
@@ -321,15 +414,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
 #pragma unroll
                 for (int c = 0; c < 64; ++c) mx = max_abs(mx, x[c]);
                 const int e = row_exponent(mx, 15);
-                const float sc = pow2_biased(268 - e);
-                s_qs[r] = pow2_biased(e - 14) * a.scale2;
-                uint32_t h[32];
+                const float sc = copysignf(pow2_biased(268 - e), a.scale2);   // the scale's sign goes to Q: s_qs >= 0
+                s_qs[r] = pow2_biased(e - 14) * fabsf(a.scale2);
+                uint32_t h[32], lo[32];
 #pragma unroll
-                for (int c = 0; c < 32; ++c) split2(x[2 * c] * sc, x[2 * c + 1] * sc, h[c], x[c]);
+                for (int c = 0; c < 32; ++c) split2(x[2 * c] * sc, x[2 * c + 1] * sc, h[c], lo[c]);
                 tmem_st32(lane_addr + kColQ, h);
-#pragma unroll
-                for (int c = 0; c < 32; ++c) h[c] = __float_as_uint(x[c]);
-                tmem_st32(lane_addr + kColQ + 32u, h);
+                tmem_st32(lane_addr + kColQ + 32u, lo);
                 asm volatile("tcgen05.fence::before_thread_sync;");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(q_full));
@@ -338,37 +429,48 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
             const float qs = s_qs[r];
             for (int j = 0; j < n.steps; ++j) {
                 const uint32_t jj = base + (uint32_t)j, b = jj & 1u;
-                ok = __all_sync(kAll, wait(&v_full[b], (jj >> 1) & 1u)) && ok;
-                ok = __all_sync(kAll, wait(&s_full[b], (jj >> 1) & 1u)) && ok;
+                ok = wait_all(&v_full[b], (jj >> 1) & 1u) && ok;
+                ok = wait_all(&s_full[b], (jj >> 1) & 1u) && ok;
                 asm volatile("tcgen05.fence::after_thread_sync;");
-                const float4* keys = reinterpret_cast<const float4*>(s_keys + (jj & 3u) * 3 * kTileKeys + 64 * hf);
-                float x[64];
-                {
-                    uint32_t v[32];
-                    tmem_ld32(lane_addr + b * kTileKeys + 64u * hf, v);
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) x[c] = __uint_as_float(v[c]);
-                    tmem_ld32(lane_addr + b * kTileKeys + 64u * hf + 32u, v);
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) x[32 + c] = __uint_as_float(v[c]);
-                }
-#pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                    const float4 ks = keys[c], ev = keys[kTileKeys / 4 + c];
-                    x[4 * c] = fmaf(x[4 * c] * qs, ks.x, ev.x);
-                    x[4 * c + 1] = fmaf(x[4 * c + 1] * qs, ks.y, ev.y);
-                    x[4 * c + 2] = fmaf(x[4 * c + 2] * qs, ks.z, ev.z);
-                    x[4 * c + 3] = fmaf(x[4 * c + 3] * qs, ks.w, ev.w);
-                }
+                const float* keys = s_keys + (jj & 3u) * 3 * kTileKeys;
                 const int pos = n.key0 + j * kTileKeys;
-                if (pos + kTileKeys - 1 > first_last) {       // the step crosses the diagonal
+                const bool diagonal = pos + kTileKeys - 1 > n.first_last;
+                uint32_t x[64];
+                tmem_ld64(lane_addr + b * kTileKeys + 64u * hf, x);
+                float mt = -INFINITY;
+                f32x2 c[4];        // a page's factor of S, and what its exponent adds
+                float ev[4];
+                if (diagonal) {
+                    // a scale per key; t in place of S
 #pragma unroll
-                    for (int c = 0; c < 64; ++c)
-                        if (pos + 64 * hf + c > last) x[c] = -INFINITY;
+                    for (int k = 0; k < 16; ++k) {
+                        const float4 ks = reinterpret_cast<const float4*>(keys + 64 * hf)[k];
+                        const float4 ee = reinterpret_cast<const float4*>(keys + kTileKeys + 64 * hf)[k];
+                        const int p0 = pos + 64 * hf + 4 * k;
+                        auto t_of = [&](int d, float f, float e) {
+                            float v = fmaf(__uint_as_float(x[4 * k + d]) * qs, f, e);
+                            if (p0 + d > last) v = -INFINITY;
+                            x[4 * k + d] = __float_as_uint(v);
+                            mt = fmaxf(mt, v);
+                        };
+                        t_of(0, ks.x, ee.x);
+                        t_of(1, ks.y, ee.y);
+                        t_of(2, ks.z, ee.z);
+                        t_of(3, ks.w, ee.w);
+                    }
+                } else {
+                    // a scale per page: the largest t is the largest S's
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const float f = qs * keys[4 * hf + g];
+                        ev[g] = keys[kTileKeys + 4 * hf + g];
+                        float sm = __uint_as_float(x[16 * g]);
+#pragma unroll
+                        for (int d = 1; d < 16; ++d) sm = fmaxf(sm, __uint_as_float(x[16 * g + d]));
+                        mt = fmaxf(mt, fmaf(sm, f, ev[g]));
+                        c[g] = pair(f, f);
+                    }
                 }
-                float mt = x[0];
-#pragma unroll
-                for (int c = 1; c < 64; ++c) mt = fmaxf(mt, x[c]);
                 s_xch[(b * 2 + hf) * kTileRows + r] = mt;
                 pair_sync();
                 mt = fmaxf(mt, s_xch[(b * 2 + (hf ^ 1)) * kTileRows + r]);
@@ -379,26 +481,43 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                     m = mt;
                 }
                 const float lift = m == -INFINITY ? 0.f : kBase - m;
-                // probabilities, their sum, and their two terms: hi[c] packs columns
-                // 2 c and 2 c + 1, x[c] then holds the bits of their lo terms
+                // probabilities, their sum, and their two terms: hi[k] packs columns
+                // 2 k and 2 k + 1, x[k] then holds their lo terms
                 uint32_t hi[32];
                 float sum = 0.f;
+                if (diagonal) {
 #pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                    const float4 iv = keys[2 * (kTileKeys / 4) + c];
-                    const float p0 = ex2_ftz(x[4 * c] + lift), p1 = ex2_ftz(x[4 * c + 1] + lift);
-                    const float p2 = ex2_ftz(x[4 * c + 2] + lift), p3 = ex2_ftz(x[4 * c + 3] + lift);
-                    sum = fmaf(p0, iv.x, sum);
-                    sum = fmaf(p1, iv.y, sum);
-                    sum = fmaf(p2, iv.z, sum);
-                    sum = fmaf(p3, iv.w, sum);
-                    split2(p0, p1, hi[2 * c], x[2 * c]);
-                    split2(p2, p3, hi[2 * c + 1], x[2 * c + 1]);
+                    for (int k = 0; k < 16; ++k) {
+                        const float4 iv = reinterpret_cast<const float4*>(keys + 2 * kTileKeys + 64 * hf)[k];
+                        const float p0 = ex2_ftz(__uint_as_float(x[4 * k]) + lift);
+                        const float p1 = ex2_ftz(__uint_as_float(x[4 * k + 1]) + lift);
+                        const float p2 = ex2_ftz(__uint_as_float(x[4 * k + 2]) + lift);
+                        const float p3 = ex2_ftz(__uint_as_float(x[4 * k + 3]) + lift);
+                        sum = fmaf(p3, iv.w, fmaf(p2, iv.z, fmaf(p1, iv.y, fmaf(p0, iv.x, sum))));
+                        split2(p0, p1, hi[2 * k], x[2 * k]);
+                        split2(p2, p3, hi[2 * k + 1], x[2 * k + 1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x2 add = pair(ev[g] + lift, ev[g] + lift);
+                        f32x2 part = pair(0.f, 0.f);
+#pragma unroll
+                        for (int d = 0; d < 8; ++d) {
+                            const int k = 8 * g + d;
+                            const float2 e = unpair(fma2(pair(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), c[g], add));
+                            const float p0 = ex2_ftz(e.x), p1 = ex2_ftz(e.y);
+                            part = add2(part, pair(p0, p1));
+                            split2(p0, p1, hi[k], x[k]);
+                        }
+                        const float2 ps = unpair(part);
+                        sum = fmaf(ps.x + ps.y, keys[2 * kTileKeys + 4 * hf + g], sum);
+                    }
                 }
                 l = fmaf(l, alpha, sum);
                 if (j > 0) {
                     // P . V of step j - 1 is done: P is free, and O can be rescaled
-                    ok = __all_sync(kAll, wait(o_full, (jj - 1) & 1u)) && ok;
+                    ok = wait_all(o_full, (jj - 1) & 1u) && ok;
                     asm volatile("tcgen05.fence::after_thread_sync;");
                     if (__any_sync(kAll, alpha != 1.f)) {
                         uint32_t v[32];
@@ -410,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                 }
                 tmem_st32(lane_addr + kColP + 32u * hf, hi);
 #pragma unroll
-                for (int c = 0; c < 32; ++c) hi[c] = __float_as_uint(x[c]);
+                for (int k = 0; k < 32; ++k) hi[k] = x[k];
                 tmem_st32(lane_addr + kColP + 64u + 32u * hf, hi);
                 asm volatile("tcgen05.fence::before_thread_sync;");
                 __syncwarp();
@@ -418,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
             }
             float o[32];
             if (n.steps > 0) {
-                ok = __all_sync(kAll, wait(o_full, (base + (uint32_t)n.steps - 1) & 1u)) && ok;
+                ok = wait_all(o_full, (base + (uint32_t)n.steps - 1) & 1u) && ok;
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 pair_sync();     // both halves have read the last maxima
                 s_xch[hf * kTileRows + r] = l;
@@ -502,21 +621,35 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
             for (int j = 0; j < n.steps; ++j) {
                 const uint32_t jj = base + (uint32_t)j, b = jj & 1u, use = jj >> 1;
                 const int pos = n.key0 + j * kTileKeys + lw * kPageRows;
-                float* keys = s_keys + (jj & 3u) * 3 * kTileKeys + lw * kPageRows;
+                float* keys = s_keys + (jj & 3u) * 3 * kTileKeys;
                 // key buffer b is free once S of step j - 2 is computed
                 if (jj >= 2 && !wait(&s_full[b], (use - 1) & 1u)) break;
                 uint8_t* kb = smem + kOffK + b * 2 * kTermBytes;
+                const bool diagonal = n.key0 + j * kTileKeys + kTileKeys - 1 > n.first_last;
+                // largest magnitudes: of each row, or of the page in every entry
+                auto magnitudes = [&](const Row8<BF16>(&r)[4], float (&mx)[4]) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float y[8];
+                        r[i].get(y);
+                        mx[i] = max_abs8(y);
+                    }
+                    if (diagonal) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mx[i] = lanes_max(mx[i], 8);
+                    } else {
+                        mx[0] = mx[1] = mx[2] = mx[3] = lanes_max(max_abs(max_abs(mx[0], mx[1]), max_abs(mx[2], mx[3])), 32);
+                    }
+                };
+                float mx[4];
+                magnitudes(kr, mx);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int row = lw * kPageRows + 4 * i + sub;
+                    const int row = lw * kPageRows + 4 * i + sub, e = row_exponent(mx[i], 15);
                     float y[8];
                     kr[i].get(y);
-                    float mx = 0.f;
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) mx = max_abs(mx, y[c]);
-                    const int e = row_exponent(group8_max(mx), 15);
                     store_terms<BF16>(kb, (uint32_t)(row * 128 + ((dl ^ (row & 7)) << 4)), y, pow2_biased(268 - e));
-                    if (dl == 0) keys[4 * i + sub] = pow2_biased(e - 14);
+                    if (diagonal ? dl == 0 : i == 0 && lane == 0) keys[diagonal ? lw * kPageRows + 4 * i + sub : lw] = pow2_biased(e - 14);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -525,33 +658,26 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                 // value buffer b is free once P . V of step j - 2 is done
                 if (jj >= 2 && !wait(&v_free[b], (use - 1) & 1u)) break;
                 uint8_t* vb = smem + kOffV + b * 2 * kTermBytes;
+                magnitudes(vr, mx);
+                if (__any_sync(kAll, !(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) < INFINITY) ||
+                                         mx[0] != mx[0] || mx[1] != mx[1] || mx[2] != mx[2] || mx[3] != mx[3])) {
+                    // rare: elements that are not finite are left to the epilogue
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (vr[i].clear_odd()) *odd_values = 1;
+                    magnitudes(vr, mx);
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int row = lw * kPageRows + 4 * i + sub;
+                    const int row = lw * kPageRows + 4 * i + sub, e = row_exponent(mx[i], 60);
                     float y[8];
                     vr[i].get(y);
-                    float mx = 0.f;
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) mx = max_abs(mx, y[c]);
-                    mx = group8_max(mx);
-                    if (__any_sync(kAll, !(mx < INFINITY))) {   // rare: leave those elements to the epilogue
-                        mx = 0.f;
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            if (!(fabsf(y[c]) < INFINITY)) {
-                                y[c] = 0.f;
-                                *odd_values = 1;
-                            }
-                            mx = max_abs(mx, y[c]);
-                        }
-                        mx = group8_max(mx);
-                    }
-                    const int e = row_exponent(mx, 60);
                     store_terms<BF16>(vb, (uint32_t)(row * 128 + ((dl ^ (row & 7)) << 4)), y, pow2_biased(268 - e));
-                    if (dl == 0) {
+                    if (diagonal ? dl == 0 : i == 0 && lane == 0) {
+                        const int at = diagonal ? row : lw;
                         const bool there = page >= 0 && pos + 4 * i + sub < n.key1;
-                        keys[kTileKeys + 4 * i + sub] = there ? (float)(e - 141) : -INFINITY;
-                        keys[2 * kTileKeys + 4 * i + sub] = pow2_biased(268 - e);
+                        keys[kTileKeys + at] = there ? (float)(e - 141) : -INFINITY;
+                        keys[2 * kTileKeys + at] = pow2_biased(268 - e);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -571,45 +697,46 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
         uint32_t base = 0, unit_no = 0;
         for (int u = blockIdx.x; u < units; u += gridDim.x) {
             const Unit n = unit_of(u);
-            if (warp == kSoftmaxWarps + kLoadWarps && lane == 0 && n.steps > 0) {
-                const uint32_t sb = smem_u32(smem);
+            const int steps = __shfl_sync(kAll, n.steps, 0);   // the same in all lanes, and known to be
+            if (warp == kSoftmaxWarps + kLoadWarps && steps > 0) {
+                const uint32_t sb = smem_u32(smem), tm = __shfl_sync(kAll, tmem, 0);
                 auto issue_s = [&](int j) -> bool {
                     const uint32_t jj = base + (uint32_t)j, b = jj & 1u;
-                    if (!wait(&k_full[b], (jj >> 1) & 1u)) return false;
+                    if (!wait_all(&k_full[b], (jj >> 1) & 1u)) return false;
                     asm volatile("tcgen05.fence::after_thread_sync;");
-                    const uint32_t kb = sb + kOffK + b * 2 * kTermBytes, d = tmem + b * kTileKeys;
+                    const uint32_t kb = sb + kOffK + b * 2 * kTermBytes, d = tm + b * kTileKeys;
 #pragma unroll
                     for (int ks = 0; ks < kHeadDim / 16; ++ks) {
-                        const uint32_t q_hi = tmem + kColQ + 8u * ks, q_lo = q_hi + 32u;
+                        const uint32_t q_hi = tm + kColQ + 8u * ks, q_lo = q_hi + 32u;
                         const uint64_t k_hi = sw128_desc(kb + 32u * ks);
                         mma_f16_ta(d, q_lo, k_hi, kIdescS, ks ? 1u : 0u);
                         if constexpr (!BF16) mma_f16_ta(d, q_hi, sw128_desc(kb + kTermBytes + 32u * ks), kIdescS, 1u);
                         mma_f16_ta(d, q_hi, k_hi, kIdescS, 1u);
                     }
-                    mma_commit(smem_u32(&s_full[b]));
+                    commit_elected(smem_u32(&s_full[b]));
                     return true;
                 };
-                bool go = wait(q_full, unit_no & 1u) && issue_s(0) && (n.steps < 2 || issue_s(1));
-                for (int j = 0; go && j < n.steps; ++j) {
+                bool go = wait_all(q_full, unit_no & 1u) && issue_s(0) && (steps < 2 || issue_s(1));
+                for (int j = 0; go && j < steps; ++j) {
                     const uint32_t jj = base + (uint32_t)j, b = jj & 1u;
-                    if (!wait(p_full, jj & 1u) || !wait(&v_full[b], (jj >> 1) & 1u)) break;
+                    if (!wait_all(p_full, jj & 1u) || !wait_all(&v_full[b], (jj >> 1) & 1u)) break;
                     asm volatile("tcgen05.fence::after_thread_sync;");
-                    const uint32_t vb = sb + kOffV + b * 2 * kTermBytes, d = tmem + kColO;
+                    const uint32_t vb = sb + kOffV + b * 2 * kTermBytes, d = tm + kColO;
 #pragma unroll
                     for (int ks = 0; ks < kTileKeys / 16; ++ks) {
-                        const uint32_t p_hi = tmem + kColP + 8u * ks, p_lo = p_hi + 64u;
+                        const uint32_t p_hi = tm + kColP + 8u * ks, p_lo = p_hi + 64u;
                         const uint64_t v_hi = sw128_desc(vb + 2048u * ks);
                         mma_f16_ta(d, p_lo, v_hi, kIdescO, (j | ks) ? 1u : 0u);
                         if constexpr (!BF16) mma_f16_ta(d, p_hi, sw128_desc(vb + kTermBytes + 2048u * ks), kIdescO, 1u);
                         mma_f16_ta(d, p_hi, v_hi, kIdescO, 1u);
                     }
-                    mma_commit(smem_u32(o_full));
-                    mma_commit(smem_u32(&v_free[b]));
+                    commit_elected(smem_u32(o_full));
+                    commit_elected(smem_u32(&v_free[b]));
                     // S of step j + 2 into the buffer that step j's softmax has read
-                    if (j + 2 < n.steps && !issue_s(j + 2)) break;
+                    if (j + 2 < steps && !issue_s(j + 2)) break;
                 }
                 // arrives once every MMA issued above has completed, also when cut short
-                mma_commit(smem_u32(drained));
+                commit_elected(smem_u32(drained));
                 const unsigned long long t0 = globaltimer_ns();
                 while (!mbar_try_wait(smem_u32(drained), unit_no & 1u))
                     if (globaltimer_ns() - t0 > kWaitLimitNs) {
