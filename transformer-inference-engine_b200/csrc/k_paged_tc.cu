@@ -2,12 +2,19 @@
 // cores (head_dim 64), for the sequences that ops_attn.cu's streaming kernel
 // leaves to it.
 //
-// One CTA per SM takes units (paged_attn.cuh): 128 rows -- new tokens times the
-// query heads of one K/V head -- against a range of keys in steps of 128, with
-// an online softmax:
+// One CTA per SM takes an equal stretch of the batch's jobs (paged_attn.cuh): a
+// job is one step over the keys of 128 rows,
 //
 //   S  = Q . K^T    M = 128 rows, N = 128 keys, K = 64 dims
 //   O += P . V      M = 128 rows, N = 64 dims,  K = 128 keys
+//
+// with an online softmax. Two streams of jobs run side by side in a CTA, each
+// with its own O, maximum and sum: the two halves of a tile of more than 128
+// rows, over the same steps (keys and values are converted once for both), or
+// else the even and the odd steps of its one half, joined at the end. Three
+// buffers of S go round, so the next S is there when a stream has written its
+// P, and nothing stops between tiles: every role runs ahead as far as its
+// buffers let it.
 //
 // Arithmetic. Results are fp32's. A 16-bit MMA runs at twice the rate of a
 // tf32 one and fp16 has tf32's 11 significant bits, so every operand is split
@@ -35,23 +42,30 @@
 // it.
 //
 // Warps (640 threads, five warpgroups that share the registers by need):
-//   0-7   softmax: warp (q, hf) = (warp % 4, warp / 4) owns TMEM lanes
-//         32 q .. 32 q + 31 (a row per thread) and half hf of the columns.
+//   0-7   softmax: stream warp / 4, TMEM lanes 32 (warp % 4) .. + 31, a row per
+//         thread. S is read twice, for the maximum and for the probabilities,
+//         32 columns at a time; P takes the columns of S as they are read.
 //         The running maximum m moves only when it has grown by more than 8
-//         (powers of two), so O is rescaled rarely. Warps 0-3 also bring Q.
+//         (powers of two), so O is rescaled rarely.
 //   8-15  loaders: warp w takes keys 16 w .. 16 w + 15 of a step, one page, 32
 //         bytes per lane and row; scales, splits and stores them in the
-//         128-byte-swizzled layout of the MMA's B operand (K: K-major; V as it
-//         lies, MN-major). The next step's rows are in registers by then.
-//   16    allocates TMEM, issues the MMAs (17-19 only complete the warpgroup).
-// TMEM (512 columns): S of two steps (256), O (64), P hi/lo (128), Q hi/lo (64).
-// Barriers as in k_tc_attn.cu; every wait is bounded.
+//         128-byte-swizzled layout of the MMA's operands (K: K-major; V as it
+//         lies, MN-major). The next step's rows are in registers by then. A
+//         tile's Q goes the same way, 16 rows a warp.
+//   16    allocates TMEM and issues the MMAs, in the order of the jobs.
+//   17    walks the CTA's stretch and leaves each tile's description in a ring.
+//   18-19 only complete the warpgroup.
+// TMEM (512 columns): three S / P (384), two O (128).
+// Every wait is bounded: on expiry it raises the abort flag, which ends every
+// other wait; the roles run out without storing, the MMAs issued are drained
+// and TMEM is freed.
 #include <cuda.h>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "paged_attn.cuh"
 
@@ -66,7 +80,7 @@ constexpr int kThreads = 640;
 // what the block was launched with
 constexpr int kRegsLaunch = 96, kRegsSoftmax = 120, kRegsLoad = 96, kRegsMma = 40;
 static_assert(256 * kRegsSoftmax + 256 * kRegsLoad + 128 * kRegsMma <= kThreads * kRegsLaunch, "register split");
-constexpr int kSoftmaxWarps = 8, kLoadWarps = 8;
+constexpr int kSoftmaxWarps = 8, kLoadWarps = 8, kMmaWarp = 16, kUnitWarp = 17;
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s
 constexpr unsigned kAll = 0xffffffffu;
 constexpr float kBase = 7.f;        // the largest probability is 2^7 when m is the maximum
@@ -74,25 +88,32 @@ constexpr float kSlack = 8.f;       // m may lag the maximum by this (probabilit
 
 // shared memory (bytes from the 1024-aligned base)
 constexpr uint32_t kTermBytes = kTileKeys * 128;          // 128 rows of 64 fp16
+constexpr int kKeyRing = 8, kUnitRing = 8, kQsRing = kUnitRing;
 constexpr uint32_t kOffK = 0;                             // two buffers of hi, lo
 constexpr uint32_t kOffV = kOffK + 4 * kTermBytes;
-constexpr uint32_t kOffKeys = kOffV + 4 * kTermBytes;     // [4][3][128] per key: scale, e, 2^-e
-constexpr uint32_t kOffQs = kOffKeys + 4 * 3 * kTileKeys * 4;   // [128] per row
-constexpr uint32_t kOffXch = kOffQs + kTileRows * 4;      // [2][2][128] partial maxima / sums
-constexpr uint32_t kOffBars = kOffXch + 4 * kTileRows * 4;
-constexpr uint32_t kOffSched = kOffBars + 128;
-// TMEM columns
-constexpr uint32_t kTmemCols = 512, kColO = 256, kColP = 320, kColQ = 448;
+constexpr uint32_t kOffQ = kOffV + 4 * kTermBytes;        // two halves of hi, lo
+constexpr uint32_t kOffKeys = kOffQ + 4 * kTermBytes;     // [8][3][128] per key (or page): scale, e, 2^-e
+constexpr uint32_t kOffQs = kOffKeys + kKeyRing * 3 * kTileKeys * 4;   // [8][256] per row
+constexpr uint32_t kOffXch = kOffQs + kQsRing * kTileRows * 4;         // [2][4][128] the streams' maxima and sums
+constexpr uint32_t kOffUnits = kOffXch + 8 * kHalfRows * 4;
+constexpr uint32_t kOffBars = kOffUnits + kUnitRing * 80;
+constexpr uint32_t kSmemBytes = kOffBars + 512;
+static_assert(kSmemBytes + 1024 <= 227 * 1024, "shared memory");
+// the line of jobs lies in the buffers that nothing uses yet
+static_assert((kOpsMaxSeqs + 1) * 8 <= (int)kOffKeys, "line of jobs");
+// TMEM columns: S / P of buffer b at 128 b, O of stream st at kColO + 64 st
+constexpr uint32_t kTmemCols = 512, kColO = 384;
 
 // kind::f16 with f16 operands, fp32 accumulation, M = 128
-constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kTileKeys >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kTileKeys >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
 constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) /* B is MN-major */ | ((uint32_t)(kHeadDim >> 3) << 17) |
-                             ((uint32_t)(kTileRows >> 4) << 24);
+                             ((uint32_t)(kHalfRows >> 4) << 24);
 
 // D += A . B with A in tensor memory (two fp16 of consecutive k per 32-bit
-// column). Called by a whole, converged warp, of which one lane issues: with
-// one lane in a branch of its own every operand of every MMA would be moved to
-// a uniform register there and then, and the MMAs would wait for the moves.
+// column), or in shared memory. Called by a whole, converged warp, of which one
+// lane issues: with one lane in a branch of its own every operand of every MMA
+// would be moved to a uniform register there and then, and the MMAs would wait
+// for the moves.
 __device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p, one;\n\t"
@@ -100,6 +121,19 @@ __device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, u
         "elect.sync _|one, 0xffffffff;\n\t"
         "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, one;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+__device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t n) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory");
 }
 
 __device__ __forceinline__ void commit_elected(uint32_t bar) {
@@ -159,27 +193,39 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
     lo = pack2(ra, rb);
 }
 
-// 64 columns of the warp's 32 lanes, by two loads and one wait
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+// 32 columns of the warp's 32 lanes, on their way until tmem_arrived(r)
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&r)[32]) {
     __syncwarp();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t* x = r + 32 * h;
-        asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-            "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-            "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-            : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]),
-              "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]),
-              "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]), "=r"(x[21]), "=r"(x[22]), "=r"(x[23]),
-              "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]), "=r"(x[31])
-            : "r"(taddr + 32u * h));
-    }
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
     // no use of a register is moved ahead of the wait
 #pragma unroll
-    for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(r[i]));
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
 }
+// the same columns written; tmem_stored() waits for all of the warp's stores
+__device__ __forceinline__ void tmem_st32_start(uint32_t taddr, const uint32_t (&r)[32]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // the larger magnitude; NaN if either is
 __device__ __forceinline__ float max_abs(float a, float b) {
@@ -206,6 +252,16 @@ struct Row8<false> {
         asm volatile("ld.global.nc.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
                      : "l"(static_cast<const float*>(base) + at));
+    }
+    // the same from a row that is only 16-byte aligned
+    __device__ __forceinline__ void load_any(const float* from) {
+        const float4 u = __ldg(reinterpret_cast<const float4*>(from)), v = __ldg(reinterpret_cast<const float4*>(from) + 1);
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+    }
+    __device__ __forceinline__ void negate() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = -x[i];
     }
     __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -278,6 +334,23 @@ __device__ __forceinline__ float max_abs8(const float (&y)[8]) {
     return max_abs(max_abs(max_abs(y[0], y[1]), max_abs(y[2], y[3])), max_abs(max_abs(y[4], y[5]), max_abs(y[6], y[7])));
 }
 
+// A tile of the CTA's stretch, as warp 17 describes it to the others.
+struct Unit {
+    int steps;            // over keys [key0, key1); negative: no more tiles
+    int both;             // the streams are the tile's two halves; else its even and odd steps
+    int g, token0;        // K/V head; the sequence's first row of q and out
+    int row0, n_rows;     // rows of the sequence
+    int key0, key1;
+    int first_last;       // the least last visible position of the rows
+    int ctx, part;        // where the result goes: partial 2 * CTA + part, or -1: out
+    int fill0, job0;      // steps and jobs of the tiles before it
+    int half0;            // Q halves used before it
+    int s;
+    int odd;              // a value is not finite (set by the loaders)
+    int pad[4];
+};
+static_assert(sizeof(Unit) == 80, "ring entry");
+
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) {
     extern __shared__ uint8_t smem_raw[];
@@ -285,48 +358,68 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
     float* s_keys = reinterpret_cast<float*>(smem + kOffKeys);
     float* s_qs = reinterpret_cast<float*>(smem + kOffQs);
     float* s_xch = reinterpret_cast<float*>(smem + kOffXch);
+    volatile Unit* units = reinterpret_cast<volatile Unit*>(smem + kOffUnits);
+    // Barriers; a phase of each is one use of what it guards, in order.
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
-    uint64_t* k_full = bars + 0;    // [2] keys of the step in buffer b written (loader warps)
-    uint64_t* v_full = bars + 2;    // [2] values and per-key numbers written (loader warps)
-    uint64_t* s_full = bars + 4;    // [2] S computed: key buffer b free (MMA commit)
-    uint64_t* v_free = bars + 6;    // [2] P . V of value buffer b done (MMA commit)
-    uint64_t* p_full = bars + 8;    // P written, O rescaled (softmax warps)
-    uint64_t* o_full = bars + 9;    // P . V done: P free (MMA commit)
-    uint64_t* drained = bars + 10;  // every MMA of the unit done (MMA commit)
-    uint64_t* q_full = bars + 11;   // Q of the unit in TMEM (softmax warps 0-3)
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
+    uint64_t* k_full = bars + 0;     // [step % 2] keys written (loader warps)
+    uint64_t* v_full = bars + 2;     // [step % 2] values and per-key numbers written (loader warps)
+    uint64_t* k_free = bars + 4;     // [step % 2] keys read by all their MMAs (two commits)
+    uint64_t* v_free = bars + 6;     // [step % 2] values likewise
+    uint64_t* q_full = bars + 8;     // [half % 2] Q half written (loader warps)
+    uint64_t* q_free = bars + 10;    // [half % 2] read by all its MMAs (commit)
+    uint64_t* s_full = bars + 12;    // [job % 3] S computed (commit)
+    uint64_t* p_full = bars + 15;    // [job % 3] P written, O rescaled (the stream's softmax warps)
+    uint64_t* o_done = bars + 18;    // [job % 3] P . V done (commit)
+    uint64_t* o_last = bars + 21;    // [stream] the tile's last P . V of the stream done (commit)
+    uint64_t* o_free = bars + 23;    // [stream] O read by the epilogue (softmax warps)
+    uint64_t* pair_in = bars + 25;   // [lane quarter] both streams' maxima and sums written
+    uint64_t* unit_full = bars + 29; // [tile % 8] description written
+    uint64_t* unit_free = bars + 37; // [tile % 8] read for good (softmax, loader and MMA warps)
+    uint64_t* drained = bars + 45;   // every MMA done (commit)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 46);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* odd_values = reinterpret_cast<volatile int*>(tmem_slot + 2);   // a value of the unit is not finite
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
 
     if (t == 0) {
         for (int b = 0; b < 2; ++b) {
             mbar_init(smem_u32(&k_full[b]), kLoadWarps);
             mbar_init(smem_u32(&v_full[b]), kLoadWarps);
-            mbar_init(smem_u32(&s_full[b]), 1);
-            mbar_init(smem_u32(&v_free[b]), 1);
+            mbar_init(smem_u32(&k_free[b]), 2);
+            mbar_init(smem_u32(&v_free[b]), 2);
+            mbar_init(smem_u32(&q_full[b]), kLoadWarps);
+            mbar_init(smem_u32(&q_free[b]), 1);
+            mbar_init(smem_u32(&o_last[b]), 1);
+            mbar_init(smem_u32(&o_free[b]), kSoftmaxWarps);
         }
-        mbar_init(smem_u32(p_full), kSoftmaxWarps);
-        mbar_init(smem_u32(o_full), 1);
+        for (int b = 0; b < 3; ++b) {
+            mbar_init(smem_u32(&s_full[b]), 1);
+            mbar_init(smem_u32(&p_full[b]), kSoftmaxWarps / 2);
+            mbar_init(smem_u32(&o_done[b]), 1);
+        }
+        for (int b = 0; b < 4; ++b) mbar_init(smem_u32(&pair_in[b]), 2);
+        for (int b = 0; b < kUnitRing; ++b) {
+            mbar_init(smem_u32(&unit_full[b]), 1);
+            mbar_init(smem_u32(&unit_free[b]), kSoftmaxWarps + kLoadWarps + 1);
+        }
         mbar_init(smem_u32(drained), 1);
-        mbar_init(smem_u32(q_full), 4);
         *abort_flag = 0;
-        *odd_values = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kSoftmaxWarps + kLoadWarps) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     __shared__ ScheduleScratch<kThreads> scratch;
-    Schedule sch;
-    build_schedule<kThreads>(a, 1, reinterpret_cast<int*>(smem + kOffSched), &scratch, t, &sch);
+    JobLine line;
+    build_line<kThreads>(a, reinterpret_cast<long long*>(smem), &scratch, t, &line);
+    const long long all = line.base[a.n_seq], g0 = blockIdx.x * line.share, g1 = min(g0 + line.share, all);
+    LineUnit here;                   // the stretch's first tile (warp 17's own)
+    if (warp == kUnitWarp && g0 < g1) here = unit_at(a, line, g0);
     asm volatile("tcgen05.fence::before_thread_sync;");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;");
     const uint32_t tmem = *tmem_slot;
-    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
 
     auto wait = [&](const uint64_t* bar, uint32_t parity) -> bool {
         const uint32_t b = smem_u32(bar);
@@ -343,137 +436,88 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
         if (a.status) atomicExch(a.status, (int)MODEL_ERR_DEVICE);
         return false;
     };
-
     auto wait_all = [&](const uint64_t* bar, uint32_t parity) -> bool { return __all_sync(kAll, wait(bar, parity)); };
-
-    const int units = sch.unit[a.n_seq];
+    // tile number n of the stretch is described
+    auto unit_there = [&](uint32_t n) -> bool { return wait_all(&unit_full[n % kUnitRing], n / kUnitRing & 1u); };
+    auto unit_read = [&](uint32_t n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&unit_free[n % kUnitRing]));
+    };
     const size_t w = (size_t)a.n_kv_head * kHeadDim;
-
-    // Each role runs its own loop over the CTA's units (a register count per
-    // role needs code of its own), all in the same order; `base` counts the
-    // steps of the units before, so buffers and parities run on.
-    struct Unit {
-        SeqShape q;
-        int s, in, sp, g, row0, n_rows, key0, key1, steps;
-        int first_last;   // the least last visible position of the rows
-        const int32_t* table;
-    };
-    auto unit_of = [&](int u) {
-        Unit x;
-        x.s = owner_of(sch.unit, a.n_seq, u);
-        x.q = seq_shape(a, x.s);
-        x.sp = splits_of(x.q, sch.chunk);
-        x.in = u - sch.unit[x.s];
-        x.g = x.in % a.n_kv_head;
-        const int split = x.in / a.n_kv_head % x.sp, tile = x.in / a.n_kv_head / x.sp;
-        x.row0 = tile * kTileRows;
-        x.n_rows = min(kTileRows, x.q.rows - x.row0);
-        // keys [key0, key1): the split's, up to the tile's last visible one
-        x.key0 = split * sch.chunk * kTileKeys;
-        const int seen = x.q.ctx + (x.row0 + x.n_rows - 1) / a.group + 1;
-        x.key1 = (int)min((long long)seen, (long long)x.key0 + (long long)sch.chunk * kTileKeys);
-        x.steps = x.key1 > x.key0 ? (x.key1 - x.key0 + kTileKeys - 1) / kTileKeys : 0;
-        x.table = a.table + (size_t)x.s * a.width;
-        x.first_last = x.q.ctx + x.row0 / a.group;
-        return x;
-    };
-    // the end of a unit, for all threads: nothing of it is in flight; false ends the loop
-    auto unit_end = [&]() -> bool {
-        asm volatile("tcgen05.fence::before_thread_sync;");
-        asm volatile("bar.sync 0;" ::: "memory");
-        asm volatile("tcgen05.fence::after_thread_sync;");
-        const bool go = !*abort_flag;
-        if (t == 0) *odd_values = 0;
-        asm volatile("bar.sync 0;" ::: "memory");
-        return go;
-    };
 
     if (warp < kSoftmaxWarps) {
         // ------------------------------------------------------------ softmax
+        // tcgen05.ld / .st are warp-collective: every condition around them is
+        // the warp's.
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        uint32_t base = 0, unit_no = 0;
-        for (int u = blockIdx.x; u < units; u += gridDim.x) {
-            const Unit n = unit_of(u);
-            // tcgen05.ld / .st and the named barriers are warp-collective: a
-            // failed wait clears `ok` and the n.steps run on, storing nothing.
-            const int qq = warp & 3, hf = warp >> 2, r = qq * 32 + lane;
-            const int i = min(n.row0 + r, n.q.rows - 1), last = n.q.ctx + i / a.group;
-            auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + qq) : "memory"); };
-            float m = -INFINITY, l = 0.f;
+        const int st = warp >> 2, qq = warp & 3, r = qq * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(qq * 32) << 16);
+        uint32_t lasts = 0, pairs = 0;      // o_last and pair_in phases so far
+        for (uint32_t un = 0;; ++un) {
+            if (!unit_there(un)) break;
+            const volatile Unit& n = units[un % kUnitRing];
+            const int steps = n.steps, both = n.both;
+            if (steps < 0) break;
+            const int row = (both ? st * kHalfRows : 0) + r, n_rows = n.n_rows;   // of the tile
+            const int i = n.row0 + min(row, n_rows - 1), last = n.ctx + i / a.group;
+            const int key0 = n.key0, first_last = n.first_last;
+            const uint32_t fill0 = (uint32_t)n.fill0, job0 = (uint32_t)n.job0;
+            float m = -INFINITY, l = 0.f, qs = 0.f;
             bool ok = true;
-            if (hf == 0 && n.steps > 0) {
-                // Q: TMEM lane = row, a thread's 64 dims
-                float x[64], mx = 0.f;
-                const float* from = a.q + (size_t)(n.q.row0 + i / a.group) * a.ldq + (n.g * a.group + i % a.group) * kHeadDim;
-#pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                    const float4 v = r < n.n_rows ? __ldg(reinterpret_cast<const float4*>(from) + c)
-                                                : make_float4(0.f, 0.f, 0.f, 0.f);
-                    x[4 * c] = v.x; x[4 * c + 1] = v.y; x[4 * c + 2] = v.z; x[4 * c + 3] = v.w;
-                }
-#pragma unroll
-                for (int c = 0; c < 64; ++c) mx = max_abs(mx, x[c]);
-                const int e = row_exponent(mx, 15);
-                const float sc = copysignf(pow2_biased(268 - e), a.scale2);   // the scale's sign goes to Q: s_qs >= 0
-                s_qs[r] = pow2_biased(e - 14) * fabsf(a.scale2);
-                uint32_t h[32], lo[32];
-#pragma unroll
-                for (int c = 0; c < 32; ++c) split2(x[2 * c] * sc, x[2 * c + 1] * sc, h[c], lo[c]);
-                tmem_st32(lane_addr + kColQ, h);
-                tmem_st32(lane_addr + kColQ + 32u, lo);
-                asm volatile("tcgen05.fence::before_thread_sync;");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(q_full));
-            }
-            pair_sync();     // the partner warp's s_qs
-            const float qs = s_qs[r];
-            for (int j = 0; j < n.steps; ++j) {
-                const uint32_t jj = base + (uint32_t)j, b = jj & 1u;
-                ok = wait_all(&v_full[b], (jj >> 1) & 1u) && ok;
-                ok = wait_all(&s_full[b], (jj >> 1) & 1u) && ok;
+            const int j0 = both ? 0 : st, dj = both ? 1 : 2;
+#pragma unroll 1
+            for (int j = j0; j < steps; j += dj) {
+                const uint32_t f = fill0 + (uint32_t)j, job = job0 + (both ? 2u * j + st : (uint32_t)j), buf = job % 3u;
+                const uint32_t col_s = lanes + buf * kTileKeys;
+                ok = ok && wait_all(&v_full[f & 1u], f >> 1 & 1u);
+                ok = ok && wait_all(&s_full[buf], job / 3u & 1u);
+                if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;");
-                const float* keys = s_keys + (jj & 3u) * 3 * kTileKeys;
-                const int pos = n.key0 + j * kTileKeys;
-                const bool diagonal = pos + kTileKeys - 1 > n.first_last;
-                uint32_t x[64];
-                tmem_ld64(lane_addr + b * kTileKeys + 64u * hf, x);
+                if (j == j0) qs = s_qs[(un % kQsRing) * kTileRows + row];   // written before the tile's first v_full
+                const float* keys = s_keys + (f % kKeyRing) * 3 * kTileKeys;
+                const int pos = key0 + j * kTileKeys;
+                const bool diagonal = pos + kTileKeys - 1 > first_last;
+                uint32_t x[32];
+                // t of four columns 4 k .. 4 k + 3 of a step on the diagonal: a scale per key
+                auto t_of4 = [&](const uint32_t* s4, int k, float (&tt)[4]) {
+                    const float4 ks = reinterpret_cast<const float4*>(keys)[k];
+                    const float4 ee = reinterpret_cast<const float4*>(keys + kTileKeys)[k];
+                    const float fk[4] = {ks.x, ks.y, ks.z, ks.w}, e[4] = {ee.x, ee.y, ee.z, ee.w};
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        tt[d] = fmaf(__uint_as_float(s4[d]) * qs, fk[d], e[d]);
+                        if (pos + 4 * k + d > last) tt[d] = -INFINITY;
+                    }
+                };
                 float mt = -INFINITY;
-                f32x2 c[4];        // a page's factor of S, and what its exponent adds
-                float ev[4];
-                if (diagonal) {
-                    // a scale per key; t in place of S
+                // one body per pass for the four chunks of 32 columns: unrolled, the
+                // roles' code together outgrows the instruction cache
+                tmem_ld32_start(col_s, x);
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    tmem_arrived(x);
+                    if (diagonal) {
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float4 ks = reinterpret_cast<const float4*>(keys + 64 * hf)[k];
-                        const float4 ee = reinterpret_cast<const float4*>(keys + kTileKeys + 64 * hf)[k];
-                        const int p0 = pos + 64 * hf + 4 * k;
-                        auto t_of = [&](int d, float f, float e) {
-                            float v = fmaf(__uint_as_float(x[4 * k + d]) * qs, f, e);
-                            if (p0 + d > last) v = -INFINITY;
-                            x[4 * k + d] = __float_as_uint(v);
-                            mt = fmaxf(mt, v);
-                        };
-                        t_of(0, ks.x, ee.x);
-                        t_of(1, ks.y, ee.y);
-                        t_of(2, ks.z, ee.z);
-                        t_of(3, ks.w, ee.w);
+                        for (int k = 0; k < 8; ++k) {
+                            float tt[4];
+                            t_of4(x + 4 * k, 8 * c + k, tt);
+                            mt = fmaxf(fmaxf(fmaxf(mt, tt[0]), tt[1]), fmaxf(tt[2], tt[3]));
+                        }
+                    } else {
+                        // a scale per page: the largest t is the largest S's
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            float s0 = __uint_as_float(x[16 * g]), s1 = __uint_as_float(x[16 * g + 1]);
+#pragma unroll
+                            for (int d = 2; d < 16; d += 2) {
+                                s0 = fmaxf(s0, __uint_as_float(x[16 * g + d]));
+                                s1 = fmaxf(s1, __uint_as_float(x[16 * g + d + 1]));
+                            }
+                            mt = fmaxf(mt, fmaf(fmaxf(s0, s1), qs * keys[2 * c + g], keys[kTileKeys + 2 * c + g]));
+                        }
                     }
-                } else {
-                    // a scale per page: the largest t is the largest S's
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const float f = qs * keys[4 * hf + g];
-                        ev[g] = keys[kTileKeys + 4 * hf + g];
-                        float sm = __uint_as_float(x[16 * g]);
-#pragma unroll
-                        for (int d = 1; d < 16; ++d) sm = fmaxf(sm, __uint_as_float(x[16 * g + d]));
-                        mt = fmaxf(mt, fmaf(sm, f, ev[g]));
-                        c[g] = pair(f, f);
-                    }
+                    tmem_ld32_start(col_s + 32u * ((c + 1) & 3), x);   // the last one begins the second pass
                 }
-                s_xch[(b * 2 + hf) * kTileRows + r] = mt;
-                pair_sync();
-                mt = fmaxf(mt, s_xch[(b * 2 + (hf ^ 1)) * kTileRows + r]);
                 float alpha = 1.f;
                 if (mt > m + kSlack || m == -INFINITY) {      // also the first finite maximum
                     alpha = ex2_ftz(m - mt);                  // m = -inf: 0 (or, mt = -inf too, unused)
@@ -481,159 +525,266 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                     m = mt;
                 }
                 const float lift = m == -INFINITY ? 0.f : kBase - m;
-                // probabilities, their sum, and their two terms: hi[k] packs columns
-                // 2 k and 2 k + 1, x[k] then holds their lo terms
-                uint32_t hi[32];
                 float sum = 0.f;
-                if (diagonal) {
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    tmem_arrived(x);
+                    uint32_t p[32];                           // hi terms of columns 2 k, 2 k + 1 in p[k], lo in p[16 + k]
+                    if (diagonal) {
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float4 iv = reinterpret_cast<const float4*>(keys + 2 * kTileKeys + 64 * hf)[k];
-                        const float p0 = ex2_ftz(__uint_as_float(x[4 * k]) + lift);
-                        const float p1 = ex2_ftz(__uint_as_float(x[4 * k + 1]) + lift);
-                        const float p2 = ex2_ftz(__uint_as_float(x[4 * k + 2]) + lift);
-                        const float p3 = ex2_ftz(__uint_as_float(x[4 * k + 3]) + lift);
-                        sum = fmaf(p3, iv.w, fmaf(p2, iv.z, fmaf(p1, iv.y, fmaf(p0, iv.x, sum))));
-                        split2(p0, p1, hi[2 * k], x[2 * k]);
-                        split2(p2, p3, hi[2 * k + 1], x[2 * k + 1]);
-                    }
-                } else {
+                        for (int k = 0; k < 8; ++k) {
+                            float tt[4];
+                            t_of4(x + 4 * k, 8 * c + k, tt);
+                            const float4 iv = reinterpret_cast<const float4*>(keys + 2 * kTileKeys)[8 * c + k];
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const f32x2 add = pair(ev[g] + lift, ev[g] + lift);
-                        f32x2 part = pair(0.f, 0.f);
-#pragma unroll
-                        for (int d = 0; d < 8; ++d) {
-                            const int k = 8 * g + d;
-                            const float2 e = unpair(fma2(pair(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), c[g], add));
-                            const float p0 = ex2_ftz(e.x), p1 = ex2_ftz(e.y);
-                            part = add2(part, pair(p0, p1));
-                            split2(p0, p1, hi[k], x[k]);
+                            for (int d = 0; d < 4; ++d) tt[d] = ex2_ftz(tt[d] + lift);
+                            sum = fmaf(tt[3], iv.w, fmaf(tt[2], iv.z, fmaf(tt[1], iv.y, fmaf(tt[0], iv.x, sum))));
+                            split2(tt[0], tt[1], p[2 * k], p[16 + 2 * k]);
+                            split2(tt[2], tt[3], p[2 * k + 1], p[16 + 2 * k + 1]);
                         }
-                        const float2 ps = unpair(part);
-                        sum = fmaf(ps.x + ps.y, keys[2 * kTileKeys + 4 * hf + g], sum);
+                    } else {
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const float fk = qs * keys[2 * c + g], e = keys[kTileKeys + 2 * c + g] + lift;
+                            const f32x2 ff = pair(fk, fk), ee = pair(e, e);
+                            f32x2 part = pair(0.f, 0.f);
+#pragma unroll
+                            for (int d = 0; d < 8; ++d) {
+                                const int k = 8 * g + d;
+                                const float2 y = unpair(fma2(pair(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), ff, ee));
+                                const float p0 = ex2_ftz(y.x), p1 = ex2_ftz(y.y);
+                                part = add2(part, pair(p0, p1));
+                                split2(p0, p1, p[k], p[16 + k]);
+                            }
+                            const float2 ps = unpair(part);
+                            sum = fmaf(ps.x + ps.y, keys[2 * kTileKeys + 2 * c + g], sum);
+                        }
                     }
+                    if (c < 3) tmem_ld32_start(col_s + 32u * (c + 1), x);
+                    tmem_st32_start(col_s + 32u * c, p);      // over the columns of S it was made from
                 }
                 l = fmaf(l, alpha, sum);
-                if (j > 0) {
-                    // P . V of step j - 1 is done: P is free, and O can be rescaled
-                    ok = wait_all(o_full, (jj - 1) & 1u) && ok;
+                if (__any_sync(kAll, alpha != 1.f && j > j0)) {
+                    // O of the stream's job before, once its P . V is done
+                    const uint32_t before = job - 2u;
+                    ok = ok && wait_all(&o_done[before % 3u], before / 3u & 1u);
+                    if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;");
-                    if (__any_sync(kAll, alpha != 1.f)) {
-                        uint32_t v[32];
-                        tmem_ld32(lane_addr + kColO + 32u * hf, v);
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        tmem_ld32_start(lanes + kColO + 64u * st + 32u * h, x);
+                        tmem_arrived(x);
 #pragma unroll
-                        for (int d = 0; d < 32; ++d) v[d] = __float_as_uint(__uint_as_float(v[d]) * alpha);
-                        tmem_st32(lane_addr + kColO + 32u * hf, v);
+                        for (int d = 0; d < 32; ++d) x[d] = __float_as_uint(__uint_as_float(x[d]) * alpha);
+                        tmem_st32_start(lanes + kColO + 64u * st + 32u * h, x);
+                        tmem_stored();
                     }
                 }
-                tmem_st32(lane_addr + kColP + 32u * hf, hi);
-#pragma unroll
-                for (int k = 0; k < 32; ++k) hi[k] = x[k];
-                tmem_st32(lane_addr + kColP + 64u + 32u * hf, hi);
+                tmem_stored();
                 asm volatile("tcgen05.fence::before_thread_sync;");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(p_full));
+                if (lane == 0) mbar_arrive(smem_u32(&p_full[buf]));
             }
-            float o[32];
-            if (n.steps > 0) {
-                ok = wait_all(o_full, (base + (uint32_t)n.steps - 1) & 1u) && ok;
-                asm volatile("tcgen05.fence::after_thread_sync;");
-                pair_sync();     // both halves have read the last maxima
-                s_xch[hf * kTileRows + r] = l;
-                pair_sync();
-                l = s_xch[r] + s_xch[kTileRows + r];
-                uint32_t v[32];
-                tmem_ld32(lane_addr + kColO + 32u * hf, v);
-#pragma unroll
-                for (int d = 0; d < 32; ++d) o[d] = __uint_as_float(v[d]);
-            } else {
-#pragma unroll
-                for (int d = 0; d < 32; ++d) o[d] = 0.f;
+            if (j0 < steps) {
+                ok = ok && wait_all(&o_last[st], lasts & 1u);
+                ++lasts;
             }
-            if (ok && r < n.n_rows) {
-                if (*odd_values) {
+            if (!ok) break;
+            // this thread's results: row `row`, dims [dim0, dim0 + 32), from o
+            auto put = [&](uint32_t (&o)[32], int dim0, float mm, float ll) {
+                if (n.odd) {
                     // values that are not finite, for the rows that see them
-                    for (int key = n.key0; key < min(n.key1, last + 1); ++key) {
-                        const int e = __ldg(n.table + key / kPageRows);
+                    const int32_t* table = a.table + (size_t)n.s * a.width;
+                    for (int key = key0; key < min(n.key1, last + 1); ++key) {
+                        const int e = __ldg(table + key / kPageRows);
                         if (e < 0 || e >= a.n_pages) continue;
-                        const size_t at = ((size_t)e * kPageRows + key % kPageRows) * w + n.g * kHeadDim + 32 * hf;
-#pragma unroll
+                        const size_t at = ((size_t)e * kPageRows + key % kPageRows) * w + n.g * kHeadDim + dim0;
+#pragma unroll 1
                         for (int d = 0; d < 32; ++d) {
-                            float x;
-                            if constexpr (BF16) x = __bfloat162float(static_cast<const __nv_bfloat16*>(a.v)[at + d]);
-                            else x = static_cast<const float*>(a.v)[at + d];
-                            if (!(fabsf(x) < INFINITY)) o[d] += x;
+                            float v;
+                            if constexpr (BF16) v = __bfloat162float(static_cast<const __nv_bfloat16*>(a.v)[at + d]);
+                            else v = static_cast<const float*>(a.v)[at + d];
+                            if (fabsf(v) < INFINITY) continue;
+#pragma unroll
+                            for (int k = 0; k < 32; ++k)
+                                if (k == d) o[k] = __float_as_uint(__uint_as_float(o[k]) + v);
                         }
                     }
                 }
-                if (n.sp == 1) {
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
-                    float4* to = reinterpret_cast<float4*>(a.out + (size_t)(n.q.row0 + i / a.group) * a.ldo +
-                                                           (n.g * a.group + i % a.group) * kHeadDim + 32 * hf);
-#pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        to[c] = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                         : make_float4(o[4 * c] * inv, o[4 * c + 1] * inv, o[4 * c + 2] * inv, o[4 * c + 3] * inv);
+                float4* to;
+                float f = 1.f;
+                if (n.part < 0) {
+                    f = ll == 0.f ? 0.f : 1.f / ll;
+                    to = reinterpret_cast<float4*>(a.out + (size_t)(n.token0 + i / a.group) * a.ldo +
+                                                   (n.g * a.group + i % a.group) * kHeadDim + dim0);
                 } else {
-                    const size_t pu = (size_t)(sch.part[n.s] + n.in) * kTileRows + r;
-                    float4* to = reinterpret_cast<float4*>(a.part_o[1] + pu * kHeadDim + 32 * hf);
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) to[c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
-                    if (hf == 0) {
-                        a.part_ml[1][2 * pu] = m == -INFINITY ? m : m - kBase;
-                        a.part_ml[1][2 * pu + 1] = l;
+                    const size_t at = (2 * (size_t)blockIdx.x + n.part) * kTileRows + row;
+                    to = reinterpret_cast<float4*>(a.part_o[1] + at * kHeadDim + dim0);
+                    if (dim0 == 0) {
+                        a.part_ml[1][2 * at] = mm == -INFINITY ? mm : mm - kBase;
+                        a.part_ml[1][2 * at + 1] = ll;
                     }
                 }
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    to[c] = f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                     : make_float4(__uint_as_float(o[4 * c]) * f, __uint_as_float(o[4 * c + 1]) * f,
+                                                   __uint_as_float(o[4 * c + 2]) * f, __uint_as_float(o[4 * c + 3]) * f);
+            };
+            uint32_t o[32];
+            if (both) {
+                asm volatile("tcgen05.fence::after_thread_sync;");
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    tmem_ld32_start(lanes + kColO + 64u * st + 32u * h, o);
+                    tmem_arrived(o);
+                    if (steps == 0) {
+                        // the stretch has the second half of a step that belongs to the CTA
+                        // before: a part with nothing in it
+#pragma unroll
+                        for (int d = 0; d < 32; ++d) o[d] = 0u;
+                    }
+                    if (row < n_rows) put(o, 32 * h, m, l);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;");
+                __syncwarp();
+                if (lane == 0) mbar_arrive_n(smem_u32(&o_free[st]), 2);
+            } else {
+                // the streams' results joined: each stream's warps do 32 dims
+                float* xch = s_xch + (un & 1u) * 4 * kHalfRows;
+                xch[(2 * st) * kHalfRows + r] = m;
+                xch[(2 * st + 1) * kHalfRows + r] = l;
+                asm volatile("tcgen05.fence::before_thread_sync;");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&pair_in[qq]));
+                if (!wait_all(&pair_in[qq], pairs & 1u)) break;
+                ++pairs;
+                asm volatile("tcgen05.fence::after_thread_sync;");
+                const float m0 = xch[r], l0 = xch[kHalfRows + r], m1 = xch[2 * kHalfRows + r], l1 = xch[3 * kHalfRows + r];
+                const float mm = fmaxf(m0, m1), base = mm == -INFINITY ? 0.f : mm;
+                const float f0 = ex2_ftz(m0 - base), f1 = ex2_ftz(m1 - base);
+                uint32_t v1[32];
+                tmem_ld32_start(lanes + kColO + 32u * st, o);
+                tmem_arrived(o);
+                tmem_ld32_start(lanes + kColO + 64u + 32u * st, v1);
+                tmem_arrived(v1);
+                asm volatile("tcgen05.fence::before_thread_sync;");
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(&o_free[0]));
+                    mbar_arrive(smem_u32(&o_free[1]));
+                }
+#pragma unroll
+                for (int d = 0; d < 32; ++d) {
+                    float v = f0 > 0.f ? __uint_as_float(o[d]) * f0 : 0.f;
+                    // a stream without steps has left nothing in its O
+                    if (f1 > 0.f) v = fmaf(__uint_as_float(v1[d]), f1, v);
+                    o[d] = __float_as_uint(v);
+                }
+                if (row < n_rows) put(o, 32 * st, mm, fmaf(l1, f1, l0 * f0));
             }
-            base += (uint32_t)n.steps;
-            unit_no += n.steps > 0;
-            if (!unit_end()) break;
+            unit_read(un);
         }
     } else if (warp < kSoftmaxWarps + kLoadWarps) {
         // ------------------------------------------------------------ loaders
-        uint32_t base = 0, unit_no = 0;
-        for (int u = blockIdx.x; u < units; u += gridDim.x) {
-            const Unit n = unit_of(u);
-            const int lw = warp - kSoftmaxWarps, sub = lane >> 3, dl = lane & 7;
-            Row8<BF16> kr[4], vr[4];
-            // this warp's page of step j: its 16 positions, or -1
-            auto page_of = [&](int j) {
-                const int p = (n.key0 + j * kTileKeys) / kPageRows + lw;
-                if (j >= n.steps || (long long)p * kPageRows >= n.key1) return -1;
-                const int e = __ldg(n.table + p);
-                return e >= 0 && e < a.n_pages ? e : -1;
-            };
-            auto load = [&](Row8<BF16>(&r)[4], const void* from, int j, int page) {
-                const int pos = n.key0 + j * kTileKeys + lw * kPageRows;
+        const int lw = warp - kSoftmaxWarps, sub = lane >> 3, dl = lane & 7;
+        Row8<BF16> kr[4], vr[4];
+        // the rows of step j of the tile in ring entry `e` that this warp has: its
+        // page (or -1), and their loads
+        auto page_of = [&](const volatile Unit& n, int j) {
+            const int p = (n.key0 + j * kTileKeys) / kPageRows + lw;
+            if (j >= n.steps || (long long)p * kPageRows >= n.key1) return -1;
+            const int e = __ldg(a.table + (size_t)n.s * a.width + p);
+            return e >= 0 && e < a.n_pages ? e : -1;
+        };
+        auto load = [&](Row8<BF16>(&rows)[4], const void* from, const volatile Unit& n, int j, int page) {
+            const int pos = n.key0 + j * kTileKeys + lw * kPageRows, key1 = n.key1, g = n.g;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = 4 * i + sub;
-                    if (page >= 0 && pos + row < n.key1)
-                        r[i].load(from, ((size_t)page * kPageRows + row) * w + n.g * kHeadDim + 8 * dl);
-                    else
-                        r[i].zero();
-                }
-            };
-            int page = page_of(0), page_next = page_of(1);
-            load(kr, a.k, 0, page);
-            load(vr, a.v, 0, page);
-            for (int j = 0; j < n.steps; ++j) {
-                const uint32_t jj = base + (uint32_t)j, b = jj & 1u, use = jj >> 1;
-                const int pos = n.key0 + j * kTileKeys + lw * kPageRows;
-                float* keys = s_keys + (jj & 3u) * 3 * kTileKeys;
-                // key buffer b is free once S of step j - 2 is computed
-                if (jj >= 2 && !wait(&s_full[b], (use - 1) & 1u)) break;
-                uint8_t* kb = smem + kOffK + b * 2 * kTermBytes;
-                const bool diagonal = n.key0 + j * kTileKeys + kTileKeys - 1 > n.first_last;
-                // largest magnitudes: of each row, or of the page in every entry
-                auto magnitudes = [&](const Row8<BF16>(&r)[4], float (&mx)[4]) {
+            for (int i = 0; i < 4; ++i) {
+                const int row = 4 * i + sub;
+                if (page >= 0 && pos + row < key1)
+                    rows[i].load(from, ((size_t)page * kPageRows + row) * w + g * kHeadDim + 8 * dl);
+                else
+                    rows[i].zero();
+            }
+        };
+        // stores this warp's 16 rows as terms; mx: what each row (in all its lanes) is scaled by
+        auto store = [&](uint8_t* to, const auto (&rows)[4], const float (&mx)[4], int lo, auto is_bf16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = lw * 16 + 4 * i + sub;
+                float y[8];
+                rows[i].get(y);
+                store_terms<decltype(is_bf16)::value>(to, (uint32_t)(row * 128 + ((dl ^ (row & 7)) << 4)), y,
+                                                      pow2_biased(268 - row_exponent(mx[i], lo)));
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        };
+        auto row_max = [&](const auto (&rows)[4], float (&mx)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float y[8];
+                rows[i].get(y);
+                mx[i] = max_abs8(y);
+            }
+        };
+        auto arrive = [&](uint64_t* bar) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(bar));
+        };
+        bool ok = unit_there(0);
+        int page = -1, page_next = -1;
+        if (ok && units[0].steps > 0) {
+            page = page_of(units[0], 0);
+            load(kr, a.k, units[0], 0, page);
+            load(vr, a.v, units[0], 0, page);
+        }
+        for (uint32_t un = 0; ok; ++un) {
+            volatile Unit& n = units[un % kUnitRing];
+            const int steps = n.steps;
+            if (steps < 0) break;
+            if (steps > 0) {
+                // Q: rows of 64 floats, a scale per row
+                const uint32_t half0 = (uint32_t)n.half0;
+                page_next = page_of(n, 1);
+#pragma unroll 1
+                for (int h = 0; h <= n.both && ok; ++h) {
+                    const uint32_t half = half0 + (uint32_t)h;
+                    Row8<false> qr[4];
+                    float mx[4];
+                    const int n_rows = n.n_rows, row0 = n.row0, token0 = n.token0, g = n.g;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float y[8];
-                        r[i].get(y);
-                        mx[i] = max_abs8(y);
+                        const int row = h * kHalfRows + lw * 16 + 4 * i + sub, at = row0 + row;
+                        if (row < n_rows)
+                            qr[i].load_any(a.q + (size_t)(token0 + at / a.group) * a.ldq +
+                                           (g * a.group + at % a.group) * kHeadDim + 8 * dl);
+                        else
+                            qr[i].zero();
                     }
+                    row_max(qr, mx);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        mx[i] = lanes_max(mx[i], 8);
+                        if (a.scale2 < 0.f) qr[i].negate();   // the scale's sign goes to Q: s_qs >= 0
+                        if (dl == 0)
+                            s_qs[(un % kQsRing) * kTileRows + h * kHalfRows + lw * 16 + 4 * i + sub] =
+                                pow2_biased(row_exponent(mx[i], 15) - 14) * fabsf(a.scale2);
+                    }
+                    if (half >= 2) ok = wait_all(&q_free[half & 1u], ((half >> 1) - 1) & 1u);
+                    if (!ok) break;
+                    store(smem + kOffQ + (half & 1u) * 2 * kTermBytes, qr, mx, 15, std::false_type{});
+                    arrive(&q_full[half & 1u]);
+                }
+            }
+#pragma unroll 1
+            for (int j = 0; j < steps && ok; ++j) {
+                const uint32_t f = (uint32_t)n.fill0 + (uint32_t)j, b = f & 1u, before = ((f >> 1) - 1) & 1u;
+                const int pos = n.key0 + j * kTileKeys + lw * kPageRows;
+                const bool diagonal = n.key0 + j * kTileKeys + kTileKeys - 1 > n.first_last;
+                float* keys = s_keys + (f % kKeyRing) * 3 * kTileKeys;
+                // largest magnitudes: of each row, or of the page in every entry
+                auto spread = [&](float (&mx)[4]) {
                     if (diagonal) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) mx[i] = lanes_max(mx[i], 8);
@@ -642,117 +793,223 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                     }
                 };
                 float mx[4];
-                magnitudes(kr, mx);
+                row_max(kr, mx);
+                spread(mx);
+                // key buffer b is free once the S of the step before last are computed
+                if (f >= 2 && !(ok = wait_all(&k_free[b], before))) break;
+                store(smem + kOffK + b * 2 * kTermBytes, kr, mx, 15, std::integral_constant<bool, BF16>{});
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = lw * kPageRows + 4 * i + sub, e = row_exponent(mx[i], 15);
-                    float y[8];
-                    kr[i].get(y);
-                    store_terms<BF16>(kb, (uint32_t)(row * 128 + ((dl ^ (row & 7)) << 4)), y, pow2_biased(268 - e));
-                    if (diagonal ? dl == 0 : i == 0 && lane == 0) keys[diagonal ? lw * kPageRows + 4 * i + sub : lw] = pow2_biased(e - 14);
+                for (int i = 0; i < 4; ++i)
+                    if (diagonal ? dl == 0 : i == 0 && lane == 0)
+                        keys[diagonal ? lw * kPageRows + 4 * i + sub : lw] = pow2_biased(row_exponent(mx[i], 15) - 14);
+                arrive(&k_full[b]);
+                // the next step's rows, of this tile or the next one
+                const bool over = j + 1 == steps;
+                const volatile Unit* nn = &n;
+                int jn = j + 1;
+                if (over) {
+                    if (!(ok = unit_there(un + 1))) break;
+                    nn = &units[(un + 1) % kUnitRing];
+                    jn = 0;
+                    page_next = nn->steps > 0 ? page_of(*nn, 0) : -1;
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&k_full[b]));
-                load(kr, a.k, j + 1, page_next);
-                // value buffer b is free once P . V of step j - 2 is done
-                if (jj >= 2 && !wait(&v_free[b], (use - 1) & 1u)) break;
-                uint8_t* vb = smem + kOffV + b * 2 * kTermBytes;
-                magnitudes(vr, mx);
-                if (__any_sync(kAll, !(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) < INFINITY) ||
-                                         mx[0] != mx[0] || mx[1] != mx[1] || mx[2] != mx[2] || mx[3] != mx[3])) {
+                if (nn->steps > 0) load(kr, a.k, *nn, jn, page_next);
+                row_max(vr, mx);
+                spread(mx);
+                if (__any_sync(kAll, !(mx[0] < INFINITY && mx[1] < INFINITY && mx[2] < INFINITY && mx[3] < INFINITY))) {
                     // rare: elements that are not finite are left to the epilogue
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (vr[i].clear_odd()) *odd_values = 1;
-                    magnitudes(vr, mx);
+                        if (vr[i].clear_odd()) n.odd = 1;
+                    row_max(vr, mx);
+                    spread(mx);
                 }
+                // value buffer b is free once the P . V of the step before last are done
+                if (f >= 2 && !(ok = wait_all(&v_free[b], before))) break;
+                store(smem + kOffV + b * 2 * kTermBytes, vr, mx, 60, std::integral_constant<bool, BF16>{});
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = lw * kPageRows + 4 * i + sub, e = row_exponent(mx[i], 60);
-                    float y[8];
-                    vr[i].get(y);
-                    store_terms<BF16>(vb, (uint32_t)(row * 128 + ((dl ^ (row & 7)) << 4)), y, pow2_biased(268 - e));
+                for (int i = 0; i < 4; ++i)
                     if (diagonal ? dl == 0 : i == 0 && lane == 0) {
-                        const int at = diagonal ? row : lw;
+                        const int at = diagonal ? lw * kPageRows + 4 * i + sub : lw, e = row_exponent(mx[i], 60);
                         const bool there = page >= 0 && pos + 4 * i + sub < n.key1;
                         keys[kTileKeys + at] = there ? (float)(e - 141) : -INFINITY;
                         keys[2 * kTileKeys + at] = pow2_biased(268 - e);
                     }
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&v_full[b]));
-                load(vr, a.v, j + 1, page_next);
+                arrive(&v_full[b]);
+                if (nn->steps > 0) load(vr, a.v, *nn, jn, page_next);
                 page = page_next;
-                page_next = page_of(j + 2);
+                page_next = over ? -1 : page_of(n, j + 2);
             }
-            base += (uint32_t)n.steps;
-            unit_no += n.steps > 0;
-            if (!unit_end()) break;
+            if (!ok) break;
+            unit_read(un);
+            if (steps == 0) {
+                // nothing was prefetched for the tile after an empty one
+                if (!(ok = unit_there(un + 1))) break;
+                const volatile Unit& x = units[(un + 1) % kUnitRing];
+                if (x.steps > 0) {
+                    page = page_of(x, 0);
+                    load(kr, a.k, x, 0, page);
+                    load(vr, a.v, x, 0, page);
+                }
+            }
         }
     } else {
-        // ---------------------------------------------------------------- MMA
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
-        uint32_t base = 0, unit_no = 0;
-        for (int u = blockIdx.x; u < units; u += gridDim.x) {
-            const Unit n = unit_of(u);
-            const int steps = __shfl_sync(kAll, n.steps, 0);   // the same in all lanes, and known to be
-            if (warp == kSoftmaxWarps + kLoadWarps && steps > 0) {
-                const uint32_t sb = smem_u32(smem), tm = __shfl_sync(kAll, tmem, 0);
-                auto issue_s = [&](int j) -> bool {
-                    const uint32_t jj = base + (uint32_t)j, b = jj & 1u;
-                    if (!wait_all(&k_full[b], (jj >> 1) & 1u)) return false;
-                    asm volatile("tcgen05.fence::after_thread_sync;");
-                    const uint32_t kb = sb + kOffK + b * 2 * kTermBytes, d = tm + b * kTileKeys;
-#pragma unroll
-                    for (int ks = 0; ks < kHeadDim / 16; ++ks) {
-                        const uint32_t q_hi = tm + kColQ + 8u * ks, q_lo = q_hi + 32u;
-                        const uint64_t k_hi = sw128_desc(kb + 32u * ks);
-                        mma_f16_ta(d, q_lo, k_hi, kIdescS, ks ? 1u : 0u);
-                        if constexpr (!BF16) mma_f16_ta(d, q_hi, sw128_desc(kb + kTermBytes + 32u * ks), kIdescS, 1u);
-                        mma_f16_ta(d, q_hi, k_hi, kIdescS, 1u);
-                    }
-                    commit_elected(smem_u32(&s_full[b]));
-                    return true;
-                };
-                bool go = wait_all(q_full, unit_no & 1u) && issue_s(0) && (steps < 2 || issue_s(1));
-                for (int j = 0; go && j < steps; ++j) {
-                    const uint32_t jj = base + (uint32_t)j, b = jj & 1u;
-                    if (!wait_all(p_full, jj & 1u) || !wait_all(&v_full[b], (jj >> 1) & 1u)) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;");
-                    const uint32_t vb = sb + kOffV + b * 2 * kTermBytes, d = tm + kColO;
-#pragma unroll
-                    for (int ks = 0; ks < kTileKeys / 16; ++ks) {
-                        const uint32_t p_hi = tm + kColP + 8u * ks, p_lo = p_hi + 64u;
-                        const uint64_t v_hi = sw128_desc(vb + 2048u * ks);
-                        mma_f16_ta(d, p_lo, v_hi, kIdescO, (j | ks) ? 1u : 0u);
-                        if constexpr (!BF16) mma_f16_ta(d, p_hi, sw128_desc(vb + kTermBytes + 2048u * ks), kIdescO, 1u);
-                        mma_f16_ta(d, p_hi, v_hi, kIdescO, 1u);
-                    }
-                    commit_elected(smem_u32(o_full));
-                    commit_elected(smem_u32(&v_free[b]));
-                    // S of step j + 2 into the buffer that step j's softmax has read
-                    if (j + 2 < steps && !issue_s(j + 2)) break;
+        if (warp == kMmaWarp) {
+            // ------------------------------------------------------------ MMA
+            const uint32_t sb = smem_u32(smem), tm = __shfl_sync(kAll, tmem, 0);
+            // a place in the line of jobs: job k of tile un
+            struct Cursor {
+                uint32_t un, job;
+                int k, jobs, both, steps;
+            };
+            // (values of the ring are the same in all lanes, and known to the compiler to be)
+            auto uniform = [&](int v) { return __shfl_sync(kAll, v, 0); };
+            // to the next tile with jobs from c.un on; false: there is none
+            auto settle = [&](Cursor& c) -> bool {
+                for (;; ++c.un) {
+                    if (!unit_there(c.un)) return false;
+                    const volatile Unit& n = units[c.un % kUnitRing];
+                    c.steps = uniform(n.steps);
+                    if (c.steps < 0) return false;
+                    c.both = uniform(n.both);
+                    c.k = 0;
+                    c.jobs = c.steps << c.both;
+                    if (c.jobs) return true;
                 }
-                // arrives once every MMA issued above has completed, also when cut short
-                commit_elected(smem_u32(drained));
-                const unsigned long long t0 = globaltimer_ns();
-                while (!mbar_try_wait(smem_u32(drained), unit_no & 1u))
-                    if (globaltimer_ns() - t0 > kWaitLimitNs) {
-                        *abort_flag = 1;
-                        if (a.status) atomicExch(a.status, (int)MODEL_ERR_DEVICE);
-                        break;
-                    }
+            };
+            Cursor sc{}, pc{};
+            bool s_more = settle(sc), failed = false;
+            // S of the next job, into the buffer that the job three before has left
+            auto issue_s = [&]() -> bool {
+                const volatile Unit& n = units[sc.un % kUnitRing];
+                const int j = sc.k >> sc.both, st = sc.k & 1;
+                const uint32_t f = (uint32_t)uniform(n.fill0) + (uint32_t)j, b = f & 1u, buf = sc.job % 3u;
+                const uint32_t half = (uint32_t)uniform(n.half0) + (sc.both ? (uint32_t)st : 0u);
+                const bool first = sc.both ? j == 0 : sc.k == 0, last = sc.both ? j == sc.steps - 1 : sc.k == sc.jobs - 1;
+                if (first && !wait_all(&q_full[half & 1u], half >> 1 & 1u)) return false;
+                if (!wait_all(&k_full[b], f >> 1 & 1u)) return false;
+                if (sc.job >= 3 && !wait_all(&o_done[buf], (sc.job / 3u - 1) & 1u)) return false;
+                asm volatile("tcgen05.fence::after_thread_sync;");
+                const uint32_t kb = sb + kOffK + b * 2 * kTermBytes, qb = sb + kOffQ + (half & 1u) * 2 * kTermBytes;
+                const uint32_t d = tm + buf * kTileKeys;
+#pragma unroll
+                for (int ks = 0; ks < kHeadDim / 16; ++ks) {
+                    const uint64_t q_hi = sw128_desc(qb + 32u * ks), q_lo = sw128_desc(qb + kTermBytes + 32u * ks);
+                    const uint64_t k_hi = sw128_desc(kb + 32u * ks);
+                    mma_f16(d, q_lo, k_hi, kIdescS, ks ? 1u : 0u);
+                    if constexpr (!BF16) mma_f16(d, q_hi, sw128_desc(kb + kTermBytes + 32u * ks), kIdescS, 1u);
+                    mma_f16(d, q_hi, k_hi, kIdescS, 1u);
+                }
+                commit_elected(smem_u32(&s_full[buf]));
+                commit_elected(smem_u32(&k_free[b]));
+                if (!sc.both) commit_elected(smem_u32(&k_free[b]));   // no other job reads the buffer
+                if (last) commit_elected(smem_u32(&q_free[half & 1u]));
+                ++sc.job;
+                if (++sc.k == sc.jobs) {
+                    ++sc.un;
+                    s_more = settle(sc);
+                }
+                return true;
+            };
+            bool p_more = s_more && settle(pc);
+            for (int k = 0; k < 3 && s_more && !failed; ++k) failed = !issue_s();
+            uint32_t freed = 0;         // tiles whose description is no longer needed
+            while (p_more && !failed) {
+                const volatile Unit& n = units[pc.un % kUnitRing];
+                const int j = pc.k >> pc.both, st = pc.k & 1;
+                const uint32_t f = (uint32_t)uniform(n.fill0) + (uint32_t)j, b = f & 1u, buf = pc.job % 3u;
+                const bool first = pc.both ? j == 0 : pc.k < 2;
+                const bool last = pc.both ? j == pc.steps - 1 : pc.k + 2 >= pc.jobs;
+                if (!wait_all(&p_full[buf], pc.job / 3u & 1u) || !wait_all(&v_full[b], f >> 1 & 1u)) break;
+                // the tile before has left O
+                if (first && pc.un && !wait_all(&o_free[st], (pc.un - 1) & 1u)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;");
+                const uint32_t vb = sb + kOffV + b * 2 * kTermBytes, p_col = tm + buf * kTileKeys, d = tm + kColO + 64u * st;
+#pragma unroll
+                for (int ks = 0; ks < kTileKeys / 16; ++ks) {
+                    // 32 columns of P: the hi terms of 32 keys, then their lo terms
+                    const uint32_t p_hi = p_col + 32u * (ks >> 1) + 8u * (ks & 1), p_lo = p_hi + 16u;
+                    const uint64_t v_hi = sw128_desc(vb + 2048u * ks);
+                    mma_f16_ta(d, p_lo, v_hi, kIdescO, (!first || ks) ? 1u : 0u);
+                    if constexpr (!BF16) mma_f16_ta(d, p_hi, sw128_desc(vb + kTermBytes + 2048u * ks), kIdescO, 1u);
+                    mma_f16_ta(d, p_hi, v_hi, kIdescO, 1u);
+                }
+                commit_elected(smem_u32(&o_done[buf]));
+                commit_elected(smem_u32(&v_free[b]));
+                if (!pc.both) commit_elected(smem_u32(&v_free[b]));
+                if (last) commit_elected(smem_u32(&o_last[st]));
+                ++pc.job;
+                if (++pc.k == pc.jobs) {
+                    ++pc.un;
+                    p_more = settle(pc);
+                    for (; freed < pc.un; ++freed) unit_read(freed);
+                }
+                if (s_more) failed = !issue_s();
             }
-            base += (uint32_t)n.steps;
-            unit_no += n.steps > 0;
-            if (!unit_end()) break;
+            for (; freed < pc.un; ++freed) unit_read(freed);
+            // every MMA issued completes before TMEM is freed, also when cut short
+            commit_elected(smem_u32(drained));
+            const unsigned long long t0 = globaltimer_ns();
+            while (!mbar_try_wait(smem_u32(drained), 0))
+                if (globaltimer_ns() - t0 > kWaitLimitNs) {
+                    *abort_flag = 1;
+                    if (a.status) atomicExch(a.status, (int)MODEL_ERR_DEVICE);
+                    break;
+                }
+        } else if (warp == kUnitWarp) {
+            // ---------------------------------------------------------- tiles
+            uint32_t un = 0;
+            int fills = 0, jobs = 0, halves = 0;
+            for (long long x = g0; x < g1; unit_next(a, here)) {
+                const long long from = max(x, here.jobs), to = min(here.end, g1);
+                x = here.end;
+                if (from >= to) {                       // only places before its jobs are in the stretch
+                    if (x >= g1) break;
+                    continue;
+                }
+                if (un >= kUnitRing && !wait_all(&unit_free[un % kUnitRing], (un / kUnitRing - 1) & 1u)) break;
+                if (lane == 0) {
+                    volatile Unit& n = units[un % kUnitRing];
+                    const int n_rows = tile_n_rows(here.q, here.tile), both = n_rows > kHalfRows;
+                    // a step belongs to the CTA that has its first job
+                    const int step0 = (int)((from - here.jobs + both) >> both), step1 = (int)((to - here.jobs + both) >> both);
+                    n.steps = step1 - step0;
+                    n.both = both;
+                    n.g = here.g;
+                    n.token0 = here.q.row0;
+                    n.row0 = here.tile * kTileRows;
+                    n.n_rows = n_rows;
+                    n.key0 = step0 * kTileKeys;
+                    n.key1 = min(step1 * kTileKeys, tile_keys(a, here.q, here.tile));
+                    n.first_last = here.q.ctx + here.tile * kTileRows / a.group;
+                    n.ctx = here.q.ctx;
+                    n.part = here.jobs < g0 ? 0 : here.end > g1 ? 1 : -1;
+                    n.fill0 = fills;
+                    n.job0 = jobs;
+                    n.half0 = halves;
+                    n.s = here.s;
+                    n.odd = 0;
+                    fills += step1 - step0;
+                    jobs += (step1 - step0) << both;
+                    if (step1 > step0) halves += 1 + both;
+                    mbar_arrive(smem_u32(&unit_full[un % kUnitRing]));
+                }
+                __syncwarp();
+                ++un;
+                if (x >= g1) break;
+            }
+            if (un < kUnitRing || wait_all(&unit_free[un % kUnitRing], (un / kUnitRing - 1) & 1u)) {
+                if (lane == 0) {
+                    units[un % kUnitRing].steps = -1;
+                    mbar_arrive(smem_u32(&unit_full[un % kUnitRing]));
+                }
+            }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;");
     __syncthreads();
-    if (warp == kSoftmaxWarps + kLoadWarps) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.fence::after_thread_sync;");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
     }
@@ -760,9 +1017,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
 
 }  // namespace
 
-cudaError_t launch_paged_attn_tc(const PagedAttnArgs& a, bool bf16, int sms, cudaStream_t st) {
+cudaError_t launch_paged_attn_tc(const PagedAttnArgs& a, bool bf16, cudaStream_t st) {
     auto* kernel = bf16 ? paged_tc_kernel<true> : paged_tc_kernel<false>;
-    const size_t smem = 1024 + kOffSched + 2 * (size_t)(a.n_seq + 1) * sizeof(int);
+    const size_t smem = 1024 + kSmemBytes;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     // the register split waits for registers that a smaller launch would not have
@@ -773,7 +1030,7 @@ cudaError_t launch_paged_attn_tc(const PagedAttnArgs& a, bool bf16, int sms, cud
         if (f.numRegs != kRegsLaunch) return cudaErrorInvalidConfiguration;
         checked[bf16] = 1;
     }
-    kernel<<<(unsigned)sms, kThreads, smem, st>>>(a);
+    kernel<<<(unsigned)a.ctas, kThreads, smem, st>>>(a);
     return cudaGetLastError();
 }
 

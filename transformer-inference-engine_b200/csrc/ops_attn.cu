@@ -145,10 +145,10 @@ __global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_rows_kerne
     __shared__ __align__(16) FewSmem sm;
     const int t = threadIdx.x;
     Schedule sch;
-    build_schedule<kFewThreads>(a, 0, s_sched, &scratch, t, &sch);
+    build_schedule<kFewThreads>(a, s_sched, &scratch, t, &sch);
     const int units = sch.unit[a.n_seq];
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
-        const int s = owner_of(sch.unit, a.n_seq, u);
+        const int s = owner_of<int>(sch.unit, a.n_seq, u);
         const SeqShape q = seq_shape(a, s);
         const int sp = splits_of(q, sch.chunk), in = u - sch.unit[s];
         const int g = in % a.n_kv_head, split = in / a.n_kv_head % sp, tile = in / a.n_kv_head / sp;
@@ -189,61 +189,84 @@ __global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_rows_kerne
 }
 
 // ------------------------------------------------------------------ the join --
-// Split sequences: a warp per (row, head) adds its splits in order, lane l dims
-// 2 l and 2 l + 1.
-constexpr int kJoinThreads = 256;
+// A warp per (row, head) of what was cut adds its parts in order, lane l dims
+// 2 l and 2 l + 1. Part k's row lies at row_at(k) of the kind's partials.
+constexpr int kJoinThreads = 256, kJoinRows = 32;
+
+template <typename RowAt>
+__device__ __forceinline__ void join_row(const PagedAttnArgs& a, int kind, int parts, const RowAt& row_at, int lane,
+                                         float* out) {
+    float mx = -INFINITY;
+    for (int k = lane; k < parts; k += 32) mx = fmaxf(mx, a.part_ml[kind][2 * row_at(k)]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, o));
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float l = 0.f, ox = 0.f, oy = 0.f;
+    for (int k = 0; k < parts; ++k) {
+        const size_t at = row_at(k);
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml[kind] + 2 * at);
+        const float f = ex2_ftz(ml.x - base);
+        const float2 v = *reinterpret_cast<const float2*>(a.part_o[kind] + at * kHeadDim + 2 * lane);
+        l = fmaf(ml.y, f, l);
+        if (f > 0.f) { ox = fmaf(v.x, f, ox); oy = fmaf(v.y, f, oy); }
+    }
+    *reinterpret_cast<float2*>(out + 2 * lane) = l == 0.f ? make_float2(0.f, 0.f) : make_float2(ox / l, oy / l);
+}
 
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(PagedAttnArgs a) {
-    extern __shared__ int s_sched[];
+    extern __shared__ long long s_line[];
     __shared__ ScheduleScratch<kJoinThreads> scratch;
-    const int t = threadIdx.x, lane = t & 31;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     pdl_wait();
-    for (int kind = 0; kind < (a.only_few ? 1 : 2); ++kind) {
+    auto out_of = [&](const SeqShape& q, int g, int i) {
+        return a.out + (size_t)(q.row0 + i / a.group) * a.ldo + (g * a.group + i % a.group) * kHeadDim;
+    };
+    if (a.group <= kFewRows) {
+        // streaming units: a sequence's split units come in groups of `splits`
+        // per (tile, head); an item is one row of one group
         Schedule sch;
-        build_schedule<kJoinThreads>(a, kind, s_sched, &scratch, t, &sch);
-        const int tr = tile_rows_of(kind);
-        // units that left partials come in groups of `splits` per (tile, head);
-        // an item is one row of one group
-        const long long items = (long long)sch.part[a.n_seq] * tr;
-        for (long long x = (long long)blockIdx.x * (kJoinThreads / 32) + (t >> 5); x < items;
+        build_schedule<kJoinThreads>(a, reinterpret_cast<int*>(s_line), &scratch, t, &sch);
+        const long long items = (long long)sch.part[a.n_seq] * kFewRows;
+        for (long long x = (long long)blockIdx.x * (kJoinThreads / 32) + warp; x < items;
              x += (long long)gridDim.x * (kJoinThreads / 32)) {
-            const int pu = (int)(x / tr), r = (int)(x % tr);
-            const int s = owner_of(sch.part, a.n_seq, pu);
+            const int pu = (int)(x / kFewRows), r = (int)(x % kFewRows);
+            const int s = owner_of<int>(sch.part, a.n_seq, pu);
             const SeqShape q = seq_shape(a, s);
             const int sp = splits_of(q, sch.chunk), in = pu - sch.part[s];
             const int g = in % a.n_kv_head, split = in / a.n_kv_head % sp, tile = in / a.n_kv_head / sp;
-            const int i = tile * tr + r;
+            const int i = tile * kFewRows + r;
             if (split || i >= q.rows) continue;
-            float mx = -INFINITY;
-            for (int k = lane; k < sp; k += 32)
-                mx = fmaxf(mx, a.part_ml[kind][2 * ((size_t)(pu + k * a.n_kv_head) * tr + r)]);
-#pragma unroll
-            for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, o));
-            const float base = mx == -INFINITY ? 0.f : mx;
-            float l = 0.f, ox = 0.f, oy = 0.f;
-            for (int k = 0; k < sp; ++k) {
-                const size_t at = (size_t)(pu + k * a.n_kv_head) * tr + r;
-                const float2 ml = *reinterpret_cast<const float2*>(a.part_ml[kind] + 2 * at);
-                const float f = ex2_ftz(ml.x - base);
-                const float2 v = *reinterpret_cast<const float2*>(a.part_o[kind] + at * kHeadDim + 2 * lane);
-                l = fmaf(ml.y, f, l);
-                if (f > 0.f) { ox = fmaf(v.x, f, ox); oy = fmaf(v.y, f, oy); }
-            }
-            *reinterpret_cast<float2*>(a.out + (size_t)(q.row0 + i / a.group) * a.ldo +
-                                       (g * a.group + i % a.group) * kHeadDim + 2 * lane) =
-                l == 0.f ? make_float2(0.f, 0.f) : make_float2(ox / l, oy / l);
+            join_row(a, 0, sp, [&](int k) { return (size_t)(pu + k * a.n_kv_head) * kFewRows + r; }, lane, out_of(q, g, i));
         }
         __syncthreads();
     }
+    if (a.only_few) return;
+    // tensor-core tiles: the one that CTA c began and did not finish lies in c's
+    // second part and the first parts of the CTAs after it
+    JobLine line;
+    build_line<kJoinThreads>(a, s_line, &scratch, t, &line);
+    const long long total = line.base[a.n_seq];
+    for (int x = blockIdx.x; x < a.ctas * (kTileRows / kJoinRows); x += gridDim.x) {
+        const int c = x / (kTileRows / kJoinRows), r0 = x % (kTileRows / kJoinRows) * kJoinRows;
+        const long long g0 = c * line.share, g1 = g0 + line.share;
+        if (g1 >= total) break;
+        const LineUnit u = unit_at(a, line, g1 - 1);
+        if (u.jobs < g0 || u.jobs >= g1 || u.end <= g1) continue;
+        const int parts = (int)((u.end - 1) / line.share) - c + 1, n_rows = tile_n_rows(u.q, u.tile);
+        for (int r = r0 + warp; r < min(r0 + kJoinRows, n_rows); r += kJoinThreads / 32)
+            join_row(a, 1, parts, [&](int k) { return ((size_t)2 * (c + k) + (k == 0)) * kTileRows + r; }, lane,
+                     out_of(u.q, u.g, u.tile * kTileRows + r));
+    }
 }
 
-// Units aimed at when sequences are split: four per SM of the streaming kernel
-// (two resident CTAs), two of the tensor-core kernel (one resident).
-int target_of(int kind, int sms) { return (kind ? 2 : 4) * sms; }
+// Streaming units aimed at when sequences are split: four per SM (two CTAs
+// resident). A split sequence has more pages than a chunk, so its units number
+// at most twice its pages over the chunk: all partials fit 2 x target units.
+int target_of(int sms) { return 4 * sms; }
 
-// A split sequence has more steps than a chunk, so its units number at most
-// twice its steps over the chunk: all partials fit 2 x target units.
-size_t part_rows(int kind, int sms) { return 2 * (size_t)target_of(kind, sms) * tile_rows_of(kind); }
+size_t part_rows(int kind, int sms) {
+    return kind ? 2 * (size_t)sms * kTileRows : 2 * (size_t)target_of(sms) * kFewRows;
+}
 size_t scratch_bytes(int sms) { return (part_rows(0, sms) + part_rows(1, sms)) * (kHeadDim + 2) * sizeof(float); }
 
 }  // namespace
@@ -271,7 +294,7 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
     if (ldq < w || ldo < w || (ldq & 3) || (ldo & 3)) return MODEL_ERR_ARG;
     if (!aligned16(q) || !aligned(k_pages, 32) || !aligned(v_pages, 32) || !aligned16(out) || !aligned16(workspace))
         return MODEL_ERR_ARG;
-    if (n_seq > kOpsMaxSeqs || pages_per_seq > kOpsMaxPages - 1) return MODEL_ERR_CAPACITY;
+    if (n_seq > kOpsMaxSeqs || pages_per_seq > kOpsMaxPages / 2) return MODEL_ERR_CAPACITY;
     // units are counted in int32: at most one per row and head, and one per
     // sequence and K/V head, before any split
     if ((long long)rows * n_head + (long long)n_seq * n_kv_head > INT_MAX / 2) return MODEL_ERR_CAPACITY;
@@ -291,7 +314,6 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
     a.out = out; a.ldo = ldo;
     float* f = static_cast<float*>(workspace);
     for (int kind = 0; kind < 2; ++kind) {
-        a.target[kind] = target_of(kind, sms);
         a.part_o[kind] = f;
         f += part_rows(kind, sms) * kHeadDim;
     }
@@ -299,13 +321,15 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
         a.part_ml[kind] = f;
         f += part_rows(kind, sms) * 2;
     }
+    a.target = target_of(sms);
+    a.ctas = sms;
     a.status = status;
     const bool bf16 = kv_format == TIE_KV_BF16;
     const long long most = (long long)max_new * a.group;      // rows of one sequence and K/V head
     a.only_few = most <= kFewRows;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const size_t smem = 2 * (size_t)(n_seq + 1) * sizeof(int);
-    if (!a.only_few) TIE_OP_CU(launch_paged_attn_tc(a, bf16, sms, st));
+    const size_t smem = (size_t)(n_seq + 1) * sizeof(long long);
+    if (!a.only_few) TIE_OP_CU(launch_paged_attn_tc(a, bf16, st));
     if (a.group <= kFewRows) {
         const int rmax = most <= 1 ? 1 : most <= 2 ? 2 : most <= 4 ? 4 : kFewRows;
         void (*kernel)(PagedAttnArgs) = nullptr;

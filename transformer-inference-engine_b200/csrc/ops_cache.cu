@@ -339,7 +339,7 @@ extern "C" model_status tie_page_plan(const int32_t* ctx_lens, const int32_t* ne
         return MODEL_ERR_ARG;
     if (n_seq <= 0 || pages_per_seq <= 0 || n_pages <= 0 || max_rows <= 0) return MODEL_ERR_ARG;
     if (free_pages ? (!n_free || !n_free_out || max_free < 0) : (n_free || n_free_out)) return MODEL_ERR_ARG;
-    if (n_seq > kOpsMaxSeqs || n_pages > kOpsMaxPages || pages_per_seq > kOpsMaxPages - 1) return MODEL_ERR_CAPACITY;
+    if (n_seq > kOpsMaxSeqs || n_pages > kOpsMaxPages || pages_per_seq > kOpsMaxPages / 2) return MODEL_ERR_CAPACITY;
     OnDeviceOf dev(row_start);
     if (dev.status() != MODEL_OK) return dev.status();
     PlanArgs a{ctx_lens, new_lens, n_seq, page_table, pages_per_seq, n_pages, free_pages, max_free, n_free, n_free_out,
@@ -389,7 +389,7 @@ extern "C" model_status tie_kv_reorder(void* k_pages, void* v_pages, int kv_form
     if (!k_pages || !v_pages || !page_table || !parent || !first || !length) return MODEL_ERR_ARG;
     if (!pool_shape_ok(kv_format, n_pages, n_kv_head) || n_layer <= 0 || pages_per_seq <= 0 || n_req <= 0 || beams <= 0)
         return MODEL_ERR_ARG;
-    if (beams > kMaxBeams || n_req > kOpsMaxSeqs || pages_per_seq > kOpsMaxPages - 1) return MODEL_ERR_CAPACITY;
+    if (beams > kMaxBeams || n_req > kOpsMaxSeqs || pages_per_seq > kOpsMaxPages / 2) return MODEL_ERR_CAPACITY;
     const size_t size = kv_format == TIE_KV_BF16 ? 2 : 4;
     const size_t row = (size_t)n_kv_head * kHeadDim;
     if (!aligned16(k_pages) || !aligned16(v_pages) || (layer_stride * size) % 16) return MODEL_ERR_ARG;

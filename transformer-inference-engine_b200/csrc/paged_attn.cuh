@@ -5,12 +5,18 @@
 // Row (i, h) of sequence s is its new token i and query head h, at position
 // ctx_s + i. The heads of one K/V head and a sequence's tokens together form
 // the rows that share keys: row index i * group + (h mod group). They are cut
-// into tiles, a tile's keys into splits; a unit is (sequence, tile, split, K/V
+// into tiles. Sequences of few rows (at most kFewRows) go to the streaming
+// kernel, the others to the tensor-core kernel; each kernel derives its
+// schedule from the lengths for itself (a scan of the lengths costs less than
+// a launch that would leave it in memory).
+//   Streaming (kind 0): a unit is (sequence, tile, split of the keys, K/V
 // head), the head fastest, so CTAs that run together read one page's
-// neighbouring rows. Sequences of few rows (at most kFewRows) are units of the
-// streaming kernel, the others of the tensor-core kernel; both kinds are
-// scheduled from the same arrays, by each kernel for itself (a scan of the
-// lengths costs less than a launch that would leave it in memory).
+// neighbouring rows.
+//   Tensor cores (kind 1): a tile's steps over the keys count as jobs (two a
+// step when the tile has more than 128 rows). All tiles of the batch stand in
+// one line -- by sequence, tile, K/V head -- each with its jobs behind a few
+// places that stand for what a tile costs besides; every CTA takes an equal
+// stretch of the line. A tile that a stretch cuts leaves partial results.
 #pragma once
 
 #include "ops.h"
@@ -18,7 +24,8 @@
 namespace tie {
 
 constexpr int kFewRows = 8;        // rows of a streaming unit
-constexpr int kTileRows = 128;     // rows of a tensor-core unit
+constexpr int kHalfRows = 128;     // rows of one MMA of the tensor-core kernel
+constexpr int kTileRows = 256;     // rows of its tiles
 constexpr int kTileKeys = 128;     // keys of one of its steps
 
 struct PagedAttnArgs {
@@ -33,23 +40,24 @@ struct PagedAttnArgs {
     float scale2;                  // score scale * log2(e): the softmax runs in powers of two
     float* out;
     int ldo;
-    // partials of split units, per kind (0 streaming, 1 tensor core)
+    // partials, per kind: of split units (streaming), two per CTA (tensor cores)
     float* part_o[2];              // [unit][tile rows][64], unnormalised
     float* part_ml[2];             // [unit][tile rows][2]: maximum (power-of-two domain), sum
-    int target[2];                 // units wanted of each kind when the work is split
+    int target;                    // streaming units wanted when the work is split
+    int ctas;                      // CTAs of the tensor-core kernel
     int only_few;                  // every sequence is of the streaming kind
     int* status;
 };
 
 __host__ __device__ inline int tile_rows_of(int kind) { return kind ? kTileRows : kFewRows; }
-__host__ __device__ inline int step_keys_of(int kind) { return kind ? kTileKeys : kPageRows; }
-// fewest steps (of step_keys_of keys) worth a unit of their own
-__host__ __device__ inline int min_steps_of(int kind) { return kind ? 2 : 8; }
+// fewest pages worth a streaming unit of their own (one for each warp), fewest
+// jobs worth a tensor-core CTA
+constexpr int kMinUnitPages = 8, kMinJobs = 2;
 
 // One sequence as the schedule sees it; rows == 0 for one to leave alone
 // (no new tokens, or lengths outside the caller's bounds).
 struct SeqShape {
-    int row0, ctx, tokens, rows, kind, tiles, steps;
+    int row0, ctx, tokens, rows, kind, tiles;
 };
 
 __device__ __forceinline__ SeqShape seq_shape(const PagedAttnArgs& a, int s) {
@@ -63,17 +71,8 @@ __device__ __forceinline__ SeqShape seq_shape(const PagedAttnArgs& a, int s) {
     q.rows = q.tokens * a.group;
     q.kind = !a.only_few && q.rows > kFewRows;
     q.tiles = (q.rows + tile_rows_of(q.kind) - 1) / tile_rows_of(q.kind);
-    q.steps = (c + q.tokens + step_keys_of(q.kind) - 1) / step_keys_of(q.kind);
     return q;
 }
-
-// The schedule of one kind in shared memory: prefix sums over the sequences of
-// the units, and of the units that leave partials.
-struct Schedule {
-    int* unit;                     // [n_seq + 1]
-    int* part;                     // [n_seq + 1]
-    int chunk;                     // steps per split
-};
 
 template <int THREADS>
 struct ScheduleScratch {
@@ -81,62 +80,77 @@ struct ScheduleScratch {
     int a[THREADS / 32], b[THREADS / 32];
 };
 
-// Splits of a sequence at `chunk` steps per split.
-__device__ __forceinline__ int splits_of(const SeqShape& q, int chunk) { return (q.steps + chunk - 1) / chunk; }
-
-// Builds the schedule of `kind` with all THREADS threads of the CTA (thread t
-// of them); ends with a barrier.
+// Sum over the CTA's threads of `v`, and in *before the sum over lower threads.
 template <int THREADS>
-__device__ __forceinline__ void build_schedule(const PagedAttnArgs& a, int kind, int* smem, ScheduleScratch<THREADS>* sc,
-                                               int t, Schedule* out) {
-    constexpr unsigned kAllLanes = 0xffffffffu;
+__device__ __forceinline__ long long scan_threads(long long v, ScheduleScratch<THREADS>* sc, int t, long long* before) {
     const int lane = t & 31, warp = t >> 5;
+    long long in = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, in, o);
+        if (lane >= o) in += u;
+    }
+    __syncthreads();
+    if (lane == 31) sc->total[warp] = in;
+    __syncthreads();
+    long long all = 0, low = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) low += sc->total[w];
+        all += sc->total[w];
+    }
+    *before = low + in - v;
+    return all;
+}
+
+// ----------------------------------------------------------- streaming units --
+// Prefix sums over the sequences of the units, and of the units that leave
+// partials, in shared memory.
+struct Schedule {
+    int* unit;                     // [n_seq + 1]
+    int* part;                     // [n_seq + 1]
+    int chunk;                     // pages per split
+};
+
+__device__ __forceinline__ int pages_of(const SeqShape& q) { return (q.ctx + q.tokens + kPageRows - 1) / kPageRows; }
+__device__ __forceinline__ int splits_of(const SeqShape& q, int chunk) { return (pages_of(q) + chunk - 1) / chunk; }
+
+// Built with all THREADS threads of the CTA (thread t of them); ends with a
+// barrier.
+template <int THREADS>
+__device__ __forceinline__ void build_schedule(const PagedAttnArgs& a, int* smem, ScheduleScratch<THREADS>* sc, int t,
+                                               Schedule* out) {
     const int per = (a.n_seq + THREADS - 1) / THREADS;
     out->unit = smem;
     out->part = smem + a.n_seq + 1;
-    long long work = 0;
+    long long work = 0, before;
     for (int k = 0; k < per; ++k) {
         const int s = t * per + k;
         if (s >= a.n_seq) break;
         const SeqShape q = seq_shape(a, s);
-        if (q.rows && q.kind == kind) work += (long long)a.n_kv_head * q.tiles * q.steps;
+        if (q.rows && !q.kind) work += (long long)a.n_kv_head * q.tiles * pages_of(q);
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) work += __shfl_xor_sync(kAllLanes, work, o);
-    if (lane == 0) sc->total[warp] = work;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) total += sc->total[w];
-    const long long even = (total + a.target[kind] - 1) / a.target[kind];
-    out->chunk = (int)(even > min_steps_of(kind) ? even : min_steps_of(kind));
-    int units = 0, parts = 0;
+    const long long even = (scan_threads<THREADS>(work, sc, t, &before) + a.target - 1) / a.target;
+    out->chunk = (int)(even > kMinUnitPages ? even : kMinUnitPages);
+    long long units = 0;           // units in the low half, units with partials in the high half
     for (int k = 0; k < per; ++k) {
         const int s = t * per + k;
         if (s >= a.n_seq) break;
         const SeqShape q = seq_shape(a, s);
-        if (!q.rows || q.kind != kind) continue;
-        const int sp = splits_of(q, out->chunk), n = a.n_kv_head * q.tiles * sp;
-        units += n;
-        if (sp > 1) parts += n;
+        if (!q.rows || q.kind) continue;
+        const int sp = splits_of(q, out->chunk);
+        const long long n = (long long)a.n_kv_head * q.tiles * sp;
+        units += n + (sp > 1 ? n << 32 : 0);
     }
-    int iu = units, ip = parts;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(kAllLanes, iu, o), p = __shfl_up_sync(kAllLanes, ip, o);
-        if (lane >= o) { iu += u; ip += p; }
-    }
-    if (lane == 31) { sc->a[warp] = iu; sc->b[warp] = ip; }
-    __syncthreads();
-    int bu = iu - units, bp = ip - parts;
-    for (int w = 0; w < warp; ++w) { bu += sc->a[w]; bp += sc->b[w]; }
+    scan_threads<THREADS>(units, sc, t, &before);
+    int bu = (int)before, bp = (int)(before >> 32);
     for (int k = 0; k < per; ++k) {
         const int s = t * per + k;
         if (s >= a.n_seq) break;
         out->unit[s] = bu;
         out->part[s] = bp;
         const SeqShape q = seq_shape(a, s);
-        if (q.rows && q.kind == kind) {
+        if (q.rows && !q.kind) {
             const int sp = splits_of(q, out->chunk), n = a.n_kv_head * q.tiles * sp;
             bu += n;
             if (sp > 1) bp += n;
@@ -146,8 +160,73 @@ __device__ __forceinline__ void build_schedule(const PagedAttnArgs& a, int kind,
     __syncthreads();
 }
 
+// ----------------------------------------------------------- tensor-core jobs --
+// The line: base[s] places before sequence s, all of them in base[n_seq]; CTA c
+// has places [c * share, (c + 1) * share).
+struct JobLine {
+    long long* base;               // [n_seq + 1], shared memory
+    long long share;
+};
+
+// places before a tile's jobs: loading Q, and the results' way out
+constexpr int kTilePlaces = 2;
+
+__device__ __forceinline__ int tile_n_rows(const SeqShape& q, int tile) { return min(kTileRows, q.rows - tile * kTileRows); }
+// keys that a tile's rows see, and its steps over them
+__device__ __forceinline__ int tile_keys(const PagedAttnArgs& a, const SeqShape& q, int tile) {
+    return q.ctx + (tile * kTileRows + tile_n_rows(q, tile) - 1) / a.group + 1;
+}
+__device__ __forceinline__ int tile_steps(const PagedAttnArgs& a, const SeqShape& q, int tile) {
+    return (tile_keys(a, q, tile) + kTileKeys - 1) / kTileKeys;
+}
+// places of a tile for one K/V head
+__device__ __forceinline__ int tile_places(const PagedAttnArgs& a, const SeqShape& q, int tile) {
+    return (tile_steps(a, q, tile) << (tile_n_rows(q, tile) > kHalfRows)) + kTilePlaces;
+}
+__device__ __forceinline__ long long seq_places(const PagedAttnArgs& a, const SeqShape& q) {
+    long long n = 0;
+    for (int tile = 0; tile < q.tiles; ++tile) n += tile_places(a, q, tile);
+    return n * a.n_kv_head;
+}
+
+template <int THREADS>
+__device__ __forceinline__ void build_line(const PagedAttnArgs& a, long long* smem, ScheduleScratch<THREADS>* sc, int t,
+                                           JobLine* out) {
+    const int per = (a.n_seq + THREADS - 1) / THREADS;
+    out->base = smem;
+    long long mine = 0, before;
+    for (int k = 0; k < per; ++k) {
+        const int s = t * per + k;
+        if (s >= a.n_seq) break;
+        const SeqShape q = seq_shape(a, s);
+        if (q.rows && q.kind) mine += seq_places(a, q);
+    }
+    const long long total = scan_threads<THREADS>(mine, sc, t, &before);
+    for (int k = 0; k < per; ++k) {
+        const int s = t * per + k;
+        if (s >= a.n_seq) break;
+        out->base[s] = before;
+        if (per > 1) {             // a thread's only sequence needs no second look
+            const SeqShape q = seq_shape(a, s);
+            if (q.rows && q.kind) before += seq_places(a, q);
+        }
+    }
+    if (t == 0) out->base[a.n_seq] = total;
+    const long long even = (total + a.ctas - 1) / a.ctas;
+    out->share = even > kTilePlaces + kMinJobs ? even : kTilePlaces + kMinJobs;
+    __syncthreads();
+}
+
+// A tile and K/V head in the line: places [first, end), its jobs from `jobs` on.
+struct LineUnit {
+    SeqShape q;
+    int s, tile, g;
+    long long first, jobs, end;
+};
+
 // The last s < n with base[s] <= x.
-__device__ __forceinline__ int owner_of(const int* base, int n, int x) {
+template <typename T>
+__device__ __forceinline__ int owner_of(const T* base, int n, T x) {
     int lo = 0, hi = n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -155,6 +234,47 @@ __device__ __forceinline__ int owner_of(const int* base, int n, int x) {
         else hi = mid;
     }
     return lo;
+}
+
+// The unit that holds place x (x < all places).
+__device__ __forceinline__ LineUnit unit_at(const PagedAttnArgs& a, const JobLine& line, long long x) {
+    LineUnit u;
+    u.s = owner_of<long long>(line.base, a.n_seq, x);
+    u.q = seq_shape(a, u.s);
+    long long at = line.base[u.s];
+    int each;
+    u.tile = 0;
+    for (;;) {
+        each = tile_places(a, u.q, u.tile);
+        const long long n = (long long)each * a.n_kv_head;
+        if (x < at + n || u.tile == u.q.tiles - 1) break;
+        at += n;
+        ++u.tile;
+    }
+    u.g = (int)((x - at) / each);
+    u.first = at + (long long)u.g * each;
+    u.jobs = u.first + kTilePlaces;
+    u.end = u.first + each;
+    return u;
+}
+
+// The unit after u: the next K/V head, tile, or sequence with rows of this kind
+// (the caller knows that there is one).
+__device__ __forceinline__ void unit_next(const PagedAttnArgs& a, LineUnit& u) {
+    if (++u.g == a.n_kv_head) {
+        u.g = 0;
+        if (++u.tile == u.q.tiles) {
+            u.tile = 0;
+            while (++u.s < a.n_seq - 1) {
+                u.q = seq_shape(a, u.s);
+                if (u.q.rows && u.q.kind) break;
+            }
+            if (u.s == a.n_seq - 1) u.q = seq_shape(a, u.s);
+        }
+    }
+    u.first = u.end;
+    u.jobs = u.first + kTilePlaces;
+    u.end = u.first + tile_places(a, u.q, u.tile);
 }
 
 // 2^x on the special-function unit (ex2.approx.ftz: relative error about
@@ -166,6 +286,6 @@ __device__ __forceinline__ float ex2_ftz(float x) {
 }
 
 // Tensor-core kernel (k_paged_tc.cu) for the sequences of kind 1.
-cudaError_t launch_paged_attn_tc(const PagedAttnArgs& a, bool bf16, int sms, cudaStream_t st);
+cudaError_t launch_paged_attn_tc(const PagedAttnArgs& a, bool bf16, cudaStream_t st);
 
 }  // namespace tie
