@@ -126,6 +126,10 @@ def test_binding_checks_shapes_and_types():
         ops.kv_reorder(pages, pages.clone(), torch.zeros(3, 2, dtype=torch.int32), ints, ints, ints, 2)
     with pytest.raises(ValueError):
         ops.page_plan(ints, ints, table, 4, ints[:2], ints, ints, ints, ints)
+    with pytest.raises(ValueError):                                            # all well but for the device
+        ops.kv_store(rows, rows, ints, pages, pages.clone())
+    with pytest.raises(ValueError):
+        ops.page_plan(ints, ints, table, 4, ints, ints, ints, ints, ints)
 
 
 def test_host_memory_is_refused():

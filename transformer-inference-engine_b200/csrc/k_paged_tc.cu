@@ -1020,15 +1020,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
 cudaError_t launch_paged_attn_tc(const PagedAttnArgs& a, bool bf16, cudaStream_t st) {
     auto* kernel = bf16 ? paged_tc_kernel<true> : paged_tc_kernel<false>;
     const size_t smem = 1024 + kSmemBytes;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // once per device and format: the shared memory, and that the register split
+    // finds the registers it will wait for
+    static std::atomic<bool> ready[64][2];
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return e;
-    // the register split waits for registers that a smaller launch would not have
-    static std::atomic<int> checked[2] = {{0}, {0}};
-    if (!checked[bf16]) {
+    if (device >= 64 || !ready[device][bf16]) {
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
         cudaFuncAttributes f;
         if ((e = cudaFuncGetAttributes(&f, kernel)) != cudaSuccess) return e;
         if (f.numRegs != kRegsLaunch) return cudaErrorInvalidConfiguration;
-        checked[bf16] = 1;
+        if (device < 64) ready[device][bf16] = true;
     }
     kernel<<<(unsigned)a.ctas, kThreads, smem, st>>>(a);
     return cudaGetLastError();

@@ -29,6 +29,7 @@ constexpr int kMaxBeams = 16;
 constexpr int kScanThreads = 256, kScanWarps = kScanThreads / 32;
 constexpr int kBatch = 8;              // elements per thread and pass
 constexpr int kPickThreads = 256, kPickWarps = kPickThreads / 32;
+constexpr int kMaxSlices = 32;         // a lane of the picking warps for each
 constexpr unsigned kAll = 0xffffffffu;
 
 // 2^x, x <= 0 here (ex2.approx.ftz: relative error about 2^-22)
@@ -92,12 +93,26 @@ beam_scan_kernel(const float* __restrict__ logits, int ldl, const int32_t* __res
             sum += (double)part;
         }
         if (__any_sync(kAll, worst_i == INT_MAX || top > worst)) {
+            // While the list is filling up, only elements that reach the k-th
+            // largest of the lanes' maxima can be among the k best: without this
+            // bound the first pass would insert one element after the other (8 us).
+            float bound = -INFINITY;
+            if (worst_i == INT_MAX) {
+                int above = 0;
+#pragma unroll 8
+                for (int j = 0; j < 32; ++j) {
+                    const float other = __shfl_sync(kAll, top, j);
+                    above += other > top || (other == top && j < lane);
+                }
+                const unsigned kth = __ballot_sync(kAll, above == k - 1);   // one lane, unless maxima are NaN
+                if (kth) bound = __shfl_sync(kAll, top, __ffs(kth) - 1);
+            }
 #pragma unroll 1
             for (int u = 0; u < kBatch; ++u) {
                 const int i = i0 + u * kScanThreads + t;
                 const float xv = fmaxf(u == 0 ? v[0] : u == 1 ? v[1] : u == 2 ? v[2] : u == 3 ? v[3]
                                        : u == 4 ? v[4] : u == 5 ? v[5] : u == 6 ? v[6] : v[7], -INFINITY);
-                unsigned todo = __ballot_sync(kAll, i < hi && better(xv, i, worst, worst_i));
+                unsigned todo = __ballot_sync(kAll, i < hi && xv >= bound && better(xv, i, worst, worst_i));
                 while (todo) {
                     const int src = __ffs(todo) - 1;
                     todo &= todo - 1;
@@ -154,129 +169,111 @@ __global__ void __launch_bounds__(kPickThreads)
 beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float* __restrict__ scores,
                  const int32_t* __restrict__ done, int32_t* __restrict__ next, int32_t* __restrict__ parent,
                  float* __restrict__ scores_out, int32_t* __restrict__ done_out) {
+    __shared__ double s_total[kMaxBeams * kMaxBeams];      // the beams' best, best first; NaN: none
+    __shared__ int s_token[kMaxBeams * kMaxBeams];
+    __shared__ double p_total[kMaxBeams];                  // the kept ones by rank
+    __shared__ int p_beam[kMaxBeams], p_token[kMaxBeams];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const size_t row0 = (size_t)blockIdx.x * k;
     pdl_wait();
-    extern __shared__ double s_total[];                    // [k * slices * k] candidates' totals
-    __shared__ double s_base[kMaxBeams];                   // score - logsumexp, or NaN
-    __shared__ float s_score[kMaxBeams];
-    __shared__ int s_done[kMaxBeams];
-    __shared__ double w_total[kPickWarps];
-    __shared__ long long w_flat[kPickWarps];
-    __shared__ int w_at[kPickWarps];
-    __shared__ double p_total[kMaxBeams];
-    __shared__ long long p_flat[kMaxBeams];
-    const int q = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const size_t row0 = (size_t)q * k;
-    if (t < k) {
-        s_done[t] = done ? done[row0 + t] != 0 : 0;
-        s_score[t] = scores[row0 + t];
-    }
-    __syncthreads();
+    // a warp per beam, a lane per slice
     for (int b = warp; b < k; b += kPickWarps) {
-        if (s_done[b]) continue;
-        const size_t at = (row0 + b) * slices;
-        float M = -INFINITY;
-        for (int s = lane; s < slices; s += 32) M = fmaxf(M, in.max[at + s]);
+        const float score = scores[row0 + b];
+        const bool finished = done && done[row0 + b] != 0;
+        const size_t at = (row0 + b) * slices + lane;
+        const bool mine = lane < slices && !finished;
+        const float m = mine ? in.max[at] : -INFINITY;
+        float M = m;
 #pragma unroll
         for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kAll, M, o));
-        double S = 0.0;
-        for (int s = lane; s < slices; s += 32)
-            if (in.max[at + s] > -INFINITY) S += in.sum[at + s] * exp((double)in.max[at + s] - (double)M);
+        double S = m > -INFINITY ? in.sum[at] * exp((double)m - (double)M) : 0.0;
 #pragma unroll
         for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(kAll, S, o);
-        // a row with no finite logit has no normaliser (NaN)
-        if (lane == 0) s_base[b] = M > -INFINITY && M < INFINITY ? (double)M + log(S) : (double)NAN;
-    }
-    __syncthreads();
-    const int per = slices * k, n = k * per;
-    auto token_of = [&](int c) {       // candidate c's token, INT_MAX for none
-        const int b = c / per, j = c % per;
-        if (s_done[b]) return j == 0 ? eos : INT_MAX;
-        const double base = (double)s_score[b] - s_base[b];
-        // a beam without a finite score: every candidate ties at -inf, the lowest tokens are its best
-        if (!(base > (double)-INFINITY)) return j < k && j < vocab ? j : INT_MAX;
-        return in.idx[(row0 + b) * per + j];
-    };
-    for (int c = t; c < n; c += kPickThreads) {
-        const int b = c / per;
-        double v = (double)-INFINITY;
-        if (s_done[b]) v = (double)s_score[b];
-        else if (c % per < per) {
-            const double base = (double)s_score[b] - s_base[b];
-            if (base > (double)-INFINITY)
-                v = (double)s_score[b] + ((double)in.val[(row0 + b) * per + c % per] - s_base[b]);
-        }
-        if (!(v > (double)-INFINITY)) v = (double)-INFINITY;       // NaN counts as -inf
-        s_total[c] = v;
-    }
-    __syncthreads();
-    // k rounds of the best remaining candidate
-    for (int round = 0; round < k; ++round) {
-        double bv = (double)-INFINITY;
-        long long bf = LLONG_MAX;
-        int bc = -1;
-        for (int c = t; c < n; c += kPickThreads) {
-            const double v = s_total[c];
-            if (!(v >= bv)) continue;                              // taken candidates are NaN
-            const int tok = token_of(c);
-            if (tok == INT_MAX) continue;
-            const long long f = (long long)(c / per) * vocab + tok;
-            if (v > bv || f < bf) { bv = v; bf = f; bc = c; }
-        }
+        // a row whose largest logit is infinite has no normaliser
+        const double lse = M > -INFINITY && M < INFINITY ? (double)M + log(S) : (double)NAN;
+        const bool scored = (double)score - lse > (double)-INFINITY;
+        // the beam's best: the lanes' sorted lists merged, best first
+        int head = 0;
+        float hv = -INFINITY;
+        int hi = INT_MAX;
+        if (mine) { hv = in.val[at * k]; hi = in.idx[at * k]; }
+        for (int r = 0; r < k; ++r) {
+            float v = hv;
+            int i = hi;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const double ov = __shfl_xor_sync(kAll, bv, o);
-            const long long of = __shfl_xor_sync(kAll, bf, o);
-            const int oc = __shfl_xor_sync(kAll, bc, o);
-            if (ov > bv || (ov == bv && of < bf)) { bv = ov; bf = of; bc = oc; }
-        }
-        if (lane == 0) { w_total[warp] = bv; w_flat[warp] = bf; w_at[warp] = bc; }
-        __syncthreads();
-        if (t == 0) {
-            for (int w = 1; w < kPickWarps; ++w)
-                if (w_total[w] > bv || (w_total[w] == bv && w_flat[w] < bf)) { bv = w_total[w]; bf = w_flat[w]; bc = w_at[w]; }
-            p_total[round] = bv;
-            p_flat[round] = bf;
-            if (bc >= 0) s_total[bc] = (double)NAN;
-        }
-        __syncthreads();
-    }
-    // a beam's best child stays in its place, the others take the free places in order
-    if (t == 0) {
-        unsigned taken = 0, heirs = 0;
-        for (int i = 0; i < k; ++i) {
-            const int b = (int)(p_flat[i] / vocab);
-            if (!(taken >> b & 1)) { taken |= 1u << b; heirs |= 1u << i; }
-        }
-        for (int i = 0; i < k; ++i) {
-            const int b = (int)(p_flat[i] / vocab), tok = (int)(p_flat[i] % vocab);
-            int place = b;
-            if (!(heirs >> i & 1)) {
-                place = __ffs((int)~taken) - 1;
-                taken |= 1u << place;
+            for (int o = 16; o; o >>= 1) {
+                const float ov = __shfl_xor_sync(kAll, v, o);
+                const int oi = __shfl_xor_sync(kAll, i, o);
+                if (better(ov, oi, v, i)) { v = ov; i = oi; }
             }
+            if (mine && hi == i && hi != INT_MAX) {
+                ++head;
+                hv = head < k ? in.val[at * k + head] : -INFINITY;
+                hi = head < k ? in.idx[at * k + head] : INT_MAX;
+            }
+            if (lane == 0) {
+                double total = (double)score + ((double)v - lse);
+                int token = i;
+                if (finished) {
+                    total = (double)score;
+                    token = r == 0 ? eos : INT_MAX;
+                } else if (!scored) {
+                    // every candidate ties at -inf, the lowest tokens are its best
+                    token = r < vocab ? r : INT_MAX;
+                }
+                if (!(total > (double)-INFINITY)) total = (double)-INFINITY;   // NaN counts as -inf
+                s_total[b * k + r] = token == INT_MAX ? (double)NAN : total;
+                s_token[b * k + r] = token;
+            }
+        }
+    }
+    __syncthreads();
+    // each candidate finds its rank among all
+    for (int c = t; c < k * k; c += kPickThreads) {
+        const double v = s_total[c];
+        if (v != v) continue;
+        const int b = c / k;
+        const long long flat = (long long)b * vocab + s_token[c];
+        int rank = 0;
+        for (int o = 0; o < k * k; ++o) {
+            const double ov = s_total[o];
+            if (ov > v || (ov == v && (long long)(o / k) * vocab + s_token[o] < flat)) ++rank;
+        }
+        if (rank < k) {
+            p_total[rank] = v;
+            p_beam[rank] = b;
+            p_token[rank] = s_token[c];
+        }
+    }
+    __syncthreads();
+    // a beam's best child stays in its place, the others take the free places in order
+    if (warp == 0) {
+        const int b = lane < k ? p_beam[lane] : kMaxBeams + lane;
+        const bool heir = __ffs((int)__match_any_sync(kAll, b)) - 1 == lane;
+        const unsigned taken = __reduce_or_sync(kAll, lane < k ? 1u << b : 0u);
+        const unsigned others = __ballot_sync(kAll, lane < k && !heir);
+        if (lane < k) {
+            const int place = heir ? b : (int)__fns(~taken, 0, __popc(others & ((1u << lane) - 1)) + 1);
+            const int tok = p_token[lane];
+            const bool was = done && done[row0 + b] != 0;
+            __syncwarp(__activemask());
             next[row0 + place] = tok;
             parent[row0 + place] = (int)row0 + b;
-            scores_out[row0 + place] = (float)p_total[i];
-            if (done_out) done_out[row0 + place] = s_done[b] || tok == eos;
+            scores_out[row0 + place] = (float)p_total[lane];
+            if (done_out) done_out[row0 + place] = was || tok == eos;
         }
     }
 }
 
 // Slices of the vocabulary per row: about four CTAs per SM in all, each of at
-// least one pass of its threads (2048 logits).
-int slices_for(long long rows, int vocab, int sms) {
+// least one pass of its threads (2048 logits), at most a lane each of the warp
+// that joins them.
+int slices_of(int n_req, int beams, int vocab, int sms) {
+    const long long rows = (long long)n_req * beams;
     const int most = (vocab + kScanThreads * kBatch - 1) / (kScanThreads * kBatch);
     const long long want = (4LL * sms + rows - 1) / rows;
-    return (int)(want < 1 ? 1 : want > most ? most : want);
-}
-
-// candidates one pick holds in shared memory
-constexpr int kMaxCandidates = 5120;
-
-int slices_of(int n_req, int beams, int vocab, int sms) {
-    const int s = slices_for((long long)n_req * beams, vocab, sms);
-    const int cap = kMaxCandidates / (beams * beams);
-    return s < cap ? s : cap;
+    const long long n = want < 1 ? 1 : want > most ? most : want;
+    return (int)(n < kMaxSlices ? n : kMaxSlices);
 }
 
 size_t scratch_bytes(int n_req, int beams, int slices) {
@@ -323,8 +320,7 @@ extern "C" model_status tie_beam_select(const float* logits, int ldl, const floa
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     beam_scan_kernel<<<(unsigned)at, kScanThreads, 0, st>>>(logits, ldl, done, vocab, slices, len, beams, p);
     TIE_OP_CU(cudaGetLastError());
-    TIE_OP_CU(launch_pdl(beam_pick_kernel, dim3((unsigned)n_req), dim3(kPickThreads),
-                         (size_t)slices * beams * beams * sizeof(double), st, p, slices, beams, vocab, eos_id, scores,
+    TIE_OP_CU(launch_pdl(beam_pick_kernel, dim3((unsigned)n_req), dim3(kPickThreads), 0, st, p, slices, beams, vocab, eos_id, scores,
                          done, next, parent, scores_out, done_out));
     return MODEL_OK;
 }

@@ -1,8 +1,7 @@
 """The operators over device memory (``include/tie_b200.h``): page plans, K/V row
 stores, attention over the paged cache, beam selection and cache reordering.
 
-Arguments are device tensors (anything with ``data_ptr``, ``shape``, ``stride``,
-``dtype`` and ``device``: torch tensors). Outputs and workspaces are the
+Arguments are torch tensors on a CUDA device. Outputs and workspaces are the
 caller's; nothing is allocated or waited for. Work runs on ``stream`` (a
 ``cudaStream_t`` as an int), by default torch's current stream of the tensors'
 device. Shapes, types and layouts that the C entry points cannot see are
@@ -14,74 +13,93 @@ The sizes of a page pool come from its tensors: ``k_pages`` and ``v_pages`` are
 """
 from __future__ import annotations
 
-from .lib import TIE_KV_BF16, TIE_KV_F32, _chk, library
+import torch
+
+from .lib import TIE_KV_BF16, TIE_KV_F32, ModelError, library
 
 PAGE_ROWS = 16
 HEAD_DIM = 64
 
-
-def _stream(t, stream):
-    if stream is not None:
-        return stream
-    import torch
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+_INT, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+# torch's current stream of a device as an integer; the public call builds a
+# Stream object first (2.3 us against 0.1 us)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-_NAMES = {}
+def _chk(rc, where):
+    if rc:
+        raise ModelError(rc, where)
 
 
-def _type(t):
-    """The element type's name, of torch.float32 as of any object that prints alike."""
-    n = _NAMES.get(t.dtype)
-    if n is None:
-        n = _NAMES[t.dtype] = str(t.dtype).rpartition(".")[2]
-    return n
+def _wrong(name, what):
+    raise ValueError(f"{name}: {what} is wanted")
 
 
 def _ints(name, t, n, device):
-    """A contiguous int32 vector of at least n elements on `device`: its address (None stays None)."""
+    """The address of a contiguous int32 tensor of at least n elements on `device` (None stays None)."""
     if t is None:
         return None
-    _need(_type(t) == "int32" and t.is_contiguous() and t.numel() >= n and t.device == device,
-          f"{name}: {n} contiguous int32 elements on {device} are wanted")
+    if t.dtype is not _INT or t.numel() < n or t.get_device() != device or not t.is_contiguous():
+        _wrong(name, f"a contiguous int32 tensor of {n} elements on device {device}")
+    return t.data_ptr()
+
+
+def _floats(name, t, n, device):
+    if t.dtype is not _F32 or t.numel() < n or t.get_device() != device or not t.is_contiguous():
+        _wrong(name, f"a contiguous float32 tensor of {n} elements on device {device}")
     return t.data_ptr()
 
 
 def _rows(name, t, width, device):
     """A float32 matrix of `width` columns whose rows are contiguous: (address, leading dimension)."""
-    _need(_type(t) == "float32" and t.dim() == 2 and t.shape[1] == width and t.stride(1) == 1 and t.device == device,
-          f"{name}: float32 [rows, {width}] with contiguous rows on {device} is wanted")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+    if t.dtype is not _F32 or t.dim() != 2 or t.get_device() != device:
+        _wrong(name, f"a float32 matrix on device {device}")
+    n, w = t.shape
+    ld, one = t.stride()
+    if w != width or (one != 1 and w > 1):
+        _wrong(name, f"[rows, {width}] with contiguous rows")
+    return t.data_ptr(), ld if n > 1 else max(ld, width)
 
 
 def _pool(k, v):
-    """(format, n_pages, n_kv_head, layers, layer stride) of a pool's two tensors."""
-    _need(k.shape == v.shape and k.dtype == v.dtype and k.device == v.device and k.is_contiguous() and v.is_contiguous(),
-          "k_pages and v_pages: two contiguous tensors of one shape, type and device are wanted")
-    shape, kind = k.shape, _type(k)
-    _need(len(shape) in (3, 4) and shape[-2] == PAGE_ROWS and shape[-1] % HEAD_DIM == 0 and kind in ("float32", "bfloat16"),
-          f"k_pages, v_pages: float32 or bfloat16 [n_pages, {PAGE_ROWS}, n_kv_head * {HEAD_DIM}] is wanted")
-    layers = shape[0] if len(shape) == 4 else 1
-    n_pages = shape[-3]
-    return (TIE_KV_BF16 if kind == "bfloat16" else TIE_KV_F32, n_pages, shape[-1] // HEAD_DIM, layers,
-            n_pages * PAGE_ROWS * shape[-1])
+    """(format, n_pages, n_kv_head, layers, layer stride, device) of a pool's two tensors."""
+    shape, dtype, device = k.shape, k.dtype, k.get_device()
+    if device < 0 or v.shape != shape or v.dtype is not dtype or v.get_device() != device or not (k.is_contiguous() and v.is_contiguous()):
+        _wrong("k_pages and v_pages", "one shape, type and CUDA device, contiguous,")
+    if dtype is _F32:
+        fmt = TIE_KV_F32
+    elif dtype is _BF16:
+        fmt = TIE_KV_BF16
+    else:
+        _wrong("k_pages, v_pages", "float32 or bfloat16")
+    if len(shape) == 3:
+        layers, (n_pages, rows, w) = 1, shape
+    elif len(shape) == 4:
+        layers, n_pages, rows, w = shape
+    else:
+        rows = 0
+    if rows != PAGE_ROWS or w % HEAD_DIM:
+        _wrong("k_pages, v_pages", f"[n_pages, {PAGE_ROWS}, n_kv_head * {HEAD_DIM}]")
+    return fmt, n_pages, w // HEAD_DIM, layers, n_pages * PAGE_ROWS * w, device
 
 
 def _table(t, device):
-    _need(_type(t) == "int32" and t.dim() == 2 and t.is_contiguous() and t.device == device,
-          f"page_table: contiguous int32 [n_seq, pages_per_seq] on {device} is wanted")
+    if t.dtype is not _INT or t.dim() != 2 or not t.is_contiguous() or t.get_device() != device or device < 0:
+        _wrong("page_table", f"a contiguous int32 [n_seq, pages_per_seq] on device {device}")
     return t.shape
+
+
+def _workspace(t, device):
+    if not t.is_contiguous() or t.get_device() != device:
+        _wrong("workspace", f"a contiguous tensor on device {device}")
+    return t.data_ptr(), t.numel() * t.element_size()
 
 
 def page_plan(ctx_lens, new_lens, page_table, n_pages, row_start, seq_of, pos_of, slot_of, status, free_pages=None,
               n_free=None, n_free_out=None, stream=None):
     """Assigns pages to new positions and writes row starts and slot maps (tie_page_plan)."""
-    d = page_table.device
+    d = page_table.get_device()
     n_seq, width = _table(page_table, d)
     rows = seq_of.numel()
     _chk(library().tie_page_plan(
@@ -89,19 +107,21 @@ def page_plan(ctx_lens, new_lens, page_table, n_pages, row_start, seq_of, pos_of
         n_pages, _ints("free_pages", free_pages, 0, d), 0 if free_pages is None else free_pages.numel(),
         _ints("n_free", n_free, 1, d), _ints("n_free_out", n_free_out, 1, d), _ints("row_start", row_start, n_seq + 1, d),
         _ints("seq_of", seq_of, rows, d), _ints("pos_of", pos_of, rows, d), _ints("slot_of", slot_of, rows, d), rows,
-        _ints("status", status, 1, d), _stream(page_table, stream)), "tie_page_plan")
+        _ints("status", status, 1, d), _raw_stream(d) if stream is None else stream), "tie_page_plan")
 
 
 def kv_store(k, v, slots, k_pages, v_pages, stream=None):
     """Rows of k and v [rows, n_kv_head * 64] (float32, any row stride that both have) into their slots (tie_kv_store)."""
-    fmt, n_pages, heads, layers, _ = _pool(k_pages, v_pages)
-    _need(layers == 1, "kv_store: the pages of one layer are wanted")
-    d, rows = k_pages.device, k.shape[0]
+    fmt, n_pages, heads, layers, _, d = _pool(k_pages, v_pages)
+    if layers != 1:
+        _wrong("k_pages, v_pages", "one layer")
+    rows = k.shape[0]
     kp, ld = _rows("k", k, heads * HEAD_DIM, d)
     vp, ldv = _rows("v", v, heads * HEAD_DIM, d)
-    _need(v.shape[0] == rows and ldv == ld, "kv_store: k and v of one shape and row stride are wanted")
+    if v.shape[0] != rows or ldv != ld:
+        _wrong("k and v", "one shape and row stride")
     _chk(library().tie_kv_store(kp, vp, ld, _ints("slots", slots, rows, d), rows, k_pages.data_ptr(), v_pages.data_ptr(),
-                                fmt, n_pages, heads, _stream(k_pages, stream)), "tie_kv_store")
+                                fmt, n_pages, heads, _raw_stream(d) if stream is None else stream), "tie_kv_store")
 
 
 def attention_paged_workspace():
@@ -113,20 +133,21 @@ def attention_paged(q, k_pages, v_pages, page_table, row_start, ctx_lens, max_ne
                     status=None, stream=None):
     """Causal attention of the new rows q over the pages that hold them (tie_attention_paged).
     scale: 1 / sqrt(64) by default."""
-    fmt, n_pages, kv_heads, layers, _ = _pool(k_pages, v_pages)
-    _need(layers == 1, "attention_paged: the pages of one layer are wanted")
-    d = k_pages.device
+    fmt, n_pages, kv_heads, layers, _, d = _pool(k_pages, v_pages)
+    if layers != 1:
+        _wrong("k_pages, v_pages", "one layer")
     n_seq, width = _table(page_table, d)
     w = q.shape[-1]
-    _need(w % HEAD_DIM == 0 and out.shape == q.shape, "attention_paged: q and out of one shape [rows, n_head * 64] are wanted")
+    if w % HEAD_DIM or out.shape != q.shape:
+        _wrong("q and out", f"one shape [rows, n_head * {HEAD_DIM}]")
     qp, ldq = _rows("q", q, w, d)
     op, ldo = _rows("out", out, w, d)
-    _need(workspace.is_contiguous() and workspace.device == d, "attention_paged: a contiguous workspace on the device is wanted")
+    wp, wn = _workspace(workspace, d)
     _chk(library().tie_attention_paged(
         qp, ldq, w // HEAD_DIM, k_pages.data_ptr(), v_pages.data_ptr(), fmt, n_pages, kv_heads, page_table.data_ptr(), width,
         _ints("row_start", row_start, n_seq + 1, d), _ints("ctx_lens", ctx_lens, n_seq, d), n_seq, max_new, q.shape[0],
-        0.125 if scale is None else scale, op, ldo, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-        _ints("status", status, 1, d), _stream(q, stream)), "tie_attention_paged")
+        0.125 if scale is None else scale, op, ldo, wp, wn, _ints("status", status, 1, d),
+        _raw_stream(d) if stream is None else stream), "tie_attention_paged")
 
 
 def beam_select_workspace(n_req, beams, vocab):
@@ -137,29 +158,26 @@ def beam_select_workspace(n_req, beams, vocab):
 def beam_select(logits, scores, beams, next_ids, parent, scores_out, workspace, done=None, done_out=None, eos_id=-1,
                 stream=None):
     """One step of beam search over logits [n_req * beams, vocab] (tie_beam_select)."""
-    d = logits.device
+    d = logits.get_device()
     n, vocab = logits.shape
-    _need(beams > 0 and n % beams == 0, "beam_select: n_req * beams rows of logits are wanted")
+    if beams <= 0 or n % beams or d < 0:
+        _wrong("logits", "n_req * beams rows on a CUDA device")
     lp, ldl = _rows("logits", logits, vocab, d)
-    for name, t in (("scores", scores), ("scores_out", scores_out)):
-        _need(_type(t) == "float32" and t.is_contiguous() and t.numel() >= n and t.device == d,
-              f"{name}: {n} contiguous float32 elements on {d} are wanted")
-    _need(workspace.is_contiguous() and workspace.device == d, "beam_select: a contiguous workspace on the device is wanted")
+    wp, wn = _workspace(workspace, d)
     _chk(library().tie_beam_select(
-        lp, ldl, scores.data_ptr(), _ints("done", done, n, d), n // beams, beams, vocab, eos_id,
-        _ints("next_ids", next_ids, n, d), _ints("parent", parent, n, d), scores_out.data_ptr(),
-        _ints("done_out", done_out, n, d), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-        _stream(logits, stream)), "tie_beam_select")
+        lp, ldl, _floats("scores", scores, n, d), _ints("done", done, n, d), n // beams, beams, vocab, eos_id,
+        _ints("next_ids", next_ids, n, d), _ints("parent", parent, n, d), _floats("scores_out", scores_out, n, d),
+        _ints("done_out", done_out, n, d), wp, wn, _raw_stream(d) if stream is None else stream), "tie_beam_select")
 
 
 def kv_reorder(k_pages, v_pages, page_table, parent, first, length, beams, stream=None):
     """Every layer's cached rows follow the beams' parents (tie_kv_reorder)."""
-    fmt, n_pages, heads, layers, stride = _pool(k_pages, v_pages)
-    d = k_pages.device
+    fmt, n_pages, heads, layers, stride, d = _pool(k_pages, v_pages)
     n, width = _table(page_table, d)
-    _need(beams > 0 and n % beams == 0, "kv_reorder: n_req * beams sequences are wanted")
+    if beams <= 0 or n % beams:
+        _wrong("page_table", "n_req * beams sequences")
     r = n // beams
     _chk(library().tie_kv_reorder(
         k_pages.data_ptr(), v_pages.data_ptr(), fmt, layers, stride, n_pages, heads, page_table.data_ptr(), width,
         _ints("parent", parent, n, d), _ints("first", first, r, d), _ints("length", length, r, d), r, beams,
-        _stream(k_pages, stream)), "tie_kv_reorder")
+        _raw_stream(d) if stream is None else stream), "tie_kv_reorder")
