@@ -28,7 +28,7 @@ namespace {
 constexpr int kMaxBeams = 16;
 constexpr int kScanThreads = 256, kScanWarps = kScanThreads / 32;
 constexpr int kBatch = 8;              // elements per thread and pass
-constexpr int kPickThreads = 256, kPickWarps = kPickThreads / 32;
+constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 64;   // pairs of warps
 constexpr int kMaxSlices = 32;         // a lane of the picking warps for each
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -49,6 +49,15 @@ struct Partials {
     int* idx;       // [rows][slices][k]
 };
 
+// floats (no NaN) as unsigned numbers of the same order, all above 0
+__device__ __forceinline__ unsigned order_key(float v) {
+    const unsigned b = __float_as_uint(v + 0.f);              // -0 and +0 are equal
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float from_order_key(unsigned k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
 __device__ __forceinline__ bool better(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
 __global__ void __launch_bounds__(kScanThreads)
@@ -59,11 +68,14 @@ beam_scan_kernel(const float* __restrict__ logits, int ldl, const int32_t* __res
     __shared__ int s_idx[kScanWarps * kMaxBeams];
     __shared__ float s_max[kScanWarps];
     __shared__ double s_sum[kScanWarps];
+    __shared__ unsigned s_bound;           // order_key of a lower bound of the slice's k-th best
     const int row = blockIdx.x / slices, slice = blockIdx.x % slices;
     if (done && done[row]) return;      // a finished beam's logits are not looked at
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int lo = slice * slice_len, hi = min(lo + slice_len, vocab);
     const float* x = logits + (size_t)row * ldl;
+    if (t == 0) s_bound = order_key(-INFINITY);
+    __syncthreads();
 
     float m = -INFINITY;
     double sum = 0.0;
@@ -72,16 +84,30 @@ beam_scan_kernel(const float* __restrict__ logits, int ldl, const int32_t* __res
     int li = INT_MAX;
     float worst = -INFINITY;            // lane k - 1's entry
     int worst_i = INT_MAX;
-    for (int i0 = lo; i0 < hi; i0 += kScanThreads * kBatch) {
+    // a pass's elements, NaN as -inf; the next pass's are on their way meanwhile
+    constexpr int kPass = kScanThreads * kBatch;
+    auto load = [&](int i0, float (&v)[kBatch]) {
+        if (i0 + kPass <= hi) {
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) v[u] = __ldcs(x + i0 + u * kScanThreads + t);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int i = i0 + u * kScanThreads + t;
+                v[u] = i < hi ? __ldcs(x + i) : -INFINITY;
+            }
+        }
+    };
+    float nv[kBatch];
+    load(lo, nv);
+    for (int i0 = lo; i0 < hi; i0 += kPass) {
         float v[kBatch];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int i = i0 + u * kScanThreads + t;
-            v[u] = i < hi ? __ldcs(x + i) : -INFINITY;
-        }
+        for (int u = 0; u < kBatch; ++u) v[u] = fmaxf(nv[u], -INFINITY);
+        if (i0 + kPass < hi) load(i0 + kPass, nv);
         float top = v[0];
 #pragma unroll
-        for (int u = 1; u < kBatch; ++u) top = fmaxf(top, v[u]);   // NaN never wins
+        for (int u = 1; u < kBatch; ++u) top = fmaxf(top, v[u]);
         if (top > m) {
             sum *= (double)ex2((m - top) * kLog2e);                // m = -inf: 0
             m = top;
@@ -89,38 +115,48 @@ beam_scan_kernel(const float* __restrict__ logits, int ldl, const int32_t* __res
         if (m > -INFINITY) {
             float part = 0.f;
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) part += v[u] == v[u] ? ex2((v[u] - m) * kLog2e) : 0.f;
+            for (int u = 0; u < kBatch; ++u) part += ex2((v[u] - m) * kLog2e);
             sum += (double)part;
         }
-        if (__any_sync(kAll, worst_i == INT_MAX || top > worst)) {
-            // While the list is filling up, only elements that reach the k-th
-            // largest of the lanes' maxima can be among the k best: without this
-            // bound the first pass would insert one element after the other (8 us).
-            float bound = -INFINITY;
-            if (worst_i == INT_MAX) {
-                int above = 0;
-#pragma unroll 8
-                for (int j = 0; j < 32; ++j) {
-                    const float other = __shfl_sync(kAll, top, j);
-                    above += other > top || (other == top && j < lane);
-                }
-                const unsigned kth = __ballot_sync(kAll, above == k - 1);   // one lane, unless maxima are NaN
-                if (kth) bound = __shfl_sync(kAll, top, __ffs(kth) - 1);
+        // The k-th best of any warp bounds the slice's k-th best from below: an
+        // element under it is in no result. The first pass has no list yet; there
+        // the k-th largest of a warp's lanes' maxima serves. (Without the shared
+        // bound each warp lists its own k best of every pass: 31 million
+        // instructions for 576 rows against 14 million.)
+        const bool filling = worst_i == INT_MAX;
+        if (i0 == lo) {
+            unsigned key = order_key(top);
+            unsigned kth = 0;
+            for (int r = 0; r < k; ++r) {
+                kth = __reduce_max_sync(kAll, key);
+                const unsigned who = __ballot_sync(kAll, key == kth);
+                if (lane == __ffs(who) - 1) key = 0;          // below every element's key
             }
-#pragma unroll 1
-            for (int u = 0; u < kBatch; ++u) {
-                const int i = i0 + u * kScanThreads + t;
-                const float xv = fmaxf(u == 0 ? v[0] : u == 1 ? v[1] : u == 2 ? v[2] : u == 3 ? v[3]
-                                       : u == 4 ? v[4] : u == 5 ? v[5] : u == 6 ? v[6] : v[7], -INFINITY);
-                unsigned todo = __ballot_sync(kAll, i < hi && xv >= bound && better(xv, i, worst, worst_i));
+            if (lane == 0) atomicMax(&s_bound, kth);
+            __syncthreads();
+        }
+        const float bound = from_order_key(*(volatile unsigned*)&s_bound);
+        if (__any_sync(kAll, top >= bound && (filling || top > worst))) {
+            unsigned lanes = __ballot_sync(kAll, top >= bound && (filling || top > worst));
+            while (lanes) {
+                const int src = __ffs(lanes) - 1;
+                lanes &= lanes - 1;
+                // lane u < kBatch: the u-th element of lane src
+                float cand = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    const float o = __shfl_sync(kAll, v[u], src);
+                    if (lane == u) cand = o;
+                }
+                const int ci0 = i0 + lane * kScanThreads + 32 * warp + src;
+                unsigned todo = __ballot_sync(kAll, lane < kBatch && ci0 < hi && cand >= bound && better(cand, ci0, worst, worst_i));
                 while (todo) {
-                    const int src = __ffs(todo) - 1;
+                    const int at = __ffs(todo) - 1;
                     todo &= todo - 1;
-                    const float cv = __shfl_sync(kAll, xv, src);
-                    const int ci = __shfl_sync(kAll, i, src);
+                    const float cv = __shfl_sync(kAll, cand, at);
+                    const int ci = __shfl_sync(kAll, ci0, at);
                     if (!better(cv, ci, worst, worst_i)) continue;
-                    const bool stays = better(lv, li, cv, ci);
-                    const int rank = __popc(__ballot_sync(kAll, stays && lane < k));
+                    const int rank = __popc(__ballot_sync(kAll, lane < k && better(lv, li, cv, ci)));
                     const float uv = __shfl_up_sync(kAll, lv, 1);
                     const int ui = __shfl_up_sync(kAll, li, 1);
                     if (lane == rank) { lv = cv; li = ci; }
@@ -129,6 +165,7 @@ beam_scan_kernel(const float* __restrict__ logits, int ldl, const int32_t* __res
                     worst_i = __shfl_sync(kAll, li, k - 1);
                 }
             }
+            if (lane == 0 && worst_i != INT_MAX) atomicMax(&s_bound, order_key(worst));
         }
     }
     // the CTA's maximum and sum
@@ -171,32 +208,40 @@ beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float
                  float* __restrict__ scores_out, int32_t* __restrict__ done_out) {
     __shared__ double s_total[kMaxBeams * kMaxBeams];      // the beams' best, best first; NaN: none
     __shared__ int s_token[kMaxBeams * kMaxBeams];
+    __shared__ float s_best[kMaxBeams * kMaxBeams];
     __shared__ double p_total[kMaxBeams];                  // the kept ones by rank
     __shared__ int p_beam[kMaxBeams], p_token[kMaxBeams];
+    __shared__ float s_val[kPickWarps][kMaxSlices * kMaxBeams];
+    __shared__ int s_idx[kPickWarps][kMaxSlices * kMaxBeams];
+    __shared__ double s_lse[kMaxBeams];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const size_t row0 = (size_t)blockIdx.x * k;
     pdl_wait();
-    // a warp per beam, a lane per slice
-    for (int b = warp; b < k; b += kPickWarps) {
-        const float score = scores[row0 + b];
-        const bool finished = done && done[row0 + b] != 0;
+    // two warps per beam, a lane per slice: one forms the logarithm of the sum of
+    // exponentials, the other merges the slices' lists
+    for (int b = warp & (kPickWarps - 1); b < k; b += kPickWarps) {
+        if (done && done[row0 + b] != 0) continue;
         const size_t at = (row0 + b) * slices + lane;
-        const bool mine = lane < slices && !finished;
-        const float m = mine ? in.max[at] : -INFINITY;
-        float M = m;
+        if (warp >= kPickWarps) {
+            const float m = lane < slices ? in.max[at] : -INFINITY;
+            float M = m;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kAll, M, o));
-        double S = m > -INFINITY ? in.sum[at] * exp((double)m - (double)M) : 0.0;
+            for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kAll, M, o));
+            double S = m > -INFINITY ? in.sum[at] * (double)ex2((m - M) * kLog2e) : 0.0;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(kAll, S, o);
-        // a row whose largest logit is infinite has no normaliser
-        const double lse = M > -INFINITY && M < INFINITY ? (double)M + log(S) : (double)NAN;
-        const bool scored = (double)score - lse > (double)-INFINITY;
-        // the beam's best: the lanes' sorted lists merged, best first
+            for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(kAll, S, o);
+            // a row whose largest logit is infinite has no normaliser
+            if (lane == 0) s_lse[b] = M > -INFINITY && M < INFINITY ? (double)M + log(S) : (double)NAN;
+            continue;
+        }
+        for (int e = lane; e < slices * k; e += 32) {
+            s_val[warp][e] = in.val[(row0 + b) * slices * k + e];
+            s_idx[warp][e] = in.idx[(row0 + b) * slices * k + e];
+        }
+        __syncwarp();
         int head = 0;
-        float hv = -INFINITY;
-        int hi = INT_MAX;
-        if (mine) { hv = in.val[at * k]; hi = in.idx[at * k]; }
+        float hv = lane < slices ? s_val[warp][lane * k] : -INFINITY;
+        int hi = lane < slices ? s_idx[warp][lane * k] : INT_MAX;
         for (int r = 0; r < k; ++r) {
             float v = hv;
             int i = hi;
@@ -206,26 +251,35 @@ beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float
                 const int oi = __shfl_xor_sync(kAll, i, o);
                 if (better(ov, oi, v, i)) { v = ov; i = oi; }
             }
-            if (mine && hi == i && hi != INT_MAX) {
+            if (hi == i && hi != INT_MAX) {
                 ++head;
-                hv = head < k ? in.val[at * k + head] : -INFINITY;
-                hi = head < k ? in.idx[at * k + head] : INT_MAX;
+                hv = head < k ? s_val[warp][lane * k + head] : -INFINITY;
+                hi = head < k ? s_idx[warp][lane * k + head] : INT_MAX;
             }
-            if (lane == 0) {
-                double total = (double)score + ((double)v - lse);
-                int token = i;
-                if (finished) {
-                    total = (double)score;
-                    token = r == 0 ? eos : INT_MAX;
-                } else if (!scored) {
-                    // every candidate ties at -inf, the lowest tokens are its best
-                    token = r < vocab ? r : INT_MAX;
-                }
-                if (!(total > (double)-INFINITY)) total = (double)-INFINITY;   // NaN counts as -inf
-                s_total[b * k + r] = token == INT_MAX ? (double)NAN : total;
-                s_token[b * k + r] = token;
-            }
+            if (lane == 0) { s_best[b * k + r] = v; s_token[b * k + r] = i; }
         }
+        __syncwarp();
+    }
+    __syncthreads();
+    // the candidates' totals
+    for (int c = t; c < k * k; c += kPickThreads) {
+        const int b = c / k, r = c % k;
+        const float score = scores[row0 + b];
+        double total = (double)score;
+        int token;
+        if (done && done[row0 + b] != 0) {
+            token = r == 0 ? eos : INT_MAX;
+        } else if ((double)score - s_lse[b] > (double)-INFINITY) {
+            token = s_token[c];
+            total += (double)s_best[c] - s_lse[b];
+        } else {
+            // every candidate ties at -inf, the lowest tokens are its best
+            token = r < vocab ? r : INT_MAX;
+            total = (double)-INFINITY;
+        }
+        if (!(total > (double)-INFINITY)) total = (double)-INFINITY;   // NaN counts as -inf
+        s_total[c] = token == INT_MAX ? (double)NAN : total;
+        s_token[c] = token;
     }
     __syncthreads();
     // each candidate finds its rank among all
@@ -252,11 +306,13 @@ beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float
         const bool heir = __ffs((int)__match_any_sync(kAll, b)) - 1 == lane;
         const unsigned taken = __reduce_or_sync(kAll, lane < k ? 1u << b : 0u);
         const unsigned others = __ballot_sync(kAll, lane < k && !heir);
+        const bool was = lane < k && done && done[row0 + b] != 0;
+        __syncwarp();                                          // done_out may be done
         if (lane < k) {
-            const int place = heir ? b : (int)__fns(~taken, 0, __popc(others & ((1u << lane) - 1)) + 1);
+            unsigned left = ~taken;                         // the free places, lowest first
+            for (int o = __popc(others & ((1u << lane) - 1)); o > 0; --o) left &= left - 1;
+            const int place = heir ? b : __ffs((int)left) - 1;
             const int tok = p_token[lane];
-            const bool was = done && done[row0 + b] != 0;
-            __syncwarp(__activemask());
             next[row0 + place] = tok;
             parent[row0 + place] = (int)row0 + b;
             scores_out[row0 + place] = (float)p_total[lane];
