@@ -27,7 +27,8 @@ namespace {
 
 constexpr int kMaxBeams = 16;
 constexpr int kScanThreads = 256, kScanWarps = kScanThreads / 32;
-constexpr int kBatch = 8;              // elements per thread and pass
+constexpr int kBatch = 8;              // elements a thread loads at a time
+constexpr int kScanResident = 8;       // CTAs per SM (64 KB of loads in flight)
 constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 64;   // pairs of warps
 constexpr int kMaxSlices = 32;         // a lane of the picking warps for each
 constexpr unsigned kAll = 0xffffffffu;
@@ -60,7 +61,7 @@ __device__ __forceinline__ float from_order_key(unsigned k) {
 
 __device__ __forceinline__ bool better(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
-__global__ void __launch_bounds__(kScanThreads)
+__global__ void __launch_bounds__(kScanThreads, kScanResident)
 beam_scan_kernel(const float* __restrict__ logits, int ldl, const int32_t* __restrict__ done, int vocab, int slices,
                  int slice_len, int k, Partials out) {
     pdl_trigger();
@@ -68,46 +69,34 @@ beam_scan_kernel(const float* __restrict__ logits, int ldl, const int32_t* __res
     __shared__ int s_idx[kScanWarps * kMaxBeams];
     __shared__ float s_max[kScanWarps];
     __shared__ double s_sum[kScanWarps];
-    __shared__ unsigned s_bound;           // order_key of a lower bound of the slice's k-th best
+    __shared__ unsigned s_key[kScanWarps * kMaxBeams], s_bound;
     const int row = blockIdx.x / slices, slice = blockIdx.x % slices;
     if (done && done[row]) return;      // a finished beam's logits are not looked at
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int lo = slice * slice_len, hi = min(lo + slice_len, vocab);
     const float* x = logits + (size_t)row * ldl;
-    if (t == 0) s_bound = order_key(-INFINITY);
-    __syncthreads();
 
+    // One pass over the slice: a thread's maximum and its sum of exponentials.
     float m = -INFINITY;
     double sum = 0.0;
-    // the warp's list: lane j < k holds its (j + 1)th best
-    float lv = -INFINITY;
-    int li = INT_MAX;
-    float worst = -INFINITY;            // lane k - 1's entry
-    int worst_i = INT_MAX;
-    // a pass's elements, NaN as -inf; the next pass's are on their way meanwhile
-    constexpr int kPass = kScanThreads * kBatch;
-    auto load = [&](int i0, float (&v)[kBatch]) {
-        if (i0 + kPass <= hi) {
+    for (int i0 = lo; i0 < hi; i0 += kScanThreads * kBatch) {
+        float v[kBatch];
+        if (i0 + kScanThreads * kBatch <= hi) {
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) v[u] = __ldcs(x + i0 + u * kScanThreads + t);
+            for (int u = 0; u < kBatch; ++u) v[u] = __ldg(x + i0 + u * kScanThreads + t);
         } else {
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
                 const int i = i0 + u * kScanThreads + t;
-                v[u] = i < hi ? __ldcs(x + i) : -INFINITY;
+                v[u] = i < hi ? __ldg(x + i) : -INFINITY;
             }
         }
-    };
-    float nv[kBatch];
-    load(lo, nv);
-    for (int i0 = lo; i0 < hi; i0 += kPass) {
-        float v[kBatch];
+        float top = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) v[u] = fmaxf(nv[u], -INFINITY);
-        if (i0 + kPass < hi) load(i0 + kPass, nv);
-        float top = v[0];
-#pragma unroll
-        for (int u = 1; u < kBatch; ++u) top = fmaxf(top, v[u]);
+        for (int u = 0; u < kBatch; ++u) {
+            v[u] = fmaxf(v[u], -INFINITY);                         // NaN counts as -inf
+            top = fmaxf(top, v[u]);
+        }
         if (top > m) {
             sum *= (double)ex2((m - top) * kLog2e);                // m = -inf: 0
             m = top;
@@ -118,54 +107,75 @@ beam_scan_kernel(const float* __restrict__ logits, int ldl, const int32_t* __res
             for (int u = 0; u < kBatch; ++u) part += ex2((v[u] - m) * kLog2e);
             sum += (double)part;
         }
-        // The k-th best of any warp bounds the slice's k-th best from below: an
-        // element under it is in no result. The first pass has no list yet; there
-        // the k-th largest of a warp's lanes' maxima serves. (Without the shared
-        // bound each warp lists its own k best of every pass: 31 million
-        // instructions for 576 rows against 14 million.)
-        const bool filling = worst_i == INT_MAX;
-        if (i0 == lo) {
-            unsigned key = order_key(top);
-            unsigned kth = 0;
-            for (int r = 0; r < k; ++r) {
-                kth = __reduce_max_sync(kAll, key);
-                const unsigned who = __ballot_sync(kAll, key == kth);
-                if (lane == __ffs(who) - 1) key = 0;          // below every element's key
-            }
-            if (lane == 0) atomicMax(&s_bound, kth);
-            __syncthreads();
+    }
+    // The k-th largest of the threads' maxima: k elements reach it, so whatever is
+    // below is in no result, and about k threads have something that is not.
+    // (Lists kept during the pass cost more instructions than the pass: 31 million
+    // for 576 rows against 9 million.)
+    auto kth_of = [&](auto next_key) {     // the warp's k largest keys, largest first; lane r gets the r-th
+        unsigned mine = 0;
+        for (int r = 0; r < k; ++r) {
+            const unsigned key = next_key(r, false), most = __reduce_max_sync(kAll, key);
+            if (lane == r) mine = most;
+            if (lane == __ffs(__ballot_sync(kAll, key == most)) - 1) next_key(r, true);
         }
-        const float bound = from_order_key(*(volatile unsigned*)&s_bound);
-        if (__any_sync(kAll, top >= bound && (filling || top > worst))) {
-            unsigned lanes = __ballot_sync(kAll, top >= bound && (filling || top > worst));
-            while (lanes) {
-                const int src = __ffs(lanes) - 1;
-                lanes &= lanes - 1;
-                // lane u < kBatch: the u-th element of lane src
-                float cand = -INFINITY;
+        return mine;
+    };
+    {
+        unsigned key = order_key(m);
+        const unsigned mine = kth_of([&](int, bool take) { return take ? key = 0u : key; });
+        if (lane < k) s_key[warp * k + lane] = mine;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        // the warps' keys, up to four a lane
+        unsigned key[kScanWarps * kMaxBeams / 32];
 #pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    const float o = __shfl_sync(kAll, v[u], src);
-                    if (lane == u) cand = o;
-                }
-                const int ci0 = i0 + lane * kScanThreads + 32 * warp + src;
-                unsigned todo = __ballot_sync(kAll, lane < kBatch && ci0 < hi && cand >= bound && better(cand, ci0, worst, worst_i));
-                while (todo) {
-                    const int at = __ffs(todo) - 1;
-                    todo &= todo - 1;
-                    const float cv = __shfl_sync(kAll, cand, at);
-                    const int ci = __shfl_sync(kAll, ci0, at);
-                    if (!better(cv, ci, worst, worst_i)) continue;
-                    const int rank = __popc(__ballot_sync(kAll, lane < k && better(lv, li, cv, ci)));
-                    const float uv = __shfl_up_sync(kAll, lv, 1);
-                    const int ui = __shfl_up_sync(kAll, li, 1);
-                    if (lane == rank) { lv = cv; li = ci; }
-                    else if (lane > rank) { lv = uv; li = ui; }
-                    worst = __shfl_sync(kAll, lv, k - 1);
-                    worst_i = __shfl_sync(kAll, li, k - 1);
-                }
+        for (int e = 0; e < kScanWarps * kMaxBeams / 32; ++e) key[e] = lane + 32 * e < kScanWarps * k ? s_key[lane + 32 * e] : 0u;
+        const unsigned mine = kth_of([&](int, bool take) {
+            unsigned most = key[0];
+#pragma unroll
+            for (int e = 1; e < kScanWarps * kMaxBeams / 32; ++e) most = max(most, key[e]);
+            if (take) {
+                bool taken = false;
+#pragma unroll
+                for (int e = 0; e < kScanWarps * kMaxBeams / 32; ++e)
+                    if (!taken && key[e] == most) { key[e] = 0u; taken = true; }
             }
-            if (lane == 0 && worst_i != INT_MAX) atomicMax(&s_bound, order_key(worst));
+            return most;
+        });
+        if (lane == k - 1) s_bound = mine;
+    }
+    __syncthreads();
+    const float bound = from_order_key(s_bound);
+    // the warp's list: lane j < k holds its (j + 1)th best
+    float lv = -INFINITY;
+    int li = INT_MAX;
+    float worst = -INFINITY;            // lane k - 1's entry
+    int worst_i = INT_MAX;
+    unsigned lanes = __ballot_sync(kAll, m >= bound);
+    while (lanes) {
+        // the elements of one lane's thread, 32 at a time
+        const int src = __ffs(lanes) - 1;
+        lanes &= lanes - 1;
+        for (int i0 = lo + 32 * warp + src; i0 < hi; i0 += 32 * kScanThreads) {
+            const int i = i0 + lane * kScanThreads;
+            const float cand = i < hi ? fmaxf(__ldg(x + i), -INFINITY) : -INFINITY;
+            unsigned todo = __ballot_sync(kAll, i < hi && cand >= bound && better(cand, i, worst, worst_i));
+            while (todo) {
+                const int at = __ffs(todo) - 1;
+                todo &= todo - 1;
+                const float cv = __shfl_sync(kAll, cand, at);
+                const int ci = __shfl_sync(kAll, i, at);
+                if (!better(cv, ci, worst, worst_i)) continue;
+                const int rank = __popc(__ballot_sync(kAll, lane < k && better(lv, li, cv, ci)));
+                const float uv = __shfl_up_sync(kAll, lv, 1);
+                const int ui = __shfl_up_sync(kAll, li, 1);
+                if (lane == rank) { lv = cv; li = ci; }
+                else if (lane > rank) { lv = uv; li = ui; }
+                worst = __shfl_sync(kAll, lv, k - 1);
+                worst_i = __shfl_sync(kAll, li, k - 1);
+            }
         }
     }
     // the CTA's maximum and sum
@@ -321,15 +331,15 @@ beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float
     }
 }
 
-// Slices of the vocabulary per row: about four CTAs per SM in all, each of at
-// least one pass of its threads (2048 logits), at most a lane each of the warp
-// that joins them.
+// Slices of the vocabulary per row: one wave of CTAs, each of at least one load
+// of its threads (2048 logits), at most a lane each of the warp that joins them.
 int slices_of(int n_req, int beams, int vocab, int sms) {
     const long long rows = (long long)n_req * beams;
     const int most = (vocab + kScanThreads * kBatch - 1) / (kScanThreads * kBatch);
-    const long long want = (4LL * sms + rows - 1) / rows;
-    const long long n = want < 1 ? 1 : want > most ? most : want;
-    return (int)(n < kMaxSlices ? n : kMaxSlices);
+    long long n = (long long)kScanResident * sms / rows;
+    if (n > most) n = most;
+    if (n > kMaxSlices) n = kMaxSlices;
+    return n < 1 ? 1 : (int)n;
 }
 
 size_t scratch_bytes(int n_req, int beams, int slices) {
