@@ -30,6 +30,7 @@ constexpr int kScanThreads = 256, kScanWarps = kScanThreads / 32;
 constexpr int kBatch = 8;              // elements a thread loads at a time
 constexpr int kScanResident = 8;       // CTAs per SM (64 KB of loads in flight)
 constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 64;   // pairs of warps
+constexpr int kWaves = 2;
 constexpr int kMaxSlices = 32;         // a lane of the picking warps for each
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -218,6 +219,7 @@ beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float
                  float* __restrict__ scores_out, int32_t* __restrict__ done_out) {
     __shared__ double s_total[kMaxBeams * kMaxBeams];      // the beams' best, best first; NaN: none
     __shared__ int s_token[kMaxBeams * kMaxBeams];
+    __shared__ long long s_flat[kMaxBeams * kMaxBeams];    // beam * vocab + token
     __shared__ float s_best[kMaxBeams * kMaxBeams];
     __shared__ double p_total[kMaxBeams];                  // the kept ones by rank
     __shared__ int p_beam[kMaxBeams], p_token[kMaxBeams];
@@ -290,22 +292,20 @@ beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float
         if (!(total > (double)-INFINITY)) total = (double)-INFINITY;   // NaN counts as -inf
         s_total[c] = token == INT_MAX ? (double)NAN : total;
         s_token[c] = token;
+        s_flat[c] = (long long)b * vocab + token;
     }
     __syncthreads();
     // each candidate finds its rank among all
     for (int c = t; c < k * k; c += kPickThreads) {
         const double v = s_total[c];
         if (v != v) continue;
-        const int b = c / k;
-        const long long flat = (long long)b * vocab + s_token[c];
+        const long long flat = s_flat[c];
         int rank = 0;
-        for (int o = 0; o < k * k; ++o) {
-            const double ov = s_total[o];
-            if (ov > v || (ov == v && (long long)(o / k) * vocab + s_token[o] < flat)) ++rank;
-        }
+#pragma unroll 4
+        for (int o = 0; o < k * k; ++o) rank += s_total[o] > v || (s_total[o] == v && s_flat[o] < flat);
         if (rank < k) {
             p_total[rank] = v;
-            p_beam[rank] = b;
+            p_beam[rank] = c / k;
             p_token[rank] = s_token[c];
         }
     }
@@ -331,12 +331,13 @@ beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float
     }
 }
 
-// Slices of the vocabulary per row: one wave of CTAs, each of at least one load
-// of its threads (2048 logits), at most a lane each of the warp that joins them.
+// Slices of the vocabulary per row: some waves of CTAs (one CTA's last steps run
+// beside another's loads), each of at least one load of its threads (2048
+// logits), at most a lane each of the warp that joins them.
 int slices_of(int n_req, int beams, int vocab, int sms) {
     const long long rows = (long long)n_req * beams;
     const int most = (vocab + kScanThreads * kBatch - 1) / (kScanThreads * kBatch);
-    long long n = (long long)kScanResident * sms / rows;
+    long long n = (long long)kWaves * kScanResident * sms / rows;
     if (n > most) n = most;
     if (n > kMaxSlices) n = kMaxSlices;
     return n < 1 ? 1 : (int)n;

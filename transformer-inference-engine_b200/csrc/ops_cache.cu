@@ -71,6 +71,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
     extern __shared__ int sm[];
     int* s_row = sm;                      // [n_seq + 1] first row of each sequence
     int* s_need = sm + a.n_seq + 1;       // [n_seq + 1] pages assigned before each sequence
+    int* s_ctx = s_need + a.n_seq + 1;    // [n_seq]
     __shared__ long long w_new[32], w_need[32];
     __shared__ int s_bad;                 // 1: a negative length, 2: a sequence beyond its table
     cg::cluster_group cluster = cg::this_cluster();
@@ -91,6 +92,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
         nw[k] = nd[k] = 0;
         if (k < per && s < a.n_seq) {
             const int c = a.ctx[s], n = a.fresh[s];
+            s_ctx[s] = c;
             if (c < 0 || n < 0) bad |= 1;
             else if ((long long)c + n > cap) bad |= 2;
             else {
@@ -157,25 +159,48 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
     const int need = s_need[a.n_seq], rows = s_row[a.n_seq];
     for (int x = g; x < need; x += G) {
         const int s = owner(s_need, x);
-        const int have = (int)(((long long)a.ctx[s] + kPageRows - 1) / kPageRows);
+        const int have = (int)(((long long)s_ctx[s] + kPageRows - 1) / kPageRows);
         a.table[(size_t)s * a.width + have + (x - s_need[s])] = a.free_pages[n_free - 1 - x];
     }
-    for (int r = g; r < a.max_rows; r += G) {
-        int seq = -1, pos = -1, slot = -1;
-        if (r < rows) {
-            seq = owner(s_row, r);
-            const int c = a.ctx[seq];
-            pos = c + (r - s_row[seq]);
-            const int j = pos / kPageRows, have = (int)(((long long)c + kPageRows - 1) / kPageRows);
+    // A warp takes 32 rows at a time, and two such groups at once (a row is two
+    // loads that depend on one another, so latency counts): the sequence of the
+    // first row by a search with all lanes, the others by walking on from there.
+    constexpr int kGroups = 2;
+    const int gw = g >> 5, GW = G >> 5;
+    for (int w0 = gw; 32 * (long long)w0 < a.max_rows; w0 += kGroups * GW) {
+        int seq[kGroups], pos[kGroups], page[kGroups];
+#pragma unroll
+        for (int x = 0; x < kGroups; ++x) {
+            const int first = 32 * (w0 + x * GW), r = first + lane;
+            seq[x] = pos[x] = page[x] = -1;
+            if (first >= rows || first < 0) continue;
+            int lo = 0, n = a.n_seq;               // s_row[lo] <= first, and not at lo + n
+            while (n > 1) {
+                const int step = (n + 31) / 32;    // lane l looks at lo + l * step
+                const bool below = lane * step < n && s_row[lo + lane * step] <= first;
+                const int at = 31 - __clz(__ballot_sync(0xffffffffu, below));
+                lo += at * step;
+                n = min(step, n - at * step);
+            }
+            if (r >= rows) continue;
+            while (s_row[lo + 1] <= r) ++lo;
+            seq[x] = lo;
+            const int c = s_ctx[lo], have = (int)(((long long)c + kPageRows - 1) / kPageRows);
+            pos[x] = c + (r - s_row[lo]);
+            const int j = pos[x] / kPageRows;
             // the entries other threads assign above are taken from the free
             // list itself, not from the table
-            const int page = a.free_pages && j >= have ? a.free_pages[n_free - 1 - (s_need[seq] + j - have)]
-                                                       : a.table[(size_t)seq * a.width + j];
-            if (page >= 0 && page < a.n_pages) slot = page * kPageRows + pos % kPageRows;
+            page[x] = a.free_pages && j >= have ? a.free_pages[n_free - 1 - (s_need[lo] + j - have)]
+                                                : a.table[(size_t)lo * a.width + j];
         }
-        a.seq_of[r] = seq;
-        a.pos_of[r] = pos;
-        a.slot_of[r] = slot;
+#pragma unroll
+        for (int x = 0; x < kGroups; ++x) {
+            const long long r = 32 * ((long long)w0 + x * GW) + lane;
+            if (r >= a.max_rows) continue;
+            a.seq_of[r] = seq[x];
+            a.pos_of[r] = pos[x];
+            a.slot_of[r] = page[x] >= 0 && page[x] < a.n_pages ? page[x] * kPageRows + pos[x] % kPageRows : -1;
+        }
     }
 }
 
@@ -286,10 +311,14 @@ __global__ void __launch_bounds__(kReorderThreads) kv_reorder_kernel(ReorderArgs
         if (r == a.n_req - 1) s_base[a.n_req] = base;
     }
     __syncthreads();
-    const long long pages = s_base[a.n_req], units = pages * 2 * a.n_layer;
+    const long long pages = s_base[a.n_req], whole = pages * 2 * a.n_layer;
     const int vecs = a.row_vecs * kPageRows;
+    // few pages: each is cut into pieces, so that every CTA has something to move
+    const int pieces = whole > 0 ? (int)max(1ll, min(gridDim.x / whole, (long long)(vecs / kReorderThreads))) : 1;
+    const int piece_vecs = (vecs + pieces - 1) / pieces;
+    const long long units = whole * pieces;
     for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-        const int pg = (int)(u % pages), lv = (int)(u / pages);
+        const int piece = (int)(u % pieces), pg = (int)(u / pieces % pages), lv = (int)(u / pieces / pages);
         int lo = 0, hi = a.n_req;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -312,8 +341,8 @@ __global__ void __launch_bounds__(kReorderThreads) kv_reorder_kernel(ReorderArgs
         }
         __syncthreads();
         uint4* pool = (lv & 1 ? a.v : a.k) + (size_t)(lv >> 1) * a.layer_vecs;
-        const int v0 = max(f - j * kPageRows, 0) * a.row_vecs;
-        const int v1 = min(len - j * kPageRows, kPageRows) * a.row_vecs;
+        const int v0 = max(max(f - j * kPageRows, 0) * a.row_vecs, piece * piece_vecs);
+        const int v1 = min(min(len - j * kPageRows, kPageRows) * a.row_vecs, (piece + 1) * piece_vecs);
         for (int i = v0 + t; i < v1; i += kReorderThreads) {
             uint4 x[BEAMS];
 #pragma unroll
@@ -349,7 +378,10 @@ extern "C" model_status tie_page_plan(const int32_t* ctx_lens, const int32_t* ne
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kPlanThreads);
-    cfg.dynamicSmemBytes = 2 * (size_t)(n_seq + 1) * sizeof(int);
+    cfg.dynamicSmemBytes = 3 * (size_t)(n_seq + 1) * sizeof(int);
+    if (cfg.dynamicSmemBytes > 46 * 1024)
+        TIE_OP_CU(cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)cfg.dynamicSmemBytes));
     cfg.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
