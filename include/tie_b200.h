@@ -269,7 +269,8 @@ model_status tie_head_argmax_noalloc(const float *x, int ldx, const float *w, in
  * captured into a graph. MODEL_ERR_ARG for a null or misaligned pointer, a
  * shape or format without meaning, or host memory; MODEL_ERR_CAPACITY for a
  * workspace too small or a limit below; MODEL_ERR_DEVICE for a CUDA failure.
- * Limits: 4096 sequences or requests, 2^27 pages (2^26 per sequence), 16 beams. */
+ * Limits: 4096 sequences or requests, 2^27 pages (2^26 per sequence), 16 beams,
+ * 2^30 logits a row. */
 enum { TIE_KV_F32 = 0, TIE_KV_BF16 = 1 };
 
 /* Page table entries, row starts and slot maps from request lengths. Sequence

@@ -77,7 +77,7 @@ def test_select_refuses(changed):
     assert _call(L.tie_beam_select, SELECT, **changed) == ARG
 
 
-@pytest.mark.parametrize("changed", [dict(beams=17), dict(n_req=4097)])
+@pytest.mark.parametrize("changed", [dict(beams=17), dict(n_req=4097), dict(vocab=(1 << 30) + 1, ldl=(1 << 30) + 1)])
 def test_select_limits(changed):
     assert _call(L.tie_beam_select, SELECT, **changed) == CAPACITY
     assert L.tie_beam_select_workspace(1, 17, 100) == 0 and L.tie_beam_select_workspace(0, 4, 100) == 0

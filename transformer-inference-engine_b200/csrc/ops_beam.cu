@@ -31,6 +31,7 @@ constexpr int kBatch = 8;              // elements a thread loads at a time
 constexpr int kScanResident = 8;       // CTAs per SM (64 KB of loads in flight)
 constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 64;   // pairs of warps
 constexpr int kWaves = 2;
+constexpr int kMaxVocab = 1 << 30;     // indices of a row stay in int32 with room for a step
 constexpr int kMaxSlices = 32;         // a lane of the picking warps for each
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -70,7 +71,9 @@ beam_scan_kernel(const float* __restrict__ logits, int ldl, const int32_t* __res
     __shared__ int s_idx[kScanWarps * kMaxBeams];
     __shared__ float s_max[kScanWarps];
     __shared__ double s_sum[kScanWarps];
-    __shared__ unsigned s_key[kScanWarps * kMaxBeams], s_bound;
+    __shared__ float s_group[2 * kScanWarps];
+    __shared__ int s_count;
+    static_assert(2 * kScanWarps >= kMaxBeams, "a bound for every list length");
     const int row = blockIdx.x / slices, slice = blockIdx.x % slices;
     if (done && done[row]) return;      // a finished beam's logits are not looked at
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -109,46 +112,24 @@ beam_scan_kernel(const float* __restrict__ logits, int ldl, const int32_t* __res
             sum += (double)part;
         }
     }
-    // The k-th largest of the threads' maxima: k elements reach it, so whatever is
-    // below is in no result, and about k threads have something that is not.
+    // The k-th largest of the half-warps' maxima: k elements reach it, so whatever
+    // is below is in no result, and few threads have something that is not.
     // (Lists kept during the pass cost more instructions than the pass: 31 million
     // for 576 rows against 9 million.)
-    auto kth_of = [&](auto next_key) {     // the warp's k largest keys, largest first; lane r gets the r-th
-        unsigned mine = 0;
-        for (int r = 0; r < k; ++r) {
-            const unsigned key = next_key(r, false), most = __reduce_max_sync(kAll, key);
-            if (lane == r) mine = most;
-            if (lane == __ffs(__ballot_sync(kAll, key == most)) - 1) next_key(r, true);
-        }
-        return mine;
-    };
+    float gm = m;
+#pragma unroll
+    for (int o = 8; o; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(kAll, gm, o));
+    if ((lane & 15) == 0) s_group[2 * warp + (lane >> 4)] = gm;
+    if (t == 0) s_count = 0;
+    __syncthreads();
+    float bound;
     {
-        unsigned key = order_key(m);
-        const unsigned mine = kth_of([&](int, bool take) { return take ? key = 0u : key; });
-        if (lane < k) s_key[warp * k + lane] = mine;
+        const float mine = lane < 2 * kScanWarps ? s_group[lane] : -INFINITY;
+        int above = 0;
+#pragma unroll
+        for (int g = 0; g < 2 * kScanWarps; ++g) above += s_group[g] > mine || (s_group[g] == mine && g < lane);
+        bound = __shfl_sync(kAll, mine, __ffs(__ballot_sync(kAll, lane < 2 * kScanWarps && above == k - 1)) - 1);
     }
-    __syncthreads();
-    if (warp == 0) {
-        // the warps' keys, up to four a lane
-        unsigned key[kScanWarps * kMaxBeams / 32];
-#pragma unroll
-        for (int e = 0; e < kScanWarps * kMaxBeams / 32; ++e) key[e] = lane + 32 * e < kScanWarps * k ? s_key[lane + 32 * e] : 0u;
-        const unsigned mine = kth_of([&](int, bool take) {
-            unsigned most = key[0];
-#pragma unroll
-            for (int e = 1; e < kScanWarps * kMaxBeams / 32; ++e) most = max(most, key[e]);
-            if (take) {
-                bool taken = false;
-#pragma unroll
-                for (int e = 0; e < kScanWarps * kMaxBeams / 32; ++e)
-                    if (!taken && key[e] == most) { key[e] = 0u; taken = true; }
-            }
-            return most;
-        });
-        if (lane == k - 1) s_bound = mine;
-    }
-    __syncthreads();
-    const float bound = from_order_key(s_bound);
     // the warp's list: lane j < k holds its (j + 1)th best
     float lv = -INFINITY;
     int li = INT_MAX;
@@ -156,26 +137,36 @@ beam_scan_kernel(const float* __restrict__ logits, int ldl, const int32_t* __res
     int worst_i = INT_MAX;
     unsigned lanes = __ballot_sync(kAll, m >= bound);
     while (lanes) {
-        // the elements of one lane's thread, 32 at a time
+        // the elements of one lane's thread, 128 at a time
         const int src = __ffs(lanes) - 1;
         lanes &= lanes - 1;
-        for (int i0 = lo + 32 * warp + src; i0 < hi; i0 += 32 * kScanThreads) {
-            const int i = i0 + lane * kScanThreads;
-            const float cand = i < hi ? fmaxf(__ldg(x + i), -INFINITY) : -INFINITY;
-            unsigned todo = __ballot_sync(kAll, i < hi && cand >= bound && better(cand, i, worst, worst_i));
-            while (todo) {
-                const int at = __ffs(todo) - 1;
-                todo &= todo - 1;
-                const float cv = __shfl_sync(kAll, cand, at);
-                const int ci = __shfl_sync(kAll, i, at);
-                if (!better(cv, ci, worst, worst_i)) continue;
-                const int rank = __popc(__ballot_sync(kAll, lane < k && better(lv, li, cv, ci)));
-                const float uv = __shfl_up_sync(kAll, lv, 1);
-                const int ui = __shfl_up_sync(kAll, li, 1);
-                if (lane == rank) { lv = cv; li = ci; }
-                else if (lane > rank) { lv = uv; li = ui; }
-                worst = __shfl_sync(kAll, lv, k - 1);
-                worst_i = __shfl_sync(kAll, li, k - 1);
+        constexpr int kAhead = 4, kStride = 32 * kScanThreads;
+        for (int i0 = lo + 32 * warp + src; i0 < hi; i0 += kAhead * kStride) {
+            float own[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int i = i0 + lane * kScanThreads + u * kStride;
+                own[u] = i < hi ? fmaxf(__ldg(x + i), -INFINITY) : -INFINITY;
+            }
+#pragma unroll 1
+            for (int u = 0; u < kAhead && i0 + u * kStride < hi; ++u) {
+                const float cand = u == 0 ? own[0] : u == 1 ? own[1] : u == 2 ? own[2] : own[3];
+                const int i = i0 + lane * kScanThreads + u * kStride;
+                unsigned todo = __ballot_sync(kAll, i < hi && cand >= bound && better(cand, i, worst, worst_i));
+                while (todo) {
+                    const int at = __ffs(todo) - 1;
+                    todo &= todo - 1;
+                    const float cv = __shfl_sync(kAll, cand, at);
+                    const int ci = __shfl_sync(kAll, i, at);
+                    if (!better(cv, ci, worst, worst_i)) continue;
+                    const int rank = __popc(__ballot_sync(kAll, lane < k && better(lv, li, cv, ci)));
+                    const float uv = __shfl_up_sync(kAll, lv, 1);
+                    const int ui = __shfl_up_sync(kAll, li, 1);
+                    if (lane == rank) { lv = cv; li = ci; }
+                    else if (lane > rank) { lv = uv; li = ui; }
+                    worst = __shfl_sync(kAll, lv, k - 1);
+                    worst_i = __shfl_sync(kAll, li, k - 1);
+                }
             }
         }
     }
@@ -187,28 +178,44 @@ beam_scan_kernel(const float* __restrict__ logits, int ldl, const int32_t* __res
 #pragma unroll
     for (int o = 16; o; o >>= 1) ws += __shfl_xor_sync(kAll, ws, o);
     if (lane == 0) { s_max[warp] = wm; s_sum[warp] = ws; }
-    if (lane < k) { s_val[warp * k + lane] = lv; s_idx[warp * k + lane] = li; }
+    // the warps' entries side by side, in any order
+    {
+        const int n = __popc(__ballot_sync(kAll, lane < k && li != INT_MAX));
+        int at = 0;
+        if (lane == 0 && n) at = atomicAdd(&s_count, n);
+        at = __shfl_sync(kAll, at, 0);
+        if (lane < n) { s_val[at + lane] = lv; s_idx[at + lane] = li; }
+    }
     __syncthreads();
     const size_t at = (size_t)row * slices + slice;
-    if (t == 0) {
-        float M = s_max[0];
-        for (int w = 1; w < kScanWarps; ++w) M = fmaxf(M, s_max[w]);
-        double S = 0.0;
-        for (int w = 0; w < kScanWarps; ++w)
-            if (s_max[w] > -INFINITY) S += s_sum[w] * exp((double)s_max[w] - (double)M);
-        out.max[at] = M;
-        out.sum[at] = S;
+    if (warp == 0) {
+        const float wm0 = lane < kScanWarps ? s_max[lane] : -INFINITY;
+        float M = wm0;
+#pragma unroll
+        for (int o = kScanWarps / 2; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kAll, M, o));
+        double S = wm0 > -INFINITY ? s_sum[lane] * (double)ex2((wm0 - M) * kLog2e) : 0.0;
+#pragma unroll
+        for (int o = kScanWarps / 2; o; o >>= 1) S += __shfl_xor_sync(kAll, S, o);
+        if (lane == 0) {
+            out.max[at] = M;
+            out.sum[at] = S;
+        }
     }
-    // each of the warps' entries finds its place among all of them
-    if (t < kScanWarps * k) {
-        const float v = s_val[t];
-        const int i = s_idx[t];
-        int rank = 0;
-        for (int j = 0; j < kScanWarps * k; ++j)
-            rank += better(s_val[j], s_idx[j], v, i) || (s_val[j] == v && s_idx[j] == i && j < t);
+    // each finds its place among all of them
+    const int count = s_count;
+    for (int e = t; e < max(count, k); e += kScanThreads) {
+        int rank = e;                   // fewer than k elements in the slice: no entry
+        float v = -INFINITY;
+        int i = INT_MAX;
+        if (e < count) {
+            v = s_val[e];
+            i = s_idx[e];
+            rank = 0;
+            for (int o = 0; o < count; ++o) rank += better(s_val[o], s_idx[o], v, i);
+        }
         if (rank < k) {
             out.val[at * k + rank] = v;
-            out.idx[at * k + rank] = i;     // INT_MAX: the slice has fewer than k elements
+            out.idx[at * k + rank] = i;
         }
     }
 }
@@ -226,20 +233,30 @@ beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float
     __shared__ float s_val[kPickWarps][kMaxSlices * kMaxBeams];
     __shared__ int s_idx[kPickWarps][kMaxSlices * kMaxBeams];
     __shared__ double s_lse[kMaxBeams];
+    __shared__ float s_score[kMaxBeams];
+    __shared__ int s_done[kMaxBeams];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const size_t row0 = (size_t)blockIdx.x * k;
     pdl_wait();
+    if (t < k) {
+        s_score[t] = scores[row0 + t];
+        s_done[t] = done && done[row0 + t] != 0;
+        p_total[t] = (double)-INFINITY;
+        p_beam[t] = t;
+        p_token[t] = 0;
+    }
     // two warps per beam, a lane per slice: one forms the logarithm of the sum of
-    // exponentials, the other merges the slices' lists
+    // exponentials, the other merges the slices' lists. (What a finished beam's
+    // rows hold is not used.)
     for (int b = warp & (kPickWarps - 1); b < k; b += kPickWarps) {
-        if (done && done[row0 + b] != 0) continue;
         const size_t at = (row0 + b) * slices + lane;
         if (warp >= kPickWarps) {
             const float m = lane < slices ? in.max[at] : -INFINITY;
+            const double part = lane < slices ? in.sum[at] : 0.0;
             float M = m;
 #pragma unroll
             for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kAll, M, o));
-            double S = m > -INFINITY ? in.sum[at] * (double)ex2((m - M) * kLog2e) : 0.0;
+            double S = m > -INFINITY ? part * (double)ex2((m - M) * kLog2e) : 0.0;
 #pragma unroll
             for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(kAll, S, o);
             // a row whose largest logit is infinite has no normaliser
@@ -252,23 +269,17 @@ beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float
         }
         __syncwarp();
         int head = 0;
-        float hv = lane < slices ? s_val[warp][lane * k] : -INFINITY;
+        unsigned key = lane < slices ? order_key(s_val[warp][lane * k]) : 0u;
         int hi = lane < slices ? s_idx[warp][lane * k] : INT_MAX;
         for (int r = 0; r < k; ++r) {
-            float v = hv;
-            int i = hi;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const float ov = __shfl_xor_sync(kAll, v, o);
-                const int oi = __shfl_xor_sync(kAll, i, o);
-                if (better(ov, oi, v, i)) { v = ov; i = oi; }
-            }
-            if (hi == i && hi != INT_MAX) {
+            const unsigned most = __reduce_max_sync(kAll, key);
+            const int first = (int)__reduce_min_sync(kAll, key == most ? (unsigned)hi : (unsigned)INT_MAX);
+            if (lane == 0) { s_best[b * k + r] = from_order_key(most); s_token[b * k + r] = first; }
+            if (key == most && hi == first && hi != INT_MAX) {
                 ++head;
-                hv = head < k ? s_val[warp][lane * k + head] : -INFINITY;
+                key = head < k ? order_key(s_val[warp][lane * k + head]) : 0u;
                 hi = head < k ? s_idx[warp][lane * k + head] : INT_MAX;
             }
-            if (lane == 0) { s_best[b * k + r] = v; s_token[b * k + r] = i; }
         }
         __syncwarp();
     }
@@ -276,10 +287,10 @@ beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float
     // the candidates' totals
     for (int c = t; c < k * k; c += kPickThreads) {
         const int b = c / k, r = c % k;
-        const float score = scores[row0 + b];
+        const float score = s_score[b];
         double total = (double)score;
         int token;
-        if (done && done[row0 + b] != 0) {
+        if (s_done[b]) {
             token = r == 0 ? eos : INT_MAX;
         } else if ((double)score - s_lse[b] > (double)-INFINITY) {
             token = s_token[c];
@@ -295,15 +306,18 @@ beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float
         s_flat[c] = (long long)b * vocab + token;
     }
     __syncthreads();
-    // each candidate finds its rank among all
-    for (int c = t; c < k * k; c += kPickThreads) {
+    // each finds its rank among all (there are always k), a warp for each
+    for (int c = warp; c < k * k; c += kPickThreads / 32) {
         const double v = s_total[c];
         if (v != v) continue;
         const long long flat = s_flat[c];
         int rank = 0;
-#pragma unroll 4
-        for (int o = 0; o < k * k; ++o) rank += s_total[o] > v || (s_total[o] == v && s_flat[o] < flat);
-        if (rank < k) {
+        for (int o0 = 0; o0 < k * k; o0 += 32) {
+            const int o = o0 + lane;
+            const bool ahead = o < k * k && (s_total[o] > v || (s_total[o] == v && s_flat[o] < flat));
+            rank += __popc(__ballot_sync(kAll, ahead));
+        }
+        if (lane == 0 && rank < k) {
             p_total[rank] = v;
             p_beam[rank] = c / k;
             p_token[rank] = s_token[c];
@@ -316,8 +330,7 @@ beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float
         const bool heir = __ffs((int)__match_any_sync(kAll, b)) - 1 == lane;
         const unsigned taken = __reduce_or_sync(kAll, lane < k ? 1u << b : 0u);
         const unsigned others = __ballot_sync(kAll, lane < k && !heir);
-        const bool was = lane < k && done && done[row0 + b] != 0;
-        __syncwarp();                                          // done_out may be done
+        const bool was = lane < k && s_done[b];
         if (lane < k) {
             unsigned left = ~taken;                         // the free places, lowest first
             for (int o = __popc(others & ((1u << lane) - 1)); o > 0; --o) left &= left - 1;
@@ -372,7 +385,7 @@ extern "C" model_status tie_beam_select(const float* logits, int ldl, const floa
     if (!shape_ok(n_req, beams, vocab) || ldl < vocab || eos_id >= vocab) return MODEL_ERR_ARG;
     if ((done || done_out) && eos_id < 0) return MODEL_ERR_ARG;
     if (!aligned16(workspace)) return MODEL_ERR_ARG;
-    if (beams > kMaxBeams || n_req > kOpsMaxSeqs) return MODEL_ERR_CAPACITY;
+    if (beams > kMaxBeams || n_req > kOpsMaxSeqs || vocab > kMaxVocab) return MODEL_ERR_CAPACITY;
     OnDeviceOf dev(next);
     if (dev.status() != MODEL_OK) return dev.status();
     const int slices = slices_of(n_req, beams, vocab, sm_count(dev.device()));
