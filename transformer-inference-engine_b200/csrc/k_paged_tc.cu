@@ -78,7 +78,7 @@ constexpr int kThreads = 640;
 // registers a thread: at launch, and after the warpgroups have shared them out
 // (softmax 2 x 128 threads, loaders 2 x 128, MMA 128); the sum must not pass
 // what the block was launched with
-constexpr int kRegsLaunch = 96, kRegsSoftmax = 120, kRegsLoad = 96, kRegsMma = 40;
+constexpr int kRegsLaunch = 96, kRegsSoftmax = 112, kRegsLoad = 104, kRegsMma = 48;
 static_assert(256 * kRegsSoftmax + 256 * kRegsLoad + 128 * kRegsMma <= kThreads * kRegsLaunch, "register split");
 constexpr int kSoftmaxWarps = 8, kLoadWarps = 8, kMmaWarp = 16, kUnitWarp = 17;
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s
@@ -130,6 +130,18 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
         "elect.sync _|one, 0xffffffff;\n\t"
         "@one tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 
 __device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t n) {
@@ -249,7 +261,7 @@ template <>
 struct Row8<false> {
     float x[8];
     __device__ __forceinline__ void load(const void* base, size_t at) {
-        asm volatile("ld.global.nc.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        asm volatile("ld.global.nc.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
                      : "l"(static_cast<const float*>(base) + at));
     }
@@ -284,7 +296,7 @@ template <>
 struct Row8<true> {
     uint32_t x[4];
     __device__ __forceinline__ void load(const void* base, size_t at) {
-        asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];"
+        asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
                      : "l"(static_cast<const __nv_bfloat16*>(base) + at));
     }
@@ -687,6 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
         }
     } else if (warp < kSoftmaxWarps + kLoadWarps) {
         // ------------------------------------------------------------ loaders
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
         const int lw = warp - kSoftmaxWarps, sub = lane >> 3, dl = lane & 7;
         Row8<BF16> kr[4], vr[4];
         // the rows of step j of the tile in ring entry `e` that this warp has: its
@@ -878,8 +891,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                     if (c.jobs) return true;
                 }
             };
+            // Whether all of the phases have completed, without waiting: the warp issues
+            // whatever is ready, the S of a later job or the P . V of an earlier one. (In
+            // a fixed order a P . V whose P has long been there waits behind an S whose
+            // keys are still on their way, and the loaders behind both.)
+            auto there = [&](const uint64_t* bar, uint32_t phase) { return mbar_test(smem_u32(bar), phase & 1u); };
             Cursor sc{}, pc{};
-            bool s_more = settle(sc), failed = false;
+            bool s_more = settle(sc), p_more = s_more && settle(pc);
             // S of the next job, into the buffer that the job three before has left
             auto issue_s = [&]() -> bool {
                 const volatile Unit& n = units[sc.un % kUnitRing];
@@ -887,9 +905,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                 const uint32_t f = (uint32_t)uniform(n.fill0) + (uint32_t)j, b = f & 1u, buf = sc.job % 3u;
                 const uint32_t half = (uint32_t)uniform(n.half0) + (sc.both ? (uint32_t)st : 0u);
                 const bool first = sc.both ? j == 0 : sc.k == 0, last = sc.both ? j == sc.steps - 1 : sc.k == sc.jobs - 1;
-                if (first && !wait_all(&q_full[half & 1u], half >> 1 & 1u)) return false;
-                if (!wait_all(&k_full[b], f >> 1 & 1u)) return false;
-                if (sc.job >= 3 && !wait_all(&o_done[buf], (sc.job / 3u - 1) & 1u)) return false;
+                if (!__all_sync(kAll, there(&k_full[b], f >> 1) && (!first || there(&q_full[half & 1u], half >> 1)) &&
+                                          (sc.job < 3 || there(&o_done[buf], sc.job / 3u - 1))))
+                    return false;
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 const uint32_t kb = sb + kOffK + b * 2 * kTermBytes, qb = sb + kOffQ + (half & 1u) * 2 * kTermBytes;
                 const uint32_t d = tm + buf * kTileKeys;
@@ -912,18 +930,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                 }
                 return true;
             };
-            bool p_more = s_more && settle(pc);
-            for (int k = 0; k < 3 && s_more && !failed; ++k) failed = !issue_s();
             uint32_t freed = 0;         // tiles whose description is no longer needed
-            while (p_more && !failed) {
+            auto issue_pv = [&]() -> bool {
                 const volatile Unit& n = units[pc.un % kUnitRing];
                 const int j = pc.k >> pc.both, st = pc.k & 1;
                 const uint32_t f = (uint32_t)uniform(n.fill0) + (uint32_t)j, b = f & 1u, buf = pc.job % 3u;
                 const bool first = pc.both ? j == 0 : pc.k < 2;
                 const bool last = pc.both ? j == pc.steps - 1 : pc.k + 2 >= pc.jobs;
-                if (!wait_all(&p_full[buf], pc.job / 3u & 1u) || !wait_all(&v_full[b], f >> 1 & 1u)) break;
-                // the tile before has left O
-                if (first && pc.un && !wait_all(&o_free[st], (pc.un - 1) & 1u)) break;
+                // (at the first job of a tile, the tile before has left O)
+                if (!__all_sync(kAll, there(&p_full[buf], pc.job / 3u) && there(&v_full[b], f >> 1) &&
+                                          (!first || !pc.un || there(&o_free[st], pc.un - 1))))
+                    return false;
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 const uint32_t vb = sb + kOffV + b * 2 * kTermBytes, p_col = tm + buf * kTileKeys, d = tm + kColO + 64u * st;
 #pragma unroll
@@ -945,7 +962,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                     p_more = settle(pc);
                     for (; freed < pc.un; ++freed) unit_read(freed);
                 }
-                if (s_more) failed = !issue_s();
+                return true;
+            };
+            unsigned long long since = globaltimer_ns();
+            for (uint32_t idle = 0; p_more;) {
+                bool some = false;
+                // (an S is at most three jobs ahead: the buffer's P . V has been issued)
+                if (s_more && sc.job < pc.job + 3u) some = issue_s();
+                if (sc.job > pc.job && issue_pv()) some = true;
+                if (some) {
+                    idle = 0;
+                } else if ((++idle & 63u) == 0) {
+                    if (__any_sync(kAll, *abort_flag != 0)) break;
+                    if (idle == 64) since = globaltimer_ns();
+                    if (__any_sync(kAll, globaltimer_ns() - since > kWaitLimitNs)) {
+                        *abort_flag = 1;
+                        if (a.status && lane == 0) atomicExch(a.status, (int)MODEL_ERR_DEVICE);
+                        break;
+                    }
+                }
             }
             for (; freed < pc.un; ++freed) unit_read(freed);
             // every MMA issued completes before TMEM is freed, also when cut short

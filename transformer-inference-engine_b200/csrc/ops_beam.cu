@@ -30,7 +30,6 @@ constexpr int kScanThreads = 256, kScanWarps = kScanThreads / 32;
 constexpr int kBatch = 8;              // elements a thread loads at a time
 constexpr int kScanResident = 8;       // CTAs per SM (64 KB of loads in flight)
 constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 64;   // pairs of warps
-constexpr int kWaves = 2;
 constexpr int kMaxVocab = 1 << 30;     // indices of a row stay in int32 with room for a step
 constexpr int kMaxSlices = 32;         // a lane of the picking warps for each
 constexpr unsigned kAll = 0xffffffffu;
@@ -344,13 +343,13 @@ beam_pick_kernel(Partials in, int slices, int k, int vocab, int eos, const float
     }
 }
 
-// Slices of the vocabulary per row: some waves of CTAs (one CTA's last steps run
-// beside another's loads), each of at least one load of its threads (2048
-// logits), at most a lane each of the warp that joins them.
+// Slices of the vocabulary per row: one wave of CTAs (576 rows of 50257: 37.5 us;
+// two, three and four waves 39.8, 42.3 and 44.8), each of at least one load of
+// its threads (2048 logits), at most a lane each of the warp that joins them.
 int slices_of(int n_req, int beams, int vocab, int sms) {
     const long long rows = (long long)n_req * beams;
     const int most = (vocab + kScanThreads * kBatch - 1) / (kScanThreads * kBatch);
-    long long n = (long long)kWaves * kScanResident * sms / rows;
+    long long n = (long long)kScanResident * sms / rows;
     if (n > most) n = most;
     if (n > kMaxSlices) n = kMaxSlices;
     return n < 1 ? 1 : (int)n;
