@@ -477,10 +477,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
             float m = -INFINITY, l = 0.f, qs = 0.f;
             bool ok = true;
             const int j0 = both ? 0 : st, dj = both ? 1 : 2;
+            // none of the warp's 32 rows exists: what P holds there reaches only rows of
+            // O that nobody reads
+            const bool idle = (both ? st * kHalfRows : 0) + qq * 32 >= n_rows;
 #pragma unroll 1
             for (int j = j0; j < steps; j += dj) {
                 const uint32_t f = fill0 + (uint32_t)j, job = job0 + (both ? 2u * j + st : (uint32_t)j), buf = job % 3u;
                 const uint32_t col_s = lanes + buf * kTileKeys;
+                if (idle) {
+                    if (!(ok = wait_all(&s_full[buf], job / 3u & 1u))) break;
+                    if (lane == 0) mbar_arrive(smem_u32(&p_full[buf]));
+                    continue;
+                }
                 ok = ok && wait_all(&v_full[f & 1u], f >> 1 & 1u);
                 ok = ok && wait_all(&s_full[buf], job / 3u & 1u);
                 if (!ok) break;
@@ -702,24 +710,27 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
         const int lw = warp - kSoftmaxWarps, sub = lane >> 3, dl = lane & 7;
         Row8<BF16> kr[4], vr[4];
-        // the rows of step j of the tile in ring entry `e` that this warp has: its
-        // page (or -1), and their loads
+        // the rows of step j of a tile that this warp has: its page (or -1), and their
+        // loads. All 16 rows of a page are read (page 0's for none) and what is not
+        // there is cleared afterwards: a branch at each load costs more than the rest.
         auto page_of = [&](const volatile Unit& n, int j) {
             const int p = (n.key0 + j * kTileKeys) / kPageRows + lw;
             if (j >= n.steps || (long long)p * kPageRows >= n.key1) return -1;
             const int e = __ldg(a.table + (size_t)n.s * a.width + p);
             return e >= 0 && e < a.n_pages ? e : -1;
         };
-        auto load = [&](Row8<BF16>(&rows)[4], const void* from, const volatile Unit& n, int j, int page) {
-            const int pos = n.key0 + j * kTileKeys + lw * kPageRows, key1 = n.key1, g = n.g;
+        const size_t lane_at = (size_t)sub * w + 8 * dl;
+        auto load = [&](Row8<BF16>(&rows)[4], const void* from, int g, int page) {
+            const size_t at = (size_t)max(page, 0) * (kPageRows * w) + g * kHeadDim + lane_at;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 4 * i + sub;
-                if (page >= 0 && pos + row < key1)
-                    rows[i].load(from, ((size_t)page * kPageRows + row) * w + g * kHeadDim + 8 * dl);
-                else
-                    rows[i].zero();
-            }
+            for (int i = 0; i < 4; ++i) rows[i].load(from, at + (size_t)(4 * i) * w);
+        };
+        // there: positions of the page that are (all of them: 16 or more)
+        auto clear = [&](Row8<BF16>(&rows)[4], int there) {
+            if (there >= kPageRows) return;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (4 * i + sub >= there) rows[i].zero();
         };
         // stores this warp's 16 rows as terms; mx: what each row (in all its lanes) is scaled by
         auto store = [&](uint8_t* to, const auto (&rows)[4], const float (&mx)[4], int lo, auto is_bf16) {
@@ -749,8 +760,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
         int page = -1, page_next = -1;
         if (ok && units[0].steps > 0) {
             page = page_of(units[0], 0);
-            load(kr, a.k, units[0], 0, page);
-            load(vr, a.v, units[0], 0, page);
+            load(kr, a.k, units[0].g, page);
+            load(vr, a.v, units[0].g, page);
         }
         for (uint32_t un = 0; ok; ++un) {
             volatile Unit& n = units[un % kUnitRing];
@@ -793,7 +804,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
 #pragma unroll 1
             for (int j = 0; j < steps && ok; ++j) {
                 const uint32_t f = (uint32_t)n.fill0 + (uint32_t)j, b = f & 1u, before = ((f >> 1) - 1) & 1u;
-                const int pos = n.key0 + j * kTileKeys + lw * kPageRows;
+                const int there = page < 0 ? 0 : n.key1 - (n.key0 + j * kTileKeys + lw * kPageRows);
                 const bool diagonal = n.key0 + j * kTileKeys + kTileKeys - 1 > n.first_last;
                 float* keys = s_keys + (f % kKeyRing) * 3 * kTileKeys;
                 // largest magnitudes: of each row, or of the page in every entry
@@ -806,6 +817,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                     }
                 };
                 float mx[4];
+                clear(kr, there);
                 row_max(kr, mx);
                 spread(mx);
                 // key buffer b is free once the S of the step before last are computed
@@ -819,14 +831,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                 // the next step's rows, of this tile or the next one
                 const bool over = j + 1 == steps;
                 const volatile Unit* nn = &n;
-                int jn = j + 1;
                 if (over) {
                     if (!(ok = unit_there(un + 1))) break;
                     nn = &units[(un + 1) % kUnitRing];
-                    jn = 0;
                     page_next = nn->steps > 0 ? page_of(*nn, 0) : -1;
                 }
-                if (nn->steps > 0) load(kr, a.k, *nn, jn, page_next);
+                const int gn = nn->steps > 0 ? nn->g : -1;
+                if (gn >= 0) load(kr, a.k, gn, page_next);
+                clear(vr, there);
                 row_max(vr, mx);
                 spread(mx);
                 if (__any_sync(kAll, !(mx[0] < INFINITY && mx[1] < INFINITY && mx[2] < INFINITY && mx[3] < INFINITY))) {
@@ -844,12 +856,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                 for (int i = 0; i < 4; ++i)
                     if (diagonal ? dl == 0 : i == 0 && lane == 0) {
                         const int at = diagonal ? lw * kPageRows + 4 * i + sub : lw, e = row_exponent(mx[i], 60);
-                        const bool there = page >= 0 && pos + 4 * i + sub < n.key1;
-                        keys[kTileKeys + at] = there ? (float)(e - 141) : -INFINITY;
+                        keys[kTileKeys + at] = (diagonal ? 4 * i + sub : 0) < there ? (float)(e - 141) : -INFINITY;
                         keys[2 * kTileKeys + at] = pow2_biased(268 - e);
                     }
                 arrive(&v_full[b]);
-                if (nn->steps > 0) load(vr, a.v, *nn, jn, page_next);
+                if (gn >= 0) load(vr, a.v, gn, page_next);
                 page = page_next;
                 page_next = over ? -1 : page_of(n, j + 2);
             }
@@ -861,8 +872,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                 const volatile Unit& x = units[(un + 1) % kUnitRing];
                 if (x.steps > 0) {
                     page = page_of(x, 0);
-                    load(kr, a.k, x, 0, page);
-                    load(vr, a.v, x, 0, page);
+                    load(kr, a.k, x.g, page);
+                    load(vr, a.v, x.g, page);
                 }
             }
         }
