@@ -13,6 +13,7 @@
 // read once through the page table.
 #include "paged_attn.cuh"
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include <climits>
@@ -20,6 +21,8 @@
 
 namespace tie {
 namespace {
+
+namespace cg = cooperative_groups;
 
 // ------------------------------------------------------- few rows: streaming --
 // Bound by the reading of K and V. A CTA of 8 warps per unit; warp w takes the
@@ -50,11 +53,12 @@ struct FewSmem {
     float o[kFewWarps][kFewRows][kHeadDim];
 };
 
-// The pages [p0, p1) of sequence s for rows tile * kFewRows .. + R - 1 (n_rows
-// of them real) of K/V head g; leaves each warp's partial in `sm`.
+// Every `stride`-th page of [p0 + warp, p1) of sequence s for rows tile *
+// kFewRows .. + R - 1 (n_rows of them real) of K/V head g; leaves each warp's
+// partial in `sm`.
 template <int R, bool BF16>
 __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const SeqShape& q, int s, int tile, int g, int p0,
-                                         int p1, int n_rows, FewSmem* sm) {
+                                         int p1, int stride, int n_rows, FewSmem* sm) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, half = lane >> 4, dl = lane & 15;
     float qv[R][4], o[R][4], m[R], l[R];
     int last[R];                       // the last position each row sees
@@ -73,9 +77,9 @@ __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const SeqShape&
     const int32_t* table = a.table + (size_t)s * a.width;
     const int own = 2 * ((dl >> 3 & 1) * 4 + (dl >> 2 & 1) * 2 + (dl >> 1 & 1)) + half;   // this lane's position of a page
     int page = p0 + warp < p1 ? __ldg(table + p0 + warp) : -1;
-    for (int p = p0 + warp; p < p1; p += kFewWarps) {
+    for (int p = p0 + warp; p < p1; p += stride) {
         const int cur = page;
-        if (p + kFewWarps < p1) page = __ldg(table + p + kFewWarps);
+        if (p + stride < p1) page = __ldg(table + p + stride);
         if (cur < 0 || cur >= a.n_pages) continue;         // an unmapped page holds no positions
         const size_t at = ((size_t)cur * kPageRows + half) * w + g * kHeadDim + 4 * dl;
         float4 kk[8], vv[8];
@@ -137,6 +141,84 @@ __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const SeqShape&
     }
 }
 
+// the same for as many rows as there are, at most RMAX
+template <int RMAX, bool BF16>
+__device__ __forceinline__ void few_rows_n(const PagedAttnArgs& a, const SeqShape& q, int s, int tile, int g, int p0,
+                                           int p1, int stride, int n_rows, FewSmem* sm) {
+    if (RMAX == 1 || n_rows == 1) few_rows<1, BF16>(a, q, s, tile, g, p0, p1, stride, n_rows, sm);
+    else if (RMAX == 2 || n_rows == 2) few_rows<(RMAX < 2 ? RMAX : 2), BF16>(a, q, s, tile, g, p0, p1, stride, n_rows, sm);
+    else if (RMAX == 4 || n_rows <= 4) few_rows<(RMAX < 4 ? RMAX : 4), BF16>(a, q, s, tile, g, p0, p1, stride, n_rows, sm);
+    else few_rows<RMAX, BF16>(a, q, s, tile, g, p0, p1, stride, n_rows, sm);
+}
+
+// Row r, dim d of the warps' partials joined.
+struct Joined {
+    float m, l, o;
+};
+__device__ __forceinline__ Joined join_warps(const FewSmem& sm, int r, int d) {
+    Joined j{sm.m[0][r], 0.f, 0.f};
+#pragma unroll
+    for (int w = 1; w < kFewWarps; ++w) j.m = fmaxf(j.m, sm.m[w][r]);
+    const float base = j.m == -INFINITY ? 0.f : j.m;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+        const float f = ex2_ftz(sm.m[w][r] - base);
+        j.l = fmaf(sm.l[w][r], f, j.l);
+        if (f > 0.f) j.o = fmaf(sm.o[w][r][d], f, j.o);
+    }
+    return j;
+}
+
+// Every sequence of the batch has few rows: a cluster of CTAs per (sequence,
+// K/V head), no schedule, no partials in memory and no second launch. The CTAs
+// take the sequence's pages 8 by 8 in turn and join through each other's shared
+// memory. The hardware hands the clusters out as SMs come free, which balances
+// ragged batches better than equal shares (256 sequences of up to 1000
+// positions: 143.7 us with few_rows_kernel, see tie_attention_paged for the
+// choice).
+template <int RMAX, bool BF16>
+__global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_cluster_kernel(PagedAttnArgs a, int ctas) {
+    __shared__ __align__(16) FewSmem sm;
+    __shared__ float c_m[kFewRows], c_l[kFewRows], c_o[kFewRows][kHeadDim];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int unit = blockIdx.x / ctas, rank = blockIdx.x % ctas, t = threadIdx.x;
+    const int g = unit % a.n_kv_head, s = unit / a.n_kv_head;
+    const SeqShape q = seq_shape(a, s);
+    if (!q.rows) return;               // the whole cluster
+    few_rows_n<RMAX, BF16>(a, q, s, 0, g, rank * kFewWarps, pages_of(q), ctas * kFewWarps, q.rows, &sm);
+    __syncthreads();
+    auto out_at = [&](int r, int d) -> float& {
+        return a.out[(size_t)(q.row0 + r / a.group) * a.ldo + (g * a.group + r % a.group) * kHeadDim + d];
+    };
+    for (int e = t; e < q.rows * kHeadDim; e += kFewThreads) {
+        const int r = e / kHeadDim, d = e % kHeadDim;
+        const Joined j = join_warps(sm, r, d);
+        if (ctas == 1) {
+            out_at(r, d) = j.l == 0.f ? 0.f : j.o / j.l;
+        } else {
+            c_o[r][d] = j.o;
+            if (d == 0) { c_m[r] = j.m; c_l[r] = j.l; }
+        }
+    }
+    if (ctas == 1) return;
+    cluster.sync();
+    for (int e = rank * kFewThreads + t; e < q.rows * kHeadDim; e += ctas * kFewThreads) {
+        const int r = e / kHeadDim, d = e % kHeadDim;
+        float mx = -INFINITY;
+        for (int c = 0; c < ctas; ++c) mx = fmaxf(mx, *cluster.map_shared_rank(&c_m[r], c));
+        const float base = mx == -INFINITY ? 0.f : mx;
+        float l = 0.f, o = 0.f;
+        for (int c = 0; c < ctas; ++c) {
+            const float f = ex2_ftz(*cluster.map_shared_rank(&c_m[r], c) - base);
+            l = fmaf(*cluster.map_shared_rank(&c_l[r], c), f, l);
+            const float v = *cluster.map_shared_rank(&c_o[r][d], c);
+            if (f > 0.f) o = fmaf(v, f, o);
+        }
+        out_at(r, d) = l == 0.f ? 0.f : o / l;
+    }
+    cluster.sync();                    // the others have read this CTA's shared memory
+}
+
 template <int RMAX, bool BF16>
 __global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_rows_kernel(PagedAttnArgs a) {
     pdl_trigger();
@@ -156,24 +238,11 @@ __global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_rows_kerne
         // the tile's last row bounds its keys
         const int keys = q.ctx + (tile * kFewRows + n_rows - 1) / a.group + 1;
         const int p0 = split * sch.chunk, p1 = min(p0 + sch.chunk, (keys + kPageRows - 1) / kPageRows);
-        if (RMAX == 1 || n_rows == 1) few_rows<1, BF16>(a, q, s, tile, g, p0, p1, n_rows, &sm);
-        else if (RMAX == 2 || n_rows == 2) few_rows<(RMAX < 2 ? RMAX : 2), BF16>(a, q, s, tile, g, p0, p1, n_rows, &sm);
-        else if (RMAX == 4 || n_rows <= 4) few_rows<(RMAX < 4 ? RMAX : 4), BF16>(a, q, s, tile, g, p0, p1, n_rows, &sm);
-        else few_rows<RMAX, BF16>(a, q, s, tile, g, p0, p1, n_rows, &sm);
+        few_rows_n<RMAX, BF16>(a, q, s, tile, g, p0, p1, kFewWarps, n_rows, &sm);
         __syncthreads();
         for (int e = t; e < n_rows * kHeadDim; e += kFewThreads) {
             const int r = e / kHeadDim, d = e % kHeadDim;
-            float mx = sm.m[0][r];
-#pragma unroll
-            for (int w = 1; w < kFewWarps; ++w) mx = fmaxf(mx, sm.m[w][r]);
-            const float base = mx == -INFINITY ? 0.f : mx;
-            float l = 0.f, o = 0.f;
-#pragma unroll
-            for (int w = 0; w < kFewWarps; ++w) {
-                const float f = ex2_ftz(sm.m[w][r] - base);
-                l = fmaf(sm.l[w][r], f, l);
-                if (f > 0.f) o = fmaf(sm.o[w][r][d], f, o);
-            }
+            const auto [mx, l, o] = join_warps(sm, r, d);
             if (sp == 1) {
                 const int i = tile * kFewRows + r;
                 a.out[(size_t)(q.row0 + i / a.group) * a.ldo + (g * a.group + i % a.group) * kHeadDim + d] =
@@ -259,6 +328,39 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(PagedAttnArgs a) {
     }
 }
 
+// CTAs per (sequence, K/V head) of few_cluster_kernel: as many as fit about four
+// per SM, at most a portable cluster. 0 where a warp may then have more than 16
+// pages (16,384 positions and more of one or two K/V heads): equal shares of the
+// keys over all SMs, joined by a second kernel, are faster there.
+int cluster_ctas(int n_seq, int n_kv_head, int pages_per_seq, int sms) {
+    const long long units = (long long)n_seq * n_kv_head;
+    int ctas = 1;
+    while (ctas < 8 && 2 * ctas * units <= 4LL * sms && ctas * kFewWarps < pages_per_seq) ctas *= 2;
+    const bool fills = units * ctas >= 2LL * sms;
+    return fills || pages_per_seq <= 16 * kFewWarps * ctas ? ctas : 0;
+}
+
+cudaError_t launch_few_cluster(const PagedAttnArgs& a, bool bf16, int rows, int ctas, cudaStream_t st) {
+    void (*kernel)(PagedAttnArgs, int) = nullptr;
+    if (bf16)
+        kernel = rows <= 1 ? few_cluster_kernel<1, true> : rows <= 2 ? few_cluster_kernel<2, true>
+                 : rows <= 4 ? few_cluster_kernel<4, true> : few_cluster_kernel<8, true>;
+    else
+        kernel = rows <= 1 ? few_cluster_kernel<1, false> : rows <= 2 ? few_cluster_kernel<2, false>
+                 : rows <= 4 ? few_cluster_kernel<4, false> : few_cluster_kernel<8, false>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.n_seq * a.n_kv_head * ctas));
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a, ctas);
+}
+
 // Streaming units aimed at when sequences are split: four per SM (two CTAs
 // resident). A split sequence has more pages than a chunk, so its units number
 // at most twice its pages over the chunk: all partials fit 2 x target units.
@@ -328,6 +430,13 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
     const long long most = (long long)max_new * a.group;      // rows of one sequence and K/V head
     a.only_few = most <= kFewRows;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a.only_few) {
+        const int ctas = cluster_ctas(n_seq, n_kv_head, pages_per_seq, sms);
+        if (ctas > 0) {
+            TIE_OP_CU(launch_few_cluster(a, bf16, (int)most, ctas, st));
+            return MODEL_OK;
+        }
+    }
     const size_t smem = (size_t)(n_seq + 1) * sizeof(long long);
     if (!a.only_few) TIE_OP_CU(launch_paged_attn_tc(a, bf16, st));
     if (a.group <= kFewRows) {
