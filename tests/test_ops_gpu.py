@@ -209,9 +209,19 @@ def test_attention_chunks_and_mixed(kv, heads, kv_heads, ctx, new):
 
 
 @pytest.mark.parametrize("kv", KV)
-@pytest.mark.parametrize("ctx,new", [([5000], [1]), ([4097], [3]), ([3900], [70])])
+@pytest.mark.parametrize("ctx,new", [
+    ([5000], [1]), ([4097], [3]), ([3900], [70]), ([17000], [1]), ([20011], [4]), ([30, 17500, 0, 9000], [1, 2, 1, 3]),
+    ([5000, 8, 2100], [2, 30, 1]), ([9000], [12])])
 def test_attention_long_contexts_split(kv, ctx, new):
     _check_attention(_batch(np.random.default_rng(7), ctx, new, 2, 1, kv))
+
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("n_seq", [40, 300])
+def test_attention_of_many_sequences(kv, n_seq):
+    """Batches that fill the GPU with one and two CTAs per sequence and head."""
+    rng = np.random.default_rng(n_seq)
+    _check_attention(_batch(rng, rng.integers(0, 300, n_seq).tolist(), rng.integers(0, 3, n_seq).tolist(), 4, 4, kv))
 
 
 @pytest.mark.parametrize("scale", [0.125, 0.01, -0.3, 0.0, 1.0])

@@ -173,9 +173,9 @@ __device__ __forceinline__ Joined join_warps(const FewSmem& sm, int r, int d) {
 // K/V head), no schedule, no partials in memory and no second launch. The CTAs
 // take the sequence's pages 8 by 8 in turn and join through each other's shared
 // memory. The hardware hands the clusters out as SMs come free, which balances
-// ragged batches better than equal shares (256 sequences of up to 1000
-// positions: 143.7 us with few_rows_kernel, see tie_attention_paged for the
-// choice).
+// ragged batches better than equal shares: 256 sequences of up to 1000 positions,
+// 12 heads, fp32 take 127 us (6.2 TB/s, 95 % of the measured copy rate) against
+// 144 us with few_rows_kernel (cluster_ctas has the choice between them).
 template <int RMAX, bool BF16>
 __global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_cluster_kernel(PagedAttnArgs a, int ctas) {
     __shared__ __align__(16) FewSmem sm;
@@ -271,13 +271,21 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs& a, int kind, int p
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, o));
     const float base = mx == -INFINITY ? 0.f : mx;
     float l = 0.f, ox = 0.f, oy = 0.f;
-    for (int k = 0; k < parts; ++k) {
-        const size_t at = row_at(k);
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml[kind] + 2 * at);
-        const float f = ex2_ftz(ml.x - base);
-        const float2 v = *reinterpret_cast<const float2*>(a.part_o[kind] + at * kHeadDim + 2 * lane);
-        l = fmaf(ml.y, f, l);
-        if (f > 0.f) { ox = fmaf(v.x, f, ox); oy = fmaf(v.y, f, oy); }
+    constexpr int kAhead = 8;          // parts on their way at a time
+    for (int k0 = 0; k0 < parts; k0 += kAhead) {
+        float2 ml[kAhead], v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const size_t at = row_at(min(k0 + u, parts - 1));
+            ml[u] = *reinterpret_cast<const float2*>(a.part_ml[kind] + 2 * at);
+            v[u] = *reinterpret_cast<const float2*>(a.part_o[kind] + at * kHeadDim + 2 * lane);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const float f = k0 + u < parts ? ex2_ftz(ml[u].x - base) : 0.f;
+            l = fmaf(ml[u].y, f, l);
+            if (f > 0.f) { ox = fmaf(v[u].x, f, ox); oy = fmaf(v[u].y, f, oy); }
+        }
     }
     *reinterpret_cast<float2*>(out + 2 * lane) = l == 0.f ? make_float2(0.f, 0.f) : make_float2(ox / l, oy / l);
 }
@@ -329,15 +337,21 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(PagedAttnArgs a) {
 }
 
 // CTAs per (sequence, K/V head) of few_cluster_kernel: as many as fit about four
-// per SM, at most a portable cluster. 0 where a warp may then have more than 16
-// pages (16,384 positions and more of one or two K/V heads): equal shares of the
-// keys over all SMs, joined by a second kernel, are faster there.
+// per SM, at most a portable cluster; 0 for few_rows_kernel, which shares the
+// keys out evenly over all SMs and joins with a second kernel. The tables' width
+// bounds the contexts; a warp of the cluster has width / (8 x CTAs) pages at
+// most. One sequence, one K/V head, bf16, on the GPU alone (cluster / shared
+// out): 1000 positions 5.1 / 11.4 us, 4000 7.1 / 11.9, 16,000 (15.6 pages a
+// warp) 15.7 / 14.8, 32,000 27.3 / 19.5; 12 heads: 16,000 17.2 / 22.2, 32,000
+// 39.7 / 35.4. Where the clusters fill the GPU (16 sequences of 12 heads, 4000
+// positions: 33.5 / 45.8) longer contexts are worth it too, up to where one long
+// sequence among short ones would be left to a single cluster.
 int cluster_ctas(int n_seq, int n_kv_head, int pages_per_seq, int sms) {
     const long long units = (long long)n_seq * n_kv_head;
     int ctas = 1;
     while (ctas < 8 && 2 * ctas * units <= 4LL * sms && ctas * kFewWarps < pages_per_seq) ctas *= 2;
     const bool fills = units * ctas >= 2LL * sms;
-    return fills || pages_per_seq <= 16 * kFewWarps * ctas ? ctas : 0;
+    return pages_per_seq <= (fills ? 64 : 16) * kFewWarps * ctas ? ctas : 0;
 }
 
 cudaError_t launch_few_cluster(const PagedAttnArgs& a, bool bf16, int rows, int ctas, cudaStream_t st) {

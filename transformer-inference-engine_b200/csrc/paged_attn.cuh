@@ -50,9 +50,9 @@ struct PagedAttnArgs {
 };
 
 __host__ __device__ inline int tile_rows_of(int kind) { return kind ? kTileRows : kFewRows; }
-// fewest pages worth a streaming unit of their own (one for each warp), fewest
+// fewest pages worth a streaming unit of their own (four for each warp), fewest
 // jobs worth a tensor-core CTA
-constexpr int kMinUnitPages = 8, kMinJobs = 2;
+constexpr int kMinUnitPages = 32, kMinJobs = 2;
 
 // One sequence as the schedule sees it; rows == 0 for one to leave alone
 // (no new tokens, or lengths outside the caller's bounds).
