@@ -105,6 +105,31 @@ model_status model_generate_greedy(model *m, const int32_t *prompts, size_t n_se
 model_status model_generate_greedy_device(model *m, const int32_t *d_prompts, size_t n_seq,
                                           size_t n_prompt, size_t n_new, int32_t *d_out_ids);
 
+/* Appends n_ids tokens to each of the pool's sequences 0 .. n_seq - 1 behind
+ * the positions it holds (ids: host, n_seq * n_ids, row-major): a prompt in
+ * pieces, the next turn of a conversation, tokens to be scored. The new tokens
+ * attend to everything cached and to one another, causally; their keys and
+ * values go into the pool and its length grows by n_ids. As for
+ * model_prefill_batch, logits_out (host, n_seq * n_ids * vocab floats, or NULL)
+ * receives the new positions' logits and next_ids (host, n_seq, or NULL) each
+ * sequence's greedy choice at its last position. Attention statistics
+ * (model_collect_attn_stats) do not cover this call. */
+model_status model_extend_batch(model *m, const int32_t *ids, size_t n_seq, size_t n_ids,
+                                float *logits_out, size_t logits_cap, int32_t *next_ids);
+
+/* Beam search: for each of n_req prompts of n_prompt tokens (host, n_req *
+ * n_prompt) the `beams` (<= 16) continuations of n_new tokens that one beam
+ * search step after the other keeps (tie_beam_select: largest sum of log
+ * probabilities, ties to the lowest beam and token). A continuation that has
+ * produced eos_id is kept with its score, filled up with eos_id; eos_id < 0:
+ * none. out_ids (host, n_req * beams * n_new) and out_scores (host, n_req *
+ * beams): each request's continuations, best first. Requires a prior
+ * model_batch_reserve covering n_req * beams sequences of n_prompt + n_new - 1
+ * positions; the pool then holds the beams in no particular order. */
+model_status model_generate_beam(model *m, const int32_t *prompts, size_t n_req, size_t n_prompt,
+                                 size_t beams, size_t n_new, int32_t eos_id, int32_t *out_ids,
+                                 float *out_scores);
+
 /* ---- diagnostics --------------------------------------------------------
  * Times `iters` back-to-back launches of one kernel of the forward pass, alone,
  * on the model's stream with CUDA events, and stores the average milliseconds

@@ -245,6 +245,12 @@ struct model {
     kv_cache* pool = nullptr;
     std::map<GraphKey, GraphEntry> graphs;
 
+    // the operators over the paged pool (model_extend_batch, model_generate_beam):
+    // their small arrays and their workspace
+    size_t ops_cap = 0, ops_ws_cap = 0;
+    int32_t* d_ops = nullptr;
+    unsigned char* d_ops_ws = nullptr;
+
     // the persistent decode step (k_step.cu)
     int step_kind = TIE_STEP_CHAINED;
     StepLayer* d_step_layers = nullptr;
@@ -271,6 +277,8 @@ thread_local char g_dev_err[256] = "";
 }  // namespace
 
 namespace tie {
+thread_local uint64_t op_launches = 0;
+
 void note_device_error(cudaError_t e, const char* what, const char* file, int line) {
     const char* base = std::strrchr(file, '/');
     std::snprintf(g_dev_err, sizeof g_dev_err, "%s (%s) at %s:%d: %s", cudaGetErrorName(e), cudaGetErrorString(e),
@@ -288,6 +296,15 @@ void note_cuda(cudaError_t e, const char* what, int line) { note_device_error(e,
     do {                                                           \
         cudaError_t e_ = (expr);                                   \
         if (e_ != cudaSuccess) { note_cuda(e_, #expr, __LINE__); cudaGetLastError(); return MODEL_ERR_DEVICE; } \
+    } while (0)
+
+// an operator of tie_b200.h: its status, and the kernels it launched
+#define OP(expr)                                                   \
+    do {                                                           \
+        const uint64_t before_ = op_launches;                      \
+        model_status s_ = (expr);                                  \
+        m->launches += op_launches - before_;                      \
+        if (s_ != MODEL_OK) return s_;                             \
     } while (0)
 
 #define LAUNCH(expr)                                               \
@@ -456,10 +473,33 @@ model_status stats_end(model* m) {
 }
 
 // --------------------------------------------------------- forward passes --
+// New tokens of the pool's sequences behind positions that are cached: what the
+// layers of run_prefill need to store and attend through the page table.
+struct PagedChunk {
+    int pos0;                                    // positions cached in every sequence
+    const int32_t *ctx, *row_start, *slots;      // device: n_seq, n_seq + 1, n_seq * T
+};
+
+// Stores the layer's new keys and values and attends over all of them: out (fp32)
+// and its tf32 split.
+model_status attend_paged(model* m, const kv_cache* c, int layer, const PagedChunk& p, int n_seq, int T) {
+    const int E = m->cfg.n_embd, H = m->cfg.n_head, R = n_seq * T, n_pages = (int)(c->rows / kPageRows);
+    const PagedKV kv = layer_view(c, layer);
+    OP(tie_kv_store(m->qkv + E, m->qkv + 2 * E, 3 * E, p.slots, R, kv.k, kv.v, TIE_KV_F32, n_pages, H, m->st));
+    OP(tie_attention_paged(m->qkv, 3 * E, H, kv.k, kv.v, TIE_KV_F32, n_pages, H, kv.page_table, kv.pages_per_seq,
+                           p.row_start, p.ctx, n_seq, T, R, (float)(1.0 / std::sqrt((double)(E / H))), m->attn, E,
+                           m->d_ops_ws, m->ops_ws_cap, m->d_err, m->st));
+    LAUNCH(launch_split_hilo(m->attn, m->attn_hi, m->attn_lo, (long long)R * E, m->st));
+    return MODEL_OK;
+}
+
 // Prefill of n_seq sequences of T tokens whose ids are in m->d_ids; leaves
 // LN_f(x) in m->xb. Keys and values go to `cache` when it is non-NULL
 // (sequences first_seq..).                                   model.c:647-763
-model_status run_prefill(model* m, int n_seq, int T, kv_cache* cache, int first_seq) {
+// With `chunk` the tokens follow positions that the pool already holds
+// (sequences 0..), which they attend to as well.
+model_status run_prefill(model* m, int n_seq, int T, kv_cache* cache, int first_seq,
+                         const PagedChunk* chunk = nullptr) {
     const int E = m->cfg.n_embd, H = m->cfg.n_head, R = n_seq * T;
     const float eps = m->cfg.layer_norm_epsilon;
     cudaStream_t st = m->st;
@@ -467,15 +507,20 @@ model_status run_prefill(model* m, int n_seq, int T, kv_cache* cache, int first_
     const Mat xb{nullptr, m->xb_hi, m->xb_lo}, attn{nullptr, m->attn_hi, m->attn_lo};
     const Mat ff{nullptr, m->ff_hi, m->ff_lo};
     model_status rc;
-    LAUNCH(launch_embed_prefill(m->d_ids, R, T, m->wte, m->wpe, m->x, E, m->cfg.vocab_size, st));
+    const size_t pos0 = chunk ? (size_t)chunk->pos0 : 0;
+    LAUNCH(launch_embed_prefill(m->d_ids, R, T, m->wte, m->wpe + pos0 * E, m->x, E, m->cfg.vocab_size, st));
     for (int l = 0; l < m->cfg.n_layer; ++l) {
         const Layer& w = m->layers[l];
         LAUNCH(launch_layernorm(m->x, w.ln1_w, w.ln1_b, nullptr, R, E, eps, st, m->xb_hi, m->xb_lo));
         if ((rc = matmul(m, false, R, xb, E, Mat{w.qkv_w, w.qkv_hi, w.qkv_lo}, 3 * E, E, w.qkv_b, EPI_BIAS,
                          m->qkv, nullptr, nullptr, 3 * E)) != MODEL_OK)
             return rc;
-        if (cache) LAUNCH(launch_kv_store_prefill(m->qkv, n_seq, T, layer_view(cache, l), first_seq, st));
-        LAUNCH(launch_attn_prefill(m->qkv, n_seq, T, H, nullptr, stats, st, m->attn_hi, m->attn_lo, m->d_err));
+        if (chunk) {
+            if ((rc = attend_paged(m, cache, l, *chunk, n_seq, T)) != MODEL_OK) return rc;
+        } else {
+            if (cache) LAUNCH(launch_kv_store_prefill(m->qkv, n_seq, T, layer_view(cache, l), first_seq, st));
+            LAUNCH(launch_attn_prefill(m->qkv, n_seq, T, H, nullptr, stats, st, m->attn_hi, m->attn_lo, m->d_err));
+        }
         if ((rc = matmul(m, false, R, attn, E, Mat{w.proj_w, w.proj_hi, w.proj_lo}, E, E, w.proj_b,
                          EPI_BIAS_RESID, m->x, nullptr, nullptr, E)) != MODEL_OK)
             return rc;
@@ -1244,6 +1289,8 @@ void model_free(model* m) {
     if (!m) return;
     if (m->st) cudaStreamSynchronize(m->st);
     drop_graphs(m);
+    cudaFree(m->d_ops);
+    cudaFree(m->d_ops_ws);
     cudaFree(m->d_weights);
     cudaFree(m->d_split);
     cudaFree(m->x);  // the activation block (x, xb, qkv, attn, ff and their splits)
@@ -1537,17 +1584,11 @@ size_t model_batch_free_pages(const model* m) {
     return m && m->pool ? (size_t)m->pool->pages.free_pages() : 0;
 }
 
-static model_status batch_prefill_impl(model* m, size_t n_seq, size_t T, float* logits_host,
-                                       int32_t* next_host, bool host_ids, const int32_t* ids) {
+// The head and the greedy choices of n_seq x T rows of LN_f(x): all logits to the
+// host, or the last positions' alone.
+static model_status prefill_logits(model* m, size_t n_seq, size_t T, float* logits_host) {
     const int V = m->cfg.vocab_size;
     model_status rc;
-    if (host_ids) {
-        if ((rc = copy_ids_to_device(m, ids, n_seq * T)) != MODEL_OK) return rc;
-    } else {
-        CU(cudaMemcpyAsync(m->d_ids, ids, n_seq * T * sizeof(int32_t), cudaMemcpyDeviceToDevice, m->st));
-    }
-    if ((rc = map_pages(m, n_seq, T)) != MODEL_OK) return rc;
-    if ((rc = run_prefill(m, (int)n_seq, (int)T, m->pool, 0)) != MODEL_OK) return rc;
     if (logits_host) {
         if ((rc = ensure_logits(m, n_seq * T)) != MODEL_OK) return rc;
         if ((rc = prefill_head(m, (int)(n_seq * T), 0, 1)) != MODEL_OK) return rc;
@@ -1559,8 +1600,21 @@ static model_status batch_prefill_impl(model* m, size_t n_seq, size_t T, float* 
         if ((rc = prefill_head(m, (int)n_seq, T - 1, (int)T)) != MODEL_OK) return rc;
         LAUNCH(launch_argmax_rows(m->logits, V, (int)n_seq, V, 1, 0, m->d_next, m->st));
     }
-    (void)next_host;
     return MODEL_OK;
+}
+
+static model_status batch_prefill_impl(model* m, size_t n_seq, size_t T, float* logits_host,
+                                       int32_t* next_host, bool host_ids, const int32_t* ids) {
+    model_status rc;
+    if (host_ids) {
+        if ((rc = copy_ids_to_device(m, ids, n_seq * T)) != MODEL_OK) return rc;
+    } else {
+        CU(cudaMemcpyAsync(m->d_ids, ids, n_seq * T * sizeof(int32_t), cudaMemcpyDeviceToDevice, m->st));
+    }
+    if ((rc = map_pages(m, n_seq, T)) != MODEL_OK) return rc;
+    if ((rc = run_prefill(m, (int)n_seq, (int)T, m->pool, 0)) != MODEL_OK) return rc;
+    (void)next_host;
+    return prefill_logits(m, n_seq, T, logits_host);
 }
 
 model_status model_prefill_batch(model* m, const int32_t* ids, size_t n_seq, size_t T, float* logits,
@@ -1604,6 +1658,46 @@ model_status model_decode_step_batch(model* m, const int32_t* ids, size_t n_seq,
         CU(cudaMemcpyAsync(next_ids, m->d_next, n_seq * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
     if ((rc = finish(m)) != MODEL_OK) return rc;
     m->pool->length += 1;
+    return MODEL_OK;
+}
+
+model_status model_extend_batch(model* m, const int32_t* ids, size_t n_seq, size_t T, float* logits,
+                                size_t cap, int32_t* next_ids) {
+    if (!m || !ids || n_seq == 0 || T == 0) return MODEL_ERR_ARG;
+    if (!m->pool || n_seq > (size_t)m->pool->n_seq) return MODEL_ERR_ARG;
+    const size_t pos0 = (size_t)m->pool->length;
+    if (T > (size_t)m->pool->capacity || pos0 + T > (size_t)m->pool->capacity) return MODEL_ERR_CAPACITY;
+    if (logits && cap < n_seq * T * (size_t)m->cfg.vocab_size) return MODEL_ERR_CAPACITY;
+    for (size_t i = 0; i < n_seq * T; ++i)
+        if (ids[i] < 0 || ids[i] >= m->cfg.vocab_size) return MODEL_ERR_RANGE;
+    const size_t rows = n_seq * T;
+    model_status rc = ensure_rows(m, rows);
+    if (rc != MODEL_OK) return rc;
+    // ctx, new, row starts, three arrays of rows, status
+    if ((rc = grow(&m->d_ops, &m->ops_cap, 3 * n_seq + 1 + 3 * rows + 1)) != MODEL_OK) return rc;
+    if ((rc = grow(&m->d_ops_ws, &m->ops_ws_cap, tie_attention_paged_workspace())) != MODEL_OK) return rc;
+    if ((rc = ensure_pinned(m, 2 * n_seq)) != MODEL_OK) return rc;
+    if ((rc = copy_ids_to_device(m, ids, rows)) != MODEL_OK) return rc;
+    int32_t *ctx = m->d_ops, *fresh = ctx + n_seq, *start = fresh + n_seq, *seq = start + n_seq + 1, *pos = seq + rows;
+    int32_t *slots = pos + rows, *status = slots + rows;
+    CU(cudaStreamSynchronize(m->st));
+    for (size_t i = 0; i < n_seq; ++i) {
+        m->h_small[i] = (int32_t)pos0;
+        m->h_small[n_seq + i] = (int32_t)T;
+    }
+    CU(cudaMemcpyAsync(ctx, m->h_small, 2 * n_seq * sizeof(int32_t), cudaMemcpyHostToDevice, m->st));
+    if ((rc = map_pages(m, n_seq, pos0 + T)) != MODEL_OK) return rc;
+    // the pool's host allocator has assigned the pages: the table is complete
+    const kv_cache* c = m->pool;
+    OP(tie_page_plan(ctx, fresh, (int)n_seq, c->d_page_table, c->pages_per_seq, (int)(c->rows / kPageRows), nullptr, 0,
+                     nullptr, nullptr, start, seq, pos, slots, (int)rows, status, m->st));
+    const PagedChunk chunk{(int)pos0, ctx, start, slots};
+    if ((rc = run_prefill(m, (int)n_seq, (int)T, m->pool, 0, &chunk)) != MODEL_OK) return rc;
+    if ((rc = prefill_logits(m, n_seq, T, logits)) != MODEL_OK) return rc;
+    if (next_ids)
+        CU(cudaMemcpyAsync(next_ids, m->d_next, n_seq * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
+    if ((rc = finish(m)) != MODEL_OK) return rc;
+    m->pool->length = (int)(pos0 + T);
     return MODEL_OK;
 }
 
@@ -1657,6 +1751,92 @@ model_status model_generate_greedy(model* m, const int32_t* prompts, size_t n_se
 model_status model_generate_greedy_device(model* m, const int32_t* d_prompts, size_t n_seq,
                                           size_t n_prompt, size_t n_new, int32_t* d_out_ids) {
     return generate_impl(m, d_prompts, n_seq, n_prompt, n_new, d_out_ids, false);
+}
+
+model_status model_generate_beam(model* m, const int32_t* prompts, size_t n_req, size_t T, size_t beams,
+                                 size_t n_new, int32_t eos_id, int32_t* out_ids, float* out_scores) {
+    if (!m || !prompts || !out_ids || !out_scores || n_req == 0 || T == 0 || beams == 0 || n_new == 0)
+        return MODEL_ERR_ARG;
+    if (beams > 16) return MODEL_ERR_CAPACITY;
+    if (!m->pool || n_req > (size_t)m->pool->n_seq || n_req * beams > (size_t)m->pool->n_seq) return MODEL_ERR_ARG;
+    const size_t cap = (size_t)m->pool->capacity;
+    if (T > cap || n_new > cap || T + n_new - 1 > cap) return MODEL_ERR_CAPACITY;
+    const int V = m->cfg.vocab_size;
+    if (eos_id >= V) return MODEL_ERR_RANGE;
+    for (size_t i = 0; i < n_req * T; ++i)
+        if (prompts[i] < 0 || prompts[i] >= V) return MODEL_ERR_RANGE;
+    const size_t S = n_req * beams;
+    model_status rc = ensure_rows(m, S * T);
+    if (rc != MODEL_OK) return rc;
+    if ((rc = ensure_slots(m, S, m->pool->capacity)) != MODEL_OK) return rc;
+    // next, parent, done, scores, first, and per step the tokens and parents
+    if ((rc = grow(&m->d_ops, &m->ops_cap, 4 * S + n_req + 2 * n_new * S)) != MODEL_OK) return rc;
+    if ((rc = grow(&m->d_ops_ws, &m->ops_ws_cap, tie_beam_select_workspace((int)n_req, (int)beams, V))) != MODEL_OK)
+        return rc;
+    int32_t *next = m->d_ops, *parent = next + S, *done = parent + S, *first = done + S + S;
+    float* scores = reinterpret_cast<float*>(done + S);
+    int32_t *tokens = first + n_req, *parents = tokens + n_new * S;   // [S][n_new], [n_new][S]
+    int32_t* done_or_null = eos_id < 0 ? nullptr : done;
+    if ((rc = stats_begin(m)) != MODEL_OK) return rc;
+
+    // every beam of a request holds the prompt; only the first has a score yet
+    std::vector<int32_t> ids(S * T);
+    for (size_t s = 0; s < S; ++s) std::memcpy(&ids[s * T], prompts + s / beams * T, T * sizeof(int32_t));
+    if ((rc = batch_prefill_impl(m, S, T, nullptr, nullptr, true, ids.data())) != MODEL_OK) return rc;
+    if ((rc = ensure_pinned(m, 3 * S + n_req)) != MODEL_OK) return rc;
+    CU(cudaStreamSynchronize(m->st));
+    int32_t *h_done = m->h_small, *h_score = h_done + S, *h_first = h_score + S, *h_len = h_first + n_req;
+    for (size_t s = 0; s < S; ++s) {
+        const float score = s % beams ? -INFINITY : 0.f;
+        h_done[s] = 0;
+        std::memcpy(&h_score[s], &score, sizeof score);
+        h_len[s] = (int32_t)T - 1;
+    }
+    for (size_t r = 0; r < n_req; ++r) h_first[r] = (int32_t)T;
+    CU(cudaMemcpyAsync(done, h_done, (2 * S + n_req) * sizeof(int32_t), cudaMemcpyHostToDevice, m->st));
+    CU(cudaMemcpyAsync(m->d_lens, h_len, S * sizeof(int32_t), cudaMemcpyHostToDevice, m->st));
+    CU(cudaMemsetAsync(m->d_step, 0, sizeof(int32_t), m->st));
+
+    const kv_cache* c = m->pool;
+    for (size_t g = 0; g < n_new; ++g) {
+        if (g) {
+            // position T + g - 1 of every beam
+            if ((rc = map_pages(m, S, T + g)) != MODEL_OK) return rc;
+            if ((rc = decode_step(m, (int)S, m->pool, false, nullptr, 0)) != MODEL_OK) return rc;
+        }
+        OP(tie_beam_select(m->logits, V, scores, done_or_null, (int)n_req, (int)beams, V, eos_id, next, parent, scores,
+                           done_or_null, m->d_ops_ws, m->ops_ws_cap, m->st));
+        // the choices become the next step's tokens, the lengths grow to T + g
+        LAUNCH(launch_step_advance(next, m->d_tokens, m->d_lens, tokens, (int)n_new, m->d_step, (int)S, m->st));
+        CU(cudaMemcpyAsync(parents + g * S, parent, S * sizeof(int32_t), cudaMemcpyDeviceToDevice, m->st));
+        // (all lengths are equal, so the first n_req stand for the requests)
+        if (g && g + 1 < n_new)
+            OP(tie_kv_reorder(c->k, c->v, TIE_KV_F32, c->n_layer, c->rows * (size_t)c->n_embd, (int)(c->rows / kPageRows),
+                              m->cfg.n_head, c->d_page_table, c->pages_per_seq, parent, first, m->d_lens, (int)n_req,
+                              (int)beams, m->st));
+    }
+    std::vector<int32_t> h_tok(n_new * S), h_par(n_new * S);
+    std::vector<float> h_sc(S);
+    CU(cudaMemcpyAsync(h_tok.data(), tokens, n_new * S * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
+    CU(cudaMemcpyAsync(h_par.data(), parents, n_new * S * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
+    CU(cudaMemcpyAsync(h_sc.data(), scores, S * sizeof(float), cudaMemcpyDeviceToHost, m->st));
+    if ((rc = finish(m)) != MODEL_OK) return rc;
+    m->pool->length = (int)(T + n_new - 1);
+    // each request's beams, best first, their tokens read back along the parents
+    std::vector<size_t> order(beams);
+    for (size_t r = 0; r < n_req; ++r) {
+        for (size_t b = 0; b < beams; ++b) order[b] = r * beams + b;
+        std::stable_sort(order.begin(), order.end(), [&](size_t x, size_t y) { return h_sc[x] > h_sc[y]; });
+        for (size_t b = 0; b < beams; ++b) {
+            size_t at = order[b];
+            out_scores[r * beams + b] = h_sc[at];
+            for (size_t g = n_new; g-- > 0;) {
+                out_ids[(r * beams + b) * n_new + g] = h_tok[at * n_new + g];
+                at = (size_t)h_par[g * S + at];
+            }
+        }
+    }
+    return MODEL_OK;
 }
 
 model_status model_step_trace(model* m, size_t rows, size_t context, uint64_t* out, size_t cap,

@@ -21,6 +21,9 @@ constexpr int kHeadDim = 64;
 // Records `e` for tie_last_device_error (model.cu).
 void note_device_error(cudaError_t e, const char* what, const char* file, int line);
 
+// Kernels launched by the operators on the calling thread.
+extern thread_local uint64_t op_launches;
+
 #define TIE_OP_CU(expr)                                                    \
     do {                                                                   \
         cudaError_t e_ = (expr);                                           \

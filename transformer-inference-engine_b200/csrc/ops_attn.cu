@@ -448,6 +448,7 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
         const int ctas = cluster_ctas(n_seq, n_kv_head, pages_per_seq, sms);
         if (ctas > 0) {
             TIE_OP_CU(launch_few_cluster(a, bf16, (int)most, ctas, st));
+            ++op_launches;
             return MODEL_OK;
         }
     }
@@ -469,5 +470,6 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
         TIE_OP_CU(cudaGetLastError());
     }
     TIE_OP_CU(launch_pdl(join_kernel, dim3((unsigned)sms * 2), dim3(kJoinThreads), smem, st, a));
+    op_launches += 1 + !a.only_few + (a.group <= kFewRows);
     return MODEL_OK;
 }

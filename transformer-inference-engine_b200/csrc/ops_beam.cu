@@ -401,5 +401,6 @@ extern "C" model_status tie_beam_select(const float* logits, int ldl, const floa
     TIE_OP_CU(cudaGetLastError());
     TIE_OP_CU(launch_pdl(beam_pick_kernel, dim3((unsigned)n_req), dim3(kPickThreads), 0, st, p, slices, beams, vocab, eos_id, scores,
                          done, next, parent, scores_out, done_out));
+    op_launches += 2;
     return MODEL_OK;
 }

@@ -390,6 +390,7 @@ extern "C" model_status tie_page_plan(const int32_t* ctx_lens, const int32_t* ne
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     TIE_OP_CU(cudaLaunchKernelEx(&cfg, page_plan_kernel, a));
+    ++op_launches;
     return MODEL_OK;
 }
 
@@ -411,6 +412,7 @@ extern "C" model_status tie_kv_store(const float* k, const float* v, int ld, con
     kernel<<<(unsigned)blocks, kStoreThreads, 0, static_cast<cudaStream_t>(stream)>>>(k, v, ld, slots, n, w / 8,
                                                                                       n_slots, k_pages, v_pages);
     TIE_OP_CU(cudaGetLastError());
+    ++op_launches;
     return MODEL_OK;
 }
 
@@ -449,5 +451,6 @@ extern "C" model_status tie_kv_reorder(void* k_pages, void* v_pages, int kv_form
     const unsigned grid = (unsigned)sm_count(dev.device()) * (2048 / kReorderThreads);
     kernel<<<grid, kReorderThreads, (size_t)(n_req + 1) * sizeof(int), static_cast<cudaStream_t>(stream)>>>(a);
     TIE_OP_CU(cudaGetLastError());
+    ++op_launches;
     return MODEL_OK;
 }

@@ -122,6 +122,9 @@ def library():
         "model_decode_step_batch": (C.c_int, [_vp, _ip, C.c_size_t, _fp, C.c_size_t, _ip]),
         "model_generate_greedy": (C.c_int, [_vp, _ip, C.c_size_t, C.c_size_t, C.c_size_t, _ip]),
         "model_generate_greedy_device": (C.c_int, [_vp, _vp, C.c_size_t, C.c_size_t, C.c_size_t, _vp]),
+        "model_extend_batch": (C.c_int, [_vp, _ip, C.c_size_t, C.c_size_t, _fp, C.c_size_t, _ip]),
+        "model_generate_beam": (C.c_int, [_vp, _ip, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_int32, _ip,
+                                          _fp]),
         "model_time_kernel": (C.c_int, [_vp, C.c_int, C.c_size_t, C.c_size_t, C.c_int, _fp]),
         "model_set_step_kernel": (C.c_int, [_vp, C.c_int]),
         "model_debug_wait_drill": (C.c_int, [_vp, C.c_uint64]),
@@ -450,6 +453,35 @@ class Model:
             _chk(rc, "model_decode_step_batch")
             return nxt, logits
         return rc, nxt, logits
+
+    def extend_batch(self, ids, want_logits=False, check=True):
+        """Appends ids [n_seq, n_ids] to the pool's sequences (model_extend_batch): like
+        prefill_batch, behind the positions already cached."""
+        ids = _ids(ids)
+        S, T = ids.shape
+        nxt = np.zeros(S, dtype=np.int32)
+        logits = np.empty((S, T, self.vocab), dtype=np.float32) if want_logits else None
+        rc = library().model_extend_batch(self.h, _ip_of(ids), S, T,
+                                          _fp_of(logits) if want_logits else None,
+                                          logits.size if want_logits else 0, _ip_of(nxt))
+        if check:
+            _chk(rc, "model_extend_batch")
+            return nxt, logits
+        return rc, nxt, logits
+
+    def generate_beam(self, prompts, beams, n_new, eos_id=-1, check=True):
+        """Beam search (model_generate_beam): ids [n_req, beams, n_new] and scores
+        [n_req, beams], best first."""
+        prompts = _ids(prompts)
+        R, T = prompts.shape
+        out = np.zeros((R, beams, n_new), dtype=np.int32)
+        scores = np.zeros((R, beams), dtype=np.float32)
+        rc = library().model_generate_beam(self.h, _ip_of(prompts), R, T, beams, n_new, eos_id, _ip_of(out),
+                                           _fp_of(scores))
+        if check:
+            _chk(rc, "model_generate_beam")
+            return out, scores
+        return rc, out, scores
 
     def generate_greedy(self, prompts, n_new, check=True):
         prompts = _ids(prompts)
