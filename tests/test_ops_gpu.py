@@ -355,6 +355,64 @@ def test_attention_and_store_beyond_32_bit_offsets(new):
     assert (np.abs(out.cpu().numpy() - want) <= ref.attention_bound(vmax, smax, rows)).all()
 
 
+def _long(kv, ctx, new, heads, scores, unmapped=0):
+    """One sequence, one K/V head, values around 1; (got, want) of some of its rows, want in 64 bits.
+
+    scores(position) is added to what every row scores the position, in units of the score."""
+    total, rng = ctx + new, np.random.default_rng(ctx + heads)
+    n_pages = ref.pages_of(total)
+    table = rng.permutation(n_pages)
+    q, k, v = rng.standard_normal((new, heads * D)), rng.standard_normal((total, D)), 1 + rng.standard_normal((total, D))
+    q, k = 0.02 * q.reshape(new, heads, D), 0.1 * k
+    q[..., 0], k[:, 0] = 1.0, scores(np.arange(total))
+    dev = lambda x: torch.from_numpy(x.astype(np.float32)).cuda()  # noqa: E731
+    q, pools = dev(q.reshape(new, -1)), []
+    for x in (k, v):
+        pool = torch.zeros(n_pages, PAGE, D, device="cuda")
+        pool[torch.from_numpy(table).cuda()] = torch.nn.functional.pad(dev(x), (0, 0, 0, -total % PAGE)).view(n_pages, PAGE, D)
+        pools.append(pool.to(kv))
+    mapped = np.where(np.arange(n_pages) < unmapped // PAGE, -1, table)
+    out = torch.full((new, heads * D), 7.0, device="cuda")
+    ops.attention_paged(q, *pools, _i(mapped[None]), _i([0, new]), _i([ctx]), new, out, _workspace(), scale=1.0)
+    pick = torch.from_numpy(np.unique(np.linspace(0, new - 1, 24).astype(int))).cuda()
+    kd, vd = (x[torch.from_numpy(table).cuda()].view(-1, D)[:total].double() for x in pools)
+    s = q.view(new, heads, D)[pick].double() @ kd.T
+    pos = torch.arange(total, device="cuda")
+    s.masked_fill_((pos > ctx + pick[:, None, None]) | (pos < unmapped), -torch.inf)
+    return out.view(new, heads, D)[pick].double(), s.softmax(-1) @ vd
+
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("heads,new", [(16, 1024), (4, 16)])
+def test_attention_of_many_keys_keeps_32_bits(kv, heads, new):
+    """30,000 keys of about the same weight: what each step cuts off its sums must not add up.
+
+    Relative bounds, each at its worst: an O of at most 64 MMAs, each of which cuts off at most one unit in
+    the last place of a sum that grows evenly, 32 x 2^-23; the split of q, k, p and v, 4 x 2^-22; scores of
+    |s| < 0.5 from 12 MMAs that cut off likewise, 12 x 2^-24; 2^x, 2^-22; 1 in 128 of the additions to the row
+    sum one after the other (240 steps, in two streams or by two CTAs or more), 120 x 2^-24. In all
+    2^-24 (64 + 16 + 12 + 4 + 120) = 1.3e-5."""
+    got, want = _long(kv, 30000, new, heads, lambda pos: 0.0 * pos)
+    assert torch.linalg.vector_norm(got - want) <= 1.3e-5 * torch.linalg.vector_norm(want)
+    # a sum that loses always in one direction shows in the mean: half of the first bound, of 64 MMAs (the rest
+    # is rounded, which has no direction, or belongs to a row's sum: 8 x 2^-24 in the mean of the rows)
+    assert abs(float((got / want)[want > 0.5].mean()) - 1) <= (32 + 8) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("ramp", [300.0, -300.0, 20.0])
+@pytest.mark.parametrize("unmapped", [0, 2064])
+def test_attention_of_maxima_that_move(kv, ramp, unmapped):
+    """Scores that rise or fall along the context by far more than a running sum can hold at one scale.
+
+    The bound of attention_bound, with the largest sum |q||k| of a row for its scores (the ramp, and 0.02 x 0.1
+    x 64 products of at most 5 deviations each way) and the values of the data."""
+    n = 6000
+    got, want = _long(kv, n, 700, 16, lambda pos: ramp * pos / n, unmapped)
+    bound = ref.attention_bound(6.0, abs(ramp) * 1.2 + 1.0, n + 700)
+    assert float((got - want).abs().max()) <= bound
+
+
 # ------------------------------------------------------------------ beam selection
 
 def _select(logits, scores, beams, done=None, eos=-1, alias=False):

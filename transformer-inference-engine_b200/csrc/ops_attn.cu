@@ -383,7 +383,10 @@ int target_of(int sms) { return 4 * sms; }
 size_t part_rows(int kind, int sms) {
     return kind ? 2 * (size_t)sms * kTileRows : 2 * (size_t)target_of(sms) * kFewRows;
 }
-size_t scratch_bytes(int sms) { return (part_rows(0, sms) + part_rows(1, sms)) * (kHeadDim + 2) * sizeof(float); }
+size_t run_floats(int sms) { return (size_t)sms * kTileRows * kHeadDim; }
+size_t scratch_bytes(int sms) {
+    return ((part_rows(0, sms) + part_rows(1, sms)) * (kHeadDim + 2) + run_floats(sms)) * sizeof(float);
+}
 
 }  // namespace
 }  // namespace tie
@@ -429,6 +432,8 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
     a.scale2 = (float)((double)scale * 1.4426950408889634);
     a.out = out; a.ldo = ldo;
     float* f = static_cast<float*>(workspace);
+    a.run_o = f;
+    f += run_floats(sms);
     for (int kind = 0; kind < 2; ++kind) {
         a.part_o[kind] = f;
         f += part_rows(kind, sms) * kHeadDim;

@@ -43,6 +43,7 @@ struct PagedAttnArgs {
     // partials, per kind: of split units (streaming), two per CTA (tensor cores)
     float* part_o[2];              // [unit][tile rows][64], unnormalised
     float* part_ml[2];             // [unit][tile rows][2]: maximum (power-of-two domain), sum
+    float* run_o;                  // [CTA][stream][64 / 4][128 rows][4]: running sums (tensor cores)
     int target;                    // streaming units wanted when the work is split
     int ctas;                      // CTAs of the tensor-core kernel
     int only_few;                  // every sequence is of the streaming kind
