@@ -113,11 +113,11 @@ model_status model_generate_greedy_device(model *m, const int32_t *d_prompts, si
  * model_prefill_batch, logits_out (host, n_seq * n_ids * vocab floats, or NULL)
  * receives the new positions' logits and next_ids (host, n_seq, or NULL) each
  * sequence's greedy choice at its last position. Attention statistics
- * (model_collect_attn_stats) do not cover this call. */
+ * (model_collect_attn_stats) do not cover this call. At most 4096 sequences. */
 model_status model_extend_batch(model *m, const int32_t *ids, size_t n_seq, size_t n_ids,
                                 float *logits_out, size_t logits_cap, int32_t *next_ids);
 
-/* Beam search: for each of n_req prompts of n_prompt tokens (host, n_req *
+/* Beam search: for each of n_req (<= 4096) prompts of n_prompt tokens (host, n_req *
  * n_prompt) the `beams` (<= 16) continuations of n_new tokens that one beam
  * search step after the other keeps (tie_beam_select: largest sum of log
  * probabilities, ties to the lowest beam and token). A continuation that has
@@ -323,8 +323,8 @@ model_status tie_page_plan(const int32_t *ctx_lens, const int32_t *new_lens, int
 
 /* Key and value rows into their slots: row r of k and v (n_kv_head * 64 floats,
  * ld floats apart) to slot slots[r] of the pool, rounded to nearest even for
- * bf16. A slot outside the pool stores nothing; of two rows with one slot
- * either may stay. rows == 0 is allowed. */
+ * bf16. A slot outside the pool stores nothing; of two rows with one slot each
+ * part of 8 elements is one or the other's. rows == 0 is allowed. */
 model_status tie_kv_store(const float *k, const float *v, int ld, const int32_t *slots, int rows,
                           void *k_pages, void *v_pages, int kv_format, int n_pages, int n_kv_head,
                           void *stream);
@@ -340,8 +340,8 @@ model_status tie_kv_store(const float *k, const float *v, int ld, const int32_t 
  * new tokens, with more than max_new, with row_start outside 0..rows or beyond
  * pages_per_seq pages is left out: its rows of out stay as they were, and so
  * do rows behind the last sequence's. Sums and softmax statistics are fp32.
- * A key or value that is not finite makes the rows that see it not finite and
- * no others. The result of a row depends, in its rounding, on how the batch
+ * A value that is not finite makes the rows that see it not finite, a key that
+ * is not finite may, and neither does it to any other row. The result of a row depends, in its rounding, on how the batch
  * splits its keys, and is the same for the same call.
  * status, if not NULL, receives MODEL_ERR_DEVICE when a bounded wait in the
  * kernel expires (the output is then incomplete); it is not written otherwise. */

@@ -413,6 +413,38 @@ def test_attention_of_maxima_that_move(kv, ramp, unmapped):
     assert float((got - want).abs().max()) <= bound
 
 
+def test_calls_of_many_sequences_on_two_threads():
+    """Numbers of sequences that ask for different amounts of shared memory, side by side."""
+    import threading
+    failed = []
+
+    def calls(n_seq, seed):
+        try:
+            rng = np.random.default_rng(seed)
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                b = _batch(rng, [3] * n_seq, [2] + [1] * (n_seq - 1), 4, 1, torch.float32)
+                b["max_new"] = 9          # not all sequences have few rows, as far as the call knows
+                first, ws = _attend(b), _workspace()
+                for _ in range(40):
+                    o = dict(row_start=_out(n_seq + 1), seq_of=_out(n_seq + 1), pos_of=_out(n_seq + 1),
+                             slot_of=_out(n_seq + 1), status=_out(1))
+                    ops.page_plan(_i([3] * n_seq), _i([1] * n_seq), _i(b["table"]), 2 * n_seq + 8, **o)
+                    again = _attend(b, workspace=ws)
+                stream.synchronize()
+                assert torch.equal(first, again) and int(o["status"][0]) == 0
+                assert o["row_start"].tolist() == list(range(n_seq + 1))
+        except Exception as e:                                     # noqa: BLE001
+            failed.append((n_seq, repr(e)))
+
+    threads = [threading.Thread(target=calls, args=(n, n)) for n in (4096, 3950)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not failed
+
+
 # ------------------------------------------------------------------ beam selection
 
 def _select(logits, scores, beams, done=None, eos=-1, alias=False):

@@ -1665,6 +1665,7 @@ model_status model_extend_batch(model* m, const int32_t* ids, size_t n_seq, size
                                 size_t cap, int32_t* next_ids) {
     if (!m || !ids || n_seq == 0 || T == 0) return MODEL_ERR_ARG;
     if (!m->pool || n_seq > (size_t)m->pool->n_seq) return MODEL_ERR_ARG;
+    if (n_seq > (size_t)kOpsMaxSeqs) return MODEL_ERR_CAPACITY;
     const size_t pos0 = (size_t)m->pool->length;
     if (T > (size_t)m->pool->capacity || pos0 + T > (size_t)m->pool->capacity) return MODEL_ERR_CAPACITY;
     if (logits && cap < n_seq * T * (size_t)m->cfg.vocab_size) return MODEL_ERR_CAPACITY;
@@ -1760,7 +1761,7 @@ model_status model_generate_beam(model* m, const int32_t* prompts, size_t n_req,
     if (beams > 16) return MODEL_ERR_CAPACITY;
     if (!m->pool || n_req > (size_t)m->pool->n_seq || n_req * beams > (size_t)m->pool->n_seq) return MODEL_ERR_ARG;
     const size_t cap = (size_t)m->pool->capacity;
-    if (T > cap || n_new > cap || T + n_new - 1 > cap) return MODEL_ERR_CAPACITY;
+    if (n_req > (size_t)kOpsMaxSeqs || T > cap || n_new > cap || T + n_new - 1 > cap) return MODEL_ERR_CAPACITY;
     const int V = m->cfg.vocab_size;
     if (eos_id >= V) return MODEL_ERR_RANGE;
     for (size_t i = 0; i < n_req * T; ++i)

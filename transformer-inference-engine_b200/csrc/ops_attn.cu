@@ -469,8 +469,10 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
             kernel = rmax == 1 ? few_rows_kernel<1, false> : rmax == 2 ? few_rows_kernel<2, false>
                      : rmax == 4 ? few_rows_kernel<4, false> : few_rows_kernel<8, false>;
         // the prefix sums of many sequences pass the 48 KB that a kernel has unasked
+        // (always the most that any call wants: calls on other threads set it too)
         if (smem + sizeof(FewSmem) > 44 * 1024)
-            TIE_OP_CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            TIE_OP_CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (kOpsMaxSeqs + 1) * (int)sizeof(long long)));
         kernel<<<(unsigned)(sms * (rmax <= 2 ? 2 : 1)), kFewThreads, smem, st>>>(a);
         TIE_OP_CU(cudaGetLastError());
     }

@@ -157,8 +157,8 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
     };
     // assigned page x of the call is free page n_free - 1 - x
     const int need = s_need[a.n_seq], rows = s_row[a.n_seq];
-    for (int x = g; x < need; x += G) {
-        const int s = owner(s_need, x);
+    for (long long at = g; at < need; at += G) {
+        const int x = (int)at, s = owner(s_need, x);
         const int have = (int)(((long long)s_ctx[s] + kPageRows - 1) / kPageRows);
         a.table[(size_t)s * a.width + have + (x - s_need[s])] = a.free_pages[n_free - 1 - x];
     }
@@ -171,9 +171,10 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
         int seq[kGroups], pos[kGroups], page[kGroups];
 #pragma unroll
         for (int x = 0; x < kGroups; ++x) {
-            const int first = 32 * (w0 + x * GW), r = first + lane;
+            const long long group = 32 * ((long long)w0 + x * GW);
             seq[x] = pos[x] = page[x] = -1;
-            if (first >= rows || first < 0) continue;
+            if (group >= rows) continue;
+            const int first = (int)group, r = first + lane < rows ? first + lane : INT_MAX;
             int lo = 0, n = a.n_seq;               // s_row[lo] <= first, and not at lo + n
             while (n > 1) {
                 const int step = (n + 31) / 32;    // lane l looks at lo + l * step
@@ -182,7 +183,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
                 lo += at * step;
                 n = min(step, n - at * step);
             }
-            if (r >= rows) continue;
+            if (r == INT_MAX) continue;
             while (s_row[lo + 1] <= r) ++lo;
             seq[x] = lo;
             const int c = s_ctx[lo], have = (int)(((long long)c + kPageRows - 1) / kPageRows);
@@ -379,9 +380,10 @@ extern "C" model_status tie_page_plan(const int32_t* ctx_lens, const int32_t* ne
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kPlanThreads);
     cfg.dynamicSmemBytes = 3 * (size_t)(n_seq + 1) * sizeof(int);
+    // (always the most that any call wants: calls on other threads set it too)
     if (cfg.dynamicSmemBytes > 46 * 1024)
         TIE_OP_CU(cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)cfg.dynamicSmemBytes));
+                                       3 * (kOpsMaxSeqs + 1) * (int)sizeof(int)));
     cfg.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
