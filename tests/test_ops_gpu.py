@@ -413,6 +413,36 @@ def test_attention_of_maxima_that_move(kv, ramp, unmapped):
     assert float((got - want).abs().max()) <= bound
 
 
+def test_binding_reads_tensors_as_they_are():
+    """Parameters, views with an offset, single rows of any stride, streams by number; refusals with the GPU's tensors."""
+    rng = np.random.default_rng(2)
+    b = _batch(rng, [20, 3], [1, 2], 2, 1, torch.float32)
+    want = _attend(b)
+    wide = torch.full((4, 200), 5.0, device="cuda")
+    out = wide[1:, 8:136]
+    got = _attend(dict(b, q=torch.nn.Parameter(b["q"].clone())), out=out)
+    assert got is out and torch.equal(out, want) and bool((wide[:, :8] == 5).all()) and bool((wide[0] == 5).all())
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    again = torch.zeros_like(want)
+    ops.attention_paged(b["q"], b["k"], b["v"], _i(b["table"]), _i(b["start"]), _i(b["ctx"]), 2, again, _workspace(),
+                        stream=stream.cuda_stream)
+    stream.synchronize()
+    assert torch.equal(again, want)
+    k1 = torch.arange(64.0, device="cuda")[None].expand(1, 64)
+    ops.kv_store(k1, k1.clone(), _i([3]), b["k"], b["v"])
+    assert torch.equal(b["k"][0, 3], k1[0]) and torch.equal(b["v"][0, 3], k1[0])
+    for bad in (dict(q=b["q"].cpu()), dict(q=b["q"].double()), dict(k=b["k"].cpu()), dict(v=b["v"].bfloat16()),
+                dict(k=b["k"][:, :8], v=b["v"][:, :8]), dict(max_new=1 << 32), dict(q=b["q"].T), dict(q=b["q"][0]),
+                dict(q=b["q"].cpu().numpy())):
+        with pytest.raises(ValueError):
+            _attend(dict(b, **bad), out=want)
+    with pytest.raises(TypeError):
+        _attend(b, scale="large")
+    with pytest.raises(ValueError):
+        ops.kv_store(k1, k1.clone(), torch.zeros(1, device="cuda"), b["k"], b["v"])
+
+
 def test_calls_of_many_sequences_on_two_threads():
     """Numbers of sequences that ask for different amounts of shared memory, side by side."""
     import threading

@@ -1,15 +1,19 @@
 """Builds libtie_b200.so in-tree with nvcc for sm_100a (no JIT cache, no torch
 extension machinery): every .cu/.cpp under csrc/ is compiled to an object in
-parallel, then linked into lib/libtie_b200.so.  Rebuilds only what changed.
+parallel, then linked into lib/libtie_b200.so; csrc/python/ops_module.cpp becomes
+tie_b200/_ops (of torch only one header is used, nothing is linked).  Rebuilds only
+what changed.
 
     python -m tie_b200.build            (from transformer-inference-engine_b200/)
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -19,6 +23,9 @@ INCLUDE = os.path.join(REPO_ROOT, "include")
 OBJ_DIR = os.path.join(PKG_ROOT, "build")
 LIB_DIR = os.path.join(PKG_ROOT, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libtie_b200.so")
+
+OPS_SRC = os.path.join(CSRC, "python", "ops_module.cpp")
+OPS_PATH = os.path.join(PKG_ROOT, "tie_b200", "_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O3",
@@ -74,7 +81,24 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None) -> str:
         if p.returncode != 0:
             raise RuntimeError(f"link failed:\n{p.stdout}\n{p.stderr}")
         os.replace(tmp, LIB_PATH)
+    build_ops_module()
     return LIB_PATH
+
+
+def build_ops_module() -> str:
+    """tie_b200/_ops, the Python side of the operators' calls."""
+    newest = max([os.path.getmtime(OPS_SRC)] + [os.path.getmtime(os.path.join(INCLUDE, f)) for f in os.listdir(INCLUDE)])
+    if os.path.exists(OPS_PATH) and os.path.getmtime(OPS_PATH) >= newest:
+        return OPS_PATH
+    torch_dir = importlib.util.find_spec("torch").submodule_search_locations[0]
+    tmp = OPS_PATH + ".tmp"
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-I" + INCLUDE,
+           "-I" + sysconfig.get_paths()["include"], "-isystem", os.path.join(torch_dir, "include"), OPS_SRC, "-o", tmp]
+    p = subprocess.run(cmd, capture_output=True, text=True)
+    if p.returncode != 0:
+        raise RuntimeError(f"g++ failed on {OPS_SRC}:\n{p.stdout}\n{p.stderr}")
+    os.replace(tmp, OPS_PATH)
+    return OPS_PATH
 
 
 if __name__ == "__main__":
