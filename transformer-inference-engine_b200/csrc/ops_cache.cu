@@ -41,7 +41,9 @@ namespace cg = cooperative_groups;
 // one cluster: every CTA scans all lengths for itself (4 per thread at most,
 // from L2) and then writes its share of the table entries and rows. One
 // cluster, because n_free_out may be n_free: the cluster barrier puts every
-// CTA's read of it before the one write.
+// CTA's read of it before the one write. 256 sequences of one row: 6.0 us on the
+// GPU, of which an empty launch has 2; 72,000 rows of 1500 sequences: 10.3 us,
+// bound by the rows' instructions on the cluster's 16 SMs.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanPerThread = kOpsMaxSeqs / kPlanThreads;
 
@@ -162,29 +164,39 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
         const int have = (int)(((long long)s_ctx[s] + kPageRows - 1) / kPageRows);
         a.table[(size_t)s * a.width + have + (x - s_need[s])] = a.free_pages[n_free - 1 - x];
     }
-    // A warp takes 32 rows at a time, and two such groups at once (a row is two
-    // loads that depend on one another, so latency counts): the sequence of the
-    // first row by a search with all lanes, the others by walking on from there.
+    // A warp takes a stretch of rows, 32 at a time and two such groups at once (a row is
+    // two loads that depend on one another, so latency counts). The sequence of its
+    // first row is found by a search with all lanes, the others by walking on.
     constexpr int kGroups = 2;
-    const int gw = g >> 5, GW = G >> 5;
-    for (int w0 = gw; 32 * (long long)w0 < a.max_rows; w0 += kGroups * GW) {
+    const long long groups = ((long long)a.max_rows + 31) / 32, per_warp = (groups + (G >> 5) - 1) / (G >> 5);
+    const long long w0 = (g >> 5) * per_warp, w1 = min(w0 + per_warp, groups);
+    int from = -1;                                 // the sequence of the last row so far
+    for (long long w = w0; w < w1; w += kGroups) {
         int seq[kGroups], pos[kGroups], page[kGroups];
 #pragma unroll
         for (int x = 0; x < kGroups; ++x) {
-            const long long group = 32 * ((long long)w0 + x * GW);
             seq[x] = pos[x] = page[x] = -1;
-            if (group >= rows) continue;
-            const int first = (int)group, r = first + lane < rows ? first + lane : INT_MAX;
-            int lo = 0, n = a.n_seq;               // s_row[lo] <= first, and not at lo + n
-            while (n > 1) {
-                const int step = (n + 31) / 32;    // lane l looks at lo + l * step
-                const bool below = lane * step < n && s_row[lo + lane * step] <= first;
-                const int at = 31 - __clz(__ballot_sync(0xffffffffu, below));
-                lo += at * step;
-                n = min(step, n - at * step);
+            if (w + x >= w1 || 32 * (w + x) >= rows) continue;
+            const int first = (int)(32 * (w + x)), r = min(first + lane, rows - 1);
+            if (from < 0) {
+                int n = a.n_seq;                   // s_row[from] <= first, and not at from + n
+                from = 0;
+                while (n > 1) {
+                    const int step = (n + 31) / 32;    // lane l looks at from + l * step
+                    const bool below = lane * step < n && s_row[from + lane * step] <= first;
+                    const int at = 31 - __clz(__ballot_sync(0xffffffffu, below));
+                    from += at * step;
+                    n = min(step, n - at * step);
+                }
             }
-            if (r == INT_MAX) continue;
-            while (s_row[lo + 1] <= r) ++lo;
+            int lo = from;
+            // (by a search of its own where many without rows lie between)
+            bool there = s_row[lo + 1] > r;
+#pragma unroll 1
+            for (int k = 0; k < 4 && !there; ++k) there = s_row[++lo + 1] > r;
+            if (!there) lo = owner(s_row, r);
+            from = __shfl_sync(0xffffffffu, lo, 31);
+            if (r != first + lane) continue;
             seq[x] = lo;
             const int c = s_ctx[lo], have = (int)(((long long)c + kPageRows - 1) / kPageRows);
             pos[x] = c + (r - s_row[lo]);
@@ -196,13 +208,42 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
         }
 #pragma unroll
         for (int x = 0; x < kGroups; ++x) {
-            const long long r = 32 * ((long long)w0 + x * GW) + lane;
-            if (r >= a.max_rows) continue;
+            const long long r = 32 * (w + x) + lane;
+            if (w + x >= w1 || r >= a.max_rows) continue;
             a.seq_of[r] = seq[x];
             a.pos_of[r] = pos[x];
             a.slot_of[r] = page[x] >= 0 && page[x] < a.n_pages ? page[x] * kPageRows + pos[x] % kPageRows : -1;
         }
     }
+}
+
+// The widest cluster of plan CTAs that the current device runs, asked once per device:
+// 16 on B200 (72,000 rows of 1500 sequences: 14.4 us with 8 CTAs, 10.3 with 16).
+// Also raises the kernel's shared memory to the most that any call wants.
+int widest_plan(int device) {
+    static std::mutex mu;
+    static int known[64] = {0};
+    std::lock_guard<std::mutex> lock(mu);
+    if (device >= 0 && device < 64 && known[device]) return known[device];
+    const int smem = 3 * (kOpsMaxSeqs + 1) * (int)sizeof(int);
+    int widest = 8, fit = 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(kPlanThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 16;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess &&
+        cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+        cudaOccupancyMaxActiveClusters(&fit, page_plan_kernel, &cfg) == cudaSuccess && fit > 0)
+        widest = 16;
+    cudaGetLastError();
+    if (device >= 0 && device < 64) known[device] = widest;
+    return widest;
 }
 
 // ---------------------------------------------------------------- row store --
@@ -374,16 +415,12 @@ extern "C" model_status tie_page_plan(const int32_t* ctx_lens, const int32_t* ne
     if (dev.status() != MODEL_OK) return dev.status();
     PlanArgs a{ctx_lens, new_lens, n_seq, page_table, pages_per_seq, n_pages, free_pages, max_free, n_free, n_free_out,
                row_start, seq_of, pos_of, slot_of, max_rows, status};
-    // a CTA per 4096 rows (four passes of its threads), at most a portable cluster
-    const int ctas = (int)min(8LL, (max_rows + 4095LL) / 4096);
+    // a CTA per 4096 rows (four of each thread), at most a cluster
+    const int ctas = (int)min((long long)widest_plan(dev.device()), (max_rows + 4095LL) / 4096);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kPlanThreads);
     cfg.dynamicSmemBytes = 3 * (size_t)(n_seq + 1) * sizeof(int);
-    // (always the most that any call wants: calls on other threads set it too)
-    if (cfg.dynamicSmemBytes > 46 * 1024)
-        TIE_OP_CU(cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       3 * (kOpsMaxSeqs + 1) * (int)sizeof(int)));
     cfg.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
