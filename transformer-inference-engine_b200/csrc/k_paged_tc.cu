@@ -471,8 +471,28 @@ struct Unit {
 };
 static_assert(sizeof(Unit) == 80, "ring entry");
 
+// Adds the values of keys [key0, key1) that are not finite to 32 elements at `to`
+// (whatever their probabilities: what sees them is not finite). Rare: out of line.
+template <bool BF16>
+__device__ __noinline__ void add_odd(const void* values, const int32_t* table, size_t w, int n_pages, float* to, int dim,
+                                     int key0, int key1) {
+    for (int key = key0; key < key1; ++key) {
+        const int e = __ldg(table + key / kPageRows);
+        if (e < 0 || e >= n_pages) continue;
+        const size_t at = ((size_t)e * kPageRows + key % kPageRows) * w + dim;
+#pragma unroll 1
+        for (int d = 0; d < 32; ++d) {
+            float v;
+            if constexpr (BF16) v = __bfloat162float(static_cast<const __nv_bfloat16*>(values)[at + d]);
+            else v = static_cast<const float*>(values)[at + d];
+            if (!(fabsf(v) < INFINITY)) to[d] += v;
+        }
+    }
+}
+
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) {
+    pdl_trigger();                     // few_rows_kernel takes the SMs that are done
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float* s_keys = reinterpret_cast<float*>(smem + kOffKeys);
@@ -720,25 +740,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
             }
             // this thread's results: row `row`, dims [dim0, dim0 + 32), from o
             auto put = [&](uint32_t (&o)[32], int dim0, float mm, float ll) {
-                if (n.odd) {
-                    // values that are not finite, for the rows that see them
-                    const int32_t* table = a.table + (size_t)n.s * a.width;
-                    for (int key = key0; key < min(n.key1, last + 1); ++key) {
-                        const int e = __ldg(table + key / kPageRows);
-                        if (e < 0 || e >= a.n_pages) continue;
-                        const size_t at = ((size_t)e * kPageRows + key % kPageRows) * w + n.g * kHeadDim + dim0;
-#pragma unroll 1
-                        for (int d = 0; d < 32; ++d) {
-                            float v;
-                            if constexpr (BF16) v = __bfloat162float(static_cast<const __nv_bfloat16*>(a.v)[at + d]);
-                            else v = static_cast<const float*>(a.v)[at + d];
-                            if (fabsf(v) < INFINITY) continue;
-#pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                if (k == d) o[k] = __float_as_uint(__uint_as_float(o[k]) + v);
-                        }
-                    }
-                }
                 float4* to;
                 float f = 1.f;
                 if (n.part < 0) {
@@ -758,6 +759,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                     to[c] = f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
                                      : make_float4(__uint_as_float(o[4 * c]) * f, __uint_as_float(o[4 * c + 1]) * f,
                                                    __uint_as_float(o[4 * c + 2]) * f, __uint_as_float(o[4 * c + 3]) * f);
+                if (n.odd && f != 0.f)
+                    add_odd<BF16>(a.v, a.table + (size_t)n.s * a.width, w, a.n_pages, reinterpret_cast<float*>(to),
+                                  n.g * kHeadDim + dim0, key0, min(n.key1, last + 1));
             };
             uint32_t o[32];
             if (both) {

@@ -255,6 +255,9 @@ __global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_rows_kerne
         }
         __syncthreads();
     }
+    // (nothing above needs the tensor-core kernel's results, but what waits for this
+    // kernel waits for both)
+    pdl_wait();
 }
 
 // ------------------------------------------------------------------ the join --
@@ -265,24 +268,30 @@ constexpr int kJoinThreads = 256, kJoinRows = 32;
 template <typename RowAt>
 __device__ __forceinline__ void join_row(const PagedAttnArgs& a, int kind, int parts, const RowAt& row_at, int lane,
                                          float* out) {
-    float mx = -INFINITY;
-    for (int k = lane; k < parts; k += 32) mx = fmaxf(mx, a.part_ml[kind][2 * row_at(k)]);
+    constexpr int kAhead = 8;          // parts on their way at a time
+    float2 ml[kAhead], v[kAhead];
+    auto ask = [&](int k0) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (u == 0 || k0 + u < parts) {
+                const size_t at = row_at(k0 + u);
+                ml[u] = *reinterpret_cast<const float2*>(a.part_ml[kind] + 2 * at);
+                v[u] = *reinterpret_cast<const float2*>(a.part_o[kind] + at * kHeadDim + 2 * lane);
+            }
+    };
+    float mx = lane < parts ? a.part_ml[kind][2 * row_at(lane)] : -INFINITY;
+    ask(0);
+    for (int k = lane + 32; k < parts; k += 32) mx = fmaxf(mx, a.part_ml[kind][2 * row_at(k)]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, o));
     const float base = mx == -INFINITY ? 0.f : mx;
     float l = 0.f, ox = 0.f, oy = 0.f;
-    constexpr int kAhead = 8;          // parts on their way at a time
     for (int k0 = 0; k0 < parts; k0 += kAhead) {
-        float2 ml[kAhead], v[kAhead];
+        if (k0) ask(k0);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const size_t at = row_at(min(k0 + u, parts - 1));
-            ml[u] = *reinterpret_cast<const float2*>(a.part_ml[kind] + 2 * at);
-            v[u] = *reinterpret_cast<const float2*>(a.part_o[kind] + at * kHeadDim + 2 * lane);
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const float f = k0 + u < parts ? ex2_ftz(ml[u].x - base) : 0.f;
+            if (k0 + u >= parts) break;
+            const float f = ex2_ftz(ml[u].x - base);
             l = fmaf(ml[u].y, f, l);
             if (f > 0.f) { ox = fmaf(v[u].x, f, ox); oy = fmaf(v[u].y, f, oy); }
         }
@@ -426,6 +435,7 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
     a.q = q; a.ldq = ldq; a.n_head = n_head;
     a.k = k_pages; a.v = v_pages;
     a.n_pages = n_pages; a.n_kv_head = n_kv_head; a.group = n_head / n_kv_head;
+    a.group_inv = a.group == 1 ? 0 : ~0ull / (unsigned)a.group + 1;
     a.table = page_table; a.width = pages_per_seq;
     a.row_start = row_start; a.ctx = ctx_lens;
     a.n_seq = n_seq; a.max_new = max_new; a.rows = rows;
@@ -473,10 +483,13 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
         if (smem + sizeof(FewSmem) > 44 * 1024)
             TIE_OP_CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            (kOpsMaxSeqs + 1) * (int)sizeof(long long)));
-        kernel<<<(unsigned)(sms * (rmax <= 2 ? 2 : 1)), kFewThreads, smem, st>>>(a);
+        // beside the tensor-core kernel's last CTAs, where there is one
+        const dim3 grid((unsigned)(sms * (rmax <= 2 ? 2 : 1)));
+        if (a.only_few) kernel<<<grid, kFewThreads, smem, st>>>(a);
+        else TIE_OP_CU(launch_pdl(kernel, grid, dim3(kFewThreads), smem, st, a));
         TIE_OP_CU(cudaGetLastError());
     }
-    TIE_OP_CU(launch_pdl(join_kernel, dim3((unsigned)sms * 2), dim3(kJoinThreads), smem, st, a));
+    TIE_OP_CU(launch_pdl(join_kernel, dim3((unsigned)sms * (a.only_few ? 2 : 8)), dim3(kJoinThreads), smem, st, a));
     op_launches += 1 + !a.only_few + (a.group <= kFewRows);
     return MODEL_OK;
 }
