@@ -224,6 +224,14 @@ def test_attention_of_many_sequences(kv, n_seq):
     _check_attention(_batch(rng, rng.integers(0, 300, n_seq).tolist(), rng.integers(0, 3, n_seq).tolist(), 4, 4, kv))
 
 
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("heads,kv_heads", [(25, 25), (36, 18)])
+def test_attention_of_more_tiles_than_buffers(kv, heads, kv_heads):
+    """Chunks and decoding sequences whose tiles are many more than the SMs and what each keeps of them."""
+    rng = np.random.default_rng(heads)
+    _check_attention(_batch(rng, rng.integers(0, 300, 80).tolist(), rng.integers(0, 40, 80).tolist(), heads, kv_heads, kv))
+
+
 @pytest.mark.parametrize("scale", [0.125, 0.01, -0.3, 0.0, 1.0])
 def test_attention_scale_and_row_strides(scale):
     _check_attention(_batch(np.random.default_rng(3), [70, 9], [3, 40], 4, 2, torch.float32, ldq_extra=2 * 4 * D), scale)

@@ -557,6 +557,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
     const long long all = line.base[a.n_seq], g0 = blockIdx.x * line.share, g1 = min(g0 + line.share, all);
     LineUnit here;                   // the stretch's first tile (warp 17's own)
     if (warp == kUnitWarp && g0 < g1) here = unit_at(a, line, g0);
+    if (warp == kUnitWarp + 1 && lane == 0) {
+        // the tile that this CTA begins and does not finish, for the join: it lies in the
+        // CTA's second part and the first parts of the CTAs after it (while the line is
+        // still there: the loaders write over it)
+        JoinRecord rec{};
+        if (g0 < g1 && g1 < all) {
+            const LineUnit u = unit_at(a, line, g1 - 1);
+            if (u.jobs >= g0 && u.jobs < g1 && u.end > g1) {
+                rec.parts = (int)((u.end - 1) / line.share) - (int)blockIdx.x + 1;
+                rec.n_rows = tile_n_rows(u.q, u.tile);
+                rec.token0 = u.q.row0;
+                rec.i0 = u.tile * kTileRows;
+                rec.g = u.g;
+            }
+        }
+        a.record[1][blockIdx.x] = rec;
+    }
     asm volatile("tcgen05.fence::before_thread_sync;");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;");

@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_rows_kerne
     Schedule sch;
     build_schedule<kFewThreads>(a, s_sched, &scratch, t, &sch);
     const int units = sch.unit[a.n_seq];
+    if (blockIdx.x == 0 && t == 0) *a.n_records = sch.part[a.n_seq];
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
         const int s = owner_of<int>(sch.unit, a.n_seq, u);
         const SeqShape q = seq_shape(a, s);
@@ -239,6 +240,8 @@ __global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_rows_kerne
         const int keys = q.ctx + (tile * kFewRows + n_rows - 1) / a.group + 1;
         const int p0 = split * sch.chunk, p1 = min(p0 + sch.chunk, (keys + kPageRows - 1) / kPageRows);
         few_rows_n<RMAX, BF16>(a, q, s, tile, g, p0, p1, kFewWarps, n_rows, &sm);
+        if (sp > 1 && t == 0)
+            a.record[0][sch.part[s] + in] = JoinRecord{split ? 0 : sp, n_rows, q.row0, tile * kFewRows, g, {0, 0, 0}};
         __syncthreads();
         for (int e = t; e < n_rows * kHeadDim; e += kFewThreads) {
             const int r = e / kHeadDim, d = e % kHeadDim;
@@ -299,49 +302,35 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs& a, int kind, int p
     *reinterpret_cast<float2*>(out + 2 * lane) = l == 0.f ? make_float2(0.f, 0.f) : make_float2(ox / l, oy / l);
 }
 
+// The kernels that cut left records of what is to be joined, so that nothing of the
+// schedule is built again (with it: 27 us after 48 mixed sequences).
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(PagedAttnArgs a) {
-    extern __shared__ long long s_line[];
-    __shared__ ScheduleScratch<kJoinThreads> scratch;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     pdl_wait();
-    auto out_of = [&](const SeqShape& q, int g, int i) {
-        return a.out + (size_t)(q.row0 + i / a.group) * a.ldo + (g * a.group + i % a.group) * kHeadDim;
+    auto out_of = [&](const JoinRecord& rec, int r) {
+        const int i = rec.i0 + r, token = i / a.group;
+        return a.out + (size_t)(rec.token0 + token) * a.ldo + (rec.g * a.group + i - token * a.group) * kHeadDim;
     };
-    if (a.group <= kFewRows) {
-        // streaming units: a sequence's split units come in groups of `splits`
-        // per (tile, head); an item is one row of one group
-        Schedule sch;
-        build_schedule<kJoinThreads>(a, reinterpret_cast<int*>(s_line), &scratch, t, &sch);
-        const long long items = (long long)sch.part[a.n_seq] * kFewRows;
-        for (long long x = (long long)blockIdx.x * (kJoinThreads / 32) + warp; x < items;
-             x += (long long)gridDim.x * (kJoinThreads / 32)) {
-            const int pu = (int)(x / kFewRows), r = (int)(x % kFewRows);
-            const int s = owner_of<int>(sch.part, a.n_seq, pu);
-            const SeqShape q = seq_shape(a, s);
-            const int sp = splits_of(q, sch.chunk), in = pu - sch.part[s];
-            const int g = in % a.n_kv_head, split = in / a.n_kv_head % sp, tile = in / a.n_kv_head / sp;
-            const int i = tile * kFewRows + r;
-            if (split || i >= q.rows) continue;
-            join_row(a, 0, sp, [&](int k) { return (size_t)(pu + k * a.n_kv_head) * kFewRows + r; }, lane, out_of(q, g, i));
+    // tensor-core tiles
+    if (!a.only_few)
+        for (int x = blockIdx.x; x < a.ctas * (kTileRows / kJoinRows); x += gridDim.x) {
+            const int c = x / (kTileRows / kJoinRows), r0 = x % (kTileRows / kJoinRows) * kJoinRows;
+            const JoinRecord rec = a.record[1][c];
+            if (!rec.parts) continue;
+            for (int r = r0 + warp; r < min(r0 + kJoinRows, rec.n_rows); r += kJoinThreads / 32)
+                join_row(a, 1, rec.parts, [&](int k) { return ((size_t)2 * (c + k) + (k == 0)) * kTileRows + r; }, lane,
+                         out_of(rec, r));
         }
-        __syncthreads();
-    }
-    if (a.only_few) return;
-    // tensor-core tiles: the one that CTA c began and did not finish lies in c's
-    // second part and the first parts of the CTAs after it
-    JobLine line;
-    build_line<kJoinThreads>(a, s_line, &scratch, t, &line);
-    const long long total = line.base[a.n_seq];
-    for (int x = blockIdx.x; x < a.ctas * (kTileRows / kJoinRows); x += gridDim.x) {
-        const int c = x / (kTileRows / kJoinRows), r0 = x % (kTileRows / kJoinRows) * kJoinRows;
-        const long long g0 = c * line.share, g1 = g0 + line.share;
-        if (g1 >= total) break;
-        const LineUnit u = unit_at(a, line, g1 - 1);
-        if (u.jobs < g0 || u.jobs >= g1 || u.end <= g1) continue;
-        const int parts = (int)((u.end - 1) / line.share) - c + 1, n_rows = tile_n_rows(u.q, u.tile);
-        for (int r = r0 + warp; r < min(r0 + kJoinRows, n_rows); r += kJoinThreads / 32)
-            join_row(a, 1, parts, [&](int k) { return ((size_t)2 * (c + k) + (k == 0)) * kTileRows + r; }, lane,
-                     out_of(u.q, u.g, u.tile * kTileRows + r));
+    // streaming units: a sequence's come in groups of `parts` per (tile, head)
+    static_assert(kJoinThreads / 32 == kFewRows, "a warp for each row of a unit");
+    if (a.group <= kFewRows) {
+        const int n = *a.n_records;
+        for (int u = blockIdx.x; u < n; u += gridDim.x) {
+            const JoinRecord rec = a.record[0][u];
+            if (warp < (rec.parts ? rec.n_rows : 0))
+                join_row(a, 0, rec.parts, [&](int k) { return (size_t)(u + k * a.n_kv_head) * kFewRows + warp; }, lane,
+                         out_of(rec, warp));
+        }
     }
 }
 
@@ -393,8 +382,10 @@ size_t part_rows(int kind, int sms) {
     return kind ? 2 * (size_t)sms * kTileRows : 2 * (size_t)target_of(sms) * kFewRows;
 }
 size_t run_floats(int sms) { return (size_t)sms * kTileRows * kHeadDim; }
+size_t records(int kind, int sms) { return kind ? sms : 2 * (size_t)target_of(sms); }
 size_t scratch_bytes(int sms) {
-    return ((part_rows(0, sms) + part_rows(1, sms)) * (kHeadDim + 2) + run_floats(sms)) * sizeof(float);
+    return ((part_rows(0, sms) + part_rows(1, sms)) * (kHeadDim + 2) + run_floats(sms)) * sizeof(float) +
+           (records(0, sms) + records(1, sms) + 1) * sizeof(JoinRecord);
 }
 
 }  // namespace
@@ -452,6 +443,10 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
         a.part_ml[kind] = f;
         f += part_rows(kind, sms) * 2;
     }
+    JoinRecord* rec = reinterpret_cast<JoinRecord*>(f);
+    a.record[0] = rec;
+    a.record[1] = rec + records(0, sms);
+    a.n_records = &a.record[1][records(1, sms)].parts;
     a.target = target_of(sms);
     a.ctas = sms;
     a.status = status;
@@ -489,7 +484,7 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
         else TIE_OP_CU(launch_pdl(kernel, grid, dim3(kFewThreads), smem, st, a));
         TIE_OP_CU(cudaGetLastError());
     }
-    TIE_OP_CU(launch_pdl(join_kernel, dim3((unsigned)sms * (a.only_few ? 2 : 8)), dim3(kJoinThreads), smem, st, a));
+    TIE_OP_CU(launch_pdl(join_kernel, dim3((unsigned)sms * (a.only_few ? 2 : 8)), dim3(kJoinThreads), 0, st, a));
     op_launches += 1 + !a.only_few + (a.group <= kFewRows);
     return MODEL_OK;
 }

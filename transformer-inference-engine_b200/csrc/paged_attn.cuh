@@ -28,6 +28,13 @@ constexpr int kHalfRows = 128;     // rows of one MMA of the tensor-core kernel
 constexpr int kTileRows = 256;     // rows of its tiles
 constexpr int kTileKeys = 128;     // keys of one of its steps
 
+// What the join has to know of a cut tile: its first part lies where the record does.
+struct __align__(16) JoinRecord {
+    int parts, n_rows;             // parts 0: nothing to join here
+    int token0, i0, g;             // the sequence's first row of out, the tile's first row, K/V head
+    int pad[3];
+};
+
 struct PagedAttnArgs {
     const float* q;
     int ldq, n_head;
@@ -45,6 +52,8 @@ struct PagedAttnArgs {
     float* part_o[2];              // [unit][tile rows][64], unnormalised
     float* part_ml[2];             // [unit][tile rows][2]: maximum (power-of-two domain), sum
     float* run_o;                  // [CTA][stream][64 / 4][128 rows][4]: running sums (tensor cores)
+    JoinRecord* record[2];         // [unit with partials], [CTA]: written by the kernels that cut
+    int* n_records;                // streaming units with partials
     int target;                    // streaming units wanted when the work is split
     int ctas;                      // CTAs of the tensor-core kernel
     int only_few;                  // every sequence is of the streaming kind
