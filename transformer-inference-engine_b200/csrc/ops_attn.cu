@@ -268,10 +268,11 @@ __global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_rows_kerne
 // 2 l and 2 l + 1. Part k's row lies at row_at(k) of the kind's partials.
 constexpr int kJoinThreads = 256, kJoinRows = 32;
 
-template <typename RowAt>
+// kAhead parts are on their way at a time: a tile is cut into two or three, one long
+// sequence into hundreds.
+template <int kAhead, typename RowAt>
 __device__ __forceinline__ void join_row(const PagedAttnArgs& a, int kind, int parts, const RowAt& row_at, int lane,
                                          float* out) {
-    constexpr int kAhead = 8;          // parts on their way at a time
     float2 ml[kAhead], v[kAhead];
     auto ask = [&](int k0) {
 #pragma unroll
@@ -304,7 +305,7 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs& a, int kind, int p
 
 // The kernels that cut left records of what is to be joined, so that nothing of the
 // schedule is built again (with it: 27 us after 48 mixed sequences).
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(PagedAttnArgs a) {
+__global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(PagedAttnArgs a) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     pdl_wait();
     auto out_of = [&](const JoinRecord& rec, int r) {
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(PagedAttnArgs a) {
             const JoinRecord rec = a.record[1][c];
             if (!rec.parts) continue;
             for (int r = r0 + warp; r < min(r0 + kJoinRows, rec.n_rows); r += kJoinThreads / 32)
-                join_row(a, 1, rec.parts, [&](int k) { return ((size_t)2 * (c + k) + (k == 0)) * kTileRows + r; }, lane,
+                join_row<4>(a, 1, rec.parts, [&](int k) { return ((size_t)2 * (c + k) + (k == 0)) * kTileRows + r; }, lane,
                          out_of(rec, r));
         }
     // streaming units: a sequence's come in groups of `parts` per (tile, head)
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(PagedAttnArgs a) {
         for (int u = blockIdx.x; u < n; u += gridDim.x) {
             const JoinRecord rec = a.record[0][u];
             if (warp < (rec.parts ? rec.n_rows : 0))
-                join_row(a, 0, rec.parts, [&](int k) { return (size_t)(u + k * a.n_kv_head) * kFewRows + warp; }, lane,
+                join_row<8>(a, 0, rec.parts, [&](int k) { return (size_t)(u + k * a.n_kv_head) * kFewRows + warp; }, lane,
                          out_of(rec, warp));
         }
     }
