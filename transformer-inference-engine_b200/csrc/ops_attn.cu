@@ -339,18 +339,20 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(PagedAttnArgs a) 
 // per SM, at most a portable cluster; 0 for few_rows_kernel, which shares the
 // keys out evenly over all SMs and joins with a second kernel. The tables' width
 // bounds the contexts; a warp of the cluster has width / (8 x CTAs) pages at
-// most. One sequence, one K/V head, bf16, on the GPU alone (cluster / shared
-// out): 1000 positions 5.1 / 11.4 us, 4000 7.1 / 11.9, 16,000 (15.6 pages a
-// warp) 15.7 / 14.8, 32,000 27.3 / 19.5; 12 heads: 16,000 17.2 / 22.2, 32,000
-// 39.7 / 35.4. Where the clusters fill the GPU (16 sequences of 12 heads, 4000
-// positions: 33.5 / 45.8) longer contexts are worth it too, up to where one long
-// sequence among short ones would be left to a single cluster.
+// most. On the GPU alone, bf16 (cluster / shared out, us):
+//   1 sequence, 1 head     1000 positions 4.1 / 9.3, 4000 6.5 / 9.5, 8000 (7.8 pages a
+//                          warp) 9.4 / 9.5, 16,000 15.4 / 10.9, 32,000 26.4 / 14.7
+//   1 sequence, 12 heads   8000 10.0 / 11.8, 16,000 (15.6) 15.8 / 17.0, 32,000 38.1 / 28.1
+//   16 sequences, 12 heads 1000 13.6 / 15.8, 4000 52.1 / 59.6, 16,000 (125) 174.6 / 188.9
+// so 8 pages a warp where the clusters take less than half of the SMs, 16 up to two a SM,
+// and 64 where they fill the GPU: up to where one long sequence among short ones would be
+// left to a single cluster.
 int cluster_ctas(int n_seq, int n_kv_head, int pages_per_seq, int sms) {
     const long long units = (long long)n_seq * n_kv_head;
     int ctas = 1;
     while (ctas < 8 && 2 * ctas * units <= 4LL * sms && ctas * kFewWarps < pages_per_seq) ctas *= 2;
-    const bool fills = units * ctas >= 2LL * sms;
-    return pages_per_seq <= (fills ? 64 : 16) * kFewWarps * ctas ? ctas : 0;
+    const int a_warp = units * ctas >= 2LL * sms ? 64 : 2 * units * ctas >= sms ? 16 : 8;
+    return pages_per_seq <= a_warp * kFewWarps * ctas ? ctas : 0;
 }
 
 cudaError_t launch_few_cluster(const PagedAttnArgs& a, bool bf16, int rows, int ctas, cudaStream_t st) {
