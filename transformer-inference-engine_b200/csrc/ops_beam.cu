@@ -10,7 +10,11 @@
 // finished beam offers only (eos, score_b). The logits are read once: a CTA
 // per (row, slice of the vocabulary) keeps the slice's maximum, its sum of
 // exponentials and its `beams` largest logits; a CTA per request then joins
-// the slices and picks. Bound by the reading of the logits.
+// the slices and picks. 96 requests of 6 beams over 50,257 tokens: 37 us (29 the scan,
+// 8 the picking), against 17.7 for the logits' bytes. All CTAs are one wave, and each has
+// its pass, its bound, a second look and its lists one after the other, so memory idles
+// in the later ones (46 % of its rate, 37 % of the issue slots). One request of 4 beams:
+// 8.7 us on the GPU, two kernels' latency.
 //
 // Totals decide an order, so they are formed in double: exponentials in fp32
 // (x - max is exact where the terms are large), their sum, the logarithm and
