@@ -93,11 +93,23 @@ namespace {
 #include "tc_ptx.cuh"
 
 constexpr int kThreads = 640;
-// registers a thread: at launch, and after the warpgroups have shared them out
-// (softmax 2 x 128 threads, loaders 2 x 128, MMA 128); the sum must not pass
-// what the block was launched with
-constexpr int kRegsLaunch = 96, kRegsSoftmax = 112, kRegsLoad = 104, kRegsMma = 48;
-static_assert(256 * kRegsSoftmax + 256 * kRegsLoad + 128 * kRegsMma <= kThreads * kRegsLaunch, "register split");
+// Registers a thread: at launch, and after the warpgroups have shared them out (softmax
+// 2 x 128 threads, loaders 2 x 128, MMA 128); the sum must not pass what the block was
+// launched with, and a share that is taken with .inc (or .dec) not be below (above) it.
+// fp32 rows take the loaders twice the registers of bf16 ones, and the mixed batch and the
+// chunk below are bound by the loaders' and the softmax's code: 112 / 104 / 48 took 286 and
+// 856 us, 112 / 112 / 32 253 and 941, 120 / 96 / 48 315 and 855, 104 / 112 / 48 265 and 1,249.
+constexpr int kRegsLaunch = 96;
+template <bool BF16>
+constexpr int kRegsSoftmax = 112;
+template <bool BF16>
+constexpr int kRegsLoad = BF16 ? 104 : 112;
+template <bool BF16>
+constexpr int kRegsMma = BF16 ? 48 : 32;
+template <bool BF16>
+constexpr bool kRegsFit = 256 * kRegsSoftmax<BF16> + 256 * kRegsLoad<BF16> + 128 * kRegsMma<BF16> <= kThreads * kRegsLaunch &&
+                          kRegsSoftmax<BF16> >= kRegsLaunch && kRegsLoad<BF16> >= kRegsLaunch && kRegsMma<BF16> <= kRegsLaunch;
+static_assert(kRegsFit<true> && kRegsFit<false>, "register split");
 constexpr int kSoftmaxWarps = 8, kLoadWarps = 8, kMmaWarp = 16, kUnitWarp = 17;
 constexpr uint32_t kWaitLimitNs = 2000000000u;  // 2 s
 constexpr unsigned kAll = 0xffffffffu;
@@ -606,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
         // ------------------------------------------------------------ softmax
         // tcgen05.ld / .st are warp-collective: every condition around them is
         // the warp's.
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax<BF16>));
         const int st = warp >> 2, qq = warp & 3, r = qq * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(qq * 32) << 16);
         uint32_t lasts = 0, pairs = 0;      // o_last and pair_in phases so far
@@ -840,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
         }
     } else if (warp < kSoftmaxWarps + kLoadWarps) {
         // ------------------------------------------------------------ loaders
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsLoad<BF16>));
         const int lw = warp - kSoftmaxWarps, sub = lane >> 3, dl = lane & 7;
         Row8<BF16> kr[4], vr[4];
         // the rows of step j of a tile that this warp has: its page (or -1), and their
@@ -1011,7 +1023,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma<BF16>));
         if (warp == kMmaWarp) {
             // ------------------------------------------------------------ MMA
             const uint32_t sb = smem_u32(smem), tm = __shfl_sync(kAll, tmem, 0);
