@@ -65,13 +65,13 @@
 //   16    allocates TMEM and issues the MMAs: whatever is ready, S up to three jobs
 //         ahead of P . V, each kind in the order of the jobs.
 //   17    walks the CTA's stretch and leaves each tile's description in a ring.
-//   18-19 only complete the warpgroup.
+//   18    leaves the join its record; 19 only completes the warpgroup.
 // The roles' loops together outgrow the instruction cache, so loops that would be
 // unrolled elsewhere are not and waits are kept short: 16 % -> 7 % of the fetches
 // missed, 1,050 -> 955 us for the chunk above, 357 -> 335 us for 48 mixed sequences.
 // In all, with the join: the chunk (32 query heads on 8) 860 us, of which 311 are its
 // MMAs at the measured rate; 48 sequences of up to 117 new rows and 900 cached, 25
-// heads, fp32: 289 us, bound by the loaders' chain of a step (convert keys, convert
+// heads, fp32: 242 us, bound by the loaders' chain of a step (convert keys, convert
 // values, wait for their buffers) and by a tile's start, not by memory (51 us).
 // TMEM (512 columns): three S / P (384), two O (128).
 // Every wait is bounded: on expiry it raises the abort flag, which ends every
@@ -96,9 +96,9 @@ constexpr int kThreads = 640;
 // Registers a thread: at launch, and after the warpgroups have shared them out (softmax
 // 2 x 128 threads, loaders 2 x 128, MMA 128); the sum must not pass what the block was
 // launched with, and a share that is taken with .inc (or .dec) not be below (above) it.
-// fp32 rows take the loaders twice the registers of bf16 ones, and the mixed batch and the
-// chunk below are bound by the loaders' and the softmax's code: 112 / 104 / 48 took 286 and
-// 856 us, 112 / 112 / 32 253 and 941, 120 / 96 / 48 315 and 855, 104 / 112 / 48 265 and 1,249.
+// fp32 rows take the loaders twice the registers of bf16 ones: 112 / 104 / 48 took 286 us
+// for the mixed batch above (fp32) and 856 for the chunk (bf16), 112 / 112 / 32 253 and 941,
+// 120 / 96 / 48 315 and 855, 104 / 112 / 48 265 and 1,249.
 constexpr int kRegsLaunch = 96;
 template <bool BF16>
 constexpr int kRegsSoftmax = 112;
@@ -1071,7 +1071,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
 #pragma unroll 1
                 for (int term = 2; term >= 0; term -= BF16 ? 2 : 1) {
                     const uint32_t qt = qb + (term == 2 ? kTermBytes : 0u), kt = kb + (term == 1 ? kTermBytes : 0u);
-#pragma unroll
+#pragma unroll (BF16 ? 4 : 1)
                     for (int ks = 0; ks < kHeadDim / 16; ++ks)
                         mma_f16(d, sw128_desc(qt + 32u * ks), sw128_desc(kt + 32u * ks), kIdescS, ks || term < 2 ? 1u : 0u);
                 }
@@ -1115,7 +1115,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
 #pragma unroll 1
                     for (int term = 2; term >= 0; --term) {
                         const uint32_t pt = term == 2 ? 16u : 0u, vt = vb + (term == 1 ? kTermBytes : 0u);
-#pragma unroll
+#pragma unroll 2
                         for (int ks = 0; ks < kTileKeys / 16; ++ks)
                             mma_f16_ta(d, p_at(ks) + pt, sw128_desc(vt + 2048u * ks), kIdescO, ks || term < 2 ? 1u : more);
                     }

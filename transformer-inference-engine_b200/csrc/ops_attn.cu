@@ -429,7 +429,6 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
     a.q = q; a.ldq = ldq; a.n_head = n_head;
     a.k = k_pages; a.v = v_pages;
     a.n_pages = n_pages; a.n_kv_head = n_kv_head; a.group = n_head / n_kv_head;
-    a.group_inv = a.group == 1 ? 0 : ~0ull / (unsigned)a.group + 1;
     a.table = page_table; a.width = pages_per_seq;
     a.row_start = row_start; a.ctx = ctx_lens;
     a.n_seq = n_seq; a.max_new = max_new; a.rows = rows;

@@ -40,7 +40,6 @@ struct PagedAttnArgs {
     int ldq, n_head;
     const void *k, *v;
     int n_pages, n_kv_head, group;
-    unsigned long long group_inv;  // 2^64 / group, rounded up (0 for group 1)
     const int32_t* table;
     int width;
     const int32_t *row_start, *ctx;
@@ -59,11 +58,6 @@ struct PagedAttnArgs {
     int only_few;                  // every sequence is of the streaming kind
     int* status;
 };
-
-// the new token that a sequence's row i belongs to: i / group, exact for 32-bit i
-__device__ __forceinline__ int token_of(const PagedAttnArgs& a, int i) {
-    return a.group == 1 ? i : (int)__umul64hi((unsigned long long)i, a.group_inv);
-}
 
 __host__ __device__ inline int tile_rows_of(int kind) { return kind ? kTileRows : kFewRows; }
 // fewest pages worth a streaming unit of their own (four for each warp), fewest
