@@ -86,11 +86,14 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None) -> str:
 
 
 def build_ops_module() -> str:
-    """tie_b200/_ops, the Python side of the operators' calls."""
+    """tie_b200/_ops, the Python side of the operators' calls ("" without torch, whose tensors it reads)."""
+    torch = importlib.util.find_spec("torch")
+    if torch is None:
+        return ""
     newest = max([os.path.getmtime(OPS_SRC)] + [os.path.getmtime(os.path.join(INCLUDE, f)) for f in os.listdir(INCLUDE)])
     if os.path.exists(OPS_PATH) and os.path.getmtime(OPS_PATH) >= newest:
         return OPS_PATH
-    torch_dir = importlib.util.find_spec("torch").submodule_search_locations[0]
+    torch_dir = torch.submodule_search_locations[0]
     tmp = OPS_PATH + ".tmp"
     cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-I" + INCLUDE,
            "-I" + sysconfig.get_paths()["include"], "-isystem", os.path.join(torch_dir, "include"), OPS_SRC, "-o", tmp]
