@@ -1,0 +1,62 @@
+"""The operators over the paged cache at the edges of the number range and of their arguments, on the GPU."""
+import os
+import sys
+
+import numpy as np
+import pytest
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+torch = pytest.importorskip("torch")
+import ops_oracle as ref  # noqa: E402
+from test_ops_gpu import KV, _attend, _batch, _i  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+PAGE, D = 16, 64
+
+
+def _positions(b, s):
+    """Pages and rows of sequence s's positions, cached and new."""
+    pos = np.arange(b["ctx"][s] + b["start"][s + 1] - b["start"][s])
+    return torch.from_numpy(b["table"][s][pos // PAGE]).cuda(), torch.from_numpy(pos % PAGE).cuda()
+
+
+# ------------------------------------------------------------------ values of very different sizes
+
+# exponents of the value rows by position (None: a row of zeros)
+SIZES = {
+    "zeros, then large": lambda pos, n: np.where(pos < n // 2, np.nan, 70),
+    "large, then zeros": lambda pos, n: np.where(pos < n // 2, 70, np.nan),
+    "tiny, then huge": lambda pos, n: np.where(pos < n // 2, -60, 100),
+    "huge, then tiny": lambda pos, n: np.where(pos < n // 2, 100, -60),
+    "ones and huge by pages": lambda pos, n: np.where(pos // PAGE % 2, 100, 0),
+    "zeros and huge by rows": lambda pos, n: np.where(pos % 2, 100, np.nan),
+    "zeros and huge by steps": lambda pos, n: np.where(pos // 128 % 2, 100, np.nan),
+    "huge at last": lambda pos, n: np.where(pos < n - 5, np.nan, 100),
+    "rising": lambda pos, n: -100 + 200 * pos // n,
+    "falling": lambda pos, n: 100 - 200 * pos // n,
+}
+
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("sizes", SIZES)
+@pytest.mark.parametrize("n_seq,kv_heads,group,ctx,new", [
+    (1, 1, 1, 700, 1), (1, 1, 1, 0, 150), (1, 1, 2, 700, 9), (1, 2, 1, 650, 150), (1, 1, 1, 3000, 40), (80, 4, 1, 300, 12)])
+def test_attention_counts_keys_whatever_their_values(kv, sizes, n_seq, kv_heads, group, ctx, new):
+    """A key's weight does not depend on how large its value is beside the others': the row sum keeps keys whose
+    values are zero or tiny when others' are huge. The bound is attention_bound's, in units of the largest value,
+    and 2^-106 for values below 2^-67, which are multiplied by 2^81 and not more: a second fp16 term of
+    subnormal size is rounded by at most 2^-25 then, 2^-106 of the value, and the weights of a row add up to 1."""
+    b = _batch(np.random.default_rng(ctx + new), [ctx] * n_seq, [new] * n_seq, kv_heads * group, kv_heads, kv)
+    for s in range(n_seq):
+        page, row = _positions(b, s)
+        e = SIZES[sizes](np.arange(ctx + new), ctx + new)
+        size = torch.from_numpy(np.where(np.isnan(e), 0.0, np.exp2(np.nan_to_num(e)))).cuda()[:, None]
+        b["v"][page, row] = (b["v"][page, row].double() * size).to(kv)
+    status = _i([0])
+    got = _attend(b, status=status).cpu().numpy().astype(np.float64)
+    want, vmax, smax = ref.attention(b["q"].cpu().numpy().astype(np.float64), b["k"].cpu().double().numpy(),
+                                     b["v"].cpu().double().numpy(), b["table"], b["start"], b["ctx"], kv_heads * group,
+                                     kv_heads, 0.125, np.zeros(got.shape))
+    assert int(status[0]) == 0
+    bad = ~(np.abs(got - want) <= ref.attention_bound(vmax, smax, ctx + new) + 2.0 ** -106)
+    assert not bad.any(), (bad.sum(), np.argwhere(bad)[:4], got[bad][:4], want[bad][:4])

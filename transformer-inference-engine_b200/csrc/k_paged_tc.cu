@@ -31,7 +31,10 @@
 //     2^(t_j - m) (v_j 2^-e_j) = 2^(s_j - m) v_j. The row sum is
 //     sum 2^(t_j - m) 2^-e_j. With m at most 8 below the largest t so far, the
 //     probabilities lie in [0, 2^15] around 2^7 and their small ones keep an
-//     absolute error of 2^-32 of the largest.
+//     absolute error of 2^-32 of the largest. What falls below 2^-126 is nothing
+//     to O, but in the row sum it may be the largest weight there is (a row of
+//     zeros beside values of 2^70). A sum that could miss such weights is small
+//     (kLeastSum), and the epilogue forms it anew from the scores alone.
 // A scale belongs to one row where rows may be masked (steps that cross the
 // diagonal), so a masked row's range costs no visible one bits; elsewhere the 16
 // rows of a page, which every query row sees, share theirs.
@@ -137,6 +140,9 @@ static_assert((kOpsMaxSeqs + 1) * 8 <= (int)kOffKeys, "line of jobs");
 template <bool BF16>
 constexpr int kFlush = BF16 ? 4 : 2;
 constexpr float kFarUp = 40.f;     // the running O is rescaled when the maximum has grown by this
+// A key whose 2^(s + e - m) flushed weighs less than 2^(81 - 126) in the row sum (e >= -81).
+// A sum of this for each of its keys has lost less than 2^-24 of itself.
+constexpr float kLeastSum = 0x1p-21f;
 
 // TMEM columns: S / P of buffer b at 128 b, O of stream st at kColO + 64 st
 constexpr uint32_t kTmemCols = 512, kColO = 384;
@@ -506,8 +512,55 @@ __device__ __noinline__ void add_odd(const void* values, const int32_t* table, s
     }
 }
 
+// four elements of a row of the pool
 template <bool BF16>
-__global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) {
+__device__ __forceinline__ float4 four_of(const void* pool, size_t at) {
+    if constexpr (BF16) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(pool) + at));
+        return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                           __uint_as_float(u.y & 0xffff0000u));
+    } else {
+        return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(pool) + at));
+    }
+}
+
+// The row sum, relative to the maximum m, of row i of the unit's sequence over those of the unit's
+// keys that it sees, from the scores alone. Rare, hence simple: four keys at a time, which a warp's
+// rows share.
+template <bool BF16>
+__device__ __noinline__ float row_sum(const PagedAttnArgs& a, const volatile Unit& n, int i, float m) {
+    const size_t w = (size_t)a.n_kv_head * kHeadDim;
+    const float* q = a.q + (size_t)(n.token0 + i / a.group) * a.ldq + (n.g * a.group + i % a.group) * kHeadDim;
+    const int32_t* table = a.table + (size_t)n.s * a.width;
+    const int key1 = min(n.key1, n.ctx + i / a.group + 1);
+    float sum = 0.f;
+    constexpr int kKeys = 4;
+#pragma unroll 1
+    for (int key = n.key0; key < key1; key += kKeys) {     // (key0 is a multiple of a page)
+        const int page = __ldg(table + key / kPageRows);
+        if (page < 0 || page >= a.n_pages) continue;
+        const size_t from = ((size_t)page * kPageRows + key % kPageRows) * w + (size_t)n.g * kHeadDim;
+        float s[kKeys] = {};
+#pragma unroll 2
+        for (int d = 0; d < kHeadDim; d += 4) {
+            const float4 x = __ldg(reinterpret_cast<const float4*>(q + d));
+#pragma unroll
+            for (int r = 0; r < kKeys; ++r) {
+                const float4 y = four_of<BF16>(a.k, from + r * w + d);
+                s[r] = fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, fmaf(x.x, y.x, s[r]))));
+            }
+        }
+        float part = 0.f;
+#pragma unroll
+        for (int r = 0; r < kKeys; ++r)
+            if (key + r < key1) part += ex2_ftz(fmaf(s[r], a.scale2, kBase - m));
+        sum += part;
+    }
+    return sum;
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_constant__ PagedAttnArgs a) {
     pdl_trigger();                     // few_rows_kernel takes the SMs that are done
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -695,15 +748,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                     }
                     tmem_ld32_start(col_s + 32u * ((c + 1) & 3), x);   // the last one begins the second pass
                 }
-                float alpha = 1.f;
+                float alpha = 1.f, sum = 0.f;
                 const float m_o = m;           // what O is relative to
                 if (mt > m + kSlack || m == -INFINITY) {      // also the first finite maximum
                     alpha = ex2_ftz(m - mt);                  // m = -inf: 0 (or, mt = -inf too, unused)
+                    if (alpha == 0.f) sum = weigh(l, m - mt); // the row sum may outweigh it
                     if (mt == -INFINITY) alpha = 1.f;
                     m = mt;
                 }
                 const float lift = m == -INFINITY ? 0.f : kBase - m;
-                float sum = 0.f;
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     tmem_arrived(x);
@@ -798,6 +851,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
             };
             uint32_t o[32];
             if (both) {
+                if (l < (float)steps * (kTileKeys * kLeastSum) && m != -INFINITY && row < n_rows) l = row_sum<BF16>(a, n, i, m);
                 asm volatile("tcgen05.fence::after_thread_sync;");
 #pragma unroll 1
                 for (int h = 0; h < 2; ++h) {
@@ -828,6 +882,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                 const float m0 = xch[r], l0 = xch[kHalfRows + r], m1 = xch[2 * kHalfRows + r], l1 = xch[3 * kHalfRows + r];
                 const float mm = fmaxf(m0, m1), base = mm == -INFINITY ? 0.f : mm;
                 const float f0 = ex2_ftz(m0 - base), f1 = ex2_ftz(m1 - base);
+                float ll = fmaf(l1, f1, l0 * f0);
+                const float far = fminf(m0, m1) - base;
+                if ((ll < (float)steps * (kTileKeys * kLeastSum) || (far < -126.f && far > -INFINITY)) && mm != -INFINITY && row < n_rows)
+                    ll = row_sum<BF16>(a, n, i, mm);
                 uint32_t v1[32];
                 tmem_ld32_start(lanes + kColO + 32u * st, o);
                 tmem_arrived(o);
@@ -846,7 +904,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(PagedAttnArgs a) 
                     if (f1 > 0.f) v = fmaf(__uint_as_float(v1[d]), f1, v);
                     o[d] = __float_as_uint(v);
                 }
-                if (row < n_rows) put(o, 32 * st, mm, fmaf(l1, f1, l0 * f0));
+                if (row < n_rows) put(o, 32 * st, mm, ll);
             }
             unit_read(un);
         }

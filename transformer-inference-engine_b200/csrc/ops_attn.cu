@@ -296,7 +296,7 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs& a, int kind, int p
         for (int u = 0; u < kAhead; ++u) {
             if (k0 + u >= parts) break;
             const float f = ex2_ftz(ml[u].x - base);
-            l = fmaf(ml[u].y, f, l);
+            l = f > 0.f ? fmaf(ml[u].y, f, l) : l + weigh(ml[u].y, ml[u].x - base);
             if (f > 0.f) { ox = fmaf(v[u].x, f, ox); oy = fmaf(v[u].y, f, oy); }
         }
     }

@@ -295,6 +295,13 @@ __device__ __forceinline__ float ex2_ftz(float x) {
     return y;
 }
 
+// l 2^d for d <= 0. The row sum of a part of the tensor-core kernel is between 2^-106 and
+// 2^126 (its maximum counts the values' exponents), so where 2^d flushes l 2^d need not.
+__device__ __forceinline__ float weigh(float l, float d) {
+    const float half = ex2_ftz(0.5f * d);
+    return d >= -126.f ? l * ex2_ftz(d) : l * half * half;
+}
+
 // Tensor-core kernel (k_paged_tc.cu) for the sequences of kind 1.
 cudaError_t launch_paged_attn_tc(const PagedAttnArgs& a, bool bf16, cudaStream_t st);
 
