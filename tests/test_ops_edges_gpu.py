@@ -60,3 +60,18 @@ def test_attention_counts_keys_whatever_their_values(kv, sizes, n_seq, kv_heads,
     assert int(status[0]) == 0
     bad = ~(np.abs(got - want) <= ref.attention_bound(vmax, smax, ctx + new) + 2.0 ** -106)
     assert not bad.any(), (bad.sum(), np.argwhere(bad)[:4], got[bad][:4], want[bad][:4])
+
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("n_seq,kv_heads,ctx,new", [
+    (1, 1, 0, 1), (1, 1, 900, 1), (1, 12, 1900, 2), (1, 1, 20011, 1), (1, 1, 20011, 4), (160, 2, 300, 1), (1, 1, 700, 9),
+    (80, 4, 300, 12), (1, 1, 5000, 40)])
+def test_attention_of_the_largest_values_is_finite(kv, n_seq, kv_heads, ctx, new):
+    """The mean of finite values is finite, also where their sum is not."""
+    b = _batch(np.random.default_rng(ctx), [ctx] * n_seq, [new] * n_seq, kv_heads, kv_heads, kv)
+    b["v"].copy_((b["v"].double().abs().clamp(max=1.0) * 0.5 + 0.4) * 2.0 ** 127)       # 0.4 to 0.9 of 2^127
+    got = _attend(b).cpu().numpy().astype(np.float64)
+    want, vmax, smax = ref.attention(b["q"].cpu().numpy().astype(np.float64), b["k"].cpu().double().numpy(),
+                                     b["v"].cpu().double().numpy(), b["table"], b["start"], b["ctx"], kv_heads, kv_heads,
+                                     0.125, np.zeros(got.shape))
+    assert (np.abs(got - want) <= ref.attention_bound(vmax, smax, ctx + new)).all()

@@ -36,6 +36,9 @@ namespace cg = cooperative_groups;
 // in shared memory.
 constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
 constexpr unsigned kAll = 0xffffffffu;
+// Weights are 2^(s - max) times this, so that the sum of as many of them as there are
+// positions (2^30) times any finite value stays finite.
+constexpr float kWeight = 0x1p-30f;
 
 template <bool BF16>
 __device__ __forceinline__ float4 load4(const void* base, size_t at) {
@@ -109,7 +112,7 @@ __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const SeqShape&
 #pragma unroll
             for (int x = 2; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, x));
             const float m_new = fmaxf(m[r], mx), base = m_new == -INFINITY ? 0.f : m_new;
-            const float alpha = ex2_ftz(m[r] - base), pr = ex2_ftz(sc - base);
+            const float alpha = ex2_ftz(m[r] - base), pr = kWeight * ex2_ftz(sc - base);
             m[r] = m_new;
             l[r] = fmaf(l[r], alpha, pr);                  // two lanes hold each position: halved at the end
 #pragma unroll
