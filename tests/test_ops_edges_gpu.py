@@ -75,3 +75,43 @@ def test_attention_of_the_largest_values_is_finite(kv, n_seq, kv_heads, ctx, new
                                      b["v"].cpu().double().numpy(), b["table"], b["start"], b["ctx"], kv_heads, kv_heads,
                                      0.125, np.zeros(got.shape))
     assert (np.abs(got - want) <= ref.attention_bound(vmax, smax, ctx + new)).all()
+
+
+# ------------------------------------------------------------------ values that are not finite
+
+# positions that score far below the others
+LOW = {
+    "one position": lambda pos, n: pos == n // 2,
+    "one warp's pages": lambda pos, n: pos // PAGE % 8 == 3,
+    "one CTA's pages": lambda pos, n: pos // 128 % 8 == 1,
+    "the first half": lambda pos, n: pos < n // 2,
+    "the second half": lambda pos, n: (pos >= n // 2) & (pos < n - 60),
+}
+
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("odd", [float("inf"), float("nan")])
+@pytest.mark.parametrize("low", LOW)
+@pytest.mark.parametrize("n_seq,kv_heads,ctx,new", [
+    (1, 1, 240, 1), (1, 1, 900, 1), (1, 12, 1900, 2), (1, 1, 20011, 1), (1, 1, 20011, 4), (160, 2, 300, 1), (1, 1, 700, 9),
+    (1, 2, 300, 60), (80, 4, 300, 12), (1, 1, 5000, 40)])
+def test_attention_values_that_are_not_finite_reach_the_rows_that_see_them(kv, odd, low, n_seq, kv_heads, ctx, new):
+    """However small its probability, and whoever read it (the maximum's warp, CTA or part, or another): a value
+    that is not finite makes its dimension of every row that sees it not finite, and nothing else."""
+    n = ctx + new
+    b = _batch(np.random.default_rng(ctx), [ctx] * n_seq, [new] * n_seq, kv_heads, kv_heads, kv)
+    b["q"].mul_(0.01)
+    b["q"][:, ::D] = 1.0
+    b["k"][..., ::D] = 0.0
+    lows = LOW[low](np.arange(n), n)
+    at = int(np.flatnonzero(lows)[lows.sum() // 2])
+    for s in range(n_seq):
+        page, row = _positions(b, s)
+        where = torch.from_numpy(lows).cuda()
+        b["k"][page[where], row[where], ::D] = -400.0        # the others score about 0
+        b["v"][page[at], row[at], 5::D] = odd
+    got = _attend(b, scale=1.0).view(n_seq, new, kv_heads, D)
+    sees = torch.arange(new, device="cuda") + ctx >= at
+    assert not bool(got[:, sees][..., 5].isfinite().any())
+    got[:, sees, :, 5] = 0.0
+    assert bool(got.isfinite().all())

@@ -154,7 +154,9 @@ __device__ __forceinline__ void few_rows_n(const PagedAttnArgs& a, const SeqShap
     else few_rows<RMAX, BF16>(a, q, s, tile, g, p0, p1, stride, n_rows, sm);
 }
 
-// Row r, dim d of the warps' partials joined.
+// Row r, dim d of the warps' partials joined. (Here and in the other joins a partial that
+// has seen no key is all zeros, and one whose factor is zero is still multiplied: a value
+// that is not finite stays so, as it does within a warp.)
 struct Joined {
     float m, l, o;
 };
@@ -167,7 +169,7 @@ __device__ __forceinline__ Joined join_warps(const FewSmem& sm, int r, int d) {
     for (int w = 0; w < kFewWarps; ++w) {
         const float f = ex2_ftz(sm.m[w][r] - base);
         j.l = fmaf(sm.l[w][r], f, j.l);
-        if (f > 0.f) j.o = fmaf(sm.o[w][r][d], f, j.o);
+        j.o = fmaf(sm.o[w][r][d], f, j.o);
     }
     return j;
 }
@@ -214,8 +216,7 @@ __global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_cluster_ke
         for (int c = 0; c < ctas; ++c) {
             const float f = ex2_ftz(*cluster.map_shared_rank(&c_m[r], c) - base);
             l = fmaf(*cluster.map_shared_rank(&c_l[r], c), f, l);
-            const float v = *cluster.map_shared_rank(&c_o[r][d], c);
-            if (f > 0.f) o = fmaf(v, f, o);
+            o = fmaf(*cluster.map_shared_rank(&c_o[r][d], c), f, o);
         }
         out_at(r, d) = l == 0.f ? 0.f : o / l;
     }
@@ -300,7 +301,8 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs& a, int kind, int p
             if (k0 + u >= parts) break;
             const float f = ex2_ftz(ml[u].x - base);
             l = f > 0.f ? fmaf(ml[u].y, f, l) : l + weigh(ml[u].y, ml[u].x - base);
-            if (f > 0.f) { ox = fmaf(v[u].x, f, ox); oy = fmaf(v[u].y, f, oy); }
+            ox = fmaf(v[u].x, f, ox);
+            oy = fmaf(v[u].y, f, oy);
         }
     }
     *reinterpret_cast<float2*>(out + 2 * lane) = l == 0.f ? make_float2(0.f, 0.f) : make_float2(ox / l, oy / l);
