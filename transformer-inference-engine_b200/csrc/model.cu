@@ -1678,6 +1678,7 @@ model_status model_extend_batch(model* m, const int32_t* ids, size_t n_seq, size
     if ((rc = grow(&m->d_ops, &m->ops_cap, 3 * n_seq + 1 + 3 * rows + 1)) != MODEL_OK) return rc;
     if ((rc = grow(&m->d_ops_ws, &m->ops_ws_cap, tie_attention_paged_workspace())) != MODEL_OK) return rc;
     if ((rc = ensure_pinned(m, 2 * n_seq)) != MODEL_OK) return rc;
+    if ((rc = stats_begin(m)) != MODEL_OK) return rc;   // (its layers add none; finish() merges what is there)
     if ((rc = copy_ids_to_device(m, ids, rows)) != MODEL_OK) return rc;
     int32_t *ctx = m->d_ops, *fresh = ctx + n_seq, *start = fresh + n_seq, *seq = start + n_seq + 1, *pos = seq + rows;
     int32_t *slots = pos + rows, *status = slots + rows;
