@@ -112,8 +112,10 @@ model_status model_generate_greedy_device(model *m, const int32_t *d_prompts, si
  * values go into the pool and its length grows by n_ids. As for
  * model_prefill_batch, logits_out (host, n_seq * n_ids * vocab floats, or NULL)
  * receives the new positions' logits and next_ids (host, n_seq, or NULL) each
- * sequence's greedy choice at its last position. Attention statistics
- * (model_collect_attn_stats) do not cover this call. At most 4096 sequences. */
+ * sequence's greedy choice at its last position. A sequence that does not hold
+ * the pool's length (never prefilled to it, released, or overwritten by a call
+ * that failed) is MODEL_ERR_ARG. Attention statistics (model_collect_attn_stats)
+ * do not cover this call. At most 4096 sequences. */
 model_status model_extend_batch(model *m, const int32_t *ids, size_t n_seq, size_t n_ids,
                                 float *logits_out, size_t logits_cap, int32_t *next_ids);
 

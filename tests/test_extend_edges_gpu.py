@@ -31,3 +31,26 @@ def test_an_extension_adds_nothing_to_the_attention_statistics(fresh):
     assert m.attn_rowsum_range() == before
     m.decode_step_batch(ids[:, 20])                  # and the next call's are counted once
     assert m.attn_rowsum_range()[2] == before[2] + before[2] // 9
+
+
+def test_an_extension_of_sequences_that_hold_less_is_refused(fresh):
+    """Released, never filled, or overwritten by a call that failed: there is nothing to attend to."""
+    m, ref = fresh
+    ids = synth.prompt_ids(m.vocab, 3, 30, seed=4)
+    m.batch_reserve_pages(3, 48, 5)
+    m.prefill_batch(ids[:2, :12])
+    assert m.extend_batch(ids[:, 12:14], check=False)[0] == ARG          # the third was never filled
+    _, lg = m.extend_batch(ids[:2, 12:14], want_logits=True)
+    m.batch_release(1)
+    assert m.extend_batch(ids[:2, 14:15], check=False)[0] == ARG
+    _, more = m.extend_batch(ids[:1, 14:16], want_logits=True)           # the first still holds its positions
+    want = ref.prefill(ids[0, :16])
+    assert np.abs(np.concatenate([lg[0], more[0]]) - want[12:16]).max() <= 1e-3
+    m.prefill_batch(ids[:2, :16])                                        # filled again
+    m.extend_batch(ids[:2, 16:17])
+    m.prefill_batch(ids[:2, :12])
+    assert m.generate_beam(ids[:1, :12], 3, 25, check=False)[0] == tie_b200.MODEL_STATUS.index("MODEL_ERR_CAPACITY")
+    assert m.extend_batch(ids[:2, 12:13], check=False)[0] == ARG         # the search had begun to overwrite them
+    m.prefill_batch(ids[:2, :8])
+    nxt, lg = m.extend_batch(ids[:2, 8:20], want_logits=True)
+    assert np.abs(lg - np.stack([ref.prefill(p[:20])[8:] for p in ids[:2]])).max() <= 1e-3

@@ -31,6 +31,7 @@ struct kv_cache {
     float* v = nullptr;
     int* d_page_table = nullptr;
     tie::PageTable pages;   // pools only
+    std::vector<int> held;  // pools only: positions of each sequence whose rows have been written
 };
 
 namespace tie {
@@ -44,6 +45,8 @@ kv_status kv_pool_create(int n_layer, int n_embd, int n_seq, int capacity, int n
 // that follow on it). KV_ERR_CAPACITY when too few pages are free (the pages
 // assigned so far stay assigned), KV_ERR_ARG for a bad range.
 kv_status kv_pool_map(kv_cache* c, int n_seq, int length, cudaStream_t st);
+// Sequences [0, n_seq) that held at least `from` positions hold `to` of them now.
+void kv_pool_hold(kv_cache* c, int n_seq, int from, int to);
 // Returns sequence seq's pages to the pool.
 kv_status kv_pool_release(kv_cache* c, int seq);
 

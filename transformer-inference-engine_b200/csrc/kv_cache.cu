@@ -44,6 +44,7 @@ static kv_status create_impl(int n_layer, int n_embd, int n_seq, int capacity, b
         for (size_t i = 0; i < entries; ++i) table[i] = (int)i;   // pages in order
     } else {
         c->pages = tie::PageTable(n_seq, capacity, n_pages);
+        c->held.assign((size_t)n_seq, 0);
         table = c->pages.device_view();                          // all entries on the scratch page
     }
     // A one-sequence cache is managed memory: its kv_cache_keys/values/*_row
@@ -92,9 +93,15 @@ kv_status kv_pool_map(kv_cache* c, int n_seq, int length, cudaStream_t st) {
     return rc;
 }
 
+void kv_pool_hold(kv_cache* c, int n_seq, int from, int to) {
+    for (int s = 0; s < n_seq; ++s)
+        if (c->held[(size_t)s] >= from) c->held[(size_t)s] = to;
+}
+
 kv_status kv_pool_release(kv_cache* c, int seq) {
     if (!c || c->contiguous || seq < 0 || seq >= c->n_seq) return KV_ERR_ARG;
     c->pages.release(seq);
+    c->held[(size_t)seq] = 0;
     return KV_OK;
 }
 

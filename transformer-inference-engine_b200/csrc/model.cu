@@ -1612,6 +1612,7 @@ static model_status batch_prefill_impl(model* m, size_t n_seq, size_t T, float* 
         CU(cudaMemcpyAsync(m->d_ids, ids, n_seq * T * sizeof(int32_t), cudaMemcpyDeviceToDevice, m->st));
     }
     if ((rc = map_pages(m, n_seq, T)) != MODEL_OK) return rc;
+    kv_pool_hold(m->pool, (int)n_seq, 0, 0);   // overwritten from here on
     if ((rc = run_prefill(m, (int)n_seq, (int)T, m->pool, 0)) != MODEL_OK) return rc;
     (void)next_host;
     return prefill_logits(m, n_seq, T, logits_host);
@@ -1633,6 +1634,7 @@ model_status model_prefill_batch(model* m, const int32_t* ids, size_t n_seq, siz
         CU(cudaMemcpyAsync(next_ids, m->d_next, n_seq * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
     if ((rc = finish(m)) != MODEL_OK) return rc;
     m->pool->length = (int)T;
+    kv_pool_hold(m->pool, (int)n_seq, 0, (int)T);
     return MODEL_OK;
 }
 
@@ -1657,6 +1659,7 @@ model_status model_decode_step_batch(model* m, const int32_t* ids, size_t n_seq,
     if (next_ids)
         CU(cudaMemcpyAsync(next_ids, m->d_next, n_seq * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
     if ((rc = finish(m)) != MODEL_OK) return rc;
+    kv_pool_hold(m->pool, (int)n_seq, m->pool->length, m->pool->length + 1);
     m->pool->length += 1;
     return MODEL_OK;
 }
@@ -1667,6 +1670,8 @@ model_status model_extend_batch(model* m, const int32_t* ids, size_t n_seq, size
     if (!m->pool || n_seq > (size_t)m->pool->n_seq) return MODEL_ERR_ARG;
     if (n_seq > (size_t)kOpsMaxSeqs) return MODEL_ERR_CAPACITY;
     const size_t pos0 = (size_t)m->pool->length;
+    for (size_t s = 0; s < n_seq; ++s)
+        if ((size_t)m->pool->held[s] < pos0) return MODEL_ERR_ARG;   // nothing to attend to
     if (T > (size_t)m->pool->capacity || pos0 + T > (size_t)m->pool->capacity) return MODEL_ERR_CAPACITY;
     if (logits && cap < n_seq * T * (size_t)m->cfg.vocab_size) return MODEL_ERR_CAPACITY;
     for (size_t i = 0; i < n_seq * T; ++i)
@@ -1700,6 +1705,7 @@ model_status model_extend_batch(model* m, const int32_t* ids, size_t n_seq, size
         CU(cudaMemcpyAsync(next_ids, m->d_next, n_seq * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
     if ((rc = finish(m)) != MODEL_OK) return rc;
     m->pool->length = (int)(pos0 + T);
+    kv_pool_hold(m->pool, (int)n_seq, 0, (int)(pos0 + T));
     return MODEL_OK;
 }
 
@@ -1741,7 +1747,8 @@ static model_status generate_impl(model* m, const int32_t* prompts, size_t n_seq
     if (host)
         CU(cudaMemcpyAsync(out_ids, d_out, n_seq * n_new * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
     m->pool->length = (int)(T + n_new - 1);
-    if (host) return finish(m);
+    if (host && (rc = finish(m)) != MODEL_OK) return rc;
+    kv_pool_hold(m->pool, (int)n_seq, 0, (int)(T + n_new - 1));
     return MODEL_OK;
 }
 
@@ -1824,6 +1831,7 @@ model_status model_generate_beam(model* m, const int32_t* prompts, size_t n_req,
     CU(cudaMemcpyAsync(h_sc.data(), scores, S * sizeof(float), cudaMemcpyDeviceToHost, m->st));
     if ((rc = finish(m)) != MODEL_OK) return rc;
     m->pool->length = (int)(T + n_new - 1);
+    kv_pool_hold(m->pool, (int)S, 0, (int)(T + n_new - 1));
     // each request's beams, best first, their tokens read back along the parents
     std::vector<size_t> order(beams);
     for (size_t r = 0; r < n_req; ++r) {
