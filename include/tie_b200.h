@@ -127,7 +127,9 @@ model_status model_extend_batch(model *m, const int32_t *ids, size_t n_seq, size
  * none. out_ids (host, n_req * beams * n_new) and out_scores (host, n_req *
  * beams): each request's continuations, best first. Requires a prior
  * model_batch_reserve covering n_req * beams sequences of n_prompt + n_new - 1
- * positions; the pool then holds the beams in no particular order. */
+ * positions. The pool then holds the continuations in the order of out_ids, all
+ * but their last tokens: sequence r * beams + i is request r's prompt and its
+ * i-th best continuation, ready for model_decode_step_batch on the last tokens. */
 model_status model_generate_beam(model *m, const int32_t *prompts, size_t n_req, size_t n_prompt,
                                  size_t beams, size_t n_new, int32_t eos_id, int32_t *out_ids,
                                  float *out_scores);

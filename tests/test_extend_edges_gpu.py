@@ -54,3 +54,24 @@ def test_an_extension_of_sequences_that_hold_less_is_refused(fresh):
     m.prefill_batch(ids[:2, :8])
     nxt, lg = m.extend_batch(ids[:2, 8:20], want_logits=True)
     assert np.abs(lg - np.stack([ref.prefill(p[:20])[8:] for p in ids[:2]])).max() <= 1e-3
+
+
+@pytest.mark.parametrize("beams,n_new,with_eos", [(3, 14, False), (5, 9, True), (4, 1, False), (1, 6, False), (2, 2, False), (6, 20, False)])
+def test_the_pool_holds_the_continuations_that_a_search_returns(fresh, beams, n_new, with_eos):
+    """Decoding or extending after a search goes on from each returned continuation, in their order (the engine's
+    contract with the oracle's logits, max-abs 1e-3)."""
+    m, ref = fresh
+    R, T = 3, 7
+    prompts = synth.prompt_ids(m.vocab, R, T, seed=beams)
+    m.batch_reserve(R * beams, T + n_new + 3)
+    eos = -1
+    if with_eos:
+        eos = int(m.generate_beam(prompts, beams, n_new)[0][0, 0, n_new // 2])
+    ids, _ = m.generate_beam(prompts, beams, n_new, eos)
+    whole = np.concatenate([np.repeat(prompts, beams, 0), ids.reshape(R * beams, n_new)], 1).astype(np.int32)
+    _, lg = m.decode_step_batch(whole[:, -1], want_logits=True)
+    more = synth.prompt_ids(m.vocab, R * beams, 3, seed=1)
+    _, lg2 = m.extend_batch(more, want_logits=True)
+    for s in range(R * beams):
+        want = ref.prefill(np.concatenate([whole[s], more[s]]).astype(np.int32))[T + n_new - 1:]
+        assert np.abs(lg[s] - want[0]).max() <= 1e-3 and np.abs(lg2[s] - want[1:]).max() <= 1e-3, s

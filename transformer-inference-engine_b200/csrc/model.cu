@@ -1829,10 +1829,9 @@ model_status model_generate_beam(model* m, const int32_t* prompts, size_t n_req,
     CU(cudaMemcpyAsync(h_tok.data(), tokens, n_new * S * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
     CU(cudaMemcpyAsync(h_par.data(), parents, n_new * S * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
     CU(cudaMemcpyAsync(h_sc.data(), scores, S * sizeof(float), cudaMemcpyDeviceToHost, m->st));
-    if ((rc = finish(m)) != MODEL_OK) return rc;
-    m->pool->length = (int)(T + n_new - 1);
-    kv_pool_hold(m->pool, (int)S, 0, (int)(T + n_new - 1));
-    // each request's beams, best first, their tokens read back along the parents
+    CU(cudaStreamSynchronize(m->st));
+    // each request's beams, best first, their tokens read back along the parents; the pool's
+    // rows, which lie where the last step's parents are, follow into the same order
     std::vector<size_t> order(beams);
     for (size_t r = 0; r < n_req; ++r) {
         for (size_t b = 0; b < beams; ++b) order[b] = r * beams + b;
@@ -1840,12 +1839,22 @@ model_status model_generate_beam(model* m, const int32_t* prompts, size_t n_req,
         for (size_t b = 0; b < beams; ++b) {
             size_t at = order[b];
             out_scores[r * beams + b] = h_sc[at];
+            m->h_small[r * beams + b] = h_par[(n_new - 1) * S + at];
             for (size_t g = n_new; g-- > 0;) {
                 out_ids[(r * beams + b) * n_new + g] = h_tok[at * n_new + g];
                 at = (size_t)h_par[g * S + at];
             }
         }
     }
+    if (n_new > 1) {
+        CU(cudaMemcpyAsync(parent, m->h_small, S * sizeof(int32_t), cudaMemcpyHostToDevice, m->st));
+        OP(tie_kv_reorder(c->k, c->v, TIE_KV_F32, c->n_layer, c->rows * (size_t)c->n_embd, (int)(c->rows / kPageRows),
+                          m->cfg.n_head, c->d_page_table, c->pages_per_seq, parent, first, m->d_lens, (int)n_req, (int)beams,
+                          m->st));
+    }
+    if ((rc = finish(m)) != MODEL_OK) return rc;
+    m->pool->length = (int)(T + n_new - 1);
+    kv_pool_hold(m->pool, (int)S, 0, (int)(T + n_new - 1));
     return MODEL_OK;
 }
 
