@@ -309,7 +309,7 @@ enum { TIE_KV_F32 = 0, TIE_KV_BF16 = 1 };
  * n_free - 1 first, in the order of sequences and positions, as the engine's
  * own pool does. n_free_out[0] receives what is left (it may be n_free).
  * Without a free list (free_pages, n_free, n_free_out NULL) the table is taken
- * as complete.
+ * as complete; an empty one (max_free 0) needs no free_pages.
  * row_start[n_seq + 1] receives the row starts; seq_of, pos_of, slot_of
  * [max_rows] each row's sequence, position and slot (-1 where that entry is
  * unmapped), and -1 for rows behind the last sequence's.
@@ -328,7 +328,8 @@ model_status tie_page_plan(const int32_t *ctx_lens, const int32_t *new_lens, int
 /* Key and value rows into their slots: row r of k and v (n_kv_head * 64 floats,
  * ld floats apart) to slot slots[r] of the pool, rounded to nearest even for
  * bf16. A slot outside the pool stores nothing; of two rows with one slot each
- * part of 8 elements is one or the other's. rows == 0 is allowed. */
+ * part of 8 elements is one or the other's. rows == 0 is allowed (k, v and slots
+ * may be NULL then). */
 model_status tie_kv_store(const float *k, const float *v, int ld, const int32_t *slots, int rows,
                           void *k_pages, void *v_pages, int kv_format, int n_pages, int n_kv_head,
                           void *stream);
@@ -340,7 +341,7 @@ model_status tie_kv_store(const float *k, const float *v, int ld, const int32_t 
  * over the positions whose page is mapped; 0 where none is left. The new
  * tokens' own keys and values are read from the pages (tie_kv_store first).
  * q and out: `rows` rows of n_head * 64 floats, ldq and ldo apart, not
- * overlapping. max_new bounds the new tokens per sequence. A sequence without
+ * overlapping (rows == 0: nothing to do, q and out may be NULL). max_new bounds the new tokens per sequence. A sequence without
  * new tokens, with more than max_new, with row_start outside 0..rows or beyond
  * pages_per_seq pages is left out: its rows of out stay as they were, and so
  * do rows behind the last sequence's. Sums and softmax statistics are fp32.

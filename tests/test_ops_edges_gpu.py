@@ -8,7 +8,8 @@ import pytest
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 torch = pytest.importorskip("torch")
 import ops_oracle as ref  # noqa: E402
-from test_ops_gpu import KV, _attend, _batch, _i  # noqa: E402
+from test_ops_gpu import KV, _attend, _batch, _check_plan, _i, _workspace  # noqa: E402
+from tie_b200 import ops  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 PAGE, D = 16, 64
@@ -115,3 +116,27 @@ def test_attention_values_that_are_not_finite_reach_the_rows_that_see_them(kv, o
     assert not bool(got[:, sees][..., 5].isfinite().any())
     got[:, sees, :, 5] = 0.0
     assert bool(got.isfinite().all())
+
+
+# ------------------------------------------------------------------ nothing to do
+
+@pytest.mark.parametrize("kv", KV)
+def test_steps_without_rows(kv):
+    """Tensors without elements: no rows to store or to attend with, no free page."""
+    b = _batch(np.random.default_rng(1), [20, 3], [0, 0], 4, 2, kv)
+    none = torch.empty(0, 2 * D, device="cuda")
+    before = b["k"].clone()
+    ops.kv_store(none, none.clone(), torch.empty(0, dtype=torch.int32, device="cuda"), b["k"], b["v"])
+    assert torch.equal(b["k"], before)
+    q = torch.empty(0, 4 * D, device="cuda")
+    for max_new in (0, 5):
+        ops.attention_paged(q, b["k"], b["v"], _i(b["table"]), _i([0, 0, 0]), _i(b["ctx"]), max_new, q.clone(), _workspace())
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("new,status", [([1, 2], ref.OK), ([1, 13], ref.OK), ([1, 14], ref.CAPACITY), ([0, 0], ref.OK)])
+def test_plan_with_an_empty_free_list(new, status):
+    """Rows that fit the pages there are; or, without a page to give, nothing."""
+    table = np.array([[4, 7], [2, 9]])
+    got = _check_plan([20, 3], new, table, 10, 16, free=np.empty(0, np.int64), n_free=0)
+    assert got[-1] == status

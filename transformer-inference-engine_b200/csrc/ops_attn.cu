@@ -413,7 +413,8 @@ extern "C" model_status tie_attention_paged(const float* q, int ldq, int n_head,
                                             const int32_t* ctx_lens, int n_seq, int max_new, int rows, float scale,
                                             float* out, int ldo, void* workspace, size_t workspace_bytes,
                                             int32_t* status, void* stream) {
-    if (!q || !k_pages || !v_pages || !page_table || !row_start || !ctx_lens || !out || !workspace) return MODEL_ERR_ARG;
+    if (!k_pages || !v_pages || !page_table || !row_start || !ctx_lens || !workspace) return MODEL_ERR_ARG;
+    if (rows && (!q || !out)) return MODEL_ERR_ARG;           // arrays without rows have no address
     if (!pool_shape_ok(kv_format, n_pages, n_kv_head) || n_head <= 0 || n_head % n_kv_head || n_head > 8192)
         return MODEL_ERR_ARG;
     if (pages_per_seq <= 0 || n_seq <= 0 || max_new < 0 || rows < 0 || !std::isfinite(scale)) return MODEL_ERR_ARG;

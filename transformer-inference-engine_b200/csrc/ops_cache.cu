@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
     if (t == 0) s_bad = 0;
     __syncthreads();
 
-    const int n_free = a.free_pages ? *a.n_free : 0;
+    const int n_free = a.n_free ? *a.n_free : 0;
     const long long cap = (long long)a.width * kPageRows;
     // per thread: kPlanPerThread consecutive sequences
     int nw[kPlanPerThread], nd[kPlanPerThread];
@@ -99,9 +99,9 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
             else if ((long long)c + n > cap) bad |= 2;
             else {
                 nw[k] = n;
-                nd[k] = a.free_pages ? (int)(((long long)c + n + kPageRows - 1) / kPageRows -
-                                             ((long long)c + kPageRows - 1) / kPageRows)
-                                     : 0;
+                nd[k] = a.n_free ? (int)(((long long)c + n + kPageRows - 1) / kPageRows -
+                                         ((long long)c + kPageRows - 1) / kPageRows)
+                                 : 0;
             }
         }
         sum_new += nw[k];
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
     const int g = rank * kPlanThreads + t, G = ctas * kPlanThreads;
     if (g == 0) {
         *a.status = st;
-        if (a.free_pages) *a.n_free_out = n_free - (ok ? (int)total_need : 0);
+        if (a.n_free) *a.n_free_out = n_free - (ok ? (int)total_need : 0);
     }
     for (int s = g; s <= a.n_seq; s += G) a.row_start[s] = s_row[s];
     // the last sequence s with base[s] <= x
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
             const int j = pos[x] / kPageRows;
             // the entries other threads assign above are taken from the free
             // list itself, not from the table
-            page[x] = a.free_pages && j >= have ? a.free_pages[n_free - 1 - (s_need[lo] + j - have)]
+            page[x] = a.n_free && j >= have ? a.free_pages[n_free - 1 - (s_need[lo] + j - have)]
                                                 : a.table[(size_t)lo * a.width + j];
         }
 #pragma unroll
@@ -415,7 +415,8 @@ extern "C" model_status tie_page_plan(const int32_t* ctx_lens, const int32_t* ne
     if (!ctx_lens || !new_lens || !page_table || !row_start || !seq_of || !pos_of || !slot_of || !status)
         return MODEL_ERR_ARG;
     if (n_seq <= 0 || pages_per_seq <= 0 || n_pages <= 0 || max_rows <= 0) return MODEL_ERR_ARG;
-    if (free_pages ? (!n_free || !n_free_out || max_free < 0) : (n_free || n_free_out)) return MODEL_ERR_ARG;
+    // n_free says whether there is a free list: an empty one has no address
+    if (n_free ? (!n_free_out || max_free < 0 || (max_free && !free_pages)) : (free_pages || n_free_out)) return MODEL_ERR_ARG;
     if (n_seq > kOpsMaxSeqs || n_pages > kOpsMaxPages || pages_per_seq > kOpsMaxPages / 2) return MODEL_ERR_CAPACITY;
     OnDeviceOf dev(row_start);
     if (dev.status() != MODEL_OK) return dev.status();
@@ -442,7 +443,8 @@ extern "C" model_status tie_page_plan(const int32_t* ctx_lens, const int32_t* ne
 extern "C" model_status tie_kv_store(const float* k, const float* v, int ld, const int32_t* slots, int rows,
                                      void* k_pages, void* v_pages, int kv_format, int n_pages, int n_kv_head,
                                      void* stream) {
-    if (!k || !v || !slots || !k_pages || !v_pages || rows < 0) return MODEL_ERR_ARG;
+    if (!k_pages || !v_pages || rows < 0) return MODEL_ERR_ARG;
+    if (rows && (!k || !v || !slots)) return MODEL_ERR_ARG;   // arrays without rows have no address
     if (!pool_shape_ok(kv_format, n_pages, n_kv_head)) return MODEL_ERR_ARG;
     const int w = n_kv_head * kHeadDim;
     if (ld < w || (ld & 3) || !aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages))
