@@ -8,12 +8,14 @@ what changed.
 """
 from __future__ import annotations
 
+import importlib.metadata
 import importlib.util
 import os
 import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 
 PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -26,6 +28,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libtie_b200.so")
 
 OPS_SRC = os.path.join(CSRC, "python", "ops_module.cpp")
 OPS_PATH = os.path.join(PKG_ROOT, "tie_b200", "_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
+OPS_STAMP = os.path.join(OBJ_DIR, "ops_module.torch")    # the torch that it was built for
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O3",
@@ -86,22 +89,46 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None) -> str:
 
 
 def build_ops_module() -> str:
-    """tie_b200/_ops, the Python side of the operators' calls ("" without torch, whose tensors it reads)."""
+    """tie_b200/_ops, the Python side of the operators' calls. The library and the model do without it, so where it
+    cannot be built (no torch, one without the interface that it reads tensors by, no compiler, no Python headers)
+    the answer is "", with a warning unless torch is absent, and tie_b200.ops refuses its calls."""
     torch = importlib.util.find_spec("torch")
     if torch is None:
         return ""
-    newest = max([os.path.getmtime(OPS_SRC)] + [os.path.getmtime(os.path.join(INCLUDE, f)) for f in os.listdir(INCLUDE)])
-    if os.path.exists(OPS_PATH) and os.path.getmtime(OPS_PATH) >= newest:
-        return OPS_PATH
     torch_dir = torch.submodule_search_locations[0]
+    try:
+        built_for = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        built_for = torch_dir
+    newest = max([os.path.getmtime(OPS_SRC)] + [os.path.getmtime(os.path.join(INCLUDE, f)) for f in os.listdir(INCLUDE)])
+    if os.path.exists(OPS_PATH):
+        if os.path.getmtime(OPS_PATH) >= newest and _read(OPS_STAMP) == built_for:
+            return OPS_PATH
+        os.remove(OPS_PATH)     # it must not be called with what has changed
+    os.makedirs(os.path.dirname(OPS_STAMP), exist_ok=True)
     tmp = OPS_PATH + ".tmp"
     cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-I" + INCLUDE,
            "-I" + sysconfig.get_paths()["include"], "-isystem", os.path.join(torch_dir, "include"), OPS_SRC, "-o", tmp]
-    p = subprocess.run(cmd, capture_output=True, text=True)
-    if p.returncode != 0:
-        raise RuntimeError(f"g++ failed on {OPS_SRC}:\n{p.stdout}\n{p.stderr}")
+    try:
+        p = subprocess.run(cmd, capture_output=True, text=True)
+        failed = p.stdout + p.stderr if p.returncode else ""
+    except OSError as e:
+        failed = str(e)
+    if failed or not os.path.exists(tmp):
+        warnings.warn(f"tie_b200._ops is not built, tie_b200.ops will not work:\n{failed[:2000]}", RuntimeWarning)
+        return ""
     os.replace(tmp, OPS_PATH)
+    with open(OPS_STAMP, "w") as f:
+        f.write(built_for)
     return OPS_PATH
+
+
+def _read(path: str) -> str:
+    try:
+        with open(path) as f:
+            return f.read()
+    except OSError:
+        return ""
 
 
 if __name__ == "__main__":
