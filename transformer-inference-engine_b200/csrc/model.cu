@@ -1786,13 +1786,14 @@ model_status model_generate_beam(model* m, const int32_t* prompts, size_t n_req,
     float* scores = reinterpret_cast<float*>(done + S);
     int32_t *tokens = first + n_req, *parents = tokens + n_new * S;   // [S][n_new], [n_new][S]
     int32_t* done_or_null = eos_id < 0 ? nullptr : done;
+    // everything the host holds: the prompts, then the start's arrays, then the results
+    if ((rc = ensure_pinned(m, std::max({S * T, 3 * S + n_req, 2 * n_new * S + 2 * S}))) != MODEL_OK) return rc;
     if ((rc = stats_begin(m)) != MODEL_OK) return rc;
 
     // every beam of a request holds the prompt; only the first has a score yet
-    std::vector<int32_t> ids(S * T);
-    for (size_t s = 0; s < S; ++s) std::memcpy(&ids[s * T], prompts + s / beams * T, T * sizeof(int32_t));
-    if ((rc = batch_prefill_impl(m, S, T, nullptr, nullptr, true, ids.data())) != MODEL_OK) return rc;
-    if ((rc = ensure_pinned(m, 3 * S + n_req)) != MODEL_OK) return rc;
+    CU(cudaStreamSynchronize(m->st));
+    for (size_t s = 0; s < S; ++s) std::memcpy(m->h_small + s * T, prompts + s / beams * T, T * sizeof(int32_t));
+    if ((rc = batch_prefill_impl(m, S, T, nullptr, nullptr, true, m->h_small)) != MODEL_OK) return rc;
     CU(cudaStreamSynchronize(m->st));
     int32_t *h_done = m->h_small, *h_score = h_done + S, *h_first = h_score + S, *h_len = h_first + n_req;
     for (size_t s = 0; s < S; ++s) {
@@ -1824,22 +1825,22 @@ model_status model_generate_beam(model* m, const int32_t* prompts, size_t n_req,
                               m->cfg.n_head, c->d_page_table, c->pages_per_seq, parent, first, m->d_lens, (int)n_req,
                               (int)beams, m->st));
     }
-    std::vector<int32_t> h_tok(n_new * S), h_par(n_new * S);
-    std::vector<float> h_sc(S);
-    CU(cudaMemcpyAsync(h_tok.data(), tokens, n_new * S * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
-    CU(cudaMemcpyAsync(h_par.data(), parents, n_new * S * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
-    CU(cudaMemcpyAsync(h_sc.data(), scores, S * sizeof(float), cudaMemcpyDeviceToHost, m->st));
+    int32_t *h_tok = m->h_small, *h_par = h_tok + n_new * S, *h_last = h_par + n_new * S;
+    float* h_sc = reinterpret_cast<float*>(h_last + S);
+    CU(cudaMemcpyAsync(h_tok, tokens, n_new * S * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
+    CU(cudaMemcpyAsync(h_par, parents, n_new * S * sizeof(int32_t), cudaMemcpyDeviceToHost, m->st));
+    CU(cudaMemcpyAsync(h_sc, scores, S * sizeof(float), cudaMemcpyDeviceToHost, m->st));
     CU(cudaStreamSynchronize(m->st));
     // each request's beams, best first, their tokens read back along the parents; the pool's
     // rows, which lie where the last step's parents are, follow into the same order
-    std::vector<size_t> order(beams);
+    size_t order[16];
     for (size_t r = 0; r < n_req; ++r) {
         for (size_t b = 0; b < beams; ++b) order[b] = r * beams + b;
-        std::stable_sort(order.begin(), order.end(), [&](size_t x, size_t y) { return h_sc[x] > h_sc[y]; });
+        std::stable_sort(order, order + beams, [&](size_t x, size_t y) { return h_sc[x] > h_sc[y]; });
         for (size_t b = 0; b < beams; ++b) {
             size_t at = order[b];
             out_scores[r * beams + b] = h_sc[at];
-            m->h_small[r * beams + b] = h_par[(n_new - 1) * S + at];
+            h_last[r * beams + b] = h_par[(n_new - 1) * S + at];
             for (size_t g = n_new; g-- > 0;) {
                 out_ids[(r * beams + b) * n_new + g] = h_tok[at * n_new + g];
                 at = (size_t)h_par[g * S + at];
@@ -1847,7 +1848,7 @@ model_status model_generate_beam(model* m, const int32_t* prompts, size_t n_req,
         }
     }
     if (n_new > 1) {
-        CU(cudaMemcpyAsync(parent, m->h_small, S * sizeof(int32_t), cudaMemcpyHostToDevice, m->st));
+        CU(cudaMemcpyAsync(parent, h_last, S * sizeof(int32_t), cudaMemcpyHostToDevice, m->st));
         OP(tie_kv_reorder(c->k, c->v, TIE_KV_F32, c->n_layer, c->rows * (size_t)c->n_embd, (int)(c->rows / kPageRows),
                           m->cfg.n_head, c->d_page_table, c->pages_per_seq, parent, first, m->d_lens, (int)n_req, (int)beams,
                           m->st));
