@@ -327,8 +327,9 @@ model_status tie_page_plan(const int32_t *ctx_lens, const int32_t *new_lens, int
 
 /* Key and value rows into their slots: row r of k and v (n_kv_head * 64 floats,
  * ld floats apart) to slot slots[r] of the pool, rounded to nearest even for
- * bf16. A slot outside the pool stores nothing; of two rows with one slot each
- * part of 8 elements is one or the other's. rows == 0 is allowed (k, v and slots
+ * bf16. A slot outside the pool stores nothing; of rows with one slot each
+ * element is one or another's (which, may differ from element to element and
+ * between keys and values). rows == 0 is allowed (k, v and slots
  * may be NULL then). */
 model_status tie_kv_store(const float *k, const float *v, int ld, const int32_t *slots, int rows,
                           void *k_pages, void *v_pages, int kv_format, int n_pages, int n_kv_head,

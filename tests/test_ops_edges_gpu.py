@@ -140,3 +140,24 @@ def test_plan_with_an_empty_free_list(new, status):
     table = np.array([[4, 7], [2, 9]])
     got = _check_plan([20, 3], new, table, 10, 16, free=np.empty(0, np.int64), n_free=0)
     assert got[-1] == status
+
+
+# ------------------------------------------------------------------ the same slot twice
+
+@pytest.mark.parametrize("kv", KV)
+def test_store_of_two_rows_with_one_slot(kv):
+    """Every element is one of the rows', in the keys and in the values, and no other slot is touched."""
+    rows, w, n_pages = 4000, 3 * D, 5
+    g = torch.Generator(device="cuda").manual_seed(7)
+    k, v = torch.randn(2, rows, w, generator=g, device="cuda")
+    slots = torch.randint(0, n_pages * PAGE // 2, (rows,), generator=g, device="cuda").to(torch.int32) * 2
+    pages = [torch.full((n_pages, PAGE, w), 9.0, device="cuda", dtype=kv) for _ in range(2)]
+    ops.kv_store(k, v, slots, *pages)
+    for p, x in zip(pages, (k, v)):
+        flat = p.view(-1, w)
+        for slot in range(n_pages * PAGE):
+            mine = x[slots == slot].to(kv)
+            if slot % 2:
+                assert bool((flat[slot] == 9.0).all())
+            else:
+                assert len(mine) > 1 and bool((mine == flat[slot]).any(0).all())
