@@ -161,3 +161,33 @@ def test_store_of_two_rows_with_one_slot(kv):
                 assert bool((flat[slot] == 9.0).all())
             else:
                 assert len(mine) > 1 and bool((mine == flat[slot]).any(0).all())
+
+
+# ------------------------------------------------------------------ very long contexts
+
+def test_attention_of_tiles_that_take_longer_than_a_wait():
+    """A tile of 72 million positions takes its CTA over 2 s, and more tiles than the CTA describes in advance stand
+    behind it. The positions are those of 64 pages again and again, so the exact result is a weighted mean over these.
+
+    A row sum is added up over half a million steps and the running output over a quarter of them, each addition
+    off by 2^-24 of the sum at worst."""
+    n, new, small = 72 << 20, 148 * 256, 20
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = torch.randn(2, 64, PAGE, D, generator=g, device="cuda").to(torch.bfloat16)
+    width = ref.pages_of(n + new)
+    table = (torch.arange(width, dtype=torch.int32, device="cuda") % 64).repeat(1 + small, 1)
+    rows = new + 9 * small
+    q = torch.randn(rows, D, generator=g, device="cuda")
+    start = _i([0] + [new + 9 * s for s in range(small + 1)])
+    out, status = torch.full((rows, D), 7.0, device="cuda"), _i([0])
+    ops.attention_paged(q, k, v, table, start, _i([n] + [0] * small), new, out, _workspace(), status=status)
+    torch.cuda.synchronize()
+    assert int(status[0]) == 0
+    kd, vd = k.double().view(-1, D), v.double().view(-1, D)
+    pick = torch.cat([torch.arange(0, new, 997, device="cuda"), torch.arange(new, rows, device="cuda")])
+    seen = torch.where(pick < new, n + pick + 1, (pick - new) % 9 + 1)[:, None]
+    count = (seen // len(kd) + (torch.arange(len(kd), device="cuda") < seen % len(kd))).double()
+    p = torch.exp(0.125 * q[pick].double() @ kd.T) * count
+    want = p / p.sum(1, keepdim=True) @ vd
+    bound = 2 * (seen / 128 + 100 + 96) * 2.0 ** -24 * vd.abs().max()
+    assert bool(((out[pick].double() - want).abs() <= bound).all())

@@ -77,9 +77,9 @@
 // heads, fp32: 242 us, bound by the loaders' chain of a step (convert keys, convert
 // values, wait for their buffers) and by a tile's start, not by memory (51 us).
 // TMEM (512 columns): three S / P (384), two O (128).
-// Every wait is bounded: on expiry it raises the abort flag, which ends every
-// other wait; the roles run out without storing, the MMAs issued are drained
-// and TMEM is freed.
+// Every wait is bounded (2 s; longer only for the place of a tile of more than 16,384
+// steps in the ring): on expiry it raises the abort flag, which ends every other wait;
+// the roles run out without storing, the MMAs issued are drained and TMEM is freed.
 #include <cuda.h>
 
 #include <cuda_bf16.h>
@@ -1220,6 +1220,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             // ---------------------------------------------------------- tiles
             uint32_t un = 0;
             int fills = 0, jobs = 0, halves = 0;
+            // a place in the ring: its tile may be a long one, so the steps that it takes (2 to 4 us
+            // each, 65 ms for 16,384) extend the wait, which the other roles cut short when they stall
+            auto place_free = [&]() -> bool {
+                if (un < kUnitRing) return true;
+                const uint32_t b = smem_u32(&unit_free[un % kUnitRing]), parity = (un / kUnitRing - 1) & 1u;
+                int more = units[un % kUnitRing].steps / 16384;
+                for (uint32_t i = 1, t0 = nanoseconds(); !mbar_try_wait(b, parity); ++i) {
+                    if ((i & 255u) != 0) continue;
+                    if (*abort_flag) return false;
+                    if (nanoseconds() - t0 <= kWaitLimitNs) continue;
+                    if (--more < 0) {
+                        *abort_flag = 1;
+                        return false;
+                    }
+                    t0 = nanoseconds();
+                }
+                return true;
+            };
             for (long long x = g0; x < g1; unit_next(a, here)) {
                 const long long from = max(x, here.jobs), to = min(here.end, g1);
                 x = here.end;
@@ -1227,7 +1245,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     if (x >= g1) break;
                     continue;
                 }
-                if (un >= kUnitRing && !wait_all(&unit_free[un % kUnitRing], (un / kUnitRing - 1) & 1u)) break;
+                if (!__all_sync(kAll, place_free())) break;
                 if (lane == 0) {
                     volatile Unit& n = units[un % kUnitRing];
                     const int n_rows = tile_n_rows(here.q, here.tile), both = n_rows > kHalfRows;
@@ -1258,7 +1276,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 ++un;
                 if (x >= g1) break;
             }
-            if (un < kUnitRing || wait_all(&unit_free[un % kUnitRing], (un / kUnitRing - 1) & 1u)) {
+            if (__all_sync(kAll, place_free())) {
                 if (lane == 0) {
                     units[un % kUnitRing].steps = -1;
                     mbar_arrive(smem_u32(&unit_full[un % kUnitRing]));
