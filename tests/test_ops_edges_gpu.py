@@ -191,3 +191,21 @@ def test_attention_of_tiles_that_take_longer_than_a_wait():
     want = p / p.sum(1, keepdim=True) @ vd
     bound = 2 * (seen / 128 + 100 + 96) * 2.0 ** -24 * vd.abs().max()
     assert bool(((out[pick].double() - want).abs() <= bound).all())
+
+
+# ------------------------------------------------------------------ queries and keys of very different sizes
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("power", [112, 60, -60, -105])
+@pytest.mark.parametrize("ctx,new", [(70, 1), (70, 9), (0, 150), (300, 40)])
+def test_attention_of_queries_and_keys_whose_products_are_ordinary(kv, power, ctx, new):
+    """Queries of 2^power and keys of 2^-power: their products are as ever, and so are the results."""
+    b = _batch(np.random.default_rng(new), [ctx], [new], 4, 2, kv)
+    b["q"].mul_(2.0 ** power)
+    b["k"].copy_((b["k"].double() * 2.0 ** -power).to(kv))
+    status = _i([0])
+    got = _attend(b, status=status).cpu().numpy().astype(np.float64)
+    want, vmax, smax = ref.attention(b["q"].cpu().numpy().astype(np.float64), b["k"].cpu().double().numpy(),
+                                     b["v"].cpu().double().numpy(), b["table"], b["start"], b["ctx"], 4, 2, 0.125,
+                                     np.zeros(got.shape))
+    assert int(status[0]) == 0 and (np.abs(got - want) <= ref.attention_bound(vmax, smax, ctx + new)).all()

@@ -715,7 +715,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     const float fk[4] = {ks.x, ks.y, ks.z, ks.w}, e[4] = {ee.x, ee.y, ee.z, ee.w};
 #pragma unroll
                     for (int d = 0; d < 4; ++d) {
-                        tt[d] = fmaf(__uint_as_float(s4[d]) * qs, fk[d], e[d]);
+                        // (the scales first: S times one of them may be beyond fp32)
+                        tt[d] = fmaf(__uint_as_float(s4[d]), qs * fk[d], e[d]);
                         if (pos + 4 * k + d > last) tt[d] = -INFINITY;
                     }
                 };
