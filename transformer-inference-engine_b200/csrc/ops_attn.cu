@@ -56,18 +56,17 @@ struct FewSmem {
     float o[kFewWarps][kFewRows][kHeadDim];
 };
 
-// Every `stride`-th page of [p0 + warp, p1) of sequence s for rows tile *
-// kFewRows .. + R - 1 (n_rows of them real) of K/V head g; leaves each warp's
-// partial in `sm`.
+// Every `stride`-th page of [p0 + warp, p1) of sequence s for its rows (R, of
+// which q.rows are real) of K/V head g; leaves each warp's partial in `sm`.
 template <int R, bool BF16>
-__device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const SeqShape& q, int s, int tile, int g, int p0,
-                                         int p1, int stride, int n_rows, FewSmem* sm) {
+__device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const SeqShape& q, int s, int g, int p0, int p1,
+                                         int stride, FewSmem* sm) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, half = lane >> 4, dl = lane & 15;
     float qv[R][4], o[R][4], m[R], l[R];
     int last[R];                       // the last position each row sees
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int i = min(tile * kFewRows + r, q.rows - 1), tok = i / a.group;
+        const int i = min(r, q.rows - 1), tok = i / a.group;
         last[r] = q.ctx + tok;
         const float4 x = __ldg(reinterpret_cast<const float4*>(a.q + (size_t)(q.row0 + tok) * a.ldq +
                                                                (g * a.group + i % a.group) * kHeadDim + 4 * dl));
@@ -136,7 +135,7 @@ __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const SeqShape&
         for (int x = 1; x < 32; x <<= 1) l[r] += __shfl_xor_sync(kAll, l[r], x);
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[r][c] += __shfl_xor_sync(kAll, o[r][c], 16);
-        if (r < n_rows) {
+        if (r < q.rows) {
             if (lane == 0) { sm->m[warp][r] = m[r]; sm->l[warp][r] = 0.5f * l[r]; }
             if (half == 0)
                 *reinterpret_cast<float4*>(&sm->o[warp][r][4 * dl]) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
@@ -146,12 +145,12 @@ __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const SeqShape&
 
 // the same for as many rows as there are, at most RMAX
 template <int RMAX, bool BF16>
-__device__ __forceinline__ void few_rows_n(const PagedAttnArgs& a, const SeqShape& q, int s, int tile, int g, int p0,
-                                           int p1, int stride, int n_rows, FewSmem* sm) {
-    if (RMAX == 1 || n_rows == 1) few_rows<1, BF16>(a, q, s, tile, g, p0, p1, stride, n_rows, sm);
-    else if (RMAX == 2 || n_rows == 2) few_rows<(RMAX < 2 ? RMAX : 2), BF16>(a, q, s, tile, g, p0, p1, stride, n_rows, sm);
-    else if (RMAX == 4 || n_rows <= 4) few_rows<(RMAX < 4 ? RMAX : 4), BF16>(a, q, s, tile, g, p0, p1, stride, n_rows, sm);
-    else few_rows<RMAX, BF16>(a, q, s, tile, g, p0, p1, stride, n_rows, sm);
+__device__ __forceinline__ void few_rows_n(const PagedAttnArgs& a, const SeqShape& q, int s, int g, int p0, int p1,
+                                           int stride, FewSmem* sm) {
+    if (RMAX == 1 || q.rows == 1) few_rows<1, BF16>(a, q, s, g, p0, p1, stride, sm);
+    else if (RMAX == 2 || q.rows == 2) few_rows<(RMAX < 2 ? RMAX : 2), BF16>(a, q, s, g, p0, p1, stride, sm);
+    else if (RMAX == 4 || q.rows <= 4) few_rows<(RMAX < 4 ? RMAX : 4), BF16>(a, q, s, g, p0, p1, stride, sm);
+    else few_rows<RMAX, BF16>(a, q, s, g, p0, p1, stride, sm);
 }
 
 // Row r, dim d of the warps' partials joined. (Here and in the other joins a partial that
@@ -190,7 +189,7 @@ __global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_cluster_ke
     const int g = unit % a.n_kv_head, s = unit / a.n_kv_head;
     const SeqShape q = seq_shape(a, s);
     if (!q.rows) return;               // the whole cluster
-    few_rows_n<RMAX, BF16>(a, q, s, 0, g, rank * kFewWarps, pages_of(q), ctas * kFewWarps, q.rows, &sm);
+    few_rows_n<RMAX, BF16>(a, q, s, g, rank * kFewWarps, pages_of(q), ctas * kFewWarps, &sm);
     __syncthreads();
     auto out_at = [&](int r, int d) -> float& {
         return a.out[(size_t)(q.row0 + r / a.group) * a.ldo + (g * a.group + r % a.group) * kHeadDim + d];
@@ -237,22 +236,16 @@ __global__ void __launch_bounds__(kFewThreads, RMAX <= 2 ? 2 : 1) few_rows_kerne
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
         const int s = owner_of<int>(sch.unit, a.n_seq, u);
         const SeqShape q = seq_shape(a, s);
-        const int sp = splits_of(q, sch.chunk), in = u - sch.unit[s];
-        const int g = in % a.n_kv_head, split = in / a.n_kv_head % sp, tile = in / a.n_kv_head / sp;
-        const int n_rows = min(kFewRows, q.rows - tile * kFewRows);
-        // the tile's last row bounds its keys
-        const int keys = q.ctx + (tile * kFewRows + n_rows - 1) / a.group + 1;
-        const int p0 = split * sch.chunk, p1 = min(p0 + sch.chunk, (keys + kPageRows - 1) / kPageRows);
-        few_rows_n<RMAX, BF16>(a, q, s, tile, g, p0, p1, kFewWarps, n_rows, &sm);
-        if (sp > 1 && t == 0)
-            a.record[0][sch.part[s] + in] = JoinRecord{split ? 0 : sp, n_rows, q.row0, tile * kFewRows, g, {0, 0, 0}};
+        const int sp = splits_of(q, sch.chunk), in = u - sch.unit[s], g = in % a.n_kv_head, split = in / a.n_kv_head;
+        const int p0 = split * sch.chunk, p1 = min(p0 + sch.chunk, pages_of(q));
+        few_rows_n<RMAX, BF16>(a, q, s, g, p0, p1, kFewWarps, &sm);
+        if (sp > 1 && t == 0) a.record[0][sch.part[s] + in] = JoinRecord{split ? 0 : sp, q.rows, q.row0, 0, g, {0, 0, 0}};
         __syncthreads();
-        for (int e = t; e < n_rows * kHeadDim; e += kFewThreads) {
+        for (int e = t; e < q.rows * kHeadDim; e += kFewThreads) {
             const int r = e / kHeadDim, d = e % kHeadDim;
             const auto [mx, l, o] = join_warps(sm, r, d);
             if (sp == 1) {
-                const int i = tile * kFewRows + r;
-                a.out[(size_t)(q.row0 + i / a.group) * a.ldo + (g * a.group + i % a.group) * kHeadDim + d] =
+                a.out[(size_t)(q.row0 + r / a.group) * a.ldo + (g * a.group + r % a.group) * kHeadDim + d] =
                     l == 0.f ? 0.f : o / l;
             } else {
                 const size_t pu = (size_t)(sch.part[s] + in) * kFewRows + r;
@@ -327,7 +320,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(PagedAttnArgs a) 
                 join_row<4>(a, 1, rec.parts, [&](int k) { return ((size_t)2 * (c + k) + (k == 0)) * kTileRows + r; }, lane,
                          out_of(rec, r));
         }
-    // streaming units: a sequence's come in groups of `parts` per (tile, head)
+    // streaming units: a sequence's come in groups of `parts` per head
     static_assert(kJoinThreads / 32 == kFewRows, "a warp for each row of a unit");
     if (a.group <= kFewRows) {
         const int n = *a.n_records;

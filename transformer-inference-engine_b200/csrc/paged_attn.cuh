@@ -4,18 +4,17 @@
 //
 // Row (i, h) of sequence s is its new token i and query head h, at position
 // ctx_s + i. The heads of one K/V head and a sequence's tokens together form
-// the rows that share keys: row index i * group + (h mod group). They are cut
-// into tiles. Sequences of few rows (at most kFewRows) go to the streaming
-// kernel, the others to the tensor-core kernel; each kernel derives its
-// schedule from the lengths for itself (a scan of the lengths costs less than
-// a launch that would leave it in memory).
-//   Streaming (kind 0): a unit is (sequence, tile, split of the keys, K/V
-// head), the head fastest, so CTAs that run together read one page's
-// neighbouring rows.
-//   Tensor cores (kind 1): a tile's steps over the keys count as jobs (two a
-// step when the tile has more than 128 rows). All tiles of the batch stand in
-// one line -- by sequence, tile, K/V head -- each with its jobs behind a few
-// places that stand for what a tile costs besides; every CTA takes an equal
+// the rows that share keys: row index i * group + (h mod group). Sequences of
+// few rows (at most kFewRows) go to the streaming kernel, the others to the
+// tensor-core kernel; each kernel derives its schedule from the lengths for
+// itself (a scan of the lengths costs less than a launch that would leave it in
+// memory).
+//   Streaming (kind 0): a unit is (sequence, split of the keys, K/V head), the
+// head fastest, so CTAs that run together read one page's neighbouring rows.
+//   Tensor cores (kind 1): the rows are cut into tiles, whose steps over the keys
+// count as jobs (two a step when the tile has more than 128 rows). All tiles of the
+// batch stand in one line -- by sequence, tile, K/V head -- each with its jobs behind
+// a few places that stand for what a tile costs besides; every CTA takes an equal
 // stretch of the line. A tile that a stretch cuts leaves partial results.
 #pragma once
 
@@ -23,7 +22,7 @@
 
 namespace tie {
 
-constexpr int kFewRows = 8;        // rows of a streaming unit
+constexpr int kFewRows = 8;        // rows of a streaming unit at most
 constexpr int kHalfRows = 128;     // rows of one MMA of the tensor-core kernel
 constexpr int kTileRows = 256;     // rows of its tiles
 constexpr int kTileKeys = 128;     // keys of one of its steps
@@ -59,7 +58,6 @@ struct PagedAttnArgs {
     int* status;
 };
 
-__host__ __device__ inline int tile_rows_of(int kind) { return kind ? kTileRows : kFewRows; }
 // fewest pages worth a streaming unit of their own (four for each warp), fewest
 // jobs worth a tensor-core CTA
 constexpr int kMinUnitPages = 32, kMinJobs = 2;
@@ -80,7 +78,7 @@ __device__ __forceinline__ SeqShape seq_shape(const PagedAttnArgs& a, int s) {
     q.tokens = r1 - r0;
     q.rows = q.tokens * a.group;
     q.kind = !a.only_few && q.rows > kFewRows;
-    q.tiles = (q.rows + tile_rows_of(q.kind) - 1) / tile_rows_of(q.kind);
+    q.tiles = (q.rows + kTileRows - 1) / kTileRows;
     return q;
 }
 
@@ -138,10 +136,11 @@ __device__ __forceinline__ void build_schedule(const PagedAttnArgs& a, int* smem
         const int s = t * per + k;
         if (s >= a.n_seq) break;
         const SeqShape q = seq_shape(a, s);
-        if (q.rows && !q.kind) work += (long long)a.n_kv_head * q.tiles * pages_of(q);
+        if (q.rows && !q.kind) work += (long long)a.n_kv_head * pages_of(q);
     }
     const long long even = (scan_threads<THREADS>(work, sc, t, &before) + a.target - 1) / a.target;
-    out->chunk = (int)(even > kMinUnitPages ? even : kMinUnitPages);
+    // (no sequence has as many pages as the pool can have)
+    out->chunk = (int)(even < kMinUnitPages ? kMinUnitPages : even < kOpsMaxPages ? even : kOpsMaxPages);
     long long units = 0;           // units in the low half, units with partials in the high half
     for (int k = 0; k < per; ++k) {
         const int s = t * per + k;
@@ -149,7 +148,7 @@ __device__ __forceinline__ void build_schedule(const PagedAttnArgs& a, int* smem
         const SeqShape q = seq_shape(a, s);
         if (!q.rows || q.kind) continue;
         const int sp = splits_of(q, out->chunk);
-        const long long n = (long long)a.n_kv_head * q.tiles * sp;
+        const long long n = (long long)a.n_kv_head * sp;
         units += n + (sp > 1 ? n << 32 : 0);
     }
     scan_threads<THREADS>(units, sc, t, &before);
@@ -161,7 +160,7 @@ __device__ __forceinline__ void build_schedule(const PagedAttnArgs& a, int* smem
         out->part[s] = bp;
         const SeqShape q = seq_shape(a, s);
         if (q.rows && !q.kind) {
-            const int sp = splits_of(q, out->chunk), n = a.n_kv_head * q.tiles * sp;
+            const int sp = splits_of(q, out->chunk), n = a.n_kv_head * sp;
             bu += n;
             if (sp > 1) bp += n;
         }
