@@ -75,3 +75,36 @@ def test_the_pool_holds_the_continuations_that_a_search_returns(fresh, beams, n_
     for s in range(R * beams):
         want = ref.prefill(np.concatenate([whole[s], more[s]]).astype(np.int32))[T + n_new - 1:]
         assert np.abs(lg[s] - want[0]).max() <= 1e-3 and np.abs(lg2[s] - want[1:]).max() <= 1e-3, s
+
+
+@pytest.mark.parametrize("kind", [tie_b200.TIE_STEP_PERSISTENT, tie_b200.TIE_STEP_STREAM])
+def test_beam_search_and_extension_with_every_step_kernel(fresh, kind):
+    m, ref = fresh
+    prompts = synth.prompt_ids(m.vocab, 2, 9, seed=12)
+    m.batch_reserve(4, 40)
+    want = m.generate_beam(prompts, 2, 16)
+    m.set_step_kernel(kind)
+    ids, scores = m.generate_beam(prompts, 2, 16)
+    assert np.abs(scores - want[1]).max() <= 2e-3 * 16
+    assert np.array_equal(ids, want[0]) or np.abs(np.diff(want[1], axis=1)).min() < 2e-3 * 16
+    whole = np.concatenate([np.repeat(prompts, 2, 0), ids.reshape(4, 16)], 1).astype(np.int32)
+    _, lg = m.decode_step_batch(whole[:, -1], want_logits=True)
+    nxt, lg2 = m.extend_batch(whole[:, :5], want_logits=True)
+    for s in range(4):
+        full = ref.prefill(np.concatenate([whole[s], whole[s, :5]]).astype(np.int32))[24:]
+        assert np.abs(lg[s] - full[0]).max() <= 1e-3 and np.abs(lg2[s] - full[1:]).max() <= 1e-3
+
+
+@pytest.mark.parametrize("fmt", [tie_b200.TIE_WEIGHTS_BF16, tie_b200.TIE_WEIGHTS_INT8])
+def test_an_extension_agrees_with_a_prefill_in_every_weight_format(fresh, fmt):
+    m, _ = fresh
+    ids = synth.prompt_ids(m.vocab, 3, 30, seed=6)
+    m.set_weight_format(fmt)
+    m.batch_reserve(3, 40)
+    _, want = m.prefill_batch(ids, want_logits=True)
+    _, a = m.prefill_batch(ids[:, :11], want_logits=True)
+    _, b = m.extend_batch(ids[:, 11:29], want_logits=True)
+    _, c = m.extend_batch(ids[:, 29:], want_logits=True)
+    assert np.abs(np.concatenate([a, b, c], 1) - want).max() <= 1e-3
+    out, scores = m.generate_beam(ids[:, :12], 1, 9)
+    assert np.array_equal(out[:, 0], m.generate_greedy(ids[:, :12], 9))
