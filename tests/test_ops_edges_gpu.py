@@ -209,3 +209,37 @@ def test_attention_of_queries_and_keys_whose_products_are_ordinary(kv, power, ct
                                      b["v"].cpu().double().numpy(), b["table"], b["start"], b["ctx"], 4, 2, 0.125,
                                      np.zeros(got.shape))
     assert int(status[0]) == 0 and (np.abs(got - want) <= ref.attention_bound(vmax, smax, ctx + new)).all()
+
+
+# ------------------------------------------------------------------ streams of a tile that end far apart
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("rows", [136, 160, 200, 256, 300])
+@pytest.mark.parametrize("odd", [2.0 ** 100, float("inf")])
+def test_attention_of_tiles_whose_halves_end_far_apart(kv, rows, odd):
+    """Tiles of two halves, of which the second has a long way out (its rows see a value that their row sums, or their
+    results, have to be completed for), each in front of tiles of one short step: the others' O is left in time, and
+    no signal for a tile comes before the last one for the tile before it."""
+    rng = np.random.default_rng(rows)
+    n, kv_heads = 24, 6
+    ctx = [v for _ in range(n) for v in (int(rng.integers(300, 700)), int(rng.integers(0, 90)), 10)]
+    new = [v for _ in range(n) for v in (rows, int(rng.integers(9, 30)), 9)]
+    b = _batch(rng, ctx, new, kv_heads, kv_heads, kv)
+    late = min(rows - 1, 130)
+    for s in range(0, 3 * n, 3):
+        page, row = _positions(b, s)
+        b["v"][page[ctx[s] + late], row[ctx[s] + late]] = odd
+    outs = [_attend(b) for _ in range(4)]
+    assert all(torch.equal(torch.nan_to_num(o), torch.nan_to_num(outs[0])) for o in outs)
+    got, start = outs[0].cpu().numpy().astype(np.float64), b["start"]
+    for s in (0, 1, 2, 33, 34, 35):
+        lo, hi = start[s], start[s + 1]
+        one = [x.cpu().double().numpy() for x in (b["q"][lo:hi], b["k"], b["v"])]
+        with np.errstate(all="ignore"):
+            want, vmax, smax = ref.attention(*one, b["table"][s:s + 1], [0, hi - lo], [ctx[s]], kv_heads, kv_heads, 0.125,
+                                             np.zeros((hi - lo, kv_heads * D)))
+        sees = s % 3 == 0 and not np.isfinite(odd)
+        live = np.arange(hi - lo) < (late if sees else hi - lo)
+        near = np.abs(got[lo:hi][live] - want[live]) <= ref.attention_bound(vmax, smax, ctx[s] + new[s])[live]
+        assert near.all()
+        assert not np.isfinite(got[lo:hi][~live]).any()

@@ -581,7 +581,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     uint64_t* p_full = bars + 15;    // [job % 3] P written, O rescaled (the stream's softmax warps)
     uint64_t* o_done = bars + 18;    // [job % 3] P . V done (commit)
     uint64_t* o_last = bars + 21;    // [stream] the tile's last P . V of the stream done (commit)
-    uint64_t* o_free = bars + 23;    // [stream] O read by the epilogue (softmax warps)
+    uint64_t* o_free = bars + 23;    // [stream] O read by the epilogue (softmax warps), a phase for each tile
+                                     // that has jobs of the stream: arrivals for one without could come
+                                     // before those of the tile before it
     uint64_t* pair_in = bars + 25;   // [lane quarter] both streams' maxima and sums written
     uint64_t* unit_full = bars + 29; // [tile % 8] description written
     uint64_t* unit_free = bars + 37; // [tile % 8] read for good (softmax, loader and MMA warps)
@@ -868,10 +870,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;");
                 __syncwarp();
-                if (lane == 0) mbar_arrive_n(smem_u32(&o_free[st]), 2);
+                if (lane == 0 && steps) mbar_arrive_n(smem_u32(&o_free[st]), 2);
             } else {
                 // the streams' results joined: each stream's warps do 32 dims
-                float* xch = s_xch + (un & 1u) * 4 * kHalfRows;
+                float* xch = s_xch + (pairs & 1u) * 4 * kHalfRows;
                 xch[(2 * st) * kHalfRows + r] = m;
                 xch[(2 * st + 1) * kHalfRows + r] = l;
                 asm volatile("tcgen05.fence::before_thread_sync;");
@@ -896,7 +898,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(smem_u32(&o_free[0]));
-                    mbar_arrive(smem_u32(&o_free[1]));
+                    if (steps > 1) mbar_arrive(smem_u32(&o_free[1]));
                 }
 #pragma unroll
                 for (int d = 0; d < 32; ++d) {
@@ -1146,16 +1148,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 return true;
             };
             uint32_t freed = 0;         // tiles whose description is no longer needed
+            uint32_t uses0 = 0, uses1 = 0;   // tiles so far that have jobs of each stream
             auto issue_pv = [&]() -> bool {
                 const volatile Unit& n = units[pc.un % kUnitRing];
                 const int j = pc.k >> pc.both, st = pc.k & 1;
                 const uint32_t f = (uint32_t)uniform(n.fill0) + (uint32_t)j, b = f & 1u, buf = pc.job % 3u;
                 const bool first = pc.both ? j == 0 : pc.k < 2;
                 const bool last = pc.both ? j == pc.steps - 1 : pc.k + 2 >= pc.jobs;
-                // (at the first job of a tile, the tile before has left O)
+                // (at the stream's first job of a tile, the tile before has left O)
+                const uint32_t uses = st ? uses1 : uses0;
                 if (!__all_sync(kAll, there(&p_full[buf], pc.job / 3u) && there(&v_full[b], f >> 1) &&
-                                          (!first || !pc.un || there(&o_free[st], pc.un - 1))))
+                                          (!first || !uses || there(&o_free[st], uses - 1))))
                     return false;
+                if (first) ++(st ? uses1 : uses0);
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 const uint32_t vb = sb + kOffV + b * 2 * kTermBytes, p_col = tm + buf * kTileKeys, d = tm + kColO + 64u * st;
                 const uint32_t more = (pc.both ? j : j >> 1) % kFlush<BF16> ? 1u : 0u;   // O goes on
