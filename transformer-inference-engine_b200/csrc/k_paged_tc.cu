@@ -489,7 +489,8 @@ struct Unit {
     int half0;            // Q halves used before it
     int s;
     int odd;              // a value is not finite (set by the loaders)
-    int pad[4];
+    int used0, used1;     // tiles before it that have jobs of each stream
+    int pad[2];
 };
 static_assert(sizeof(Unit) == 80, "ring entry");
 
@@ -1148,7 +1149,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 return true;
             };
             uint32_t freed = 0;         // tiles whose description is no longer needed
-            uint32_t uses0 = 0, uses1 = 0;   // tiles so far that have jobs of each stream
             auto issue_pv = [&]() -> bool {
                 const volatile Unit& n = units[pc.un % kUnitRing];
                 const int j = pc.k >> pc.both, st = pc.k & 1;
@@ -1156,11 +1156,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 const bool first = pc.both ? j == 0 : pc.k < 2;
                 const bool last = pc.both ? j == pc.steps - 1 : pc.k + 2 >= pc.jobs;
                 // (at the stream's first job of a tile, the tile before has left O)
-                const uint32_t uses = st ? uses1 : uses0;
+                const int used = first ? uniform(st ? n.used1 : n.used0) : 0;
                 if (!__all_sync(kAll, there(&p_full[buf], pc.job / 3u) && there(&v_full[b], f >> 1) &&
-                                          (!first || !uses || there(&o_free[st], uses - 1))))
+                                          (!used || there(&o_free[st], (uint32_t)used - 1))))
                     return false;
-                if (first) ++(st ? uses1 : uses0);
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 const uint32_t vb = sb + kOffV + b * 2 * kTermBytes, p_col = tm + buf * kTileKeys, d = tm + kColO + 64u * st;
                 const uint32_t more = (pc.both ? j : j >> 1) % kFlush<BF16> ? 1u : 0u;   // O goes on
@@ -1225,7 +1224,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         } else if (warp == kUnitWarp) {
             // ---------------------------------------------------------- tiles
             uint32_t un = 0;
-            int fills = 0, jobs = 0, halves = 0;
+            int fills = 0, jobs = 0, halves = 0, used0 = 0, used1 = 0;
             // a place in the ring: its tile may be a long one, so the steps that it takes (2 to 4 us
             // each, 65 ms for 16,384) extend the wait, which the other roles cut short when they stall
             auto place_free = [&]() -> bool {
@@ -1273,9 +1272,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     n.half0 = halves;
                     n.s = here.s;
                     n.odd = 0;
+                    n.used0 = used0;
+                    n.used1 = used1;
                     fills += step1 - step0;
                     jobs += (step1 - step0) << both;
-                    if (step1 > step0) halves += 1 + both;
+                    if (step1 > step0) {
+                        halves += 1 + both;
+                        ++used0;
+                        if (both || step1 > step0 + 1) ++used1;
+                    }
                     mbar_arrive(smem_u32(&unit_full[un % kUnitRing]));
                 }
                 __syncwarp();
