@@ -291,8 +291,8 @@ model_status tie_head_argmax_noalloc(const float *x, int ldx, const float *w, in
  *
  * Pointers are DEVICE pointers of one device (made current for the call) and
  * `stream` a cudaStream_t of it (NULL: the legacy default stream); work is
- * enqueued and not waited for. Activations and workspaces are 16-byte, pages 32-byte
- * aligned, leading dimensions multiples of 4 floats. A workspace holds nothing
+ * enqueued and not waited for. Activations, workspaces and pages are 16-byte aligned
+ * (pages that tie_attention_paged reads 32-byte), leading dimensions multiples of 4 floats. A workspace holds nothing
  * from one call to the next, but two calls that overlap on the GPU (streams,
  * replayed graphs) need one each. Nothing is allocated, and every call may be
  * captured into a graph. MODEL_ERR_ARG for a null or misaligned pointer, a
@@ -329,8 +329,8 @@ model_status tie_page_plan(const int32_t *ctx_lens, const int32_t *new_lens, int
  * ld floats apart) to slot slots[r] of the pool, rounded to nearest even for
  * bf16. A slot outside the pool stores nothing; of rows with one slot each
  * element is one or another's (which, may differ from element to element and
- * between keys and values). rows == 0 is allowed (k, v and slots
- * may be NULL then). */
+ * between keys and values). rows == 0 is allowed (k, v and slots may be NULL
+ * then). */
 model_status tie_kv_store(const float *k, const float *v, int ld, const int32_t *slots, int rows,
                           void *k_pages, void *v_pages, int kv_format, int n_pages, int n_kv_head,
                           void *stream);
@@ -342,15 +342,21 @@ model_status tie_kv_store(const float *k, const float *v, int ld, const int32_t 
  * over the positions whose page is mapped; 0 where none is left. The new
  * tokens' own keys and values are read from the pages (tie_kv_store first).
  * q and out: `rows` rows of n_head * 64 floats, ldq and ldo apart, not
- * overlapping (rows == 0: nothing to do, q and out may be NULL). max_new bounds the new tokens per sequence. A sequence without
- * new tokens, with more than max_new, with row_start outside 0..rows or beyond
- * pages_per_seq pages is left out: its rows of out stay as they were, and so
- * do rows behind the last sequence's. Sums and softmax statistics are fp32.
+ * overlapping (rows == 0: nothing to do, q and out may be NULL). max_new bounds
+ * the new tokens per sequence. A sequence without new tokens, with more than
+ * max_new, with row_start outside 0..rows or beyond pages_per_seq pages is left
+ * out: its rows of out stay as they were, and so do rows behind the last
+ * sequence's. Sums and softmax statistics are fp32.
+ * Operands of many rows are held in 22 bits of the largest element of their
+ * query, of their 16 keys or of their 16 values (an element below 2^-17 of it
+ * to 2^-40 of it), and values to 2^-106 at the least.
  * A value that is not finite makes the rows that see it not finite, a key that
- * is not finite may, and neither does it to any other row. The result of a row depends, in its rounding, on how the batch
- * splits its keys, and is the same for the same call.
+ * is not finite may, and neither does it to any other row. The result of a row
+ * depends, in its rounding, on how the batch splits its keys, and is the same
+ * for the same call.
  * status, if not NULL, receives MODEL_ERR_DEVICE when a bounded wait in the
- * kernel expires (the output is then incomplete); it is not written otherwise. */
+ * kernel expires (the output is then incomplete, and nothing else tells); it is
+ * not written otherwise. */
 size_t tie_attention_paged_workspace(void);
 model_status tie_attention_paged(const float *q, int ldq, int n_head, const void *k_pages,
                                  const void *v_pages, int kv_format, int n_pages, int n_kv_head,

@@ -72,9 +72,9 @@
 // The roles' loops together outgrow the instruction cache, so loops that would be
 // unrolled elsewhere are not and waits are kept short: 16 % -> 7 % of the fetches
 // missed, 1,050 -> 955 us for the chunk above, 357 -> 335 us for 48 mixed sequences.
-// In all, with the join: the chunk (32 query heads on 8) 860 us, of which 311 are its
+// In all, with the join: the chunk (32 query heads on 8) 881 us, of which 311 are its
 // MMAs at the measured rate; 48 sequences of up to 117 new rows and 900 cached, 25
-// heads, fp32: 242 us, bound by the loaders' chain of a step (convert keys, convert
+// heads, fp32: 245 us, bound by the loaders' chain of a step (convert keys, convert
 // values, wait for their buffers) and by a tile's start, not by memory (51 us).
 // TMEM (512 columns): three S / P (384), two O (128).
 // Every wait is bounded (2 s; longer only for the place of a tile of more than 16,384
@@ -99,9 +99,11 @@ constexpr int kThreads = 640;
 // Registers a thread: at launch, and after the warpgroups have shared them out (softmax
 // 2 x 128 threads, loaders 2 x 128, MMA 128); the sum must not pass what the block was
 // launched with, and a share that is taken with .inc (or .dec) not be below (above) it.
-// fp32 rows take the loaders twice the registers of bf16 ones: 112 / 104 / 48 took 286 us
-// for the mixed batch above (fp32) and 856 for the chunk (bf16), 112 / 112 / 32 253 and 941,
-// 120 / 96 / 48 315 and 855, 104 / 112 / 48 265 and 1,249.
+// fp32 rows take the loaders twice the registers of bf16 ones. Both splits with both types
+// (us, 112 / 104 / 48 and 112 / 112 / 32): 48 sequences of 60 new rows behind 450, 25 heads,
+// fp32 274 and 232, bf16 184 and 200; 8 of 256 behind 512, 12 heads, fp32 88 and 84, bf16 68
+// and 72; the chunk, bf16 864 and 995, but fp32 1,264 and 1,452: there the shape would want
+// the other split. (120 / 96 / 48 and 104 / 112 / 48 were slower for one or the other.)
 constexpr int kRegsLaunch = 96;
 template <bool BF16>
 constexpr int kRegsSoftmax = 112;
@@ -527,7 +529,7 @@ __device__ __forceinline__ float4 four_of(const void* pool, size_t at) {
 
 // The row sum, relative to the maximum m, of row i of the unit's sequence over those of the unit's
 // keys that it sees, from the scores alone. Rare, hence simple: four keys at a time, which a warp's
-// rows share.
+// rows share (0.6 us a key and tile: the waits of the other roles bound a tile to 3 million keys).
 template <bool BF16>
 __device__ __noinline__ float row_sum(const PagedAttnArgs& a, const volatile Unit& n, int i, float m) {
     const size_t w = (size_t)a.n_kv_head * kHeadDim;

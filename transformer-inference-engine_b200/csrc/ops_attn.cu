@@ -344,7 +344,12 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(PagedAttnArgs a) 
 //   16 sequences, 12 heads 1000 13.6 / 15.8, 4000 52.1 / 59.6, 16,000 (125) 174.6 / 188.9
 // so 8 pages a warp where the clusters take less than half of the SMs, 16 up to two a SM,
 // and 64 where they fill the GPU: up to where one long sequence among short ones would be
-// left to a single cluster.
+// left to a single cluster. The same rule was measured for fp32 and for 4 and 8 rows, whose
+// CTAs an SM holds one of (cluster / shared out, a call after a flush of the caches, about 6 us
+// of it the call's own; fp32, bf16 within 10 % but for the last line):
+//   1 sequence, 1 head     8 rows: 4000 20 / 22, 8000 31 / 25, 16,000 49 / 27; 1 row: 8000 16 / 16
+//   1 sequence, 12 heads   8 rows: 8000 33 / 43, 16,000 55 / 61, 32,000 94 / 96; 1 row: 16,000 35 / 37
+//   16 sequences, 12 heads 8 rows: 4000 145 / 197, 16,000 488 / 641; 1 row: 4000 88 / 92 (bf16 68 / 72)
 int cluster_ctas(int n_seq, int n_kv_head, int pages_per_seq, int sms) {
     const long long units = (long long)n_seq * n_kv_head;
     int ctas = 1;

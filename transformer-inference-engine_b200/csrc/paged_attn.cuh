@@ -22,7 +22,15 @@
 
 namespace tie {
 
-constexpr int kFewRows = 8;        // rows of a streaming unit at most
+// Rows of a streaming unit at most. Streaming and tensor cores, each for all rows, 8 K/V heads
+// (us, a call after a flush of the caches, about 6 of them the call's own; fp32, bf16 in brackets):
+//   1 sequence, 1000 cached:   1 row 10 and 43 (10, 37), 8 rows 14 and 43 (14, 39),
+//                              16 rows 31 and 45 (32, 39), 48 rows 33 and 47 (37, 41)
+//   8 sequences, 1000 cached:  8 rows 49 and 53 (49, 45), 12 rows 45 and 57 (47, 47), 24 rows 66 and 57 (64, 47)
+//   64 sequences, 4000 cached: 1 row 174 and 520 (117, 360), 4 rows 240 and 522 (234, 362),
+//                              8 rows 334 and 522 (336, 364), 12 rows 522 and 526 (494, 371)
+// So the rule holds where there are many sequences; one alone would stream up to 48 rows.
+constexpr int kFewRows = 8;
 constexpr int kHalfRows = 128;     // rows of one MMA of the tensor-core kernel
 constexpr int kTileRows = 256;     // rows of its tiles
 constexpr int kTileKeys = 128;     // keys of one of its steps
@@ -177,7 +185,9 @@ struct JobLine {
     long long share;
 };
 
-// places before a tile's jobs: loading Q, and the results' way out
+// places before a tile's jobs: loading Q, and the results' way out (1, 2, 3, 4: 48 sequences of 60
+// new rows behind 450, 25 heads, fp32 239, 233, 236, 232 us, bf16 190, 184, 186, 182; 8 of 256 behind
+// 512, 12 heads, fp32 84, 84, 84, 88; a long chunk 860 with each)
 constexpr int kTilePlaces = 2;
 
 __device__ __forceinline__ int tile_n_rows(const SeqShape& q, int tile) { return min(kTileRows, q.rows - tile * kTileRows); }

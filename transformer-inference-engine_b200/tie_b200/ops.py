@@ -66,7 +66,8 @@ def attention_paged_workspace():
 def attention_paged(q, k_pages, v_pages, page_table, row_start, ctx_lens, max_new, out, workspace, scale=None,
                     status=None, stream=None):
     """Causal attention of the new rows q over the pages that hold them (tie_attention_paged).
-    scale: 1 / sqrt(64) by default."""
+    scale: 1 / sqrt(64) by default. status: an int32 tensor that receives an error code when a bounded wait in
+    the kernel has expired, which nothing else tells."""
     rc = (_module or _ops()).attention_paged(q, k_pages, v_pages, page_table, row_start, ctx_lens, max_new, out, workspace,
                                              0.125 if scale is None else scale, status, stream)
     if rc:
