@@ -18,7 +18,8 @@ data of each configuration's shapes.
     python bench.py [--gpus N] [--steps K] [--warmup W] [--workload NAME]
                     [--workloads auto|none|NAME,...] [--impl ours|reference]
 
-N > 1 runs under torchrun, one rank per GPU; rank 0 prints one JSON line and
+N > 1 runs under torchrun, one rank per GPU; rank 0 prints one JSON line (the
+headline and a number for each workload; their tables go to a details file) and
 writes a results record in the reference harness's format (tie_b200.results).
 """
 from __future__ import annotations
@@ -741,10 +742,25 @@ def run_ours(args, rank, local_rank, world):
             path = results.write(args.results_dir, f"gpt2_{args.workload}_n{world}", results.header("b200", dev),
                                  records)
             line["results_record"] = os.path.relpath(path, ROOT)
+            details = os.path.join(args.results_dir, f"gpt2_{args.workload}_n{world}_details.json")
+            with open(details, "w") as f:
+                json.dump(line, f, indent=1)
+            line["details"] = os.path.relpath(details, ROOT)
         except OSError as e:
             line["results_record"] = f"not written: {e}"
-        print(json.dumps(line), flush=True)
+        print(json.dumps(short_line(line)), flush=True)
     return 0
+
+
+def short_line(line):
+    """What goes to stdout: one line that a log's last 3 KB hold (all of it with every workload is 32 KB, and stays
+    in the details file). Tables become one number for each entry."""
+    out = {k: v for k, v in line.items() if k not in ("kernels", "workloads", "cpu_baseline", "peaks", "phases")}
+    if "workloads" in line:
+        out["workloads"] = {n: float(f"{w['value']:.6g}") for n, w in line["workloads"].items() if w.get("value")}
+    if "cpu_baseline" in line:
+        out["cpu_baseline"] = {k: line["cpu_baseline"][k] for k in ("value", "unit", "cores", "kind")}
+    return out
 
 
 def run_kernel(args):
