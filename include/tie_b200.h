@@ -300,7 +300,11 @@ model_status tie_head_argmax_noalloc(const float *x, int ldx, const float *w, in
  * workspace too small or a limit below; MODEL_ERR_DEVICE for a CUDA failure.
  * Limits: 4096 sequences or requests, 2^27 pages (2^26 per sequence), 16 beams,
  * 2^30 logits a row. */
-enum { TIE_KV_F32 = 0, TIE_KV_BF16 = 1 };
+enum {
+    TIE_KV_F32 = 0,
+    TIE_KV_BF16 = 1,
+    TIE_KV_INT8 = 2   /* pages with scales: the entry points that take scales */
+};
 
 /* Page table entries, row starts and slot maps from request lengths. Sequence
  * s has ctx_lens[s] positions cached and appends new_lens[s] (>= 0). Its
@@ -399,6 +403,99 @@ model_status tie_kv_reorder(void *k_pages, void *v_pages, int kv_format, int n_l
                             const int32_t *page_table, int pages_per_seq, const int32_t *parent,
                             const int32_t *first, const int32_t *length, int n_req, int beams,
                             void *stream);
+
+/* ---- the cache in 8 bits --------------------------------------------------
+ * A pool in 8 bits (TIE_KV_INT8) is, for keys and for values, n_pages pages of
+ * KV_CACHE_PAGE_ROWS rows of n_kv_head * 64 int8 levels, and a scale per row and
+ * head: fp32 [n_pages][n_kv_head][KV_CACHE_PAGE_ROWS]. An element is level *
+ * scale; scale = max |x| / 127 of the head's 64 elements, level = x / scale to
+ * the nearest integer, ties to even (of the exact quotient), 0 where the scale
+ * is 0. A head's row with an element that is not finite gets a scale that is NaN
+ * and levels 0. Pointers, streams and errors are those of the paged cache above. */
+
+/* tie_kv_store into a pool in 8 bits. */
+model_status tie_kv_store_q8(const float *k, const float *v, int ld, const int32_t *slots, int rows,
+                             void *k_pages, void *v_pages, float *k_scales, float *v_scales,
+                             int n_pages, int n_kv_head, void *stream);
+
+/* Rows of a pool of any format read back: row r of k and v (n_kv_head * 64
+ * floats, ld floats apart) receives what slot slots[r] holds. A slot outside the
+ * pool leaves its row as it was; a slot may be read by any number of rows.
+ * k_scales and v_scales: those of TIE_KV_INT8, NULL for the other formats.
+ * rows == 0 is allowed (k, v and slots may be NULL then). */
+model_status tie_kv_load(const int32_t *slots, int rows, const void *k_pages, const void *v_pages,
+                         const float *k_scales, const float *v_scales, int kv_format, int n_pages,
+                         int n_kv_head, float *k, float *v, int ld, void *stream);
+
+/* Attention of new tokens over their sequences' own pages and over pages that
+ * groups of sequences share: beams and answers of one prompt, requests behind one
+ * instruction. Group g is sequences group_start[g] .. group_start[g + 1] - 1
+ * (group_start[n_group + 1], ascending); its first prefix_lens[g] positions lie in
+ * the pages of prefix_table (n_group rows of pages_per_prefix entries) and are read
+ * once for all its rows. A sequence's own pages (page_table, ctx_lens) hold what
+ * comes behind them, from a page's first row on. For row r of sequence s, its new
+ * token i, and query head h,
+ *   out[r][h] = sum_j softmax_j(scale * q[r][h] . k[j]) v[j]
+ * over the group's shared positions and the sequence's own positions 0 ..
+ * ctx_lens[s] + i whose page is mapped; 0 where none is left. A sequence in no
+ * group has its own positions only, and so have those of a group whose range or
+ * length has no meaning (outside 0..n_seq or pages_per_prefix pages). n_group 0:
+ * no groups (prefix_table, prefix_lens and group_start NULL). kv_format may be
+ * TIE_KV_INT8, with the pool's scales (NULL for the others).
+ * All else is as for tie_attention_paged: rows, limits, what is left out, and what
+ * is not finite. Sums and softmax statistics are fp32, products of all of their
+ * operands' 24 bits. The result of a row depends, in its rounding, on how the
+ * batch splits its keys, and is the same for the same call.
+ * workspace: tie_attention_shared_workspace(rows, n_head) bytes (on the current
+ * device) or more. */
+size_t tie_attention_shared_workspace(int rows, int n_head);
+model_status tie_attention_shared(const float *q, int ldq, int n_head, const void *k_pages,
+                                  const void *v_pages, const float *k_scales,
+                                  const float *v_scales, int kv_format, int n_pages, int n_kv_head,
+                                  const int32_t *page_table, int pages_per_seq,
+                                  const int32_t *row_start, const int32_t *ctx_lens, int n_seq,
+                                  int max_new, int rows, const int32_t *prefix_table,
+                                  int pages_per_prefix, const int32_t *prefix_lens,
+                                  const int32_t *group_start, int n_group, float scale, float *out,
+                                  int ldo, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- 4-bit weights --------------------------------------------------------
+ * A weight matrix W of n rows (outputs) of k weights, cut along k into groups of
+ * 32, 64 or 128. A group has a scale = max |w| / 7 in fp32, rounded to bf16, and
+ * levels -7 .. 7 = w / scale to the nearest integer, ties to even (of the exact
+ * quotient); a weight is level * scale. A group with a weight that is not finite
+ * gets a scale that is NaN and levels 0, one whose scale is 0 levels 0.
+ * packed: tie_q4_bytes(n, k) bytes, 16-byte aligned; a row is blocks of 128
+ * weights in 64 bytes, the last one filled up with zeros. The 32-bit word 4 t + j
+ * of a block (t, j = 0 .. 3) holds its weights 32 j + 8 t + i, i = 0 .. 7, as
+ * level + 8 in bits 4 i .. 4 i + 3. scales: bf16 [n][ceil(k / group)].
+ * Pointers are DEVICE pointers of one device; any k and leading dimension is
+ * taken (fp32 rows that are 16-byte aligned are read faster). Streams and errors
+ * are those of the paged cache above; MODEL_ERR_CAPACITY for k above 2^24 or more
+ * than 2^31 thread blocks of work. */
+
+/* Bytes of the packed levels (0 for sizes without meaning). */
+size_t tie_q4_bytes(int n, int k);
+
+/* fp32 weights (ldw floats from row to row) to levels and scales, and back. */
+model_status tie_quantize_q4(const float *w, long long ldw, int n, int k, int group, void *packed,
+                             void *scales, void *stream);
+model_status tie_dequantize_q4(const void *packed, const void *scales, int n, int k, int group,
+                               float *w, long long ldw, void *stream);
+
+/* y[r] = act(x[r] W^T + bias) + residual[r] for `rows` rows of activations (ldx,
+ * ldr, ldy floats apart): the matmul of a decode step with its epilogue (the
+ * bias, GELU and residual forms of model.c:735-752).
+ * bias [n] and residual may be NULL; gelu 1: act is GELU (model.c:615-623), 0:
+ * none. residual may be y itself, x must not overlap y. Products are exact and
+ * sums fp32 (a group's, then the groups'), in an order that depends on n and k
+ * only, so a row's result does not depend on the rows beside it except by their
+ * number being at most 2 or above. The weights are read once for every 8 rows.
+ * rows == 0 is allowed (x and y may be NULL then); at most 524,280 rows. */
+model_status tie_matvec_q4(const float *x, long long ldx, int rows, const void *packed,
+                           const void *scales, int n, int k, int group, const float *bias,
+                           const float *residual, long long ldr, int gelu, float *y, long long ldy,
+                           void *stream);
 
 #ifdef __cplusplus
 }

@@ -29,6 +29,13 @@ decltype(&tie_kv_store) kv_store_fn = nullptr;
 decltype(&tie_attention_paged) attention_paged_fn = nullptr;
 decltype(&tie_beam_select) beam_select_fn = nullptr;
 decltype(&tie_kv_reorder) kv_reorder_fn = nullptr;
+decltype(&tie_kv_store_q8) kv_store_q8_fn = nullptr;
+decltype(&tie_kv_load) kv_load_fn = nullptr;
+decltype(&tie_attention_shared) attention_shared_fn = nullptr;
+decltype(&tie_quantize_q4) quantize_q4_fn = nullptr;
+decltype(&tie_dequantize_q4) dequantize_q4_fn = nullptr;
+decltype(&tie_matvec_q4) matvec_q4_fn = nullptr;
+decltype(&tie_q4_bytes) q4_bytes_fn = nullptr;
 
 // Thrown after a Python error has been set.
 struct Refused {};
@@ -125,7 +132,8 @@ struct Pool {
     void *k, *v;
     int format, n_pages, heads, layers, device;
     size_t layer_stride;
-    Pool(PyObject* ko, PyObject* vo) {
+    // levels: 8-bit pages are taken too (with scales, below)
+    Pool(PyObject* ko, PyObject* vo, bool levels = false) {
         const Tensor a("k_pages", ko), b("v_pages", vo);
         bool same = a.t.ndim == b.t.ndim && a.t.dtype.code == b.t.dtype.code && a.t.dtype.bits == b.t.dtype.bits &&
                     a.device() >= 0 && a.device() == b.device() && a.contiguous() && b.contiguous();
@@ -133,7 +141,8 @@ struct Pool {
         if (!same) wrong("k_pages and v_pages", "one shape, type and CUDA device, contiguous, are");
         if (a.is(kDLFloat, 32)) format = TIE_KV_F32;
         else if (a.is(kDLBfloat, 16)) format = TIE_KV_BF16;
-        else wrong("k_pages, v_pages", "float32 or bfloat16 is");
+        else if (levels && a.is(kDLInt, 8)) format = TIE_KV_INT8;
+        else wrong("k_pages, v_pages", levels ? "float32, bfloat16 or int8 is" : "float32 or bfloat16 is");
         const int64_t* s = a.t.shape + (a.t.ndim == 4);
         if ((a.t.ndim != 3 && a.t.ndim != 4) || s[1] != KV_CACHE_PAGE_ROWS || s[2] % kHeadDim)
             wrong("k_pages, v_pages", "[n_pages, 16, n_kv_head * 64] is");
@@ -150,18 +159,40 @@ struct Pool {
     }
 };
 
+// the scales of a pool in 8 bits, or none for one that is not
+struct Scales {
+    float *k = nullptr, *v = nullptr;
+    Scales(const Pool& pool, PyObject* ko, PyObject* vo) {
+        pool.one_layer();
+        if (pool.format != TIE_KV_INT8) {
+            if (ko != Py_None || vo != Py_None) wrong("k_scales, v_scales", "int8 pages are");
+            return;
+        }
+        k = one(pool, "k_scales", ko);
+        v = one(pool, "v_scales", vo);
+    }
+    static float* one(const Pool& pool, const char* name, PyObject* o) {
+        if (o == Py_None) wrong(name, "a scale per row and head (int8 pages) is");
+        const Tensor x(name, o);
+        if (!x.is(kDLFloat, 32) || x.t.ndim != 3 || x.t.shape[0] != pool.n_pages || x.t.shape[1] != pool.heads ||
+            x.t.shape[2] != KV_CACHE_PAGE_ROWS || !x.contiguous() || x.device() != pool.device)
+            wrong(name, "a contiguous float32 [n_pages, n_kv_head, 16] on the pool's device is");
+        return static_cast<float*>(x.data());
+    }
+};
+
 struct Table {
     int32_t* p;
     int n_seq, width, device;
     // any: on the device that the table itself is on
-    Table(PyObject* o, int on, bool any = false) {
-        const Tensor x("page_table", o);
+    Table(PyObject* o, int on, bool any = false, const char* name = "page_table") {
+        const Tensor x(name, o);
         device = x.device();
         if (!x.is(kDLInt, 32) || x.t.ndim != 2 || !x.contiguous() || device < 0 || (!any && device != on))
-            wrong("page_table", "a contiguous int32 [n_seq, pages_per_seq] on the pool's device is");
+            wrong(name, "a contiguous int32 [n_seq, pages_per_seq] on the pool's device is");
         p = static_cast<int32_t*>(x.data());
-        n_seq = as_int("page_table", x.t.shape[0]);
-        width = as_int("page_table", x.t.shape[1]);
+        n_seq = as_int(name, x.t.shape[0]);
+        width = as_int(name, x.t.shape[1]);
     }
 };
 
@@ -322,10 +353,160 @@ PyObject* kv_reorder(PyObject*, PyObject* const* v, Py_ssize_t n) {
     });
 }
 
-// torch.Tensor, its exchange interface, the addresses of the five entry points
+// k, v, slots, k_pages, v_pages, k_scales, v_scales, stream
+PyObject* kv_store_q8(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    return guarded(n, 8, [&] {
+        const Pool pool(v[3], v[4], true);
+        if (pool.format != TIE_KV_INT8) wrong("k_pages, v_pages", "int8 is");
+        const Scales sc(pool, v[5], v[6]);
+        const int64_t w = (int64_t)pool.heads * kHeadDim;
+        const Rows a("k", v[0], w, pool.device), b("v", v[1], w, pool.device);
+        if (a.rows != b.rows || a.ld != b.ld) wrong("k and v", "one shape and row stride is");
+        int32_t* slots = ints("slots", v[2], a.rows, pool.device);
+        void* st = stream_of(v[7], pool.device);
+        return unlocked([&] {
+            return kv_store_q8_fn(a.p, b.p, a.ld, slots, (int)a.rows, pool.k, pool.v, sc.k, sc.v, pool.n_pages, pool.heads, st);
+        });
+    });
+}
+
+// slots, k_pages, v_pages, k_out, v_out, k_scales, v_scales, stream
+PyObject* kv_load(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    return guarded(n, 8, [&] {
+        const Pool pool(v[1], v[2], true);
+        const Scales sc(pool, v[5], v[6]);
+        const int64_t w = (int64_t)pool.heads * kHeadDim;
+        const Rows a("k_out", v[3], w, pool.device), b("v_out", v[4], w, pool.device);
+        if (a.rows != b.rows || a.ld != b.ld) wrong("k_out and v_out", "one shape and row stride is");
+        int32_t* slots = ints("slots", v[0], a.rows, pool.device);
+        void* st = stream_of(v[7], pool.device);
+        return unlocked([&] {
+            return kv_load_fn(slots, (int)a.rows, pool.k, pool.v, sc.k, sc.v, pool.format, pool.n_pages, pool.heads, a.p, b.p,
+                              a.ld, st);
+        });
+    });
+}
+
+// q, k_pages, v_pages, page_table, row_start, ctx_lens, max_new, out, workspace, k_scales, v_scales,
+// prefix_table, prefix_lens, group_start, scale, stream
+PyObject* attention_shared(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    return guarded(n, 16, [&] {
+        const Pool pool(v[1], v[2], true);
+        const Scales sc(pool, v[9], v[10]);
+        const int d = pool.device;
+        const Table table(v[3], d);
+        const Tensor qt("q", v[0]);
+        const int64_t w = qt.t.ndim == 2 ? qt.t.shape[1] : -1;
+        if (w < 0 || w % kHeadDim) wrong("q and out", "one shape [rows, n_head * 64] is");
+        const Rows q("q", v[0], w, d), out("out", v[7], w, d);
+        if (q.rows != out.rows) wrong("q and out", "one shape [rows, n_head * 64] is");
+        int32_t* start = ints("row_start", v[4], (int64_t)table.n_seq + 1, d);
+        int32_t* ctx = ints("ctx_lens", v[5], table.n_seq, d);
+        const int max_new = as_int("max_new", v[6]);
+        const Workspace ws(v[8], d);
+        int32_t *prefix = nullptr, *lens = nullptr, *groups = nullptr;
+        int n_group = 0, prefix_width = 0;
+        if (v[11] != Py_None) {
+            const Table t(v[11], d, false, "prefix_table");
+            prefix = t.p;
+            prefix_width = t.width;
+            n_group = t.n_seq;
+            if (n_group <= 0) wrong("prefix_table", "a row for each group is");
+            lens = ints("prefix_lens", v[12], n_group, d);
+            groups = ints("group_start", v[13], (int64_t)n_group + 1, d);
+        } else if (v[12] != Py_None || v[13] != Py_None) {
+            wrong("prefix_table", "a table beside prefix_lens and group_start is");
+        }
+        const double scale = PyFloat_AsDouble(v[14]);
+        if (scale == -1.0 && PyErr_Occurred()) throw Refused{};
+        void* st = stream_of(v[15], d);
+        return unlocked([&] {
+            return attention_shared_fn(q.p, q.ld, (int)(w / kHeadDim), pool.k, pool.v, sc.k, sc.v, pool.format, pool.n_pages,
+                                       pool.heads, table.p, table.width, start, ctx, table.n_seq, max_new, (int)q.rows, prefix,
+                                       prefix_width, lens, groups, n_group, (float)scale, out.p, out.ld, ws.p, ws.bytes, st);
+        });
+    });
+}
+
+// The levels and scales of 4-bit weights of n rows of k.
+struct Q4 {
+    void *packed, *scales;
+    int n, k, group, device;
+    Q4(PyObject* po, PyObject* so, PyObject* go, int64_t columns) {
+        const Tensor p("packed", po), s("scales", so);
+        group = as_int("group", go);
+        if (group != 32 && group != 64 && group != 128) wrong("group", "32, 64 or 128 is");
+        device = p.device();
+        k = as_int("k", columns);
+        if (p.t.ndim != 2 || !p.is(kDLUInt, 8) || !p.contiguous() || device < 0 || k <= 0 || p.t.shape[0] <= 0 ||
+            (size_t)p.t.shape[1] != q4_bytes_fn(1, k))
+            wrong("packed", "a contiguous uint8 [n, 64 ceil(k / 128)] on a CUDA device is");
+        n = as_int("packed", p.t.shape[0]);
+        if (s.t.ndim != 2 || !s.is(kDLBfloat, 16) || !s.contiguous() || s.device() != device || s.t.shape[0] != n ||
+            s.t.shape[1] != (k + (int64_t)group - 1) / group)
+            wrong("scales", "a contiguous bfloat16 [n, ceil(k / group)] beside packed is");
+        packed = p.data();
+        scales = s.data();
+    }
+};
+int64_t columns_of(const char* name, PyObject* o) {
+    const Tensor x(name, o);
+    if (x.t.ndim != 2) wrong(name, "a float32 matrix is");
+    return x.t.shape[1];
+}
+
+// w, packed, scales, group, stream
+PyObject* quantize_q4(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    return guarded(n, 5, [&] {
+        const Q4 z(v[1], v[2], v[3], columns_of("w", v[0]));
+        const Rows w("w", v[0], z.k, z.device);
+        if (w.rows != z.n) wrong("w and packed", "one number of rows is");
+        void* st = stream_of(v[4], z.device);
+        return unlocked([&] { return quantize_q4_fn(w.p, w.ld, z.n, z.k, z.group, z.packed, z.scales, st); });
+    });
+}
+
+// packed, scales, group, w, stream
+PyObject* dequantize_q4(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    return guarded(n, 5, [&] {
+        const Q4 z(v[0], v[1], v[2], columns_of("w", v[3]));
+        const Rows w("w", v[3], z.k, z.device);
+        if (w.rows != z.n) wrong("w and packed", "one number of rows is");
+        void* st = stream_of(v[4], z.device);
+        return unlocked([&] { return dequantize_q4_fn(z.packed, z.scales, z.n, z.k, z.group, w.p, w.ld, st); });
+    });
+}
+
+// x, packed, scales, group, y, bias, residual, gelu, stream
+PyObject* matvec_q4(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    return guarded(n, 9, [&] {
+        const Q4 z(v[1], v[2], v[3], columns_of("x", v[0]));
+        const Rows x("x", v[0], z.k, z.device), y("y", v[4], z.n, z.device);
+        if (x.rows != y.rows) wrong("x and y", "one number of rows is");
+        float* bias = v[5] == Py_None ? nullptr : vector_of<float>("bias", v[5], z.n, z.device);
+        float* residual = nullptr;
+        int ldr = 0;
+        if (v[6] != Py_None) {
+            const Rows r("residual", v[6], z.n, z.device);
+            if (r.rows != y.rows) wrong("residual and y", "one shape is");
+            residual = r.p;
+            ldr = r.ld;
+        }
+        const int gelu = PyObject_IsTrue(v[7]);
+        if (gelu < 0) throw Refused{};
+        void* st = stream_of(v[8], z.device);
+        return unlocked([&] {
+            return matvec_q4_fn(x.p, x.ld, (int)x.rows, z.packed, z.scales, z.n, z.k, z.group, bias, residual, ldr, gelu, y.p,
+                                y.ld, st);
+        });
+    });
+}
+
+// torch.Tensor, its exchange interface, the addresses of the entry points in the order below
 PyObject* init(PyObject*, PyObject* const* v, Py_ssize_t n) {
-    if (n != 7 || !PyType_Check(v[0])) {
-        PyErr_SetString(PyExc_TypeError, "torch.Tensor, its exchange interface and five addresses are wanted");
+    constexpr Py_ssize_t kFns = 12;
+    if (n != 2 + kFns || !PyType_Check(v[0])) {
+        PyErr_SetString(PyExc_TypeError, "torch.Tensor, its exchange interface and the entry points' addresses are wanted");
         return nullptr;
     }
     const auto* got = static_cast<const DLPackExchangeAPI*>(PyCapsule_GetPointer(v[1], "dlpack_exchange_api"));
@@ -335,14 +516,21 @@ PyObject* init(PyObject*, PyObject* const* v, Py_ssize_t n) {
         PyErr_SetString(PyExc_ImportError, "tie_b200._ops was built for another version of torch's tensors");
         return nullptr;
     }
-    void* at[5];
-    for (int i = 0; i < 5; ++i)
+    void* at[kFns];
+    for (int i = 0; i < kFns; ++i)
         if (!(at[i] = PyLong_AsVoidPtr(v[2 + i]))) return PyErr_Occurred() ? nullptr : (PyErr_SetString(PyExc_ValueError, "address"), nullptr);
     page_plan_fn = reinterpret_cast<decltype(page_plan_fn)>(at[0]);
     kv_store_fn = reinterpret_cast<decltype(kv_store_fn)>(at[1]);
     attention_paged_fn = reinterpret_cast<decltype(attention_paged_fn)>(at[2]);
     beam_select_fn = reinterpret_cast<decltype(beam_select_fn)>(at[3]);
     kv_reorder_fn = reinterpret_cast<decltype(kv_reorder_fn)>(at[4]);
+    kv_store_q8_fn = reinterpret_cast<decltype(kv_store_q8_fn)>(at[5]);
+    kv_load_fn = reinterpret_cast<decltype(kv_load_fn)>(at[6]);
+    attention_shared_fn = reinterpret_cast<decltype(attention_shared_fn)>(at[7]);
+    quantize_q4_fn = reinterpret_cast<decltype(quantize_q4_fn)>(at[8]);
+    dequantize_q4_fn = reinterpret_cast<decltype(dequantize_q4_fn)>(at[9]);
+    matvec_q4_fn = reinterpret_cast<decltype(matvec_q4_fn)>(at[10]);
+    q4_bytes_fn = reinterpret_cast<decltype(q4_bytes_fn)>(at[11]);
     Py_INCREF(v[0]);
     tensor_type = reinterpret_cast<PyTypeObject*>(v[0]);
     api = got;
@@ -356,6 +544,12 @@ PyMethodDef methods[] = {{"init", fast(init), METH_FASTCALL, nullptr},
                          {"attention_paged", fast(attention_paged), METH_FASTCALL, nullptr},
                          {"beam_select", fast(beam_select), METH_FASTCALL, nullptr},
                          {"kv_reorder", fast(kv_reorder), METH_FASTCALL, nullptr},
+                         {"kv_store_q8", fast(kv_store_q8), METH_FASTCALL, nullptr},
+                         {"kv_load", fast(kv_load), METH_FASTCALL, nullptr},
+                         {"attention_shared", fast(attention_shared), METH_FASTCALL, nullptr},
+                         {"quantize_q4", fast(quantize_q4), METH_FASTCALL, nullptr},
+                         {"dequantize_q4", fast(dequantize_q4), METH_FASTCALL, nullptr},
+                         {"matvec_q4", fast(matvec_q4), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", "Argument checks and calls of tie_b200.ops", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

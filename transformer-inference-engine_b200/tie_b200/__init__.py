@@ -12,6 +12,6 @@ from .lib import (  # noqa: F401
     gemm_naive, gemm_naive_bt, gemm_tiled, gemm_tiled_bt, layernorm_normalize, attention_prefill, argmax,
     MODEL_PATH_NOCACHE, MODEL_PATH_CACHE, TIE_STEP_PERSISTENT, TIE_STEP_CHAINED, TIE_STEP_STREAM,
     TIE_WEIGHTS_F32, TIE_WEIGHTS_BF16, TIE_WEIGHTS_INT8, MODEL_CPROJ_AS_STORED, MODEL_CPROJ_TRANSPOSED,
-    TIE_KV_F32, TIE_KV_BF16,
+    TIE_KV_F32, TIE_KV_BF16, TIE_KV_INT8,
     EXPORTED_SYMBOLS,
 )

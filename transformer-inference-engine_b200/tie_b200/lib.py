@@ -21,7 +21,7 @@ for _i, _n in enumerate(MODEL_STATUS + KV_STATUS):
 MODEL_PATH_NOCACHE, MODEL_PATH_CACHE = 0, 1
 TIE_STEP_PERSISTENT, TIE_STEP_CHAINED, TIE_STEP_STREAM = 0, 1, 2
 TIE_WEIGHTS_F32, TIE_WEIGHTS_BF16, TIE_WEIGHTS_INT8 = 0, 1, 2
-TIE_KV_F32, TIE_KV_BF16 = 0, 1
+TIE_KV_F32, TIE_KV_BF16, TIE_KV_INT8 = 0, 1, 2
 MODEL_CPROJ_AS_STORED, MODEL_CPROJ_TRANSPOSED = 0, 1
 
 _fp = C.POINTER(C.c_float)
@@ -148,6 +148,17 @@ def library():
                                       _vp, C.c_size_t, _vp]),
         "tie_kv_reorder": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_size_t, C.c_int, C.c_int, _vp, C.c_int, _vp,
                                      _vp, _vp, C.c_int, C.c_int, _vp]),
+        "tie_kv_store_q8": (C.c_int, [_vp, _vp, C.c_int, _vp, C.c_int, _vp, _vp, _vp, _vp, C.c_int, C.c_int, _vp]),
+        "tie_kv_load": (C.c_int, [_vp, C.c_int, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp]),
+        "tie_attention_shared_workspace": (C.c_size_t, [C.c_int, C.c_int]),
+        "tie_attention_shared": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp,
+                                           C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp,
+                                           C.c_int, C.c_float, _vp, C.c_int, _vp, C.c_size_t, _vp]),
+        "tie_q4_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+        "tie_quantize_q4": (C.c_int, [_vp, C.c_longlong, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp]),
+        "tie_dequantize_q4": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, _vp, C.c_longlong, _vp]),
+        "tie_matvec_q4": (C.c_int, [_vp, C.c_longlong, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp,
+                                    C.c_longlong, C.c_int, _vp, C.c_longlong, _vp]),
         "kv_cache_footprint_for": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
         "kv_cache_create": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(_vp)]),
         "kv_cache_destroy": (None, [_vp]),
