@@ -13,9 +13,11 @@
 // Work. An item is 8 NT rows that share keys (a sequence's new tokens or a group's, times
 // the query heads of one K/V head) and all pages of those keys. All items of a call stand
 // in one line, each as many places as it has steps of PG pages, and one for what it
-// costs besides; every warp of the grid takes an equal stretch of the line, whatever
-// the lengths are, and works alone (no barriers). An item that a stretch cuts leaves parts,
-// which a second kernel joins; it finds them from the lengths, as the first one cut them.
+// costs besides. A team of as many warps as there are K/V heads, each with one of them, takes an
+// equal stretch of the line, whatever the lengths are; every warp works alone (no barriers).
+// Heads side by side read whole rows of a page at about one time: a warp that walked its head's
+// pages by itself, head after head, got 3.3 TB/s out of 8-bit pages (64 bytes of a row, with
+// nobody beside it). An item that a stretch cuts leaves parts, which a second kernel joins.
 //
 // Products run on bf16 MMAs (m16n8k16). An fp32 number is exactly the sum of three bf16
 // terms, a level of 8 bits and a bf16 number are one; products of terms below 2^-24 of the
@@ -29,6 +31,7 @@
 
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "paged_attn.cuh"
 #include "quant.cuh"
@@ -36,29 +39,46 @@
 namespace tie {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr unsigned kAll = 0xffffffffu;
 // Weights are 2^(s - max) times this, so that the sum of as many of them as there are
 // positions (2^30) times any finite value stays finite.
 constexpr float kWeight = 0x1p-30f;
 // fewest steps worth a warp's stretch
-constexpr int kMinShare = 3;
+constexpr int kMinShare = 2;
 
-// Pages of a step: as many as keep 8 KB of a warp's loads on their way, with few rows.
+// Pages of a step.
 template <int FMT, int NT>
-constexpr int kPages = FMT == TIE_KV_F32 ? 1 : FMT == TIE_KV_BF16 ? (NT > 2 ? 1 : 2) : (NT > 2 ? 2 : 4);
+constexpr int kPages = FMT == TIE_KV_F32 ? 1 : FMT == TIE_KV_BF16 ? (NT > 1 ? 1 : 2) : 2;
+
+// CTAs on an SM
+template <int FMT, int NT>
+constexpr int kCtas = NT <= 2 ? 3 : 2;
 
 // A line: units [u0, u1) (a unit below n_group is a group's prefix, the others are
-// sequences), cut into stretches for `warps` warps.
+// sequences), cut into stretches for `teams` teams of warps.
 struct Line {
-    int u0, u1, nt, pages, warps;      // nt: of the items; pages: of a step
+    int u0, u1, nt, pages, teams;      // nt: of the items; pages: of a step
     float* part_o;                     // [2 * warps][8 nt][64]: a warp's parts of the item it goes on with
     float* part_ml;                    // and of the one that it begins; (maximum, sum)
 };
 
+// n / d for 0 <= n < 2^31 (the multiplier is 2^(32 + shift) / d, rounded up, less 2^32)
+struct Divisor {
+    int d, shift;
+    unsigned mul;
+    __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi(mul, (unsigned)n) + (unsigned)n) >> shift); }
+};
+Divisor divisor(int d) {
+    int shift = 0;
+    while ((1LL << shift) < d) ++shift;
+    return Divisor{d, shift, (unsigned)(((1ULL << 32) * ((1ULL << shift) - (unsigned long long)d)) / (unsigned long long)d + 1)};
+}
+
 struct SharedArgs {
     const float* q;
     int ldq, n_head, group, n_kv_head;
+    Divisor by_group;
     const void *k, *v;
     const float *ks, *vs;
     int n_pages;
@@ -75,8 +95,9 @@ struct SharedArgs {
     int ldo;
     float* whole_o[2];                 // [prefix, own][row][head][64]: items that no stretch cuts
     float* whole_ml[2];                // (only where rows have two sources)
+    int2* place[2];                    // [prefix, own][row][head]: the row of its first part in the line's parts,
+                                       // or -1: whole; how many parts
     Line line[2];                      // of the prefixes and of the sequences; line[1] may be line[0]
-    int one_line;
 };
 
 // What a unit's rows are, and its keys. rows == 0: nothing to do.
@@ -114,12 +135,15 @@ __device__ __forceinline__ int unit_places(const UnitShape& s, const Line& l) {
     const int step = l.pages * kPageRows;
     return (s.keys - 1) / step + 2;
 }
-__device__ __forceinline__ long long unit_items(const SharedArgs& a, const UnitShape& s, const Line& l) {
-    return (long long)((s.rows + 8 * l.nt - 1) / (8 * l.nt)) * a.n_kv_head;
+__device__ __forceinline__ long long unit_items(const UnitShape& s, const Line& l) { return (s.rows + 8 * l.nt - 1) / (8 * l.nt); }
+
+// x / y of numbers that are nearly always small (a division of 64 bits is a hundred instructions)
+__device__ __forceinline__ long long quotient(long long x, long long y) {
+    return ((x | y) >> 32) == 0 ? (long long)((unsigned)x / (unsigned)y) : x / y;
 }
 
 __device__ __forceinline__ long long share_of(const Line& l, long long total) {
-    const long long even = (total + l.warps - 1) / l.warps;
+    const long long even = quotient(total + l.teams - 1, l.teams);
     return even > kMinShare ? even : kMinShare;
 }
 
@@ -133,7 +157,7 @@ __device__ __forceinline__ void build_base(const SharedArgs& a, int u0, int u1, 
         if (u >= u1) break;
         const UnitShape s = unit_shape(a, u);
         const Line& l = a.line[u >= a.n_group];
-        if (s.rows) mine += unit_items(a, s, l) * unit_places(s, l);
+        if (s.rows) mine += unit_items(s, l) * unit_places(s, l);
     }
     const long long total = scan_threads<kThreads>(mine, sc, t, &before);
     for (int i = 0; i < per; ++i) {
@@ -143,7 +167,7 @@ __device__ __forceinline__ void build_base(const SharedArgs& a, int u0, int u1, 
         if (per > 1) {                 // a thread's only unit needs no second look
             const UnitShape s = unit_shape(a, u);
             const Line& l = a.line[u >= a.n_group];
-            if (s.rows) before += unit_items(a, s, l) * unit_places(s, l);
+            if (s.rows) before += unit_items(s, l) * unit_places(s, l);
         }
     }
     if (t == 0) base[n] = total;
@@ -170,17 +194,9 @@ __device__ __forceinline__ void load_words(const void* base, size_t byte, uint32
     }
 }
 
-// Bytes 0 and 2 of a word, as signed levels, in a pair of bf16: 0x4300 | u is 128 + u for
-// u < 128, and 0x4380 is 256, so (128 + low 7 bits) - (128 + sign bit) is the level.
-__device__ __forceinline__ uint32_t levels2(uint32_t w) {
-    const uint32_t low = (w & 0x007f007fu) | 0x43004300u, sign = (w & 0x00800080u) | 0x43004300u;
-    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&low), *reinterpret_cast<const __nv_bfloat162*>(&sign));
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 
@@ -197,20 +213,26 @@ __device__ __forceinline__ void split3(float lo, float hi, uint32_t (&x)[3]) {
 // sets: d += the largest terms' product, and e += the others', which are 2^-8 of it (a product of
 // terms below 2^-24 of the whole is left out). With all in one chain of 24 MMAs the error of the
 // result was 2.0e-6 over fp32 pages (2-norm, 1000 positions), in two sets it is 4.0e-7.
-__device__ __forceinline__ void main_product(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b0)[3],
-                                             const uint32_t (&b1)[3]) {
-    mma_bf16(d, a, b0[0], b1[0]);
-}
+// Products of terms (of A, of B) in the order they are added; the last one is the largest.
 template <int NA>
-__device__ __forceinline__ void small_products(float (&e)[4], const uint32_t (&a)[NA][4], const uint32_t (&b0)[3],
-                                               const uint32_t (&b1)[3]) {
-    if constexpr (NA == 3) mma_bf16(e, a[2], b0[0], b1[0]);
-    mma_bf16(e, a[0], b0[2], b1[2]);
-    if constexpr (NA == 3) {
-        mma_bf16(e, a[1], b0[1], b1[1]);
-        mma_bf16(e, a[1], b0[0], b1[0]);
-    }
-    mma_bf16(e, a[0], b0[1], b1[1]);
+struct Products {
+    static constexpr int kSmall = NA == 3 ? 5 : 2;
+    // 0 2, 2 0, 1 1, 1 0, 0 1, 0 0 and, of a single term, 0 2, 0 1, 0 0
+    static __device__ __forceinline__ constexpr int a(int x) { return NA == 1 ? 0 : x == 1 ? 2 : x == 2 || x == 3 ? 1 : 0; }
+    static __device__ __forceinline__ constexpr int b(int x) { return NA == 1 ? 2 - x : x == 0 ? 2 : x == 2 || x == 4 ? 1 : 0; }
+};
+// Products [FROM, TO) for R accumulators, which take turns: an MMA that waits for the one before it
+// waits its whole latency.
+template <bool FIRST, int FROM, int TO, int R, int NA, typename A, typename B0, typename B1>
+__device__ __forceinline__ void add_products(float (&d)[R][4], const A& fa, const B0& b0, const B1& b1) {
+#pragma unroll
+    for (int x = FROM; x < TO; ++x)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            using P = Products<NA>;
+            if (FIRST && x == FROM) mma_bf16(d[r], fa(r, P::a(x)), b0(r, P::b(x)), b1(r, P::b(x)), {0.f, 0.f, 0.f, 0.f});
+            else mma_bf16(d[r], fa(r, P::a(x)), b0(r, P::b(x)), b1(r, P::b(x)));
+        }
 }
 
 // --------------------------------------------------------------- the products --
@@ -245,7 +267,6 @@ struct Format<TIE_KV_F32> {
             a[2][r] = x[2];
         }
     }
-    static constexpr int kApart = 1;   // from the first of a pair of dims to the second
 };
 template <>
 struct Format<TIE_KV_BF16> {
@@ -258,48 +279,38 @@ struct Format<TIE_KV_BF16> {
 #pragma unroll
         for (int r = 0; r < 4; ++r) a[0][r] = __byte_perm(v[2 * (r >> 1)][i], v[2 * (r >> 1) + 1][i], r & 1 ? 0x7632 : 0x5410);
     }
-    static constexpr int kApart = 1;
 };
 template <>
 struct Format<TIE_KV_INT8> {
-    static constexpr int kBytes = 1, kTerms = 1;
-    static __device__ __forceinline__ void keys(const uint32_t (&k)[2][4], int s, uint32_t (&a)[1][4]) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) a[0][r] = levels2(k[r & 1][s] >> (8 * (r >> 1)));
-    }
-    static __device__ __forceinline__ void values(const uint32_t (&v)[4][2], int i, uint32_t (&a)[1][4]) {
-#pragma unroll
-        for (int r = 0; r < 4; r += 2) {
-            const uint32_t w = __byte_perm(v[r][i >> 1], v[r + 1][i >> 1], i & 1 ? 0x7632 : 0x5410);
-            a[0][r] = levels2(w);
-            a[0][r + 1] = levels2(w >> 8);
-        }
-    }
-    static constexpr int kApart = 2;   // bytes 0 and 2 of a word make a pair, and 1 and 3
+    static constexpr int kBytes = 1;
 };
 
-// An item's rows, for one warp: their place in q and out.
+// An item, or a part of one, as one warp has it. It lies in shared memory and is read (volatile)
+// where it is needed: in registers it would take those of the operands.
 struct Item {
-    int row0, rows, i0, head;          // unit's first row, its rows, the item's first of them, K/V head
+    int row0, rows, i0;                // unit's first row, its rows, the item's first of them
     int ctx, keys;                     // UnitShape's
-    bool own;
+    int b0, b1;                        // steps
+    int own, whole, parts;             // whole: no stretch cuts it; parts: how many it has, if this is the first
     const int32_t* table;
-    __device__ __forceinline__ int row(const SharedArgs& a, int i) const { return row0 + min(i, rows - 1) / a.group; }
-    __device__ __forceinline__ int q_head(const SharedArgs& a, int i) const { return head * a.group + min(i, rows - 1) % a.group; }
+    __device__ __forceinline__ int pages() const volatile { return (keys + kPageRows - 1) / kPageRows; }
     // the last position that row i sees
-    __device__ __forceinline__ int last(const SharedArgs& a, int i) const { return own ? ctx + min(i, rows - 1) / a.group : keys - 1; }
+    __device__ __forceinline__ int last(const SharedArgs& a, int i) const volatile {
+        return own ? ctx + a.by_group(min(i, rows - 1)) : keys - 1;
+    }
 };
+using ItemAt = const volatile Item*;
 
 // The values that are not finite of keys [key0, key1) that some of the item's rows see and
 // others do not, for the rows that see them. Rare: out of line.
 template <int FMT>
-__device__ __noinline__ void add_odd(const SharedArgs& a, const Item& it, int key0, int key1, int last0, int last1, int dim,
+__device__ __noinline__ void add_odd(const SharedArgs& a, const int32_t* table, int head, int key0, int key1, int last0, int last1, int dim,
                                      float* o0, float* o1) {
     constexpr int kBytes = Format<FMT>::kBytes;
     for (int key = key0; key < key1; ++key) {
-        const int e = __ldg(it.table + key / kPageRows);
+        const int e = __ldg(table + key / kPageRows);
         if (e < 0 || e >= a.n_pages) continue;
-        const size_t at = (((size_t)e * kPageRows + key % kPageRows) * a.n_kv_head + it.head) * kHeadDim + dim;
+        const size_t at = (((size_t)e * kPageRows + key % kPageRows) * a.n_kv_head + head) * kHeadDim + dim;
         for (int d = 0; d < 8; ++d) {
             float v;
             if constexpr (kBytes == 2) v = __bfloat162float(static_cast<const __nv_bfloat16*>(a.v)[at + d]);
@@ -311,120 +322,163 @@ __device__ __noinline__ void add_odd(const SharedArgs& a, const Item& it, int ke
     }
 }
 
-template <int FMT, int NT>
+template <int NT>
 struct WarpState {
     float o[NT][4][4];                 // [i][e]: dim 8 g + 2 i + e / 2 of column 2 c + e % 2
     float m[NT][2], l[NT][2];          // of columns 2 c, 2 c + 1 (l: this lane's keys only)
 };
 
-// Steps [b0, b1) of an item. qs: the warp's operands of Q in shared memory.
+// What a warp has in its registers of the step it is at: each half is loaded as soon as the
+// half before it has been used, so that the keys of the next step are on their way
+// during this one's softmax and values, and its values during the next one's scores. (The
+// registers that hold a step anyway are the buffer.)
+template <int FMT, int PG>
+struct StepLoads {
+    static constexpr int kBytes = Format<FMT>::kBytes, KW = 4 * kBytes, VW = 2 * kBytes;
+    uint32_t k[PG][2][KW], v[PG][4][VW];
+    float ks[PG][2], vs[PG][2];
+    int entry[PG];                     // of the step that is loaded next
+    unsigned mapped;                   // of its pages
+    const char *k_at, *v_at;           // this lane's place in a page of the head
+    const char *ks_at, *vs_at;
+    unsigned page, scale_page;         // from page to page: bytes
+    int w;                             // from row to row: bytes
+    int head;
+    __device__ __forceinline__ void start(const SharedArgs& a, int of_head, int g, int c) {
+        head = of_head;
+        w = a.n_kv_head * kHeadDim * kBytes;
+        page = (unsigned)w * kPageRows;
+        k_at = static_cast<const char*>(a.k) + head * kHeadDim * kBytes + (size_t)g * w + 16 * c * kBytes;
+        v_at = static_cast<const char*>(a.v) + head * kHeadDim * kBytes + (size_t)(2 * c) * w + 8 * g * kBytes;
+        if constexpr (FMT == TIE_KV_INT8) {
+            ks_at = reinterpret_cast<const char*>(a.ks + head * kPageRows + g);
+            vs_at = reinterpret_cast<const char*>(a.vs + head * kPageRows + g);
+            scale_page = (unsigned)a.n_kv_head * kPageRows * (unsigned)sizeof(float);
+        }
+    }
+    // (what is not mapped is read from the pool's first page, and counts for nothing)
+    __device__ __forceinline__ void entries(const int32_t* table, int b, int table_pages, int n_pages) {
+        mapped = 0;
+#pragma unroll
+        for (int p = 0; p < PG; ++p) {
+            const int e = b * PG + p < table_pages ? __ldg(table + b * PG + p) : -1;
+            const bool ok = e >= 0 && e < n_pages;
+            entry[p] = ok ? e : 0;
+            mapped |= (unsigned)ok << p;
+        }
+    }
+    __device__ __forceinline__ void keys() {
+#pragma unroll
+        for (int p = 0; p < PG; ++p) {
+            const char* at = k_at + (unsigned long long)(unsigned)entry[p] * page;
+            load_words<KW>(at, 0, k[p][0]);
+            load_words<KW>(at, 8 * w, k[p][1]);
+            if constexpr (FMT == TIE_KV_INT8) {
+                const float* s = reinterpret_cast<const float*>(ks_at + (unsigned long long)(unsigned)entry[p] * scale_page);
+                ks[p][0] = __ldg(s);
+                ks[p][1] = __ldg(s + 8);
+            }
+        }
+    }
+    __device__ __forceinline__ void values() {
+#pragma unroll
+        for (int p = 0; p < PG; ++p) {
+            const char* at = v_at + (unsigned long long)(unsigned)entry[p] * page;
+            load_words<VW>(at, 0, v[p][0]);
+            load_words<VW>(at, w, v[p][1]);
+            load_words<VW>(at, 8 * w, v[p][2]);
+            load_words<VW>(at, 9 * w, v[p][3]);
+            if constexpr (FMT == TIE_KV_INT8) {
+                const float* s = reinterpret_cast<const float*>(vs_at + (unsigned long long)(unsigned)entry[p] * scale_page);
+                vs[p][0] = __ldg(s);
+                vs[p][1] = __ldg(s + 8);
+            }
+        }
+    }
+};
+
+// The largest of a column's numbers: over the lanes that hold its keys.
+__device__ __forceinline__ float column_max(float x) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(kAll, x, o));
+    return x;
+}
+
+// The running maximum takes in a step's; the factor of what is there already.
+__device__ __forceinline__ float move_max(float& m, float& l, float step_max, float* from) {
+    const float m_new = fmaxf(m, step_max);
+    *from = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = ex2_ftz(m - *from);
+    m = m_new;
+    l *= alpha;
+    return alpha;
+}
+
+// ---- fp32 and bf16 pages
+// The steps of an item, the first of which is in `in` (at the end: the next item's first, if
+// there is one). qs: the warp's operands of Q in shared memory.
 template <int FMT, int NT>
-__device__ __forceinline__ void run_steps(const SharedArgs& a, const Item& it, int b0, int b1, const uint4* qs, int lane,
-                                          WarpState<FMT, NT>& st) {
+__device__ __forceinline__ void run_steps(const SharedArgs& a, ItemAt it, ItemAt next, StepLoads<FMT, kPages<FMT, NT>>& in,
+                                          const uint2* qs, int lane, WarpState<NT>& st) {
     using F = Format<FMT>;
-    constexpr int PG = kPages<FMT, NT>, KW = 4 * F::kBytes, VW = 2 * F::kBytes, T = F::kTerms;
-    const int g = lane >> 2, c = lane & 3;
-    const size_t w = (size_t)a.n_kv_head * kHeadDim * F::kBytes;      // bytes of a row
-    const int n_pages = (it.keys + kPageRows - 1) / kPageRows;
+    constexpr int PG = kPages<FMT, NT>, VW = 2 * F::kBytes, T = F::kTerms;
+    const int g = lane >> 2, c = lane & 3, i0 = it->i0, table_pages = it->pages();
+    const int32_t* const table = it->table;
     int last[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) last[n][e] = it.last(a, it.i0 + 8 * n + 2 * c + e);
-    const int least = it.last(a, it.i0), most = it.last(a, it.i0 + 8 * NT - 1);
-    b1 = min(b1, most / (PG * kPageRows) + 1);     // later positions are seen by none of the rows
-    int entry[PG];
-    auto entries = [&](int b) {
-#pragma unroll
-        for (int p = 0; p < PG; ++p) entry[p] = b * PG + p < n_pages ? __ldg(it.table + b * PG + p) : -1;
-    };
-    if (b0 < b1) entries(b0);
-    for (int b = b0; b < b1; ++b) {
-        uint32_t kw[PG][2][KW], vw[PG][4][VW];
-        float ks[PG][2], vs[PG][2];
-        bool mapped[PG];
+        for (int e = 0; e < 2; ++e) last[n][e] = it->last(a, i0 + 8 * n + 2 * c + e);
+    const int least = it->last(a, i0), most = it->last(a, i0 + 8 * NT - 1);
+    // (positions behind `most` are seen by none of the rows; an item's own part may have no others)
+    const int b1 = max(min(it->b1, most / (PG * kPageRows) + 1), it->b0 + 1);
+    for (int b = it->b0; b < b1; ++b) {
         const int pos0 = b * PG * kPageRows;
-        bool whole = pos0 + PG * kPageRows - 1 <= least;
+        const unsigned mapped = in.mapped;
+        const bool whole = pos0 + PG * kPageRows - 1 <= least && mapped == (1u << PG) - 1;
+        const bool more = b + 1 < b1 || next;
+        if (b + 1 < b1) in.entries(table, b + 1, table_pages, a.n_pages);
+        else if (next) in.entries(next->table, next->b0, next->pages(), a.n_pages);
+        // scores of keys g, g + 8 of each page: s[n PG + p][e], e / 2 the key, e % 2 the column
+        constexpr int kAcc = NT * PG, kSmall = Products<T>::kSmall;
+        float s[kAcc][4], s_small[kAcc][4];
+        auto k_step = [&](auto first, int step) {              // of 16 dims
+            constexpr bool kFirst = decltype(first)::value;
+            uint32_t fa[PG][T][4];
+            uint2 u[NT][3];
 #pragma unroll
-        for (int p = 0; p < PG; ++p) {
-            mapped[p] = entry[p] >= 0 && entry[p] < a.n_pages;
-            whole = whole && mapped[p];
-            if (mapped[p]) {
-                const size_t at = (size_t)entry[p] * kPageRows * w + (size_t)it.head * kHeadDim * F::kBytes;
+            for (int p = 0; p < PG; ++p) F::keys(in.k[p], step, fa[p]);
 #pragma unroll
-                for (int r = 0; r < 2; ++r) load_words<KW>(a.k, at + (g + 8 * r) * w + 16 * c * F::kBytes, kw[p][r]);
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    load_words<VW>(a.v, at + (2 * c + (r & 1) + 8 * (r >> 1)) * w + 8 * g * F::kBytes, vw[p][r]);
-                if constexpr (FMT == TIE_KV_INT8) {
-                    const size_t s = ((size_t)entry[p] * a.n_kv_head + it.head) * kPageRows + g;
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        ks[p][r] = __ldg(a.ks + s + 8 * r);
-                        vs[p][r] = __ldg(a.vs + s + 8 * r);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-#pragma unroll
-                    for (int i = 0; i < KW; ++i) kw[p][r][i] = 0u;
-                    ks[p][r] = vs[p][r] = 0.f;
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int i = 0; i < VW; ++i) vw[p][r][i] = 0u;
-            }
-        }
-        bool odd = false;
-        if (b + 1 < b1) entries(b + 1);
-        // scores of keys g, g + 8 of each page: s[n][p][e], e / 2 the key, e % 2 the column
-        float s[NT][PG][4], s_small[NT][PG][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int p = 0; p < PG; ++p)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[n][p][e] = s_small[n][p][e] = 0.f;
-#pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2) {           // two k steps of 16 dims
-            uint32_t fa[2][PG][T][4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int p = 0; p < PG; ++p) F::keys(kw[p], 2 * k2 + h, fa[h][p]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                uint4 u[3];
-#pragma unroll
-                for (int e = 0; e < 3; ++e) u[e] = qs[((n * 2 + k2) * 3 + e) * 32 + lane];
-                const uint32_t x0[3] = {u[0].x, u[1].x, u[2].x}, x1[3] = {u[0].y, u[1].y, u[2].y};
-                const uint32_t y0[3] = {u[0].z, u[1].z, u[2].z}, y1[3] = {u[0].w, u[1].w, u[2].w};
-#pragma unroll
-                for (int p = 0; p < PG; ++p) {
-                    small_products<T>(s_small[n][p], fa[0][p], x0, x1);
-                    small_products<T>(s_small[n][p], fa[1][p], y0, y1);
-                    main_product(s[n][p], fa[0][p][0], x0, x1);
-                    main_product(s[n][p], fa[1][p][0], y0, y1);
-                }
-            }
-        }
+                for (int e = 0; e < 3; ++e) u[n][e] = qs[((n * 4 + step) * 3 + e) * 32 + lane];
+            auto a_of = [&](int r, int t) -> const uint32_t(&)[4] { return fa[r % PG][t]; };
+            auto b0_of = [&](int r, int t) { return u[r / PG][t].x; };
+            auto b1_of = [&](int r, int t) { return u[r / PG][t].y; };
+            add_products<kFirst, 0, kSmall, kAcc, T>(s_small, a_of, b0_of, b1_of);
+            add_products<kFirst, kSmall, kSmall + 1, kAcc, T>(s, a_of, b0_of, b1_of);
+        };
+        k_step(std::true_type{}, 0);
+        k_step(std::false_type{}, 1);
+        k_step(std::false_type{}, 2);
+        k_step(std::false_type{}, 3);
+        if (more) in.keys();
         // values that no row of the item sees are zero; one that is not finite and that only
         // some rows see is left to add_odd
+        bool odd = false;
         if (!whole) {
 #pragma unroll
             for (int p = 0; p < PG; ++p)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int pos = pos0 + p * kPageRows + 2 * c + (r & 1) + 8 * (r >> 1);
-                    if (pos > most) {
+                    if (pos > most || !(mapped >> p & 1)) {
 #pragma unroll
-                        for (int i = 0; i < VW; ++i) vw[p][r][i] = 0u;
-                    } else if (FMT != TIE_KV_INT8 && pos > least) {
+                        for (int i = 0; i < VW; ++i) in.v[p][r][i] = 0u;
+                    } else if (pos > least) {
 #pragma unroll
                         for (int i = 0; i < VW; ++i) {
-                            uint32_t& x = vw[p][r][i];
+                            uint32_t& x = in.v[p][r][i];
                             if constexpr (FMT == TIE_KV_F32) {
                                 if (magnitude(__uint_as_float(x)) >= kNotFinite) { x = 0u; odd = true; }
                             } else {
@@ -435,85 +489,268 @@ __device__ __forceinline__ void run_steps(const SharedArgs& a, const Item& it, i
                     }
                 }
         }
-        float alpha[NT][2];
-        uint32_t pb[NT][PG][2][3];     // the weights as B operands: [keys below 8, others][term]
+        float alpha[NT][2], from[NT][2];
+#pragma unroll
+        for (int r = 0; r < kAcc; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[r][e] += s_small[r][e];
+        if (!whole) {
+#pragma unroll
+            for (int r = 0; r < kAcc; ++r)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!(mapped >> (r % PG) & 1) || pos0 + (r % PG) * kPageRows + g + 8 * (e >> 1) > last[r / PG][e & 1])
+                        s[r][e] = -INFINITY;
+        }
+        float mx[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                mx[n][e] = fmaxf(s[n * PG][e], s[n * PG][2 + e]);
+#pragma unroll
+                for (int p = 1; p < PG; ++p) mx[n][e] = fmaxf(mx[n][e], fmaxf(s[n * PG + p][e], s[n * PG + p][2 + e]));
+            }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) mx[n][e] = fmaxf(mx[n][e], __shfl_xor_sync(kAll, mx[n][e], o));
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) alpha[n][e] = move_max(st.m[n][e], st.l[n][e], mx[n][e], &from[n][e]);
+#pragma unroll
+        for (int p = 0; p < PG; ++p) {
+            uint32_t pb[NT][2][3];     // the page's weights as B operands: [keys below 8, others][term]
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float w[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        w[e] = kWeight * ex2_ftz(s[n * PG + p][2 * h + e] - from[n][e]);
+                        st.l[n][e] += w[e];
+                    }
+                    uint32_t x[3];
+                    split3(w[0], w[1], x);
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) pb[n][h][e] = transposed(x[e]);
+                }
+            constexpr int kI = NT == 1 ? 2 : 1;    // dims' operands at a time: two accumulators at least take turns
+#pragma unroll
+            for (int i = 0; i < 4; i += kI) {
+                uint32_t fv[kI][T][4];
+#pragma unroll
+                for (int j = 0; j < kI; ++j) F::values(in.v[p], i + j, fv[j]);
+                float d[kI * NT][4];
+                add_products<true, 0, kSmall + 1, kI * NT, T>(
+                    d, [&](int r, int t) -> const uint32_t(&)[4] { return fv[r / NT][t]; },
+                    [&](int r, int t) { return pb[r % NT][0][t]; }, [&](int r, int t) { return pb[r % NT][1][t]; });
+#pragma unroll
+                for (int r = 0; r < kI * NT; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float& o = st.o[r % NT][i + r / NT][e];
+                        o = p == 0 ? fmaf(o, alpha[r % NT][e & 1], d[r][e]) : o + d[r][e];
+                    }
+            }
+        }
+        if (more) in.values();
+        if (__any_sync(kAll, odd)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float extra[2][8] = {};
+                add_odd<FMT>(a, it->table, in.head, max(pos0, least + 1), min(pos0 + PG * kPageRows, most + 1), last[n][0], last[n][1], 8 * g,
+                             extra[0], extra[1]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) st.o[n][i][e] += extra[e & 1][2 * i + (e >> 1)];
+            }
+        }
+    }
+}
+
+// ---- pages in 8 bits
+// Levels are operands of integer MMAs (m16n8k32, at the bf16 ones' rate for twice the sums)
+// as they lie in memory. A query's elements become integers of 24 bits, relative to its
+// largest, and a step's weights (times their values' scales) integers of 23, relative to
+// the step's largest of their row: three 8-bit digits each, the top one signed. Sums of a
+// digit are exact, and need no conversion: a digit's sum over 64 is below 2^21, so where it starts at the
+// bits of 1.5 2^23 it ends as the bits of the fp32 number 1.5 2^23 + sum.
+// Against bf16 terms (levels converted, three MMAs of half the depth) that is half the MMAs and a third
+// of the instructions.
+
+// Sums of digits start as floats of these bits: 1.5 2^23 for digit 0, 1.5 2^31 for digit 1 (whose
+// last place is worth 256), 1.5 2^39 for digit 2 (65536).
+constexpr int kStart0 = 0x4b400000, kStart1 = 0x4f400000, kStart2 = 0x53400000;
+
+// d = a b + c, all of c `START`, if FIRST, else d
+template <bool SIGNED, bool FIRST, int START>
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    const int c0 = FIRST ? START : d[0], c1 = FIRST ? START : d[1], c2 = FIRST ? START : d[2], c3 = FIRST ? START : d[3];
+    if constexpr (SIGNED)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%10, %11, %12, %13};"
+                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%10, %11, %12, %13};"
+                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
+}
+// the three digits' sums
+template <bool FIRST>
+__device__ __forceinline__ void mma_digits(int (&d)[3][4], const uint32_t (&a)[4], const uint32_t (&b0)[3], const uint32_t (&b1)[3]) {
+    mma_s8<false, FIRST, kStart0>(d[0], a, b0[0], b1[0]);
+    mma_s8<false, FIRST, kStart1>(d[1], a, b0[1], b1[1]);
+    mma_s8<true, FIRST, kStart2>(d[2], a, b0[2], b1[2]);
+}
+// d0 + 256 d1 + 65536 d2 of the digits' sums: each step but the last addition is exact or to the last place of
+// its result
+__device__ __forceinline__ float joined(int d0, int d1, int d2) {
+    const float high = __int_as_float(d2) - __int_as_float(kStart2);
+    const float low = __int_as_float(d1) - (__int_as_float(kStart1) + __int_as_float(kStart0));
+    return high + (low + __int_as_float(d0));
+}
+// the larger magnitude; NaN if either is
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
+}
+__device__ __forceinline__ float pow2_biased(int e) { return __uint_as_float((uint32_t)e << 23); }
+
+template <int NT>
+__device__ __forceinline__ void run_steps_q8(const SharedArgs& a, ItemAt it, ItemAt next,
+                                             StepLoads<TIE_KV_INT8, kPages<TIE_KV_INT8, NT>>& in, const uint4* qs,
+                                             const float* q_unit, int lane, WarpState<NT>& st) {
+    constexpr int PG = kPages<TIE_KV_INT8, NT>;
+    const int g = lane >> 2, c = lane & 3, i0 = it->i0, table_pages = it->pages();
+    const int32_t* const table = it->table;
+    int last[NT][2];
+    float unit[NT][2];                 // what 1 in a column's integers stands for
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            last[n][e] = it->last(a, i0 + 8 * n + 2 * c + e);
+            unit[n][e] = q_unit[8 * n + 2 * c + e];
+        }
+    const int least = it->last(a, i0), most = it->last(a, i0 + 8 * NT - 1);
+    const int b1 = max(min(it->b1, most / (PG * kPageRows) + 1), it->b0 + 1);
+    for (int b = it->b0; b < b1; ++b) {
+        const int pos0 = b * PG * kPageRows;
+        const unsigned mapped = in.mapped;
+        const bool whole = pos0 + PG * kPageRows - 1 <= least && mapped == (1u << PG) - 1;
+        const bool more = b + 1 < b1 || next;
+        if (b + 1 < b1) in.entries(table, b + 1, table_pages, a.n_pages);
+        else if (next) in.entries(next->table, next->b0, next->pages(), a.n_pages);
+        float s[NT][PG][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float mx[2] = {-INFINITY, -INFINITY};
+            uint4 u[3];
+#pragma unroll
+            for (int e = 0; e < 3; ++e) u[e] = qs[(n * 3 + e) * 32 + lane];
+#pragma unroll
+            for (int p = 0; p < PG; ++p) {
+                int d[3][4];
+                const uint32_t f0[4] = {in.k[p][0][0], in.k[p][1][0], in.k[p][0][1], in.k[p][1][1]};
+                const uint32_t f1[4] = {in.k[p][0][2], in.k[p][1][2], in.k[p][0][3], in.k[p][1][3]};
+                mma_digits<true>(d, f0, {u[0].x, u[1].x, u[2].x}, {u[0].y, u[1].y, u[2].y});
+                mma_digits<false>(d, f1, {u[0].z, u[1].z, u[2].z}, {u[0].w, u[1].w, u[2].w});
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    s[n][p][e] = joined(d[0][e], d[1][e], d[2][e]) * unit[n][e & 1] * in.ks[p][e >> 1];
+            }
+        }
+        if (more) in.keys();
+        uint32_t vt[PG][8];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float mx[2] = {-INFINITY, -INFINITY}, alpha[2], from[2], top[2] = {0.f, 0.f}, up[2], down[2];
+            if (!whole) {
+#pragma unroll
+                for (int p = 0; p < PG; ++p)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!(mapped >> p & 1) || pos0 + p * kPageRows + g + 8 * (e >> 1) > last[n][e & 1]) s[n][p][e] = -INFINITY;
+            }
+#pragma unroll
+            for (int p = 0; p < PG; ++p)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx[e & 1] = fmaxf(mx[e & 1], s[n][p][e]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) alpha[e] = move_max(st.m[n][e], st.l[n][e], column_max(mx[e]), &from[e]);
 #pragma unroll
             for (int p = 0; p < PG; ++p)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float& x = s[n][p][e];
-                    x += s_small[n][p][e];
-                    if constexpr (FMT == TIE_KV_INT8) x *= ks[p][e >> 1];
-                    if (!whole && (!mapped[p] || pos0 + p * kPageRows + g + 8 * (e >> 1) > last[n][e & 1])) x = -INFINITY;
-                    mx[e & 1] = fmaxf(mx[e & 1], x);
+                    const float w = ex2_ftz(x - from[e & 1]);
+                    st.l[n][e & 1] = fmaf(w, kWeight, st.l[n][e & 1]);
+                    // (a scale of a key that the row does not see may be anything)
+                    const bool none = !whole && x == -INFINITY;
+                    x = w * in.vs[p][e >> 1];
+                    if (none) x = 0.f;
+                    top[e & 1] = max_abs(top[e & 1], x);
                 }
-            float from[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(kAll, mx[e], o));
-                const float m_new = fmaxf(st.m[n][e], mx[e]);
-                from[e] = m_new == -INFINITY ? 0.f : m_new;
-                alpha[n][e] = ex2_ftz(st.m[n][e] - from[e]);
-                st.m[n][e] = m_new;
-                st.l[n][e] *= alpha[n][e];
+                for (int o = 4; o < 32; o <<= 1) top[e] = max_abs(top[e], __shfl_xor_sync(kAll, top[e], o));
+                // the largest is below 2^(x - 126): times 2^(148 - x), it is at most 2^22
+                const int x = max((int)(__float_as_uint(top[e]) >> 23), 53);
+                up[e] = pow2_biased(275 - x);
+                down[e] = x >= 255 ? top[e] * 0.f : pow2_biased(x - 51);       // (times kWeight; NaN where there is no largest)
             }
+            uint32_t wb[PG][3];            // digits of four keys' weights
 #pragma unroll
             for (int p = 0; p < PG; ++p) {
-                float w4[4];
+                int w[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float x = s[n][p][e];
-                    w4[e] = kWeight * ex2_ftz(x - from[e & 1]);
-                    st.l[n][e & 1] += w4[e];
-                    if constexpr (FMT == TIE_KV_INT8) {
-                        // (a scale of a key that the row does not see may be anything)
-                        const bool seen = whole || (mapped[p] && pos0 + p * kPageRows + g + 8 * (e >> 1) <= last[n][e & 1]);
-                        w4[e] = seen ? w4[e] * vs[p][e >> 1] : 0.f;
+                for (int e = 0; e < 4; ++e) w[e] = __float_as_int(fmaf(s[n][p][e], up[e & 1], __int_as_float(kStart0))) - kStart0;
+                const uint32_t x = transposed(__byte_perm(w[0], w[1], 0x5410)), y = transposed(__byte_perm(w[2], w[3], 0x5410));
+                const uint32_t z = transposed(__byte_perm(__byte_perm(w[0], w[2], 0x0062), __byte_perm(w[1], w[3], 0x0062), 0x5410));
+                wb[p][0] = __byte_perm(x, y, 0x6420);
+                wb[p][1] = __byte_perm(x, y, 0x7531);
+                wb[p][2] = __byte_perm(z, z, 0x3120);
+            }
+            if (n == 0) {
+                // the values of four keys of a dim side by side (not sooner: they are still on their
+                // way during the scores and the softmax)
+#pragma unroll
+                for (int p = 0; p < PG; ++p)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t(&v)[4][2] = in.v[p];
+                        const uint32_t x = __byte_perm(v[0][h], v[1][h], 0x5140), y = __byte_perm(v[0][h], v[1][h], 0x7362);
+                        const uint32_t z = __byte_perm(v[2][h], v[3][h], 0x5140), w = __byte_perm(v[2][h], v[3][h], 0x7362);
+                        vt[p][4 * h] = __byte_perm(x, z, 0x5410);
+                        vt[p][4 * h + 1] = __byte_perm(x, z, 0x7632);
+                        vt[p][4 * h + 2] = __byte_perm(y, w, 0x5410);
+                        vt[p][4 * h + 3] = __byte_perm(y, w, 0x7632);
+                    }
+                            }
+#pragma unroll
+            for (int p = 0; p < PG; p += 2)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    int d[3][4];
+                    const uint32_t fv[4] = {vt[p][2 * i], vt[p][2 * i + 1], vt[p + 1][2 * i], vt[p + 1][2 * i + 1]};
+                    mma_digits<true>(d, fv, wb[p], wb[p + 1]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float& o = st.o[n][i][e];
+                        o = fmaf(joined(d[0][e], d[1][e], d[2][e]), down[e & 1], p == 0 ? o * alpha[e & 1] : o);
                     }
                 }
-                uint32_t x[3];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    split3(w4[2 * h], w4[2 * h + 1], x);
-#pragma unroll
-                    for (int e = 0; e < 3; ++e) pb[n][p][h][e] = transposed(x[e]);
-                }
-            }
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t fv[PG][T][4];
-#pragma unroll
-            for (int p = 0; p < PG; ++p) F::values(vw[p], i, fv[p]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float d[4] = {};
-#pragma unroll
-                for (int p = 0; p < PG; ++p) small_products<T>(d, fv[p], pb[n][p][0], pb[n][p][1]);
-#pragma unroll
-                for (int p = 0; p < PG; ++p) main_product(d, fv[p][0], pb[n][p][0], pb[n][p][1]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) st.o[n][i][e] = fmaf(st.o[n][i][e], alpha[n][e & 1], d[e]);
-            }
-        }
-        if constexpr (FMT != TIE_KV_INT8) {
-            if (__any_sync(kAll, odd)) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float more[2][8] = {};
-                    add_odd<FMT>(a, it, max(pos0, least + 1), min(pos0 + PG * kPageRows, most + 1), last[n][0], last[n][1],
-                                 8 * g, more[0], more[1]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) st.o[n][i][e] += more[e & 1][2 * i + (e >> 1)];
-                }
-            }
-        }
+        if (more) in.values();
     }
 }
 
@@ -522,11 +759,12 @@ template <int NT>
 constexpr int kQBytes = NT * 2 * 3 * 32 * (int)sizeof(uint4);
 
 template <int FMT, int NT>
-__global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) shared_kernel(const __grid_constant__ SharedArgs a, int which) {
-    using F = Format<FMT>;
+__global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const __grid_constant__ SharedArgs a, int which) {
     pdl_trigger();
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ ScheduleScratch<kThreads> scratch;
+    __shared__ Item s_items[kWarps][2];
+    __shared__ float s_unit[kWarps][8 * NT];       // pages in 8 bits: run_steps_q8's q_unit
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c = lane & 3;
     const Line& line = a.line[which];
     uint4* qs = reinterpret_cast<uint4*>(smem) + (size_t)warp * (kQBytes<NT> / sizeof(uint4));
@@ -534,57 +772,105 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) shared_kernel(const
     build_base(a, line.u0, line.u1, base, &scratch, t);
     const int n_units = line.u1 - line.u0;
     const long long total = base[n_units], share = share_of(line, total);
-    const int me = blockIdx.x * kWarps + warp;
-    long long x = me * share;
-    const long long end = min(x + share, total);
+    const int me = blockIdx.x * kWarps + warp, team = me / a.n_kv_head;
+    long long x = team * share;
+    const long long end = team < line.teams ? min(x + share, total) : 0;
     int u = x < end ? owner_of<long long>(base, n_units, x) : 0;
-    while (x < end) {
-        while (base[u + 1] <= x) ++u;  // (units without rows have no places)
-        const UnitShape s = unit_shape(a, line.u0 + u);
-        const int places = unit_places(s, line);
-        const long long in = x - base[u], item = in / places;
-        const int off = (int)(in - item * places);
-        const int stop = (int)min((long long)places, off + (end - x));
-        const long long first = x - off;           // the item's first place
-        x += stop - off;
-        const int b0 = max(off - 1, 0), b1 = stop - 1;
-        if (b1 <= b0) continue;
-        Item it;
-        it.own = line.u0 + u >= a.n_group;
-        it.row0 = s.row0;
-        it.rows = s.rows;
-        it.head = (int)(item % a.n_kv_head);
-        it.i0 = (int)(item / a.n_kv_head) * 8 * NT;
-        it.ctx = s.ctx;
-        it.keys = s.keys;
-        it.table = it.own ? a.table + (size_t)(line.u0 + u - a.n_group) * a.width : a.ptable + (size_t)u * a.pwidth;
-        // Q, scaled, in three terms, as B operands: column g, the lane's four dims of each k step
+    // the next part of this warp's stretch that has steps
+    auto find = [&](Item* to) -> bool {
+        while (x < end) {
+            while (base[u + 1] <= x) ++u;          // (units without rows have no places)
+            const UnitShape s = unit_shape(a, line.u0 + u);
+            const int places = unit_places(s, line);
+            const long long in = x - base[u], item = quotient(in, places);
+            const int off = (int)(in - item * places);
+            const int stop = (int)min((long long)places, off + (end - x));
+            const long long first = x - off;       // the item's first place
+            x += stop - off;
+            if (stop - 1 <= max(off - 1, 0)) continue;
+            // (the item's first step is in this warp's stretch, and its last place in this one or a later one's)
+            const bool begins = first + 1 >= team * share, whole = begins && first + places <= (team + 1) * share;
+            __syncwarp();
+            if (lane == 0) {
+                const bool own = line.u0 + u >= a.n_group;
+                to->own = own;
+                to->row0 = s.row0;
+                to->rows = s.rows;
+                to->i0 = (int)item * 8 * NT;
+                to->ctx = s.ctx;
+                to->keys = s.keys;
+                to->b0 = max(off - 1, 0);
+                to->b1 = stop - 1;
+                to->table = own ? a.table + (size_t)(line.u0 + u - a.n_group) * a.width : a.ptable + (size_t)u * a.pwidth;
+                to->whole = whole;
+                to->parts = whole ? 1 : begins ? 1 + (int)quotient(first + places - 1 - team * share, share) : 0;
+            }
+            __syncwarp();
+            return true;
+        }
+        return false;
+    };
+    const int head = me - team * a.n_kv_head;
+    int at = 0;                        // which of the warp's two items is this one
+    StepLoads<FMT, kPages<FMT, NT>> in;
+    bool here = find(&s_items[warp][0]);
+    if (here) {
+        ItemAt it = &s_items[warp][0];
+        in.start(a, head, g, c);
+        in.entries(it->table, it->b0, it->pages(), a.n_pages);
+        in.keys();
+        in.values();
+    }
+    while (here) {
+        ItemAt it = &s_items[warp][at];
+        // Q, scaled, as B operands: column g, this lane's 16 dims
         __syncwarp();
+        const int row0 = it->row0, n_rows = it->rows, i0 = it->i0;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int i = it.i0 + 8 * n + g;
-            const float* q = a.q + (size_t)it.row(a, i) * a.ldq + it.q_head(a, i) * kHeadDim + 16 * c;
+            const int i = min(i0 + 8 * n + g, n_rows - 1), tok = a.by_group(i);
+            const float* q = a.q + (size_t)(row0 + tok) * a.ldq + (head * a.group + i - tok * a.group) * kHeadDim + 16 * c;
             float y[16];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float4 v = __ldg(reinterpret_cast<const float4*>(q) + j);
                 y[4 * j] = v.x * a.scale2; y[4 * j + 1] = v.y * a.scale2; y[4 * j + 2] = v.z * a.scale2; y[4 * j + 3] = v.w * a.scale2;
             }
+            if constexpr (FMT == TIE_KV_INT8) {
+                float top = 0.f;
 #pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2) {
+                for (int j = 0; j < 16; ++j) top = max_abs(top, y[j]);
+                top = max_abs(top, __shfl_xor_sync(kAll, top, 1));
+                top = max_abs(top, __shfl_xor_sync(kAll, top, 2));
+                const int x = max((int)(__float_as_uint(top) >> 23), 23);    // the largest is below 2^(x - 126)
+                const float up = pow2_biased(276 - x);
                 uint32_t z[4][3];
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {      // k step 2 k2 + h / 2, register h % 2
-                    const int d = 8 * k2 + 4 * (h >> 1) + (h & 1) * (3 - F::kApart);
-                    split3(y[d], y[d + F::kApart], z[h]);
+                for (int j = 0; j < 4; ++j) {
+                    int w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = min(__float2int_rn(y[4 * j + e] * up), (1 << 23) - 1);
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        z[j][e] = __byte_perm(__byte_perm(w[0], w[1], 0x40 + 0x11 * e), __byte_perm(w[2], w[3], 0x40 + 0x11 * e), 0x5410);
                 }
 #pragma unroll
-                for (int e = 0; e < 3; ++e)
-                    qs[((n * 2 + k2) * 3 + e) * 32 + lane] = make_uint4(z[0][e], z[1][e], z[2][e], z[3][e]);
+                for (int e = 0; e < 3; ++e) qs[(n * 3 + e) * 32 + lane] = make_uint4(z[0][e], z[1][e], z[2][e], z[3][e]);
+                if (c == 0) s_unit[warp][8 * n + g] = x >= 255 ? top * 0.f : pow2_biased(x - 22);
+            } else {
+                uint2* const to = reinterpret_cast<uint2*>(qs);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t x[3], z[3];
+                    split3(y[4 * k], y[4 * k + 1], x);
+                    split3(y[4 * k + 2], y[4 * k + 3], z);
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) to[((n * 4 + k) * 3 + e) * 32 + lane] = make_uint2(x[e], z[e]);
+                }
             }
         }
         __syncwarp();
-        WarpState<FMT, NT> st;
+        WarpState<NT> st;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -594,27 +880,31 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) shared_kernel(const
 #pragma unroll
                 for (int e = 0; e < 4; ++e) st.o[n][i][e] = 0.f;
         }
-        run_steps<FMT, NT>(a, it, b0, b1, qs, lane, st);
+        const bool more = find(&s_items[warp][at ^ 1]);
+        ItemAt next = more ? &s_items[warp][at ^ 1] : nullptr;
+        if constexpr (FMT == TIE_KV_INT8) run_steps_q8<NT>(a, it, next, in, qs, s_unit[warp], lane, st);
+        else run_steps<FMT, NT>(a, it, next, in, reinterpret_cast<const uint2*>(qs), lane, st);
         // where the result goes: out, the rows' own place, or a part of this warp's
-        const int w_first = (int)((first + 1) / share), w_last = (int)((first + places - 1) / share);
-        const bool all = w_first == w_last;
-        const size_t slot = (2 * (size_t)me + (me == w_first)) * (8 * NT);
+        const int whole = it->whole, parts = it->parts, own = it->own, end_row0 = it->row0, end_rows = it->rows, end_i0 = it->i0;
+        const size_t slot = (2 * (size_t)me + (parts > 0)) * (8 * NT);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) st.l[n][e] += __shfl_xor_sync(kAll, st.l[n][e], o);
-                const int in_item = 8 * n + 2 * c + e, i = it.i0 + in_item;
-                if (i >= it.rows) continue;
-                const size_t row = it.row(a, i), at = row * a.n_head + it.q_head(a, i);
+                const int in_item = 8 * n + 2 * c + e, i = end_i0 + in_item;
+                if (i >= end_rows) continue;
+                const int tok = a.by_group(i), h = head * a.group + i - tok * a.group;
+                const size_t row = end_row0 + tok, place = row * a.n_head + h;
+                if (parts && g == 0) a.place[own][place] = make_int2(whole ? -1 : (int)slot + in_item, parts);
                 float f = 1.f, *to;
-                if (all && a.n_group == 0) {
+                if (whole && a.n_group == 0) {
                     f = st.l[n][e] == 0.f ? 0.f : 1.f / st.l[n][e];
-                    to = a.out + row * a.ldo + it.q_head(a, i) * kHeadDim;
+                    to = a.out + row * a.ldo + h * kHeadDim;
                 } else {
-                    to = all ? a.whole_o[it.own] + at * kHeadDim : line.part_o + (slot + in_item) * kHeadDim;
-                    float* ml = all ? a.whole_ml[it.own] + 2 * at : line.part_ml + 2 * (slot + in_item);
+                    to = whole ? a.whole_o[own] + place * kHeadDim : line.part_o + (slot + in_item) * kHeadDim;
+                    float* ml = whole ? a.whole_ml[own] + 2 * place : line.part_ml + 2 * (slot + in_item);
                     if (g == 0) *reinterpret_cast<float2*>(ml) = make_float2(st.m[n][e], st.l[n][e]);
                 }
                 float4* p = reinterpret_cast<float4*>(to + 8 * g);
@@ -626,6 +916,8 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) shared_kernel(const
                     p[1] = make_float4(o[2][e] * f, o[2][2 + e] * f, o[3][e] * f, o[3][2 + e] * f);
                 }
             }
+        at ^= 1;
+        here = more;
     }
     // (nothing above needs another kernel's results, but what waits for this kernel waits
     // for the one before it too)
@@ -633,58 +925,39 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) shared_kernel(const
 }
 
 // ------------------------------------------------------------------ the join --
-// What a row's parts are, and where: `n` of them from `o`, `ml` on, in steps; part 0 of a cut
-// item lies in its warp's second place, the others in their warps' first ones.
-struct Source {
-    const float *o, *ml;
-    int n;
-    size_t step;                       // rows of parts from part 0 to part 1, ...
-    size_t first;                      // from part 0 to part 1
-    __device__ __forceinline__ size_t row(int k) const { return k == 0 ? 0 : first + (size_t)(k - 1) * step; }
+// A row's parts from both sources, in one line: the sequence's own first. Part 0 of a cut
+// item lies in its warp's second place, the others in the first ones of the head's warps in
+// the teams that follow.
+struct Parts {
+    const float *o[2], *ml[2];         // [prefix, own]: the part that is first
+    int n[2], per[2], heads;           // per: rows of a place
+    __device__ __forceinline__ void at(int k, const float** to, const float** ml_to) const {
+        const int w = k < n[1], j = w ? k : k - n[1];
+        const size_t row = j == 0 ? 0 : ((size_t)2 * j * heads - 1) * per[w];
+        *to = o[w] + row * kHeadDim;
+        *ml_to = ml[w] + 2 * row;
+    }
 };
 
-__device__ __forceinline__ Source source_of(const SharedArgs& a, const long long* base, int u, const UnitShape& s, int i, int row,
-                                            int h, bool own) {
-    Source z{};
-    const Line& l = a.line[own];
-    const int per = 8 * l.nt, places = unit_places(s, l);
-    const long long item = (long long)(i / per) * a.n_kv_head + h / a.group;
-    const long long origin = base[l.u0], total = base[l.u1] - origin, share = share_of(l, total);
-    const long long first = base[u] - origin + item * places;
-    const int w0 = (int)((first + 1) / share), w1 = (int)((first + places - 1) / share);
-    if (w0 == w1) {
-        const size_t at = (size_t)row * a.n_head + h;
-        z.o = a.whole_o[own] + at * kHeadDim;
-        z.ml = a.whole_ml[own] + 2 * at;
-        z.n = 1;
-    } else {
-        const size_t at = (2 * (size_t)w0 + 1) * per + i % per;
-        z.o = l.part_o + at * kHeadDim;
-        z.ml = l.part_ml + 2 * at;
-        z.n = w1 - w0 + 1;
-        z.first = per;                 // slots 2 w0 + 1, 2 w0 + 2, 2 w0 + 4, ...
-        z.step = 2 * (size_t)per;
-    }
-    return z;
-}
-
-// A warp adds parts k0, k0 + dk, ... of a source to what it has of a row: lane l dims 2 l, 2 l + 1.
+// A warp adds parts k0, k0 + dk, ... to what it has of a row: lane l dims 2 l, 2 l + 1.
 struct RowSum {
     float m, l, x, y;
 };
-__device__ __forceinline__ void add_parts(RowSum& r, const Source& z, int k0, int dk, int lane) {
+__device__ __forceinline__ void add_parts(RowSum& r, const Parts& z, int k0, int dk, int lane) {
     constexpr int kAhead = 4;
-    for (int k = k0; k < z.n; k += kAhead * dk) {
+    const int n = z.n[0] + z.n[1];
+    for (int k = k0; k < n; k += kAhead * dk) {
         float2 ml[kAhead], v[kAhead];
         float m = r.m;
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             ml[j] = make_float2(-INFINITY, 0.f);
             v[j] = make_float2(0.f, 0.f);
-            if (k + j * dk < z.n) {
-                const size_t at = z.row(k + j * dk);
-                ml[j] = __ldcg(reinterpret_cast<const float2*>(z.ml + 2 * at));
-                v[j] = __ldcg(reinterpret_cast<const float2*>(z.o + at * kHeadDim) + lane);
+            if (k + j * dk < n) {
+                const float *o, *of;
+                z.at(k + j * dk, &o, &of);
+                ml[j] = __ldcg(reinterpret_cast<const float2*>(of));
+                v[j] = __ldcg(reinterpret_cast<const float2*>(o) + lane);
             }
         }
 #pragma unroll
@@ -706,42 +979,49 @@ __device__ __forceinline__ void add_parts(RowSum& r, const Source& z, int k0, in
     }
 }
 
-// A row and query head by a warp, or by all warps of the CTA where there are few rows (and
-// many parts of each, then).
+// CTAs (s, y) take sequence s's rows: a row and query head by a warp, or by all warps of the
+// CTA where there are few rows (and many parts of each, then). What the rows of a sequence
+// that is left out hold in `place` is nothing: they are told by the lengths.
 template <bool WIDE>
 __global__ void __launch_bounds__(kThreads) shared_join_kernel(const __grid_constant__ SharedArgs a) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ ScheduleScratch<kThreads> scratch;
+    __shared__ int s_group;
     __shared__ RowSum s_sum[kWarps][32];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int n_units = a.n_group + a.n_seq;
-    long long* base = reinterpret_cast<long long*>(smem);
-    int* starts = reinterpret_cast<int*>(base + n_units + 1);        // the rows' sequences are looked for here
-    int* groups = starts + a.n_seq + 1;
-    for (int i = t; i <= a.n_seq; i += kThreads) starts[i] = __ldg(a.row_start + i);
-    for (int i = t; i <= a.n_group && a.n_group; i += kThreads) groups[i] = __ldg(a.gstart + i);
-    build_base(a, 0, n_units, base, &scratch, t);
-    pdl_wait();
-    const long long pairs = (long long)a.rows * a.n_head;
-    for (long long at = WIDE ? blockIdx.x : (long long)blockIdx.x * kWarps + warp; at < pairs;
-         at += WIDE ? gridDim.x : (long long)gridDim.x * kWarps) {
-        const int row = (int)(at / a.n_head), h = (int)(at % a.n_head);
-        const int q = owner_of<int>(starts, a.n_seq, row);
-        const UnitShape s = unit_shape(a, a.n_group + q);
-        if (!s.rows || row < s.row0 || row >= s.row0 + s.tokens) continue;
-        const Source own = source_of(a, base, a.n_group + q, s, (row - s.row0) * a.group + h % a.group, row, h, true);
-        Source shared{};
-        if (a.n_group) {
-            const int u = owner_of<int>(groups, a.n_group, q);
-            const UnitShape p = unit_shape(a, u);
-            if (p.rows && q >= groups[u] && q < groups[u + 1] && row >= p.row0 && row < p.row0 + p.tokens)
-                shared = source_of(a, base, u, p, (row - p.row0) * a.group + h % a.group, row, h, false);
-        } else if (own.n == 1) {
-            continue;                  // written already
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, q = blockIdx.x;
+    const UnitShape s = unit_shape(a, a.n_group + q);
+    if (!s.rows) return;
+    bool grouped = false;
+    if (a.n_group) {
+        if (t == 0) s_group = -1;
+        __syncthreads();
+        for (int u = t; u < a.n_group; u += kThreads)
+            if (__ldg(a.gstart + u) <= q && q < __ldg(a.gstart + u + 1)) atomicMax(&s_group, u);
+        __syncthreads();
+        if (s_group >= 0) {
+            const UnitShape p = unit_shape(a, s_group);
+            grouped = p.rows && s.row0 >= p.row0 && s.row0 + s.tokens <= p.row0 + p.tokens;
         }
+    }
+    pdl_wait();
+    const long long pairs = (long long)s.tokens * a.n_head;
+    for (long long i = WIDE ? blockIdx.y : (long long)blockIdx.y * kWarps + warp; i < pairs;
+         i += WIDE ? gridDim.y : (long long)gridDim.y * kWarps) {
+        const int row = s.row0 + (int)((unsigned)i / (unsigned)a.n_head), h = (int)((unsigned)i % (unsigned)a.n_head);
+        const size_t at = (size_t)row * a.n_head + h;
+        Parts z;
+        z.heads = a.n_kv_head;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const bool there = w || grouped;
+            const int2 where = there ? __ldcg(a.place[w] + at) : make_int2(0, 0);
+            const Line& l = a.line[w];
+            z.n[w] = where.y;
+            z.per[w] = 8 * l.nt;
+            z.o[w] = where.x < 0 ? a.whole_o[w] + at * kHeadDim : l.part_o + (size_t)where.x * kHeadDim;
+            z.ml[w] = where.x < 0 ? a.whole_ml[w] + 2 * at : l.part_ml + 2 * (size_t)where.x;
+        }
+        if (a.n_group == 0 && z.n[1] == 1) continue;      // written already
         RowSum r{-INFINITY, 0.f, 0.f, 0.f};
-        add_parts(r, own, WIDE ? warp : 0, WIDE ? kWarps : 1, lane);
-        add_parts(r, shared, WIDE ? warp : 0, WIDE ? kWarps : 1, lane);
+        add_parts(r, z, WIDE ? warp : 0, WIDE ? kWarps : 1, lane);
         if constexpr (WIDE) {
             s_sum[warp][lane] = r;
             __syncthreads();
@@ -754,11 +1034,11 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(const __grid_cons
                 r = RowSum{m, r.l * f, r.x * f, r.y * f};
 #pragma unroll
                 for (int v = 1; v < kWarps; ++v) {
-                    const RowSum z = s_sum[v][lane];
-                    f = ex2_ftz(z.m - from);
-                    r.l = fmaf(z.l, f, r.l);
-                    r.x = fmaf(z.x, f, r.x);
-                    r.y = fmaf(z.y, f, r.y);
+                    const RowSum u = s_sum[v][lane];
+                    f = ex2_ftz(u.m - from);
+                    r.l = fmaf(u.l, f, r.l);
+                    r.x = fmaf(u.x, f, r.x);
+                    r.y = fmaf(u.y, f, r.y);
                 }
             }
         }
@@ -771,17 +1051,21 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(const __grid_cons
 }
 
 // --------------------------------------------------------------- the entry ----
-constexpr int kMaxCtas = 2;            // CTAs of shared_kernel on an SM
-int most_warps(int sms) { return sms * kMaxCtas * kWarps; }
+int most_warps(int sms) { return sms * 16; }
 
 // floats of the workspace: parts of two lines, and the whole items of two sources
 size_t part_floats(int sms) { return (size_t)2 * most_warps(sms) * 32 * (kHeadDim + 2); }
-size_t workspace_floats(int sms, long long pairs) { return 2 * part_floats(sms) + (size_t)2 * pairs * (kHeadDim + 2); }
+// (and their places)
+size_t workspace_floats(int sms, long long pairs) { return 2 * part_floats(sms) + (size_t)2 * pairs * (kHeadDim + 2 + 2); }
 
 using Kernel = void (*)(SharedArgs, int);
 template <int FMT>
 Kernel kernel_of(int nt) {
     return nt == 1 ? shared_kernel<FMT, 1> : nt == 2 ? shared_kernel<FMT, 2> : shared_kernel<FMT, 4>;
+}
+template <int FMT>
+int ctas_of(int nt) {
+    return nt == 1 ? kCtas<FMT, 1> : nt == 2 ? kCtas<FMT, 2> : kCtas<FMT, 4>;
 }
 template <int FMT>
 int pages_of(int nt) {
@@ -832,7 +1116,7 @@ extern "C" model_status tie_attention_shared(const float* q, int ldq, int n_head
     const int sms = sm_count(dev.device());
     if (workspace_bytes < workspace_floats(sms, pairs) * sizeof(float)) return MODEL_ERR_CAPACITY;
     SharedArgs a{};
-    a.q = q; a.ldq = ldq; a.n_head = n_head; a.group = n_head / n_kv_head; a.n_kv_head = n_kv_head;
+    a.q = q; a.ldq = ldq; a.n_head = n_head; a.group = n_head / n_kv_head; a.by_group = divisor(a.group); a.n_kv_head = n_kv_head;
     a.k = k_pages; a.v = v_pages; a.ks = k_scales; a.vs = v_scales; a.n_pages = n_pages;
     a.table = page_table; a.width = pages_per_seq; a.row_start = row_start; a.ctx = ctx_lens;
     a.n_seq = n_seq; a.max_new = max_new; a.rows = rows;
@@ -849,21 +1133,25 @@ extern "C" model_status tie_attention_shared(const float* q, int ldq, int n_head
     for (int i = 0; i < 2; ++i) {
         a.whole_o[i] = f + i * pairs * kHeadDim;
         a.whole_ml[i] = f + 2 * pairs * kHeadDim + i * pairs * 2;
+        a.place[i] = reinterpret_cast<int2*>(f + 2 * pairs * (kHeadDim + 2) + i * pairs * 2);
     }
     // rows that share keys, at most of a sequence and on average of a group: the items' height
     auto height = [](long long most) { return most <= 8 ? 1 : most <= 16 ? 2 : 4; };
     const long long per_seq = (long long)max_new * a.group, per_group = n_group ? ((long long)rows * a.group - 1) / n_group + 1 : 0;
     const int nt[2] = {n_group ? height(per_group) : 0, height(per_seq)};
-    a.one_line = n_group && nt[0] == nt[1];
+    const bool one_line = n_group && nt[0] == nt[1];
+    int ctas[2];
     for (int i = 0; i < 2; ++i) {
         Line& l = a.line[i];
         l.nt = nt[i] ? nt[i] : nt[1];
         l.pages = q8 ? pages_of<TIE_KV_INT8>(l.nt) : kv_format == TIE_KV_BF16 ? pages_of<TIE_KV_BF16>(l.nt) : pages_of<TIE_KV_F32>(l.nt);
+        ctas[i] = sms * (q8 ? ctas_of<TIE_KV_INT8>(l.nt) : kv_format == TIE_KV_BF16 ? ctas_of<TIE_KV_BF16>(l.nt) : ctas_of<TIE_KV_F32>(l.nt));
         l.u0 = i ? n_group : 0;
         l.u1 = i ? n_group + n_seq : n_group;
-        l.warps = sms * (l.nt <= 2 ? kMaxCtas : 1) * kWarps;
+        l.teams = ctas[i] * kWarps / n_kv_head;
+        if (l.teams == 0) return MODEL_ERR_CAPACITY;          // (the K/V heads that are taken fit the GPU's warps)
     }
-    if (a.one_line) {
+    if (one_line) {
         a.line[0].u1 = n_group + n_seq;
         a.line[1] = a.line[0];
     }
@@ -872,7 +1160,7 @@ extern "C" model_status tie_attention_shared(const float* q, int ldq, int n_head
     bool first = true;
     for (int i = 0; i < 2; ++i) {
         const Line& l = a.line[i];
-        if (l.u1 == l.u0 || (i == 1 && a.one_line)) continue;
+        if (l.u1 == l.u0 || (i == 1 && one_line)) continue;
         Kernel kernel = q8 ? kernel_of<TIE_KV_INT8>(l.nt) : kv_format == TIE_KV_BF16 ? kernel_of<TIE_KV_BF16>(l.nt) : kernel_of<TIE_KV_F32>(l.nt);
         const size_t q_bytes = (size_t)kWarps * (l.nt == 1 ? kQBytes<1> : l.nt == 2 ? kQBytes<2> : kQBytes<4>);
         const size_t smem = q_bytes + (size_t)(l.u1 - l.u0 + 1) * sizeof(long long);
@@ -880,22 +1168,18 @@ extern "C" model_status tie_attention_shared(const float* q, int ldq, int n_head
         if (smem > 32 * 1024)
             TIE_OP_CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            (int)(q_bytes + most_units * sizeof(long long))));
-        const dim3 grid((unsigned)(l.warps / kWarps));
+        const dim3 grid((unsigned)ctas[i]);
         if (first) kernel<<<grid, kThreads, smem, st>>>(a, i);
         else TIE_OP_CU(launch_pdl(kernel, grid, dim3(kThreads), smem, st, a, i));
         TIE_OP_CU(cudaGetLastError());
         ++op_launches;
         first = false;
     }
-    const size_t units = (size_t)n_group + n_seq;
-    const size_t smem = (units + 1) * sizeof(long long) + (units + 2) * sizeof(int);
+    const long long most_pairs = (long long)max_new * n_head;         // of a sequence
     const bool wide = pairs <= 8LL * sms;
     auto* join = wide ? shared_join_kernel<true> : shared_join_kernel<false>;
-    if (smem > 32 * 1024)
-        TIE_OP_CU(cudaFuncSetAttribute(join, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)(most_units * (sizeof(long long) + sizeof(int)) + 64)));
-    const long long ctas = wide ? pairs : (pairs + kWarps - 1) / kWarps;
-    TIE_OP_CU(launch_pdl(join, dim3((unsigned)(ctas < 8LL * sms ? ctas : 8LL * sms)), dim3(kThreads), smem, st, a));
+    const long long y = wide ? most_pairs : (most_pairs + kWarps - 1) / kWarps;
+    TIE_OP_CU(launch_pdl(join, dim3((unsigned)n_seq, (unsigned)(y < 256 ? y : 256)), dim3(kThreads), 0, st, a));
     ++op_launches;
     return MODEL_OK;
 }
