@@ -472,7 +472,7 @@ model_status tie_attention_shared(const float *q, int ldq, int n_head, const voi
  * Pointers are DEVICE pointers of one device; any k and leading dimension is
  * taken (fp32 rows that are 16-byte aligned are read faster). Streams and errors
  * are those of the paged cache above; MODEL_ERR_CAPACITY for k above 2^24 or more
- * than 2^31 thread blocks of work. */
+ * than 2^31 - 1 blocks of 128 weights. */
 
 /* Bytes of the packed levels (0 for sizes without meaning). */
 size_t tie_q4_bytes(int n, int k);
@@ -485,13 +485,15 @@ model_status tie_dequantize_q4(const void *packed, const void *scales, int n, in
 
 /* y[r] = act(x[r] W^T + bias) + residual[r] for `rows` rows of activations (ldx,
  * ldr, ldy floats apart): the matmul of a decode step with its epilogue (the
- * bias, GELU and residual forms of model.c:735-752).
- * bias [n] and residual may be NULL; gelu 1: act is GELU (model.c:615-623), 0:
- * none. residual may be y itself, x must not overlap y. Products are exact and
- * sums fp32 (a group's, then the groups'), in an order that depends on n and k
- * only, so a row's result does not depend on the rows beside it except by their
- * number being at most 2 or above. The weights are read once for every 8 rows.
- * rows == 0 is allowed (x and y may be NULL then); at most 524,280 rows. */
+ * bias, GELU and residual forms of model.c:735-752). bias [n] and residual may be
+ * NULL; gelu 1: act is GELU (model.c:615-623), 0: none. residual may be y itself, x
+ * must not overlap y. An activation is held to 2^-32 of the largest of its 128
+ * columns (and to 2^-128), its products with levels and their sums over a group are
+ * exact, sums over groups fp32. A row's result does not depend on the rows beside
+ * it, except by their number being above 2; a row with an element that is not finite
+ * is not finite. The weights are read once for every 8 rows (every 2, where k is
+ * above about 6,000). rows == 0 is allowed (x and y may be NULL then); at most 16,384
+ * columns and 131,070 rows (MODEL_ERR_CAPACITY). */
 model_status tie_matvec_q4(const float *x, long long ldx, int rows, const void *packed,
                            const void *scales, int n, int k, int group, const float *bias,
                            const float *residual, long long ldr, int gelu, float *y, long long ldy,

@@ -76,13 +76,18 @@ def gelu(x):
 def matvec(x, w, bias=None, residual=None, act=False):
     """y in 64 bits and how far an fp32 result may be from it.
 
-    Products are exact (three terms of x times a level). A group's sum is a chain of at most 24 MMAs, each of
-    which adds 16 products and cuts off: at most 2^-23 of the sum of magnitudes each, 48 x 2^-24 with the last bits of
-    its inner sums; the scale's product, the groups' sums (one rounding each) and those of eight warps and three
-    terms: k / 32 + 16 of 2^-24 at most. Bias, GELU (of slope at most 1.13; tanhf and its products a few
+    An element of x is held to 2^-31 of the largest of its 128 (and to 2^-127), a rounding of half that; its
+    products with levels and a group's sum are exact. Joining the digits' sums rounds five times, the scale's
+    product and the groups' sums twice for each group, those of 16 warps and four digits once each: at most
+    k / 16 + 27 times 2^-24 of the sum of magnitudes. Bias, GELU (of slope at most 1.13; tanhf and its products a few
     2^-24 of the value) and residual add a rounding each."""
+    k = x.shape[1]
+    wide = np.zeros((len(x), -(-k // 128) * 128))
+    wide[:, :k] = np.abs(x)
+    tops = np.repeat(wide.reshape(len(x), -1, 128).max(-1), 128, 1)[:, :k]
+    held = (np.maximum(tops * 2.0 ** -31, 2.0 ** -127)) @ np.abs(w).T
     y = x.astype(np.float64) @ w.T
-    err = (np.abs(x).astype(np.float64) @ np.abs(w).T) * (48 + x.shape[1] / 32 + 16) * EPS
+    err = (np.abs(x).astype(np.float64) @ np.abs(w).T) * (k / 16 + 27) * EPS + held
     if bias is not None:
         y = y + bias
         err = err + np.abs(y) * EPS

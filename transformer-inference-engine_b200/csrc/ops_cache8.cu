@@ -17,93 +17,107 @@ namespace tie {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kLanes = 16;             // of a head's row: four elements each
+constexpr int kLanes = 8;              // of a head's row: eight elements each
 
-// Four elements of a head's row to levels, by 16 lanes; what the row's scale is.
-__device__ __forceinline__ uint32_t quantise4(const float4& x, float* scale) {
-    const float v[4] = {x.x, x.y, x.z, x.w};
+// Eight elements of a head's row to levels, by 8 lanes; what the row's scale is.
+__device__ __forceinline__ uint2 quantise8(const float (&x)[8], float* scale) {
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, magnitude(v[i]));
+    for (int i = 0; i < 8; ++i) top = max(top, magnitude(x[i]));
 #pragma unroll
     for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (top >= kNotFinite) {           // no value of the row is finite then
         *scale = __uint_as_float(0x7fffffffu);
-        return 0u;
+        return make_uint2(0u, 0u);
     }
     const float s = __fdiv_rn(__uint_as_float(top), 127.f);
     *scale = s;
-    if (s == 0.f) return 0u;
-    const float inv = reciprocal_of(s);
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w |= ((uint32_t)level_of(v[i], s, inv, 127.f) & 255u) << (8 * i);
-    return w;
+    if (s == 0.f) return make_uint2(0u, 0u);
+    uint32_t q[8];
+    levels_of(x, s, 127.f, q);
+    return make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410));
 }
 
-// Memory bound: 8 bytes in and 2 out for an element of keys and of values. 16 lanes take
-// a head's row of both, four elements of each a lane; they are in one warp.
+// A thread's place: row r, head h and the lane's eight elements.
+struct Place {
+    int r, h, lane;
+    __device__ __forceinline__ Place(long long i, const Divisor& heads) {
+        lane = (int)(i % kLanes);
+        const int unit = (int)(i / kLanes);
+        r = heads(unit);
+        h = unit - r * heads.d;
+    }
+};
+
+// Memory bound: 8 bytes in and 2 out for an element of keys and of values. 8 lanes take
+// a head's row of both, eight elements of each a lane; they are in one warp.
+template <int VEC>
 __global__ void __launch_bounds__(kThreads)
 kv_store_q8_kernel(const float* __restrict__ k, const float* __restrict__ v, int ld, const int32_t* __restrict__ slots,
-                   long long n, int heads, long long n_slots, int8_t* __restrict__ k_pages,
+                   long long n, Divisor heads, long long n_slots, int8_t* __restrict__ k_pages,
                    int8_t* __restrict__ v_pages, float* __restrict__ k_scales, float* __restrict__ v_scales) {
     const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
     const bool live = i < n;           // (all lanes take part in the shuffles)
-    const int lane = (int)(i % kLanes);
-    const long long unit = live ? i / kLanes : 0;
-    const int r = (int)(unit / heads), h = (int)(unit % heads);
-    const size_t from = (size_t)r * ld + h * kHeadDim + 4 * lane;
-    const float4 x = __ldcs(reinterpret_cast<const float4*>(k + from));
-    const float4 y = __ldcs(reinterpret_cast<const float4*>(v + from));
-    const int slot = __ldg(slots + r);
+    const Place at(live ? i : i % kLanes, heads);
+    const size_t from = (size_t)at.r * ld + at.h * kHeadDim + 8 * at.lane;
+    float x[8], y[8];
+    load8<VEC>(k + from, x);
+    load8<VEC>(v + from, y);
+    const int slot = __ldg(slots + at.r);
     float sk, sv;
-    const uint32_t a = quantise4(x, &sk), b = quantise4(y, &sv);
+    const uint2 a = quantise8(x, &sk), b = quantise8(y, &sv);
     if (!live || slot < 0 || slot >= n_slots) return;
-    const size_t to = (size_t)slot * heads * kHeadDim + h * kHeadDim + 4 * lane;
-    *reinterpret_cast<uint32_t*>(k_pages + to) = a;
-    *reinterpret_cast<uint32_t*>(v_pages + to) = b;
-    if (lane == 0) {
-        const size_t at = ((size_t)(slot / kPageRows) * heads + h) * kPageRows + slot % kPageRows;
-        k_scales[at] = sk;
-        v_scales[at] = sv;
+    const size_t to = (size_t)slot * heads.d * kHeadDim + at.h * kHeadDim + 8 * at.lane;
+    *reinterpret_cast<uint2*>(k_pages + to) = a;
+    *reinterpret_cast<uint2*>(v_pages + to) = b;
+    if (at.lane == 0) {
+        const size_t s = ((size_t)(slot / kPageRows) * heads.d + at.h) * kPageRows + slot % kPageRows;
+        k_scales[s] = sk;
+        v_scales[s] = sv;
     }
 }
 
 template <int FMT>
-__device__ __forceinline__ float4 row4(const void* pages, const float* scales, size_t at, size_t scale_at) {
+__device__ __forceinline__ void row8(const void* pages, const float* scales, size_t at, size_t scale_at, float (&x)[8]) {
     if constexpr (FMT == TIE_KV_F32) {
-        return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(pages) + at));
+        load8<4>(static_cast<const float*>(pages) + at, x);
     } else if constexpr (FMT == TIE_KV_BF16) {
-        const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(pages) + at));
-        return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                           __uint_as_float(u.y & 0xffff0000u));
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(pages) + at));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
     } else {
-        const char4 u = __ldg(reinterpret_cast<const char4*>(static_cast<const int8_t*>(pages) + at));
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const int8_t*>(pages) + at));
         const float s = __ldg(scales + scale_at);
-        return make_float4(u.x * s, u.y * s, u.z * s, u.w * s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (float)(int8_t)((i < 4 ? u.x : u.y) >> (8 * (i & 3))) * s;
     }
 }
 
-// The way back, memory bound as well: a lane takes four elements of a row of keys and
+// The way back, memory bound as well: a lane takes eight elements of a row of keys and
 // of its row of values.
-template <int FMT>
+template <int FMT, int VEC>
 __global__ void __launch_bounds__(kThreads)
-kv_load_kernel(const int32_t* __restrict__ slots, long long n, int heads, long long n_slots,
+kv_load_kernel(const int32_t* __restrict__ slots, long long n, Divisor heads, long long n_slots,
                const void* __restrict__ k_pages, const void* __restrict__ v_pages, const float* __restrict__ k_scales,
                const float* __restrict__ v_scales, float* __restrict__ k, float* __restrict__ v, int ld) {
     const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
     if (i >= n) return;
-    const int lane = (int)(i % kLanes);
-    const long long unit = i / kLanes;
-    const int r = (int)(unit / heads), h = (int)(unit % heads);
-    const int slot = __ldg(slots + r);
+    const Place at(i, heads);
+    const int slot = __ldg(slots + at.r);
     if (slot < 0 || slot >= n_slots) return;
-    const size_t from = (size_t)slot * heads * kHeadDim + h * kHeadDim + 4 * lane;
-    const size_t at = ((size_t)(slot / kPageRows) * heads + h) * kPageRows + slot % kPageRows;
-    const float4 x = row4<FMT>(k_pages, k_scales, from, at), y = row4<FMT>(v_pages, v_scales, from, at);
-    const size_t to = (size_t)r * ld + h * kHeadDim + 4 * lane;
-    __stcs(reinterpret_cast<float4*>(k + to), x);
-    __stcs(reinterpret_cast<float4*>(v + to), y);
+    const size_t from = (size_t)slot * heads.d * kHeadDim + at.h * kHeadDim + 8 * at.lane;
+    const size_t s = ((size_t)(slot / kPageRows) * heads.d + at.h) * kPageRows + slot % kPageRows;
+    float x[8], y[8];
+    row8<FMT>(k_pages, k_scales, from, s, x);
+    row8<FMT>(v_pages, v_scales, from, s, y);
+    const size_t to = (size_t)at.r * ld + at.h * kHeadDim + 8 * at.lane;
+    store8<VEC>(k + to, x);
+    store8<VEC>(v + to, y);
 }
 
 // What both entry points ask of the pool and of the rows.
@@ -130,10 +144,11 @@ extern "C" model_status tie_kv_store_q8(const float* k, const float* v, int ld, 
     if (bad != MODEL_OK || rows == 0) return bad;
     OnDeviceOf dev(k_pages);
     if (dev.status() != MODEL_OK) return dev.status();
+    if ((long long)rows * n_kv_head > INT_MAX) return MODEL_ERR_CAPACITY;
     const long long n = (long long)rows * n_kv_head * kLanes, blocks = (n + kThreads - 1) / kThreads;
-    if (blocks > INT_MAX) return MODEL_ERR_CAPACITY;
-    kv_store_q8_kernel<<<(unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        k, v, ld, slots, n, n_kv_head, (long long)n_pages * kPageRows, static_cast<int8_t*>(k_pages),
+    const bool wide = ld % 8 == 0 && aligned(k, 32) && aligned(v, 32);
+    (wide ? kv_store_q8_kernel<8> : kv_store_q8_kernel<4>)<<<(unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+        k, v, ld, slots, n, divisor(n_kv_head), (long long)n_pages * kPageRows, static_cast<int8_t*>(k_pages),
         static_cast<int8_t*>(v_pages), k_scales, v_scales);
     TIE_OP_CU(cudaGetLastError());
     ++op_launches;
@@ -150,12 +165,15 @@ extern "C" model_status tie_kv_load(const int32_t* slots, int rows, const void* 
     if (bad != MODEL_OK || rows == 0) return bad;
     OnDeviceOf dev(k_pages);
     if (dev.status() != MODEL_OK) return dev.status();
+    if ((long long)rows * n_kv_head > INT_MAX) return MODEL_ERR_CAPACITY;
     const long long n = (long long)rows * n_kv_head * kLanes, blocks = (n + kThreads - 1) / kThreads;
-    if (blocks > INT_MAX) return MODEL_ERR_CAPACITY;
-    auto* kernel = q8 ? kv_load_kernel<TIE_KV_INT8>
-                      : kv_format == TIE_KV_BF16 ? kv_load_kernel<TIE_KV_BF16> : kv_load_kernel<TIE_KV_F32>;
+    const bool wide = ld % 8 == 0 && aligned(k, 32) && aligned(v, 32);
+    auto of = [&](auto* with8, auto* with4) { return wide ? with8 : with4; };
+    auto* kernel = q8 ? of(kv_load_kernel<TIE_KV_INT8, 8>, kv_load_kernel<TIE_KV_INT8, 4>)
+                      : kv_format == TIE_KV_BF16 ? of(kv_load_kernel<TIE_KV_BF16, 8>, kv_load_kernel<TIE_KV_BF16, 4>)
+                                                 : of(kv_load_kernel<TIE_KV_F32, 8>, kv_load_kernel<TIE_KV_F32, 4>);
     kernel<<<(unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        slots, n, n_kv_head, (long long)n_pages * kPageRows, k_pages, v_pages, k_scales, v_scales, k, v, ld);
+        slots, n, divisor(n_kv_head), (long long)n_pages * kPageRows, k_pages, v_pages, k_scales, v_scales, k, v, ld);
     TIE_OP_CU(cudaGetLastError());
     ++op_launches;
     return MODEL_OK;

@@ -19,7 +19,7 @@
 namespace tie {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;         // of the kernels that make weights and read them back
 constexpr int kBlock = 128, kBlockBytes = kBlock / 2;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -27,68 +27,80 @@ __host__ __device__ inline int blocks_of(int k) { return (k + kBlock - 1) / kBlo
 
 // ------------------------------------------------------------ made, read back --
 // Memory bound. 16 lanes take a block, 8 consecutive weights a lane.
-template <bool VEC>
-__device__ __forceinline__ void load8(const float* row, int c, int k, float (&x)[8]) {
+// Weights c .. c + 7 of a row of k, zeros behind it.
+template <int VEC>
+__device__ __forceinline__ void weights8(const float* row, int c, int k, float (&x)[8]) {
     if (VEC && c + 8 <= k) {
-        const float4 a = __ldcs(reinterpret_cast<const float4*>(row + c));
-        const float4 b = __ldcs(reinterpret_cast<const float4*>(row + c) + 1);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        load8<VEC>(row + c, x);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = c + i < k ? __ldg(row + c + i) : 0.f;
     }
 }
 
-template <bool VEC>
+// Blocks per 16 lanes: both are loaded before either is used (a block at a time: 50257 x 1600 in
+// 95 us, two: 90).
+constexpr int kUnits = 2;
+
+template <int VEC>
 __global__ void __launch_bounds__(kThreads)
-quantize_q4_kernel(const float* __restrict__ w, long long ldw, long long units, int k, int blocks, int lanes,
+quantize_q4_kernel(const float* __restrict__ w, long long ldw, int units, int k, Divisor blocks, int shift,
                    uint32_t* __restrict__ packed, __nv_bfloat16* __restrict__ scales, int groups) {
-    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-    const bool live = i < 16 * units;              // (all lanes take part in the shuffles)
-    const long long unit = live ? i / 16 : 0;
-    const long long row = unit / blocks;
-    const int b = (int)(unit % blocks), l = (int)(i % 16);
-    float x[8];
-    load8<VEC>(w + row * ldw, b * kBlock + 8 * l, k, x);
-    uint32_t top = 0;
+    const int l = threadIdx.x % 16;
+    const long long first = (long long)blockIdx.x * (kThreads / 16 * kUnits) + threadIdx.x / 16;
+    float x[kUnits][8];
+    int row[kUnits], c[kUnits];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, magnitude(x[e]));
-    for (int o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(kAll, top, o));
-    const bool odd = top >= kNotFinite;            // a weight is not finite: no value of the group is
-    const __nv_bfloat16 sb = odd ? __ushort_as_bfloat16((unsigned short)0x7fff)
-                                 : __float2bfloat16_rn(__fdiv_rn(__uint_as_float(top), 7.f));
-    const float s = __bfloat162float(sb);
-    const float inv = reciprocal_of(s);
-    uint32_t word = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int q = odd || s == 0.f ? 0 : level_of(x[e], s, inv, 7.f);
-        word |= (uint32_t)(q + 8) << (4 * e);
+    for (int j = 0; j < kUnits; ++j) {
+        // (all lanes take part in the shuffles)
+        const int unit = (int)min(first + j * (kThreads / 16), (long long)units - 1);
+        row[j] = blocks(unit);
+        c[j] = (unit - row[j] * blocks.d) * kBlock + 8 * l;
+        weights8<VEC>(w + (long long)row[j] * ldw, c[j], k, x[j]);
     }
-    if (!live) return;
-    packed[unit * 16 + 4 * (l % 4) + l / 4] = word;
-    if (l % lanes == 0 && b * kBlock + 8 * l < k) scales[row * groups + (b * 16 + l) / lanes] = sb;
+#pragma unroll
+    for (int j = 0; j < kUnits; ++j) {
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max_abs(top, x[j][e]);
+#pragma unroll
+        for (int o = 0; o < 4; ++o)
+            if (o < shift) top = max_abs(top, __shfl_xor_sync(kAll, top, 1 << o));
+        const bool odd = !(top < INFINITY);        // a weight is not finite: no value of the group is
+        const __nv_bfloat16 sb = odd ? __ushort_as_bfloat16((unsigned short)0x7fff) : __float2bfloat16_rn(__fdiv_rn(top, 7.f));
+        const float s = __bfloat162float(sb);
+        uint32_t word = 0x88888888u;               // zeros
+        if (!odd && s != 0.f) {
+            uint32_t q[8];
+            levels_of(x[j], s, 7.f, q);
+            word = 0u;
+#pragma unroll
+            for (int e = 7; e >= 0; --e) word = word * 16u + q[e];
+            word -= (kLevelBase - 8u) * 0x11111111u;   // what each level was added to, less 8
+        }
+        const long long unit = first + j * (kThreads / 16);
+        if (unit >= units) continue;
+        packed[unit * 16 + 4 * (l % 4) + l / 4] = word;
+        if ((l & ((1 << shift) - 1)) == 0 && c[j] < k) scales[(long long)row[j] * groups + (c[j] >> (shift + 3))] = sb;
+    }
 }
 
-template <bool VEC>
+template <int VEC>
 __global__ void __launch_bounds__(kThreads)
-dequantize_q4_kernel(const uint32_t* __restrict__ packed, const __nv_bfloat16* __restrict__ scales, long long units, int k,
-                     int blocks, int lanes, int groups, float* __restrict__ w, long long ldw) {
+dequantize_q4_kernel(const uint32_t* __restrict__ packed, const __nv_bfloat16* __restrict__ scales, int units, int k,
+                     Divisor blocks, int shift, int groups, float* __restrict__ w, long long ldw) {
     const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= 16 * units) return;
-    const long long unit = i / 16, row = unit / blocks;
-    const int b = (int)(unit % blocks), l = (int)(i % 16), c = b * kBlock + 8 * l;
+    if (i >= 16LL * units) return;
+    const int unit = (int)(i / 16), row = blocks(unit), b = unit - row * blocks.d, l = (int)(i % 16), c = b * kBlock + 8 * l;
     if (c >= k) return;
-    const uint32_t word = __ldg(packed + unit * 16 + 4 * (l % 4) + l / 4);
-    const float s = __bfloat162float(scales[row * groups + (b * 16 + l) / lanes]);
+    const uint32_t word = __ldg(packed + unit * 16LL + 4 * (l % 4) + l / 4);
+    const float s = __bfloat162float(scales[(long long)row * groups + ((b * 16 + l) >> shift)]);
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = (float)((int)(word >> (4 * e) & 15u) - 8) * s;
-    float* out = w + row * ldw + c;
+    float* out = w + (long long)row * ldw + c;
     if (VEC && c + 8 <= k) {
-        __stcs(reinterpret_cast<float4*>(out), make_float4(x[0], x[1], x[2], x[3]));
-        __stcs(reinterpret_cast<float4*>(out) + 1, make_float4(x[4], x[5], x[6], x[7]));
+        store8<VEC>(out, x);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -97,22 +109,31 @@ dequantize_q4_kernel(const uint32_t* __restrict__ packed, const __nv_bfloat16* _
 }
 
 // ------------------------------------------------------------------- products --
-// y[r] = act(x[r] W^T + bias) + residual[r] for up to 8 rows of x a CTA, on bf16 MMAs
-// (m16n8k16): 16 rows of W are the A operand, the columns of B are rows of x. A level is
-// exact in bf16, and an fp32 activation is exactly the sum of three bf16 terms (its 24
-// bits in 8-bit pieces), so every product is exact and sums are fp32's: a group's sum of
-// level * x in the MMA, times the group's scale, added in fp32. One or two rows of x put
-// their terms into six of B's columns, one MMA for 16 weights of each row; up to 8 rows
-// take three MMAs into the same sums.
+// y[r] = act(x[r] W^T + bias) + residual[r] for up to 8 rows of x a CTA, on integer MMAs
+// (m16n8k32): 16 rows of W are the A operand, as the nibbles level + 8 lie in a word (a mask, a
+// shift and a mask for eight of them), the columns of B are rows of x. The elements of 128
+// columns of x become integers of 31 bits, relative to their largest, in four signed 8-bit
+// digits. A group's sum of each digit is exact; it starts at -8 times the digits' own sum, which takes the
+// 8 out of the levels, and at the bits of an fp32 number (quant.cuh), so that it ends as fp32 and needs no
+// conversion. Then come the group's scale and the sum over groups, in fp32. One or
+// two rows of x put their digits into B's eight columns, one MMA for 32 weights of each
+// row; up to 8 rows take four. (On bf16 terms of x the levels had to be converted, 11 instructions for eight
+// weights instead of 3: 50257 x 1600 took 24.7 us for 2 rows and 28.8 for 8.)
 //
-// The k blocks of a tile are dealt to the CTA's warps, whose sums are added in order.
+// Bound by the reading of W where that is large, by the chain of a strip's steps where it is
+// small. A CTA takes an equal share of the strips of 16 rows of W and turns x into digits once, in shared
+// memory, in the order that the lanes read them. The share's steps (a strip's blocks of 128
+// columns) form a line that its 16 warps cut into equal stretches; a warp has the weights of
+// kAhead steps on their way in registers, over the ends of strips. A strip that one warp has all of
+// goes out at once, the others' sums through shared memory and the CTA's only barrier, in
+// order. 50257 x 1600, 42 MB, takes 17 us for 2 rows and 20 for 8; the loads alone, in this order, take 10.
 struct MatvecArgs {
     const float* x;
     long long ldx;
     int rows;
     const uint8_t* packed;
     const __nv_bfloat16* scales;
-    int n, k, blocks, groups;
+    int n, k, blocks, groups, strips;
     const float* bias;
     const float* residual;
     long long ldr;
@@ -121,124 +142,293 @@ struct MatvecArgs {
     long long ldy;
 };
 
-constexpr int kWarps = kThreads / 32;
+constexpr int kWarps = 16, kAhead = 3;
 
-// Levels i and i + 4 of a word, for i = 0 .. 3, as pairs of bf16: 0x4300 | u is 128 + u.
-__device__ __forceinline__ void levels8(uint32_t w, uint32_t (&p)[4]) {
-    const __nv_bfloat162 off = __floats2bfloat162_rn(136.f, 136.f);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-        const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), off);
-        p[i] = *reinterpret_cast<const uint32_t*>(&v);
-    }
+// d = c + a b on levels (unsigned) and digits (signed), m16n8k32
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const int (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+}
+// where a digit's sum starts: 1.5 2^23, 2^31, 2^39, 2^47, whose last places are worth 1, 256, ...
+__host__ __device__ constexpr int start_of(int digit) { return 0x4b400000 + (digit << 26); }
+
+// A block of x in shared memory: digits [j][digit pair][lane] (few: [j][lane]), where sums start
+// [group][digit][column], what 1 is worth [column].
+template <bool FEW, int G>
+struct XBlock {
+    static constexpr int kDigits = FEW ? 1 : 4, kGroups = kBlock / G;
+    static constexpr int kDigitBytes = 4 * kDigits * 32 * 8, kStartBytes = kGroups * kDigits * 8 * 4;
+    static constexpr int kBytes = kDigitBytes + kStartBytes + 8 * 4;
+};
+constexpr int kSumBytes = 16 * 8 * 4;              // a warp's sums of a strip
+
+// y of row r0 + r, output j, from the sum of its products
+__device__ __forceinline__ void put(const MatvecArgs& a, int r, int j, float sum) {
+    if (j >= a.n) return;
+    if (a.bias) sum = __fadd_rn(sum, __ldg(a.bias + j));
+    if (a.gelu) sum = gelu_new_ref(sum);
+    if (a.residual) sum = __fadd_rn(a.residual[(long long)r * a.ldr + j], sum);
+    a.y[(long long)r * a.ldy + j] = sum;
 }
 
-template <bool FEW, int MT, int G, bool VEC>
-__global__ void __launch_bounds__(kThreads) matvec_q4_kernel(MatvecArgs a) {
-    constexpr int kTerms = FEW ? 1 : 3;            // MMAs for each 16 weights
-    __shared__ float s_sum[kWarps][MT * 16][9];
+template <bool FEW, int G, bool VEC>
+__global__ void __launch_bounds__(kWarps * 32, 1) matvec_q4_kernel(const __grid_constant__ MatvecArgs a) {
+    using X = XBlock<FEW, G>;
+    constexpr int kDigits = X::kDigits, kGroups = X::kGroups, kRows = FEW ? 2 : 8;
+    extern __shared__ __align__(16) uint8_t smem[];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c = lane & 3;
-    const int n0 = blockIdx.x * MT * 16, r0 = blockIdx.y * 8, rows = min(8, a.rows - r0);
-    // the row of x that this lane's column of B stands for, and (FEW) which of its terms
-    const int xr = FEW ? g / 3 : g, term = FEW ? g % 3 : 0;
-    const bool real = xr < rows && (!FEW || g < 6);
+    const int r0 = blockIdx.y * kRows, rows = min(kRows, a.rows - r0);
+    const int strip0 = (int)((long long)a.strips * blockIdx.x / gridDim.x);
+    const int strip1 = (int)((long long)a.strips * (blockIdx.x + 1) / gridDim.x);
+    const int steps = (strip1 - strip0) * a.blocks;          // (fits: 2^27 strips of at most 128 blocks over the SMs)
+    auto from_step = [&](int w) { return (int)((unsigned long long)(unsigned)steps * (unsigned)w / kWarps); };
+    const int q0 = from_step(warp), q1 = from_step(warp + 1);
+    pdl_wait();
+
+    // weights and scales (of group c of the block; the others have theirs from lane c) on their way
+    uint4 w[kAhead][2];
+    unsigned short sc[kAhead][2];
+    const uint8_t* w_at[2];
+    const unsigned short* s_at[2];
+    int left = q1 - q0, next_strip = strip0 + q0 / a.blocks, next_kb = q0 % a.blocks;
+    auto rows_of = [&]() {                         // of next_strip
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const long long row = min(next_strip * 16 + 8 * h + g, a.n - 1);
+            w_at[h] = a.packed + (row * a.blocks + next_kb) * kBlockBytes + 16 * c;
+            s_at[h] = reinterpret_cast<const unsigned short*>(a.scales) + row * a.groups;
+        }
+    };
+    rows_of();
+    auto load = [&](uint4 (&to)[2], unsigned short (&s)[2]) {
+        if (left <= 0) return;
+        --left;
+        const int grp = min(next_kb * kGroups + (c & (kGroups - 1)), a.groups - 1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(to[h].x), "=r"(to[h].y), "=r"(to[h].z), "=r"(to[h].w)
+                         : "l"(w_at[h]));
+            s[h] = __ldg(s_at[h] + grp);
+            w_at[h] += kBlockBytes;
+        }
+        if (++next_kb == a.blocks) {
+            next_kb = 0;
+            ++next_strip;
+            rows_of();
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) load(w[d], sc[d]);
+
+    // the row of x that this lane's column g of B stands for, and (FEW) which of its digits
+    const int xr = FEW ? g >> 2 : g;
+    const bool real = xr < rows;
     const float* x = a.x + (long long)(r0 + min(xr, rows - 1)) * a.ldx;
-    float acc[MT][4] = {};
-    for (int kb = warp; kb < a.blocks; kb += kWarps) {
-        uint4 w[MT][2];
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = min(n0 + 16 * m + 8 * h + g, a.n - 1);
-                w[m][h] = __ldg(reinterpret_cast<const uint4*>(a.packed + ((size_t)row * a.blocks + kb) * kBlockBytes) + c);
-            }
-        uint32_t b[kTerms][4][4];                  // [term][j][pair i, i + 4]
+    // block kb of x, by one warp
+    auto x_of = [&](int kb) {
+        uint8_t* const to = smem + (size_t)kb * X::kBytes;
+        float top = 0.f, v[4][8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float v[8];
-            load8<VEC>(x, kb * kBlock + 32 * j + 8 * c, real ? a.k : 0, v);
+            weights8<VEC ? 4 : 0>(x, kb * kBlock + 32 * j + 8 * c, real ? a.k : 0, v[j]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float lo = v[i], hi = v[i + 4];
+            for (int i = 0; i < 8; ++i) top = max_abs(top, v[j][i]);
+        }
+        top = max_abs(top, __shfl_xor_sync(kAll, top, 1));
+        top = max_abs(top, __shfl_xor_sync(kAll, top, 2));
+        // the largest is below 2^(e - 126): times 2^(156 - e), it is at most 2^30
+        const int e = max((int)(__float_as_uint(top) >> 23), 29);
+        const float up = __uint_as_float((uint32_t)(283 - e) << 23);
+        // (2^-127 is the smallest unit; a row with an element that is not finite gets NaN)
+        float one = e >= 255 ? top * 0.f : __uint_as_float(e == 29 ? 0x00400000u : (uint32_t)(e - 29) << 23);
+        if constexpr (FEW) one *= (float)(1 << (8 * (g & 3)));
+        int sum[kDigits][kGroups] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t b[kDigits][2];
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = ((uint32_t)__float2int_rn(v[j][2 * i + o] * up) + 0x00808080u) ^ 0x00808080u;
+                uint32_t d[4];                     // digit by digit
+                const uint32_t lo0 = __byte_perm(w[0], w[1], 0x5140), lo1 = __byte_perm(w[2], w[3], 0x5140);
+                const uint32_t hi0 = __byte_perm(w[0], w[1], 0x7362), hi1 = __byte_perm(w[2], w[3], 0x7362);
+                d[0] = __byte_perm(lo0, lo1, 0x5410);
+                d[1] = __byte_perm(lo0, lo1, 0x7632);
+                d[2] = __byte_perm(hi0, hi1, 0x5410);
+                d[3] = __byte_perm(hi0, hi1, 0x7632);
+#pragma unroll
+                for (int z = 0; z < kDigits; ++z) {
+                    b[z][o] = FEW ? ((g & 2) ? (g & 1 ? d[3] : d[2]) : (g & 1 ? d[1] : d[0])) : d[z];
+                    sum[z][j / (G / 32)] = __dp4a((int)b[z][o], 0x01010101, sum[z][j / (G / 32)]);
+                }
+            }
+            if constexpr (FEW) {
+                reinterpret_cast<uint2*>(to)[j * 32 + lane] = make_uint2(b[0][0], b[0][1]);
+            } else {
+                reinterpret_cast<uint4*>(to)[(2 * j) * 32 + lane] = make_uint4(b[0][0], b[0][1], b[1 % kDigits][0], b[1 % kDigits][1]);
+                reinterpret_cast<uint4*>(to)[(2 * j + 1) * 32 + lane] =
+                    make_uint4(b[2 % kDigits][0], b[2 % kDigits][1], b[3 % kDigits][0], b[3 % kDigits][1]);
+            }
+        }
+        int* const starts = reinterpret_cast<int*>(to + X::kDigitBytes);
+#pragma unroll
+        for (int z = 0; z < kDigits; ++z)
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) {
+                int y = sum[z][i];
+                y += __shfl_xor_sync(kAll, y, 1);
+                y += __shfl_xor_sync(kAll, y, 2);
+                if (c == 0) starts[(i * kDigits + z) * 8 + g] = start_of(z) - 8 * y;
+            }
+        if (c == 0) reinterpret_cast<float*>(to + X::kDigitBytes + X::kStartBytes)[g] = one;
+    };
+    for (int kb = warp; kb < a.blocks; kb += kWarps) x_of(kb);
+    __syncthreads();
+
+    float acc[4] = {}, ended[4];                   // ended: of the strip that the warp goes on with
+    bool went_on = false;
+    int strip = strip0 + q0 / a.blocks, kb = q0 % a.blocks, first = kb;
+    auto add = [&](uint4 (&wd)[2], unsigned short (&sd)[2]) {
+        const uint32_t w0[4] = {wd[0].x, wd[0].y, wd[0].z, wd[0].w}, w1[4] = {wd[1].x, wd[1].y, wd[1].z, wd[1].w};
+        const float s[2] = {__uint_as_float((uint32_t)sd[0] << 16), __uint_as_float((uint32_t)sd[1] << 16)};
+        load(wd, sd);
+        const uint8_t* const xb = smem + (size_t)kb * X::kBytes;
+        const int* const starts = reinterpret_cast<const int*>(xb + X::kDigitBytes) + 2 * c;
+        const float2 unit = *reinterpret_cast<const float2*>(xb + X::kDigitBytes + X::kStartBytes + 8 * c);
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) {
+            int d[kDigits][4];
+#pragma unroll
+            for (int z = 0; z < kDigits; ++z) {
+                const int2 from = *reinterpret_cast<const int2*>(starts + (i * kDigits + z) * 8);
+                d[z][0] = d[z][2] = from.x;
+                d[z][1] = d[z][3] = from.y;
+            }
+#pragma unroll
+            for (int j = i * (G / 32); j < (i + 1) * (G / 32); ++j) {
+                const uint32_t frag[4] = {w0[j] & 0x0f0f0f0fu, w1[j] & 0x0f0f0f0fu, (w0[j] >> 4) & 0x0f0f0f0fu,
+                                          (w1[j] >> 4) & 0x0f0f0f0fu};
                 if constexpr (FEW) {
-                    if (term) { lo = rest(lo); hi = rest(hi); }
-                    if (term == 2) { lo = rest(lo); hi = rest(hi); }
-                    b[0][j][i] = terms2(lo, hi);
+                    const uint2 u = reinterpret_cast<const uint2*>(xb)[j * 32 + lane];
+                    mma_u8s8(d[0], frag, u.x, u.y, d[0]);
                 } else {
-                    b[0][j][i] = terms2(lo, hi);
-                    lo = rest(lo); hi = rest(hi);
-                    b[1][j][i] = terms2(lo, hi);
-                    b[2][j][i] = terms2(rest(lo), rest(hi));
+                    const uint4 u = reinterpret_cast<const uint4*>(xb)[(2 * j) * 32 + lane];
+                    const uint4 v = reinterpret_cast<const uint4*>(xb)[(2 * j + 1) * 32 + lane];
+                    mma_u8s8(d[0], frag, u.x, u.y, d[0]);
+                    mma_u8s8(d[1 % kDigits], frag, u.z, u.w, d[1 % kDigits]);
+                    mma_u8s8(d[2 % kDigits], frag, v.x, v.y, d[2 % kDigits]);
+                    mma_u8s8(d[3 % kDigits], frag, v.z, v.w, d[3 % kDigits]);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float f = kGroups == 1 ? s[h] : __shfl_sync(kAll, s[h], (lane & ~3) | i);
+                const float f2[2] = {f * unit.x, f * unit.y};
+#pragma unroll
+                for (int e = 2 * h; e < 2 * h + 2; ++e) {
+                    float y;
+                    if constexpr (FEW) {
+                        y = __int_as_float(d[0][e]) - __int_as_float(start_of(0));
+                    } else {
+                        const float high = (__int_as_float(d[3 % kDigits][e]) - __int_as_float(start_of(3))) +
+                                           (__int_as_float(d[2 % kDigits][e]) - __int_as_float(start_of(2)));
+                        const float low = __int_as_float(d[1 % kDigits][e]) - (__int_as_float(start_of(1)) + __int_as_float(start_of(0)));
+                        y = high + (low + __int_as_float(d[0][e]));
+                    }
+                    acc[e] = fmaf(y, f2[e & 1], acc[e]);
                 }
             }
         }
+        if (++kb < a.blocks) return;
+        // the strip's end
+        if (first == 0) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const uint32_t w0[4] = {w[m][0].x, w[m][0].y, w[m][0].z, w[m][0].w};
-            const uint32_t w1[4] = {w[m][1].x, w[m][1].y, w[m][1].z, w[m][1].w};
+            for (int h = 0; h < 2; ++h) {
+                const int j = strip * 16 + 8 * h + g;
+                if constexpr (FEW) {               // columns 4 r .. 4 r + 3 are row r's digits
+                    float y = acc[2 * h] + acc[2 * h + 1];
+                    y += __shfl_xor_sync(kAll, y, 1);
+                    if ((c & 1) == 0 && (c >> 1) < rows) put(a, r0 + (c >> 1), j, y);
+                } else {
 #pragma unroll
-            for (int j0 = 0; j0 < 4; j0 += G / 32) {
-                float d[4] = {};
-#pragma unroll
-                for (int j = j0; j < j0 + G / 32; ++j) {
-                    uint32_t p[4], q[4];
-                    levels8(w0[j], p);
-                    levels8(w1[j], q);
-#pragma unroll
-                    for (int i = 0; i < 4; i += 2) {
-                        const uint32_t frag[4] = {p[i], q[i], p[i + 1], q[i + 1]};
-#pragma unroll
-                        for (int e = 0; e < kTerms; ++e) mma_bf16(d, frag, b[e][j][i], b[e][j][i + 1]);
-                    }
+                    for (int e = 0; e < 2; ++e)
+                        if (2 * c + e < rows) put(a, r0 + 2 * c + e, j, acc[2 * h + e]);
                 }
-                const int grp = (kb * kBlock + 32 * j0) / G;
+            }
+        } else {
+            went_on = true;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int row = min(n0 + 16 * m + 8 * h + g, a.n - 1);
-                    const float s = grp < a.groups ? __bfloat162float(a.scales[(size_t)row * a.groups + grp]) : 0.f;
-                    acc[m][2 * h] = fmaf(s, d[2 * h], acc[m][2 * h]);
-                    acc[m][2 * h + 1] = fmaf(s, d[2 * h + 1], acc[m][2 * h + 1]);
-                }
+            for (int e = 0; e < 4; ++e) ended[e] = acc[e];
+        }
+        acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
+        kb = first = 0;
+        ++strip;
+    };
+    for (int q = q0; q < q1; q += kAhead) {
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d)
+            if (q + d < q1) add(w[d], sc[d]);
+    }
+    // (a strip that is not at its end here: begun by this warp, or, within the stretch, gone on with)
+    const bool open = q0 < q1 && kb > 0, begun = open && first == 0;
+    // Sums of a warp's cut strips, where x was: of the one that it goes on with, of the one that it begins.
+    float* const sums = reinterpret_cast<float*>(smem);
+    auto keep = [&](int slot, const float (&y)[4]) {
+        float* const to = sums + (size_t)(2 * warp + slot) * (kSumBytes / 4);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) *reinterpret_cast<float2*>(to + (8 * h + g) * 8 + 2 * c) = make_float2(y[2 * h], y[2 * h + 1]);
+    };
+    __syncthreads();
+    if (went_on) keep(0, ended);
+    if (open) keep(begun, acc);
+    __syncthreads();
+    if (!begun) return;
+    // the warp that began a cut strip adds the sums of those that went on with it, in order
+    int last = warp + 1;
+    while (from_step(last + 1) < (strip - strip0 + 1) * a.blocks) ++last;
+    const int o = lane & 15;
+    float sum[kRows / 2] = {};
+    for (int v = warp; v <= last; ++v) {
+        if (v > warp && from_step(v) == from_step(v + 1)) continue;          // a warp without steps
+        const float* z = sums + (size_t)(2 * v + (v == warp)) * (kSumBytes / 4) + o * 8;
+#pragma unroll
+        for (int i = 0; i < kRows / 2; ++i) {
+            const int r = 2 * i + (lane >> 4);
+            if constexpr (FEW) {
+                const float4 d = *reinterpret_cast<const float4*>(z + 4 * r);
+                sum[i] += (d.x + d.y) + (d.z + d.w);
+            } else {
+                sum[i] += z[r];
             }
         }
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s_sum[warp][16 * m + 8 * (e >> 1) + g][2 * c + (e & 1)] = acc[m][e];
-    __syncthreads();
-    for (int i = t; i < MT * 16 * rows; i += kThreads) {
-        const int o = i % (MT * 16), r = i / (MT * 16), j = n0 + o;
-        if (j >= a.n) continue;
-        float sum = 0.f;
-#pragma unroll
-        for (int v = 0; v < kWarps; ++v) {
-            if constexpr (FEW) sum += s_sum[v][o][3 * r] + (s_sum[v][o][3 * r + 1] + s_sum[v][o][3 * r + 2]);
-            else sum += s_sum[v][o][r];
-        }
-        if (a.bias) sum = __fadd_rn(sum, __ldg(a.bias + j));
-        if (a.gelu) sum = gelu_new_ref(sum);
-        if (a.residual) sum = __fadd_rn(a.residual[(long long)(r0 + r) * a.ldr + j], sum);
-        a.y[(long long)(r0 + r) * a.ldy + j] = sum;
+    for (int i = 0; i < kRows / 2; ++i) {
+        const int r = 2 * i + (lane >> 4);
+        if (r < rows) put(a, r0 + r, strip * 16 + o, sum[i]);
     }
 }
 
-template <bool FEW, int MT, bool VEC>
-void (*matvec_of(int group))(MatvecArgs) {
-    return group == 32 ? matvec_q4_kernel<FEW, MT, 32, VEC>
-                       : group == 64 ? matvec_q4_kernel<FEW, MT, 64, VEC> : matvec_q4_kernel<FEW, MT, 128, VEC>;
-}
 template <bool FEW, bool VEC>
-void (*matvec_of(int mt, int group))(MatvecArgs) {
-    return mt == 1 ? matvec_of<FEW, 1, VEC>(group) : mt == 2 ? matvec_of<FEW, 2, VEC>(group) : matvec_of<FEW, 4, VEC>(group);
+void (*matvec_of(int group))(MatvecArgs) {
+    return group == 32 ? matvec_q4_kernel<FEW, 32, VEC> : group == 64 ? matvec_q4_kernel<FEW, 64, VEC> : matvec_q4_kernel<FEW, 128, VEC>;
+}
+template <bool FEW>
+size_t x_block_bytes(int group) {
+    return group == 32 ? XBlock<FEW, 32>::kBytes : group == 64 ? XBlock<FEW, 64>::kBytes : XBlock<FEW, 128>::kBytes;
 }
 
 // Shapes that the 4-bit entry points share.
 bool q4_shape_ok(int n, int k, int group) {
     return n > 0 && k > 0 && (group == 32 || group == 64 || group == 128);
 }
+// the lanes that share a group: 2 to this
+int shift_of(int group) { return group == 32 ? 2 : group == 64 ? 3 : 4; }
+constexpr int kMostInputs = 16384;                 // of a product: two rows of x fit in shared memory
 constexpr int kMostColumns = 1 << 24;              // a k whose block count and padded width stay far inside int32
 
 }  // namespace
@@ -254,13 +444,13 @@ extern "C" model_status tie_quantize_q4(const float* w, long long ldw, int n, in
                                         void* stream) {
     if (!w || !packed || !scales || !q4_shape_ok(n, k, group) || ldw < k) return MODEL_ERR_ARG;
     if (!aligned(w, 4) || !aligned16(packed) || !aligned(scales, 2)) return MODEL_ERR_ARG;
-    const long long units = (long long)n * blocks_of(k), grid = (16 * units + kThreads - 1) / kThreads;
-    if (k > kMostColumns || grid > INT_MAX) return MODEL_ERR_CAPACITY;
+    const long long units = (long long)n * blocks_of(k), per = kThreads / 16 * kUnits, grid = (units + per - 1) / per;
+    if (k > kMostColumns || units > INT_MAX) return MODEL_ERR_CAPACITY;
     OnDeviceOf dev(packed);
     if (dev.status() != MODEL_OK) return dev.status();
-    const bool vec = aligned16(w) && ldw % 4 == 0;
-    (vec ? quantize_q4_kernel<true> : quantize_q4_kernel<false>)<<<(unsigned)grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        w, ldw, units, k, blocks_of(k), group / 8, static_cast<uint32_t*>(packed), static_cast<__nv_bfloat16*>(scales),
+    const bool vec8 = aligned(w, 32) && ldw % 8 == 0, vec4 = aligned16(w) && ldw % 4 == 0;
+    (vec8 ? quantize_q4_kernel<8> : vec4 ? quantize_q4_kernel<4> : quantize_q4_kernel<0>)<<<(unsigned)grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+        w, ldw, (int)units, k, divisor(blocks_of(k)), shift_of(group), static_cast<uint32_t*>(packed), static_cast<__nv_bfloat16*>(scales),
         (k + group - 1) / group);
     TIE_OP_CU(cudaGetLastError());
     ++op_launches;
@@ -272,12 +462,12 @@ extern "C" model_status tie_dequantize_q4(const void* packed, const void* scales
     if (!w || !packed || !scales || !q4_shape_ok(n, k, group) || ldw < k) return MODEL_ERR_ARG;
     if (!aligned(w, 4) || !aligned16(packed) || !aligned(scales, 2)) return MODEL_ERR_ARG;
     const long long units = (long long)n * blocks_of(k), grid = (16 * units + kThreads - 1) / kThreads;
-    if (k > kMostColumns || grid > INT_MAX) return MODEL_ERR_CAPACITY;
+    if (k > kMostColumns || units > INT_MAX) return MODEL_ERR_CAPACITY;
     OnDeviceOf dev(w);
     if (dev.status() != MODEL_OK) return dev.status();
-    const bool vec = aligned16(w) && ldw % 4 == 0;
-    (vec ? dequantize_q4_kernel<true> : dequantize_q4_kernel<false>)<<<(unsigned)grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<const uint32_t*>(packed), static_cast<const __nv_bfloat16*>(scales), units, k, blocks_of(k), group / 8,
+    const bool vec8 = aligned(w, 32) && ldw % 8 == 0, vec4 = aligned16(w) && ldw % 4 == 0;
+    (vec8 ? dequantize_q4_kernel<8> : vec4 ? dequantize_q4_kernel<4> : dequantize_q4_kernel<0>)<<<(unsigned)grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const uint32_t*>(packed), static_cast<const __nv_bfloat16*>(scales), (int)units, k, divisor(blocks_of(k)), shift_of(group),
         (k + group - 1) / group, w, ldw);
     TIE_OP_CU(cudaGetLastError());
     ++op_launches;
@@ -293,20 +483,26 @@ extern "C" model_status tie_matvec_q4(const float* x, long long ldx, int rows, c
     if (!aligned(x, 4) || !aligned(y, 4) || !aligned(bias, 4) || !aligned(residual, 4) || !aligned16(packed) ||
         !aligned(scales, 2))
         return MODEL_ERR_ARG;
-    if (k > kMostColumns || rows > 8 * 65535) return MODEL_ERR_CAPACITY;
+    if (k > kMostInputs || rows > 2 * 65535) return MODEL_ERR_CAPACITY;
     if (rows == 0) return MODEL_OK;
     OnDeviceOf dev(y);
     if (dev.status() != MODEL_OK) return dev.status();
+    const int strips = (n - 1) / 16 + 1, sms = sm_count(dev.device()), blocks = blocks_of(k);
+    const size_t sums = (size_t)kWarps * 2 * kSumBytes, most = 227 * 1024;
+    // two rows at a time also where 8 rows of x do not fit
+    const bool few = rows <= 2 || blocks * x_block_bytes<false>(group) > most;
+    const size_t x_bytes = few ? x_block_bytes<true>(group) : x_block_bytes<false>(group);
+    const int passes = (rows - 1) / (few ? 2 : 8) + 1;
     MatvecArgs a{x, ldx, rows, static_cast<const uint8_t*>(packed), static_cast<const __nv_bfloat16*>(scales), n, k,
-                 blocks_of(k), (k + group - 1) / group, bias, residual, ldr, gelu, y, ldy};
-    const int tiles = (n - 1) / 16 + 1, sms = sm_count(dev.device());
-    const int mt = tiles >= 8 * sms ? 4 : tiles >= 2 * sms ? 2 : 1;
+                 blocks, (k + group - 1) / group, strips, bias, residual, ldr, gelu, y, ldy};
     const bool vec = aligned16(x) && ldx % 4 == 0;
-    auto* kernel = rows <= 2 ? (vec ? matvec_of<true, true>(mt, group) : matvec_of<true, false>(mt, group))
-                             : (vec ? matvec_of<false, true>(mt, group) : matvec_of<false, false>(mt, group));
-    kernel<<<dim3((unsigned)((tiles - 1) / mt + 1), (unsigned)((rows - 1) / 8 + 1)), kThreads, 0,
-             static_cast<cudaStream_t>(stream)>>>(a);
-    TIE_OP_CU(cudaGetLastError());
+    auto* kernel = few ? (vec ? matvec_of<true, true>(group) : matvec_of<true, false>(group))
+                       : (vec ? matvec_of<false, true>(group) : matvec_of<false, false>(group));
+    // (always the most that any call wants: calls on other threads set it too)
+    TIE_OP_CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    const size_t smem = blocks * x_bytes > sums ? blocks * x_bytes : sums;
+    TIE_OP_CU(launch_pdl(kernel, dim3((unsigned)(strips < sms ? strips : sms), (unsigned)passes), dim3(32 * kWarps), smem,
+                         static_cast<cudaStream_t>(stream), a));
     ++op_launches;
     return MODEL_OK;
 }

@@ -63,18 +63,6 @@ struct Line {
     float* part_ml;                    // and of the one that it begins; (maximum, sum)
 };
 
-// n / d for 0 <= n < 2^31 (the multiplier is 2^(32 + shift) / d, rounded up, less 2^32)
-struct Divisor {
-    int d, shift;
-    unsigned mul;
-    __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi(mul, (unsigned)n) + (unsigned)n) >> shift); }
-};
-Divisor divisor(int d) {
-    int shift = 0;
-    while ((1LL << shift) < d) ++shift;
-    return Divisor{d, shift, (unsigned)(((1ULL << 32) * ((1ULL << shift) - (unsigned long long)d)) / (unsigned long long)d + 1)};
-}
-
 struct SharedArgs {
     const float* q;
     int ldq, n_head, group, n_kv_head;
@@ -616,12 +604,6 @@ __device__ __forceinline__ float joined(int d0, int d1, int d2) {
     const float high = __int_as_float(d2) - __int_as_float(kStart2);
     const float low = __int_as_float(d1) - (__int_as_float(kStart1) + __int_as_float(kStart0));
     return high + (low + __int_as_float(d0));
-}
-// the larger magnitude; NaN if either is
-__device__ __forceinline__ float max_abs(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
-    return r;
 }
 __device__ __forceinline__ float pow2_biased(int e) { return __uint_as_float((uint32_t)e << 23); }
 

@@ -12,8 +12,15 @@ namespace tie {
 constexpr uint32_t kNotFinite = 0x7f800000u;
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// the larger magnitude; NaN if either is
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
+}
+
 // 1 / s for level_of, 0 where s is so small that its reciprocal may be beyond fp32.
-__device__ __forceinline__ float reciprocal_of(float s) { return s < 0x1p-120f ? 0.f : __frcp_rn(s); }
+__device__ __forceinline__ float reciprocal_of(float s) { return s < 0x1p-100f ? 0.f : __frcp_rn(s); }
 
 // The level of x at scale s > 0: the integer nearest to the exact quotient, ties to even,
 // within +-most. The approximate quotient's nearest integer q is off by one at most; the
@@ -26,6 +33,69 @@ __device__ __forceinline__ int level_of(float x, float s, float inv, float most)
     if (r2 > s || (r2 == s && odd)) q += 1.f;
     if (r2 < -s || (r2 == -s && odd)) q -= 1.f;
     return (int)fminf(most, fmaxf(-most, q));
+}
+
+// Levels of N numbers as integers added to kLevelBase (the bits of 1.5 2^23): all of them that are
+// clearly nearest to one, which a product with 1 / s tells (its error is below 2^-15 of a level);
+// the others, about one of 20,000, by level_of.
+constexpr uint32_t kLevelBase = 0x4b400000u;
+template <int N>
+__device__ __forceinline__ void levels_of(const float (&x)[N], float s, float most, uint32_t (&level)[N]) {
+    const float inv = reciprocal_of(s), base = __uint_as_float(kLevelBase);
+    float far = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float t = x[i] * inv, y = t + base;
+        level[i] = __float_as_uint(y);
+        far = fmaxf(far, fabsf(t - (y - base)));
+    }
+    if (far > 0.49996f || inv == 0.f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) level[i] = kLevelBase + (uint32_t)level_of(x[i], s, inv, most);
+    }
+}
+
+// 8 fp32 side by side: 32-byte aligned (VEC 8), 16-byte aligned (4) or anywhere (0)
+template <int VEC>
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+    if constexpr (VEC == 8) {
+        asm volatile("ld.global.nc.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
+                     : "l"(p));
+    } else if constexpr (VEC == 4) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __ldg(p + i);
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+    if constexpr (VEC == 8) {
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]),
+                     "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+                     : "memory");
+    } else if constexpr (VEC == 4) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = x[i];
+    }
+}
+
+// n / d for 0 <= n < 2^31 (the multiplier is 2^(32 + shift) / d, rounded up, less 2^32)
+struct Divisor {
+    int d, shift;
+    unsigned mul;
+    __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi(mul, (unsigned)n) + (unsigned)n) >> shift); }
+};
+inline Divisor divisor(int d) {
+    int shift = 0;
+    while ((1LL << shift) < d) ++shift;
+    return Divisor{d, shift, (unsigned)(((1ULL << 32) * ((1ULL << shift) - (unsigned long long)d)) / (unsigned long long)d + 1)};
 }
 
 // An fp32 value is the sum of three bf16 terms, its 24 bits in pieces of 8: the term is
