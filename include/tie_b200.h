@@ -457,7 +457,8 @@ model_status tie_attention_shared(const float *q, int ldq, int n_head, const voi
                                   int max_new, int rows, const int32_t *prefix_table,
                                   int pages_per_prefix, const int32_t *prefix_lens,
                                   const int32_t *group_start, int n_group, float scale, float *out,
-                                  int ldo, void *workspace, size_t workspace_bytes, void *stream);
+                                  int ldo, void *workspace, size_t workspace_bytes,
+                                  int32_t *status, void *stream);
 
 /* ---- 4-bit weights --------------------------------------------------------
  * A weight matrix W of n rows (outputs) of k weights, cut along k into groups of

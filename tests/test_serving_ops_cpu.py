@@ -33,7 +33,7 @@ LOAD = dict(slots=P, rows=3, k_pages=P, v_pages=P, k_scales=P, v_scales=P, fmt=I
             stream=None)
 ATTN = dict(q=P, ldq=256, heads=4, k=P, v=P, k_scales=P, v_scales=P, fmt=INT8, n_pages=8, kv_heads=2, table=P, width=4,
             row_start=P, ctx=P, n_seq=2, max_new=3, rows=5, ptable=P, pwidth=3, plen=P, gstart=P, n_group=1, scale=0.125,
-            out=P, ldo=256, ws=P, ws_bytes=1 << 40, stream=None)
+            out=P, ldo=256, ws=P, ws_bytes=1 << 40, status=None, stream=None)
 MAKE = dict(w=P, ldw=100, n=7, k=100, group=64, packed=P, scales=P, stream=None)
 BACK = dict(packed=P, scales=P, n=7, k=100, group=64, w=P, ldw=100, stream=None)
 MATVEC = dict(x=P, ldx=100, rows=2, packed=P, scales=P, n=7, k=100, group=64, bias=P, residual=P, ldr=7, gelu=0, y=P, ldy=7,

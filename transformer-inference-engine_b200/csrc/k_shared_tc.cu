@@ -1,0 +1,585 @@
+// k_shared_tc.cu -- attention over a prefix that many rows share, on tcgen05: 128 rows of a
+// group (its new tokens times the query heads of a K/V head) against 64 keys a step.
+//
+// The numbers are those of ops_shared.cu: Q, scaled, the weights P and, over fp32 pages, K and
+// V are sums of three bf16 terms, exactly; levels of 8 bits and bf16 numbers are one. S = Q K^T
+// and the step's O = P V are sums of the terms' products (six for fp32, three for the others),
+// the small ones first, since the MMA cuts its sums off. Each step's O starts at zero and is
+// added, in fp32 registers, to what a row has: O = O 2^(m_before - m) + step's.
+//
+// A CTA has all roles, one step after another, and half of an SM: two CTAs fill each
+// other's waits, so no role needs a second buffer. 16 warps:
+//   0-7   softmax: two threads per row, 32 keys and 32 dims each. Read S from TMEM twice
+//         (maximum; weights), write P, three terms of two bf16 a column, into TMEM, and keep
+//         the row's O.
+//   8-11  loaders: a page of 16 keys each; K and V as terms into 128-byte-swizzled rows
+//         (K K-major; V as it lies, MN-major). The next step's rows are in registers by then.
+//   12    allocates TMEM and issues the MMAs. 13-15 only complete the warpgroup.
+// TMEM (256 columns): P 96, S 64, O 64. Shared memory: Q 48 KB, K and V 8 KB a term each.
+// What a step waits for: K stored -> S -> P written -> O. S's completion also says that the step
+// before has read its V (the MMAs complete in order), so four barriers do.
+//
+// Every wait is bounded (2 s): on expiry it raises the abort flag, which ends every other wait;
+// the roles run out without storing, the MMAs issued are drained and TMEM is freed.
+#include <cuda.h>
+
+#include <cuda_bf16.h>
+
+#include "shared_attn.cuh"
+
+namespace tie {
+namespace {
+
+#include "tc_ptx.cuh"
+
+constexpr int kThreads = 512, kSoftmaxWarps = 8, kLoadWarps = 4, kMmaWarp = 12;
+constexpr unsigned kAll = 0xffffffffu;
+constexpr uint32_t kWaitLimitNs = 2000000000u;
+constexpr int kKeys = kTcPages * kPageRows;            // of a step
+// registers a thread: at launch, and as the warpgroups share them out (fp32 rows take the
+// loaders more)
+constexpr int kRegsLaunch = 64, kRegsMma = 32;
+template <int FMT>
+constexpr int kRegsSoftmax = FMT == TIE_KV_F32 ? 72 : 80;
+template <int FMT>
+constexpr int kRegsLoad = FMT == TIE_KV_F32 ? 80 : 64;
+template <int FMT>
+constexpr bool kRegsFit = 128 * (2 * kRegsSoftmax<FMT> + kRegsLoad<FMT> + kRegsMma) <= kThreads * kRegsLaunch;
+static_assert(kRegsFit<TIE_KV_F32> && kRegsFit<TIE_KV_BF16>, "register split");
+
+constexpr uint32_t kQTerm = kTcRows * 128, kKvTerm = kKeys * 128;    // bytes of a term
+constexpr uint32_t kColP = 0, kColS = 96, kColO = 160, kTmemCols = 256;
+
+template <int FMT>
+struct Tc {
+    static constexpr int kTerms = FMT == TIE_KV_F32 ? 3 : 1;
+    static constexpr uint32_t kOffQ = 0, kOffK = 3 * kQTerm, kOffV = kOffK + kTerms * kKvTerm;
+    static constexpr uint32_t kOffScales = kOffV + kTerms * kKvTerm;     // [step % 2][key, value][64]
+    static constexpr uint32_t kOffThere = kOffScales + 4 * kKeys * 4;    // [step % 2][page]: its positions
+    static constexpr uint32_t kOffTop = kOffThere + 2 * kTcPages * 4;     // [step % 2][half][row]: maxima, at the end sums
+    static constexpr uint32_t kOffBars = kOffTop + 4 * kTcRows * 4;
+    static constexpr uint32_t kBytes = kOffBars + 64;
+};
+
+// kind::f16 with bf16 operands, fp32 accumulation, M = 128, N = 64
+constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (64u >> 3 << 17) | ((uint32_t)(kTcRows >> 4) << 24);
+constexpr uint32_t kIdescO = kIdesc | (1u << 16);      // B is MN-major
+
+// D += A . B, A in shared memory or in tensor memory; a whole, converged warp calls, one lane
+// issues (as in k_paged_tc.cu).
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, one;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, one;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void commit_elected(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred one;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t nanoseconds() {
+    uint32_t t;
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+    return t;
+}
+// 16 columns of the warp's 32 lanes read, 8 written
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    __syncwarp();
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
+// Bytes 0 and 2 of a word, as signed levels, in a pair of bf16: 0x4300 | u is 128 + u for
+// u < 128, and 0x4380 is 256, so (128 + low 7 bits) - (128 + sign bit) is the level.
+__device__ __forceinline__ uint32_t levels2(uint32_t w) {
+    const uint32_t low = (w & 0x007f007fu) | 0x43004300u, sign = (w & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&low), *reinterpret_cast<const __nv_bfloat162*>(&sign));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// 8 elements of a row of a page, as they lie
+template <int FMT>
+struct Row8 {
+    static constexpr int kWords = FMT == TIE_KV_F32 ? 8 : FMT == TIE_KV_BF16 ? 4 : 2;
+    uint32_t x[kWords];
+    __device__ __forceinline__ void load(const char* p) {
+        if constexpr (kWords == 8)
+            asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7])
+                         : "l"(p));
+        else if constexpr (kWords == 4)
+            asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                         : "l"(p));
+        else
+            asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "l"(p));
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) x[i] = 0u;
+    }
+    // its terms, 16 bytes each, `term` bytes apart
+    __device__ __forceinline__ void store(uint8_t* to, uint32_t term) const {
+        if constexpr (FMT == TIE_KV_F32) {
+            uint32_t t[4][3];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) split3(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]), t[i]);
+#pragma unroll
+            for (int e = 0; e < 3; ++e) *reinterpret_cast<uint4*>(to + e * term) = make_uint4(t[0][e], t[1][e], t[2][e], t[3][e]);
+        } else if constexpr (FMT == TIE_KV_BF16) {
+            *reinterpret_cast<uint4*>(to) = make_uint4(x[0], x[1], x[2], x[3]);
+        } else {
+            uint32_t y[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {          // bytes 0, 2 and 1, 3 as pairs, then in order
+                const uint32_t even = levels2(x[i]), odd = levels2(x[i] >> 8);
+                y[2 * i] = __byte_perm(even, odd, 0x5410);
+                y[2 * i + 1] = __byte_perm(even, odd, 0x7632);
+            }
+            *reinterpret_cast<uint4*>(to) = make_uint4(y[0], y[1], y[2], y[3]);
+        }
+    }
+};
+
+// A part of an item, as every role finds it for itself.
+struct Job {
+    int row0, rows, i0, head, keys;    // the unit's first row and its rows, the item's first of them, K/V head, positions
+    int b0, b1;                        // steps
+    int whole, parts;                  // whole: no stretch cuts it; parts: how many the item has, if this is the first
+    const int32_t* table;
+};
+
+template <int FMT>
+__global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_constant__ SharedArgs a) {
+    using T = Tc<FMT>;
+    constexpr int kTerms = T::kTerms;
+    // (what comes before the call is done before the kernel after this one may begin)
+    pdl_wait();
+    pdl_trigger();
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* s_scales = reinterpret_cast<float*>(smem + T::kOffScales);
+    int* s_there = reinterpret_cast<int*>(smem + T::kOffThere);
+    float* s_top = reinterpret_cast<float*>(smem + T::kOffTop);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + T::kOffBars);
+    uint64_t* q_full = bars;             // an item's Q written (loader warps)
+    uint64_t* k_full = bars + 1;         // a step's keys written (loader warps)
+    uint64_t* v_full = bars + 2;         // a step's values written (loader warps)
+    uint64_t* s_full = bars + 3;         // a step's S computed, and all MMAs before it (commit); its scales and
+                                         // what is there of it written (loader warps)
+    uint64_t* p_full = bars + 4;         // a step's P written, the O before it read (softmax warps)
+    uint64_t* o_last = bars + 5;         // an item's last O computed (commit)
+    uint64_t* drained = bars + 6;        // every MMA done (commit)
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile int s_abort;
+    __shared__ ScheduleScratch<kThreads> scratch;
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const Line& line = a.line[0];
+
+    if (t == 0) {
+        mbar_init(smem_u32(q_full), kLoadWarps);
+        mbar_init(smem_u32(k_full), kLoadWarps);
+        mbar_init(smem_u32(v_full), kLoadWarps);
+        mbar_init(smem_u32(s_full), 1 + kLoadWarps);
+        mbar_init(smem_u32(p_full), kSoftmaxWarps);
+        mbar_init(smem_u32(o_last), 1);
+        mbar_init(smem_u32(drained), 1);
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(&s_tmem)), "r"(kTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // (the line lies behind everything else: the roles walk it to the end)
+    const Plan plan = build_plan<kThreads>(a, line.u0, line.u1, smem + T::kBytes, &scratch, t);
+    const long long* const base = plan.base;
+    asm volatile("tcgen05.fence::before_thread_sync;");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    const uint32_t tmem = s_tmem;
+    const int n_units = line.u1 - line.u0, me = blockIdx.x;
+    const long long total = base[n_units], share = share_of(line, total);
+    long long x = me * share;
+    const long long end = min(x + share, total);
+    int u = x < end ? owner_of<long long>(base, n_units, x) : 0;
+    // the next part of this CTA's stretch that has steps
+    auto find = [&](Job& job) -> bool {
+        while (x < end) {
+            while (base[u + 1] <= x) ++u;          // (units without rows have no places)
+            const UnitShape s = unit_shape(a, plan.n, line.u0 + u);
+            const int places = unit_places(s, line);
+            const long long in = x - base[u], item = quotient(in, places);
+            const int off = (int)(in - item * places);
+            const int stop = (int)min((long long)places, off + (end - x));
+            const long long first = x - off;       // the item's first place
+            x += stop - off;
+            if (stop - 1 <= max(off - 1, 0)) continue;
+            const int tile = (int)quotient(item, line.heads);
+            job.row0 = s.row0;
+            job.rows = s.rows;
+            job.i0 = tile * kTcRows;
+            job.head = (int)item - tile * line.heads;
+            job.keys = s.keys;
+            job.b0 = max(off - 1, 0);
+            job.b1 = stop - 1;
+            job.table = a.ptable + (size_t)(line.u0 + u) * a.pwidth;
+            const bool begins = first + 1 >= me * share;
+            job.whole = begins && first + places <= (me + 1) * share;
+            job.parts = job.whole ? 1 : begins ? 1 + (int)quotient(first + places - 1 - me * share, share) : 0;
+            return true;
+        }
+        return false;
+    };
+    auto wait = [&](const uint64_t* bar, uint32_t parity) -> bool {
+        const uint32_t b = smem_u32(bar), t0 = nanoseconds();
+        for (uint32_t i = 1; !mbar_try_wait(b, parity); ++i)
+            if ((i & 255u) == 0 && (s_abort || nanoseconds() - t0 > kWaitLimitNs)) {
+                s_abort = 1;
+                return false;
+            }
+        return true;
+    };
+    auto wait_all = [&](const uint64_t* bar, uint32_t phase) -> bool { return __all_sync(kAll, wait(bar, phase & 1u)); };
+    auto arrive = [&](const uint64_t* bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(bar));
+    };
+    Job job;
+    uint32_t f = 0, un = 0;              // steps and items so far
+    bool ok = true;
+
+    if (warp < kSoftmaxWarps) {
+        // ------------------------------------------------------------ softmax
+        // (tcgen05.ld and .st are the warp's: so is every condition around them)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax<FMT>));
+        const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+        // both threads of the quarter's rows
+        auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory"); };
+        for (; ok && find(job); ++un) {
+            float m = -INFINITY, l = 0.f, alpha = 1.f, o[32];
+#pragma unroll
+            for (int d = 0; d < 32; ++d) o[d] = 0.f;
+            // the step before has left its O: it is relative to that step's maximum
+            auto add_step = [&]() {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t y[16];
+                    tmem_ld16(lanes + kColO + 32u * half + 16u * h, y);
+#pragma unroll
+                    for (int d = 0; d < 16; ++d) o[16 * h + d] = fmaf(o[16 * h + d], alpha, __uint_as_float(y[d]));
+                }
+            };
+#pragma unroll 1
+            for (int b = job.b0; b < job.b1; ++b, ++f) {
+                if (!(ok = wait_all(s_full, f))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;");
+                const int* there = s_there + (f & 1u) * kTcPages + 2 * half;
+                const bool all = there[0] + there[1] == 2 * kPageRows;
+                const float4* ks = reinterpret_cast<const float4*>(s_scales + (f & 1u) * 2 * kKeys) + 8 * half;
+                const float4* vs = ks + kKeys / 4;
+                // page h (of this thread's two) of S as scores
+                auto scores = [&](int h, uint32_t (&y)[16]) {
+                    tmem_ld16(lanes + kColS + 32u * half + 16u * h, y);
+                    if constexpr (FMT == TIE_KV_INT8) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float4 z = ks[4 * h + i];
+                            y[4 * i] = __float_as_uint(__uint_as_float(y[4 * i]) * z.x);
+                            y[4 * i + 1] = __float_as_uint(__uint_as_float(y[4 * i + 1]) * z.y);
+                            y[4 * i + 2] = __float_as_uint(__uint_as_float(y[4 * i + 2]) * z.z);
+                            y[4 * i + 3] = __float_as_uint(__uint_as_float(y[4 * i + 3]) * z.w);
+                        }
+                    }
+                    if (!all) {
+                        const int n = there[h];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (i >= n) y[i] = 0xff800000u;
+                    }
+                };
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t y[16];
+                    scores(h, y);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, __uint_as_float(y[i]));
+                }
+                float* const tops = s_top + (f & 1u) * 2 * kTcRows;
+                tops[half * kTcRows + r] = top;
+                if (b > job.b0) add_step();
+                meet();
+                top = fmaxf(top, tops[(half ^ 1) * kTcRows + r]);
+                const float m_new = fmaxf(m, top), from = m_new == -INFINITY ? 0.f : m_new;
+                alpha = ex2_ftz(m - from);
+                m = m_new;
+                l *= alpha;
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t y[16];
+                    scores(h, y);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float w = kWeight * ex2_ftz(__uint_as_float(y[i]) - from);
+                        l += w;
+                        y[i] = __float_as_uint(w);
+                    }
+                    if constexpr (FMT == TIE_KV_INT8) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float4 z = vs[4 * h + i];
+                            y[4 * i] = __float_as_uint(__uint_as_float(y[4 * i]) * z.x);
+                            y[4 * i + 1] = __float_as_uint(__uint_as_float(y[4 * i + 1]) * z.y);
+                            y[4 * i + 2] = __float_as_uint(__uint_as_float(y[4 * i + 2]) * z.z);
+                            y[4 * i + 3] = __float_as_uint(__uint_as_float(y[4 * i + 3]) * z.w);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) {
+                        uint32_t p[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            p[i] = __byte_perm(y[2 * i], y[2 * i + 1], 0x7632);
+                            if (e < 2) {
+                                y[2 * i] = __float_as_uint(rest(__uint_as_float(y[2 * i])));
+                                y[2 * i + 1] = __float_as_uint(rest(__uint_as_float(y[2 * i + 1])));
+                            }
+                        }
+                        tmem_st8(lanes + kColP + 32u * e + 16u * half + 8u * h, p);
+                    }
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;");
+                arrive(p_full);
+            }
+            if (!ok || !(ok = wait_all(o_last, un))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            add_step();
+            // (the next item's first P, which lets its O begin, is written after this; the last
+            // step's maxima have been read, and the ones of the step before, whose place this is)
+            float* const sums = s_top + (f & 1u) * 2 * kTcRows;
+            sums[half * kTcRows + r] = l;
+            meet();
+            l += sums[(half ^ 1) * kTcRows + r];
+            meet();
+            const int i = job.i0 + r;
+            if (i < job.rows) {
+                const size_t slot = (2 * (size_t)me + (job.parts > 0)) * kTcRows + r;
+                const int tok = a.by_group(i), h = job.head * a.group + i - tok * a.group;
+                const size_t place = (size_t)(job.row0 + tok) * a.n_head + h;
+                float* to = (job.whole ? a.whole_o[0] + place * kHeadDim : line.part_o + slot * kHeadDim) + 32 * half;
+                if (half == 0) {
+                    if (job.parts) a.place[0][place] = make_int2(job.whole ? -1 : (int)slot, job.parts);
+                    *reinterpret_cast<float2*>(job.whole ? a.whole_ml[0] + 2 * place : line.part_ml + 2 * slot) = make_float2(m, l);
+                }
+#pragma unroll
+                for (int d = 0; d < 8; ++d)
+                    reinterpret_cast<float4*>(to)[d] = make_float4(o[4 * d], o[4 * d + 1], o[4 * d + 2], o[4 * d + 3]);
+            }
+            __syncwarp();
+        }
+    } else if (warp < kSoftmaxWarps + kLoadWarps) {
+        // ------------------------------------------------------------ loaders
+        // (.inc or .dec: more, or no fewer, than at launch)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsLoad<FMT>));
+        constexpr int kBytes = FMT == TIE_KV_F32 ? 4 : FMT == TIE_KV_BF16 ? 2 : 1;
+        const int lw = warp - kSoftmaxWarps, sub = lane >> 3, dl = lane & 7;
+        const size_t w = (size_t)a.n_kv_head * kHeadDim * kBytes;     // bytes of a row
+        Row8<FMT> k[4], v[4];
+        float ks = 0.f, vs = 0.f;
+        int page = 0, there = 0;             // of the step that is loaded: this warp's page, its positions
+        auto page_of = [&](int b) {
+            const int p = b * kTcPages + lw, left = job.keys - p * kPageRows;
+            const int e = left > 0 ? __ldg(job.table + p) : -1;
+            const bool mapped = e >= 0 && e < a.n_pages;
+            page = mapped ? e : 0;           // (what is not there is read from the pool's first page, and cleared)
+            there = mapped ? min(left, kPageRows) : 0;
+        };
+        auto row_at = [&](const void* pool, int i) {
+            return static_cast<const char*>(pool) + ((size_t)page * kPageRows + 4 * i + sub) * w + (size_t)job.head * kHeadDim * kBytes +
+                   8 * dl * kBytes;
+        };
+        auto load_k = [&]() {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) k[i].load(row_at(a.k, i));
+            if constexpr (FMT == TIE_KV_INT8) ks = __ldg(a.ks + ((size_t)page * a.n_kv_head + job.head) * kPageRows + (lane & 15));
+        };
+        auto load_v = [&]() {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i].load(row_at(a.v, i));
+            if constexpr (FMT == TIE_KV_INT8) vs = __ldg(a.vs + ((size_t)page * a.n_kv_head + job.head) * kPageRows + (lane & 15));
+        };
+        auto store = [&](uint8_t* to, Row8<FMT>(&rows)[4], int n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (4 * i + sub >= n) rows[i].zero();
+                const int row = lw * kPageRows + 4 * i + sub;
+                rows[i].store(to + row * 128 + ((dl ^ (row & 7)) << 4), kKvTerm);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        };
+        for (; ok && find(job); ++un) {
+            page_of(job.b0);
+            if constexpr (FMT != TIE_KV_F32) {
+                load_k();
+                load_v();
+            }
+            // Q: 32 rows a warp, four times four. (The last S of the item before has been waited for.)
+#pragma unroll 1
+            for (int i0 = 0; i0 < 8; i0 += 4) {
+                Row8<TIE_KV_F32> q[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = job.i0 + lw * 32 + 4 * (i0 + i) + sub;
+                    if (at < job.rows) {
+                        const int tok = a.by_group(at), h = job.head * a.group + at - tok * a.group;
+                        const float4* from = reinterpret_cast<const float4*>(a.q + (size_t)(job.row0 + tok) * a.ldq + h * kHeadDim + 8 * dl);
+                        const float4 y = __ldg(from), z = __ldg(from + 1);
+                        const float s[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+#pragma unroll
+                        for (int d = 0; d < 8; ++d) q[i].x[d] = __float_as_uint(s[d]);
+                    } else {
+                        q[i].zero();
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = lw * 32 + 4 * (i0 + i) + sub;
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) q[i].x[d] = __float_as_uint(__uint_as_float(q[i].x[d]) * a.scale2);
+                    q[i].store(smem + T::kOffQ + row * 128 + ((dl ^ (row & 7)) << 4), kQTerm);
+                }
+            }
+            if constexpr (FMT == TIE_KV_F32) {     // (in registers that Q has left)
+                load_k();
+                load_v();
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            arrive(q_full);
+#pragma unroll 1
+            for (int b = job.b0; b < job.b1; ++b, ++f) {
+                // (the step before's S has been waited for: K is free)
+                const int now = there;
+                store(smem + T::kOffK, k, now);
+                if constexpr (FMT == TIE_KV_INT8) {
+                    if (lane < kPageRows) {
+                        float* to = s_scales + (f & 1u) * 2 * kKeys + lw * kPageRows + lane;
+                        to[0] = lane < now ? ks : 0.f;
+                        to[kKeys] = lane < now ? vs : 0.f;
+                    }
+                }
+                if (lane == 0) s_there[(f & 1u) * kTcPages + lw] = now;
+                arrive(s_full);
+                if (lane == 0) mbar_arrive(smem_u32(k_full));
+                if (b + 1 < job.b1) {
+                    page_of(b + 1);
+                    load_k();
+                }
+                if (!(ok = wait_all(s_full, f))) break;      // K has been read, and the step before's V
+                store(smem + T::kOffV, v, now);
+                arrive(v_full);
+                if (b + 1 < job.b1) load_v();
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
+        if (warp == kMmaWarp) {
+            // ------------------------------------------------------------ MMA
+            const uint32_t sb = __shfl_sync(kAll, smem_u32(smem), 0), tm = __shfl_sync(kAll, tmem, 0);
+            // products of terms (of A, of B), the smallest first: two and zero, ...
+            constexpr int kProducts = kTerms == 3 ? 6 : 3;
+            constexpr uint32_t kA = kTerms == 3 ? 0x001102u : 0x012u;      // a digit each, the first lowest
+            constexpr uint32_t kB = kTerms == 3 ? 0x010120u : 0x000u;
+            for (; ok && find(job); ++un) {
+                if (!(ok = wait_all(q_full, un))) break;
+                const int steps = __shfl_sync(kAll, job.b1 - job.b0, 0);
+#pragma unroll 1
+                for (int b = 0; b < steps; ++b, ++f) {
+                    if (!(ok = wait_all(k_full, f))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+#pragma unroll 1
+                    for (int z = 0; z < kProducts; ++z) {
+                        const uint32_t q = sb + T::kOffQ + (kA >> (4 * z) & 15u) * kQTerm;
+                        const uint32_t k = sb + T::kOffK + (kB >> (4 * z) & 15u) * kKvTerm;
+#pragma unroll
+                        for (int s = 0; s < 4; ++s)
+                            mma_ss(tm + kColS, sw128_desc(q + 32u * s), sw128_desc(k + 32u * s), kIdesc, z || s ? 1u : 0u);
+                    }
+                    commit_elected(smem_u32(s_full));
+                    if (!(ok = wait_all(p_full, f) && wait_all(v_full, f))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+#pragma unroll 1
+                    for (int z = 0; z < kProducts; ++z) {
+                        const uint32_t p = tm + kColP + (kA >> (4 * z) & 15u) * 32u;
+                        const uint32_t v = sb + T::kOffV + (kB >> (4 * z) & 15u) * kKvTerm;
+#pragma unroll
+                        for (int s = 0; s < 4; ++s)
+                            mma_ts(tm + kColO, p + 8u * s, sw128_desc(v + 2048u * s), kIdescO, z || s ? 1u : 0u);
+                    }
+                    if (b + 1 == steps) commit_elected(smem_u32(o_last));
+                }
+            }
+            // every MMA issued completes before TMEM is freed, also when cut short
+            commit_elected(smem_u32(drained));
+            const uint32_t t0 = nanoseconds();
+            while (!mbar_try_wait(smem_u32(drained), 0))
+                if (nanoseconds() - t0 > kWaitLimitNs) {
+                    s_abort = 1;
+                    break;
+                }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    if (warp == kMmaWarp)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    if (t == 0 && s_abort && a.status) *a.status = MODEL_ERR_DEVICE;
+}
+
+}  // namespace
+
+int shared_tc_ctas(int sms) { return 2 * sms; }
+
+cudaError_t launch_shared_tc(const SharedArgs& a, int format, cudaStream_t st) {
+    auto* kernel = format == TIE_KV_INT8 ? shared_tc_kernel<TIE_KV_INT8>
+                                         : format == TIE_KV_BF16 ? shared_tc_kernel<TIE_KV_BF16> : shared_tc_kernel<TIE_KV_F32>;
+    const size_t fixed = 1024 + (format == TIE_KV_INT8 ? Tc<TIE_KV_INT8>::kBytes
+                                                       : format == TIE_KV_BF16 ? Tc<TIE_KV_BF16>::kBytes : Tc<TIE_KV_F32>::kBytes);
+    // (always the most that any call wants: calls on other threads set it too)
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)(fixed + plan_bytes(kOpsMaxSeqs, kOpsMaxSeqs, kOpsMaxSeqs)));
+    if (e != cudaSuccess) return e;
+    const size_t smem = fixed + plan_bytes(a.line[0].u1 - a.line[0].u0, a.n_seq, a.n_group);
+    return launch_pdl(kernel, dim3((unsigned)a.line[0].teams), dim3(kThreads), smem, st, a);
+}
+
+}  // namespace tie

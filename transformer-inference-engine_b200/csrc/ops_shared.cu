@@ -33,20 +33,13 @@
 #include <cmath>
 #include <type_traits>
 
-#include "paged_attn.cuh"
-#include "quant.cuh"
+#include "shared_attn.cuh"
 
 namespace tie {
 namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr unsigned kAll = 0xffffffffu;
-// Weights are 2^(s - max) times this, so that the sum of as many of them as there are
-// positions (2^30) times any finite value stays finite.
-constexpr float kWeight = 0x1p-30f;
-// fewest steps worth a warp's stretch
-constexpr int kMinShare = 2;
-
 // Pages of a step.
 template <int FMT, int NT>
 constexpr int kPages = FMT == TIE_KV_F32 ? 1 : FMT == TIE_KV_BF16 ? (NT > 1 ? 1 : 2) : 2;
@@ -54,113 +47,6 @@ constexpr int kPages = FMT == TIE_KV_F32 ? 1 : FMT == TIE_KV_BF16 ? (NT > 1 ? 1 
 // CTAs on an SM
 template <int FMT, int NT>
 constexpr int kCtas = NT <= 2 ? 3 : 2;
-
-// A line: units [u0, u1) (a unit below n_group is a group's prefix, the others are
-// sequences), cut into stretches for `teams` teams of warps.
-struct Line {
-    int u0, u1, nt, pages, teams;      // nt: of the items; pages: of a step
-    float* part_o;                     // [2 * warps][8 nt][64]: a warp's parts of the item it goes on with
-    float* part_ml;                    // and of the one that it begins; (maximum, sum)
-};
-
-struct SharedArgs {
-    const float* q;
-    int ldq, n_head, group, n_kv_head;
-    Divisor by_group;
-    const void *k, *v;
-    const float *ks, *vs;
-    int n_pages;
-    const int32_t* table;
-    int width;
-    const int32_t *row_start, *ctx;
-    int n_seq, max_new, rows;
-    const int32_t* ptable;
-    int pwidth;
-    const int32_t *plen, *gstart;
-    int n_group;
-    float scale2;                      // score scale * log2(e): the softmax runs in powers of two
-    float* out;
-    int ldo;
-    float* whole_o[2];                 // [prefix, own][row][head][64]: items that no stretch cuts
-    float* whole_ml[2];                // (only where rows have two sources)
-    int2* place[2];                    // [prefix, own][row][head]: the row of its first part in the line's parts,
-                                       // or -1: whole; how many parts
-    Line line[2];                      // of the prefixes and of the sequences; line[1] may be line[0]
-};
-
-// What a unit's rows are, and its keys. rows == 0: nothing to do.
-struct UnitShape {
-    int row0, tokens, rows, keys;      // keys: positions in its pages
-    int ctx;                           // own: row i sees positions <= ctx + i / group; prefix: all
-};
-
-__device__ __forceinline__ UnitShape unit_shape(const SharedArgs& a, int u) {
-    UnitShape s{};
-    if (u < a.n_group) {
-        const int s0 = __ldg(a.gstart + u), s1 = __ldg(a.gstart + u + 1), n = __ldg(a.plen + u);
-        if (s0 < 0 || s1 <= s0 || s1 > a.n_seq || n <= 0 || n > (long long)a.pwidth * kPageRows) return s;
-        const int r0 = __ldg(a.row_start + s0), r1 = __ldg(a.row_start + s1);
-        if (r0 < 0 || r1 <= r0 || r1 > a.rows) return s;
-        s.row0 = r0;
-        s.tokens = r1 - r0;
-        s.keys = n;
-        s.ctx = n;
-    } else {
-        const int q = u - a.n_group;
-        const int r0 = __ldg(a.row_start + q), r1 = __ldg(a.row_start + q + 1), c = __ldg(a.ctx + q);
-        if (r0 < 0 || r1 <= r0 || r1 > a.rows || r1 - r0 > a.max_new || c < 0) return s;
-        if ((long long)c + (r1 - r0) > (long long)a.width * kPageRows) return s;
-        s.row0 = r0;
-        s.tokens = r1 - r0;
-        s.keys = c + s.tokens;
-        s.ctx = c;
-    }
-    s.rows = s.tokens * a.group;
-    return s;
-}
-// places of one of its items, and its items
-__device__ __forceinline__ int unit_places(const UnitShape& s, const Line& l) {
-    const int step = l.pages * kPageRows;
-    return (s.keys - 1) / step + 2;
-}
-__device__ __forceinline__ long long unit_items(const UnitShape& s, const Line& l) { return (s.rows + 8 * l.nt - 1) / (8 * l.nt); }
-
-// x / y of numbers that are nearly always small (a division of 64 bits is a hundred instructions)
-__device__ __forceinline__ long long quotient(long long x, long long y) {
-    return ((x | y) >> 32) == 0 ? (long long)((unsigned)x / (unsigned)y) : x / y;
-}
-
-__device__ __forceinline__ long long share_of(const Line& l, long long total) {
-    const long long even = quotient(total + l.teams - 1, l.teams);
-    return even > kMinShare ? even : kMinShare;
-}
-
-// base[u - u0] places before unit u, all of them in base[u1 - u0]. Ends with a barrier.
-__device__ __forceinline__ void build_base(const SharedArgs& a, int u0, int u1, long long* base,
-                                           ScheduleScratch<kThreads>* sc, int t) {
-    const int n = u1 - u0, per = (n + kThreads - 1) / kThreads;
-    long long mine = 0, before;
-    for (int i = 0; i < per; ++i) {
-        const int u = u0 + t * per + i;
-        if (u >= u1) break;
-        const UnitShape s = unit_shape(a, u);
-        const Line& l = a.line[u >= a.n_group];
-        if (s.rows) mine += unit_items(s, l) * unit_places(s, l);
-    }
-    const long long total = scan_threads<kThreads>(mine, sc, t, &before);
-    for (int i = 0; i < per; ++i) {
-        const int u = u0 + t * per + i;
-        if (u >= u1) break;
-        base[u - u0] = before;
-        if (per > 1) {                 // a thread's only unit needs no second look
-            const UnitShape s = unit_shape(a, u);
-            const Line& l = a.line[u >= a.n_group];
-            if (s.rows) before += unit_items(s, l) * unit_places(s, l);
-        }
-    }
-    if (t == 0) base[n] = total;
-    __syncthreads();
-}
 
 // ------------------------------------------------------------------ operands --
 template <int WORDS>
@@ -186,15 +72,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
-}
-
-// Terms of two numbers: [0] the largest.
-__device__ __forceinline__ void split3(float lo, float hi, uint32_t (&x)[3]) {
-    x[0] = terms2(lo, hi);
-    lo = rest(lo);
-    hi = rest(hi);
-    x[1] = terms2(lo, hi);
-    x[2] = terms2(rest(lo), rest(hi));
 }
 
 // The MMA cuts its sums off, towards zero, so the products of the terms are added in two
@@ -741,7 +618,10 @@ template <int NT>
 constexpr int kQBytes = NT * 2 * 3 * 32 * (int)sizeof(uint4);
 
 template <int FMT, int NT>
-__global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const __grid_constant__ SharedArgs a, int which) {
+__global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const __grid_constant__ SharedArgs a, int which, int first) {
+    // (the call's first kernel waits for what comes before the call, and only then lets the next one
+    // begin, which does not wait for it)
+    if (first) pdl_wait();
     pdl_trigger();
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ ScheduleScratch<kThreads> scratch;
@@ -750,8 +630,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const 
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c = lane & 3;
     const Line& line = a.line[which];
     uint4* qs = reinterpret_cast<uint4*>(smem) + (size_t)warp * (kQBytes<NT> / sizeof(uint4));
-    long long* base = reinterpret_cast<long long*>(smem + kWarps * kQBytes<NT>);
-    build_base(a, line.u0, line.u1, base, &scratch, t);
+    const Plan plan = build_plan<kThreads>(a, line.u0, line.u1, smem + kWarps * kQBytes<NT>, &scratch, t);
+    const long long* const base = plan.base;
     const int n_units = line.u1 - line.u0;
     const long long total = base[n_units], share = share_of(line, total);
     const int me = blockIdx.x * kWarps + warp, team = me / a.n_kv_head;
@@ -762,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const 
     auto find = [&](Item* to) -> bool {
         while (x < end) {
             while (base[u + 1] <= x) ++u;          // (units without rows have no places)
-            const UnitShape s = unit_shape(a, line.u0 + u);
+            const UnitShape s = unit_shape(a, plan.n, line.u0 + u);
             const int places = unit_places(s, line);
             const long long in = x - base[u], item = quotient(in, places);
             const int off = (int)(in - item * places);
@@ -912,10 +792,10 @@ __global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const 
 // the teams that follow.
 struct Parts {
     const float *o[2], *ml[2];         // [prefix, own]: the part that is first
-    int n[2], per[2], heads;           // per: rows of a place
+    int n[2], per[2], apart[2];        // per: rows of a place; apart: warps or CTAs from part to part
     __device__ __forceinline__ void at(int k, const float** to, const float** ml_to) const {
         const int w = k < n[1], j = w ? k : k - n[1];
-        const size_t row = j == 0 ? 0 : ((size_t)2 * j * heads - 1) * per[w];
+        const size_t row = j == 0 ? 0 : ((size_t)2 * j * apart[w] - 1) * per[w];
         *to = o[w] + row * kHeadDim;
         *ml_to = ml[w] + 2 * row;
     }
@@ -926,7 +806,7 @@ struct RowSum {
     float m, l, x, y;
 };
 __device__ __forceinline__ void add_parts(RowSum& r, const Parts& z, int k0, int dk, int lane) {
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;
     const int n = z.n[0] + z.n[1];
     for (int k = k0; k < n; k += kAhead * dk) {
         float2 ml[kAhead], v[kAhead];
@@ -969,7 +849,8 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(const __grid_cons
     __shared__ int s_group;
     __shared__ RowSum s_sum[kWarps][32];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, q = blockIdx.x;
-    const UnitShape s = unit_shape(a, a.n_group + q);
+    const Lengths lengths{a.row_start, a.ctx, a.gstart, a.plen};
+    const UnitShape s = unit_shape(a, lengths, a.n_group + q);
     if (!s.rows) return;
     bool grouped = false;
     if (a.n_group) {
@@ -979,7 +860,7 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(const __grid_cons
             if (__ldg(a.gstart + u) <= q && q < __ldg(a.gstart + u + 1)) atomicMax(&s_group, u);
         __syncthreads();
         if (s_group >= 0) {
-            const UnitShape p = unit_shape(a, s_group);
+            const UnitShape p = unit_shape(a, lengths, s_group);
             grouped = p.rows && s.row0 >= p.row0 && s.row0 + s.tokens <= p.row0 + p.tokens;
         }
     }
@@ -990,7 +871,6 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(const __grid_cons
         const int row = s.row0 + (int)((unsigned)i / (unsigned)a.n_head), h = (int)((unsigned)i % (unsigned)a.n_head);
         const size_t at = (size_t)row * a.n_head + h;
         Parts z;
-        z.heads = a.n_kv_head;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             const bool there = w || grouped;
@@ -998,6 +878,7 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(const __grid_cons
             const Line& l = a.line[w];
             z.n[w] = where.y;
             z.per[w] = 8 * l.nt;
+            z.apart[w] = l.heads == 1 ? a.n_kv_head : 1;
             z.o[w] = where.x < 0 ? a.whole_o[w] + at * kHeadDim : l.part_o + (size_t)where.x * kHeadDim;
             z.ml[w] = where.x < 0 ? a.whole_ml[w] + 2 * at : l.part_ml + 2 * (size_t)where.x;
         }
@@ -1033,6 +914,11 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(const __grid_cons
 }
 
 // --------------------------------------------------------------- the entry ----
+// Rows of a group and K/V head, on average, from which its prefix goes to k_shared_tc.cu.
+#ifndef TCFROM
+#define TCFROM 64
+#endif
+constexpr int kTcFrom = TCFROM;
 int most_warps(int sms) { return sms * 16; }
 
 // floats of the workspace: parts of two lines, and the whole items of two sources
@@ -1040,7 +926,7 @@ size_t part_floats(int sms) { return (size_t)2 * most_warps(sms) * 32 * (kHeadDi
 // (and their places)
 size_t workspace_floats(int sms, long long pairs) { return 2 * part_floats(sms) + (size_t)2 * pairs * (kHeadDim + 2 + 2); }
 
-using Kernel = void (*)(SharedArgs, int);
+using Kernel = void (*)(SharedArgs, int, int);
 template <int FMT>
 Kernel kernel_of(int nt) {
     return nt == 1 ? shared_kernel<FMT, 1> : nt == 2 ? shared_kernel<FMT, 2> : shared_kernel<FMT, 4>;
@@ -1072,7 +958,8 @@ extern "C" model_status tie_attention_shared(const float* q, int ldq, int n_head
                                              const int32_t* row_start, const int32_t* ctx_lens, int n_seq, int max_new,
                                              int rows, const int32_t* prefix_table, int pages_per_prefix,
                                              const int32_t* prefix_lens, const int32_t* group_start, int n_group, float scale,
-                                             float* out, int ldo, void* workspace, size_t workspace_bytes, void* stream) {
+                                             float* out, int ldo, void* workspace, size_t workspace_bytes, int32_t* status,
+                                             void* stream) {
     if (!k_pages || !v_pages || !page_table || !row_start || !ctx_lens || !workspace) return MODEL_ERR_ARG;
     if (rows && (!q || !out)) return MODEL_ERR_ARG;           // arrays without rows have no address
     const bool q8 = kv_format == TIE_KV_INT8;
@@ -1104,7 +991,7 @@ extern "C" model_status tie_attention_shared(const float* q, int ldq, int n_head
     a.n_seq = n_seq; a.max_new = max_new; a.rows = rows;
     a.ptable = prefix_table; a.pwidth = pages_per_prefix; a.plen = prefix_lens; a.gstart = group_start; a.n_group = n_group;
     a.scale2 = (float)((double)scale * 1.4426950408889634);
-    a.out = out; a.ldo = ldo;
+    a.out = out; a.ldo = ldo; a.status = status;
     float* f = static_cast<float*>(workspace);
     for (int i = 0; i < 2; ++i) {
         a.line[i].part_o = f;
@@ -1120,8 +1007,10 @@ extern "C" model_status tie_attention_shared(const float* q, int ldq, int n_head
     // rows that share keys, at most of a sequence and on average of a group: the items' height
     auto height = [](long long most) { return most <= 8 ? 1 : most <= 16 ? 2 : 4; };
     const long long per_seq = (long long)max_new * a.group, per_group = n_group ? ((long long)rows * a.group - 1) / n_group + 1 : 0;
+    // (prefixes of many rows: tensor cores of their own)
+    const bool tc = per_group >= kTcFrom;
     const int nt[2] = {n_group ? height(per_group) : 0, height(per_seq)};
-    const bool one_line = n_group && nt[0] == nt[1];
+    const bool one_line = n_group && !tc && nt[0] == nt[1];
     int ctas[2];
     for (int i = 0; i < 2; ++i) {
         Line& l = a.line[i];
@@ -1131,28 +1020,38 @@ extern "C" model_status tie_attention_shared(const float* q, int ldq, int n_head
         l.u0 = i ? n_group : 0;
         l.u1 = i ? n_group + n_seq : n_group;
         l.teams = ctas[i] * kWarps / n_kv_head;
+        l.heads = 1;
         if (l.teams == 0) return MODEL_ERR_CAPACITY;          // (the K/V heads that are taken fit the GPU's warps)
+    }
+    if (tc) {
+        a.line[0].nt = kTcRows / 8;
+        a.line[0].pages = kTcPages;
+        a.line[0].heads = n_kv_head;
+        a.line[0].teams = shared_tc_ctas(sms);
     }
     if (one_line) {
         a.line[0].u1 = n_group + n_seq;
         a.line[1] = a.line[0];
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const size_t most_units = (size_t)2 * kOpsMaxSeqs + 1;
     bool first = true;
     for (int i = 0; i < 2; ++i) {
         const Line& l = a.line[i];
         if (l.u1 == l.u0 || (i == 1 && one_line)) continue;
+        if (i == 0 && tc) {
+            TIE_OP_CU(launch_shared_tc(a, kv_format, st));
+            ++op_launches;
+            first = false;
+            continue;
+        }
         Kernel kernel = q8 ? kernel_of<TIE_KV_INT8>(l.nt) : kv_format == TIE_KV_BF16 ? kernel_of<TIE_KV_BF16>(l.nt) : kernel_of<TIE_KV_F32>(l.nt);
         const size_t q_bytes = (size_t)kWarps * (l.nt == 1 ? kQBytes<1> : l.nt == 2 ? kQBytes<2> : kQBytes<4>);
-        const size_t smem = q_bytes + (size_t)(l.u1 - l.u0 + 1) * sizeof(long long);
+        const size_t smem = q_bytes + plan_bytes(l.u1 - l.u0, n_seq, n_group);
         // (always the most that any call wants: calls on other threads set it too)
         if (smem > 32 * 1024)
             TIE_OP_CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           (int)(q_bytes + most_units * sizeof(long long))));
-        const dim3 grid((unsigned)ctas[i]);
-        if (first) kernel<<<grid, kThreads, smem, st>>>(a, i);
-        else TIE_OP_CU(launch_pdl(kernel, grid, dim3(kThreads), smem, st, a, i));
+                                           (int)(q_bytes + plan_bytes(2 * kOpsMaxSeqs, kOpsMaxSeqs, kOpsMaxSeqs))));
+        TIE_OP_CU(launch_pdl(kernel, dim3((unsigned)ctas[i]), dim3(kThreads), smem, st, a, i, (int)first));
         TIE_OP_CU(cudaGetLastError());
         ++op_launches;
         first = false;

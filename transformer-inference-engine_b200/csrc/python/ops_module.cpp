@@ -388,9 +388,9 @@ PyObject* kv_load(PyObject*, PyObject* const* v, Py_ssize_t n) {
 }
 
 // q, k_pages, v_pages, page_table, row_start, ctx_lens, max_new, out, workspace, k_scales, v_scales,
-// prefix_table, prefix_lens, group_start, scale, stream
+// prefix_table, prefix_lens, group_start, scale, status, stream
 PyObject* attention_shared(PyObject*, PyObject* const* v, Py_ssize_t n) {
-    return guarded(n, 16, [&] {
+    return guarded(n, 17, [&] {
         const Pool pool(v[1], v[2], true);
         const Scales sc(pool, v[9], v[10]);
         const int d = pool.device;
@@ -419,11 +419,13 @@ PyObject* attention_shared(PyObject*, PyObject* const* v, Py_ssize_t n) {
         }
         const double scale = PyFloat_AsDouble(v[14]);
         if (scale == -1.0 && PyErr_Occurred()) throw Refused{};
-        void* st = stream_of(v[15], d);
+        int32_t* status = ints_or_none("status", v[15], 1, d);
+        void* st = stream_of(v[16], d);
         return unlocked([&] {
             return attention_shared_fn(q.p, q.ld, (int)(w / kHeadDim), pool.k, pool.v, sc.k, sc.v, pool.format, pool.n_pages,
                                        pool.heads, table.p, table.width, start, ctx, table.n_seq, max_new, (int)q.rows, prefix,
-                                       prefix_width, lens, groups, n_group, (float)scale, out.p, out.ld, ws.p, ws.bytes, st);
+                                       prefix_width, lens, groups, n_group, (float)scale, out.p, out.ld, ws.p, ws.bytes, status,
+                                       st);
         });
     });
 }

@@ -153,7 +153,7 @@ def library():
         "tie_attention_shared_workspace": (C.c_size_t, [C.c_int, C.c_int]),
         "tie_attention_shared": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp,
                                            C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp,
-                                           C.c_int, C.c_float, _vp, C.c_int, _vp, C.c_size_t, _vp]),
+                                           C.c_int, C.c_float, _vp, C.c_int, _vp, C.c_size_t, _vp, _vp]),
         "tie_q4_bytes": (C.c_size_t, [C.c_int, C.c_int]),
         "tie_quantize_q4": (C.c_int, [_vp, C.c_longlong, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp]),
         "tie_dequantize_q4": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, _vp, C.c_longlong, _vp]),

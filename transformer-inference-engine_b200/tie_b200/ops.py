@@ -121,14 +121,14 @@ def attention_shared_workspace(rows, n_head):
 
 
 def attention_shared(q, k_pages, v_pages, page_table, row_start, ctx_lens, max_new, out, workspace, k_scales=None,
-                     v_scales=None, prefix_table=None, prefix_lens=None, group_start=None, scale=None, stream=None):
+                     v_scales=None, prefix_table=None, prefix_lens=None, group_start=None, scale=None, status=None, stream=None):
     """Attention of the new rows q over their sequences' own pages and over the pages that groups of sequences
     share (tie_attention_shared). prefix_table: [n_group, pages_per_prefix]; prefix_lens: the positions that each
     group shares; group_start: the groups' first sequences, and the end of the last. All three, or none.
-    scale: 1 / sqrt(64) by default."""
+    scale: 1 / sqrt(64) by default. status: as for attention_paged."""
     rc = (_module or _ops()).attention_shared(q, k_pages, v_pages, page_table, row_start, ctx_lens, max_new, out, workspace,
                                               k_scales, v_scales, prefix_table, prefix_lens, group_start,
-                                              0.125 if scale is None else scale, stream)
+                                              0.125 if scale is None else scale, status, stream)
     if rc:
         raise ModelError(rc, "tie_attention_shared")
 
