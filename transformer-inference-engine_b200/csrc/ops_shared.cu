@@ -42,7 +42,7 @@ constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr unsigned kAll = 0xffffffffu;
 // Pages of a step.
 template <int FMT, int NT>
-constexpr int kPages = FMT == TIE_KV_F32 ? 1 : FMT == TIE_KV_BF16 ? (NT > 1 ? 1 : 2) : 2;
+constexpr int kPages = FMT == TIE_KV_F32 ? 1 : FMT == TIE_KV_BF16 ? (NT > 2 ? 1 : 2) : 2;
 
 // CTAs on an SM
 template <int FMT, int NT>
@@ -617,8 +617,10 @@ __device__ __forceinline__ void run_steps_q8(const SharedArgs& a, ItemAt it, Ite
 template <int NT>
 constexpr int kQBytes = NT * 2 * 3 * 32 * (int)sizeof(uint4);
 
-template <int FMT, int NT>
-__global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const __grid_constant__ SharedArgs a, int which, int first) {
+// Items of prefixes have 8 NP rows, those of sequences 8 NO; both stand in one line, so a decode
+// step's products with a prefix run beside the reading of its sequences' pages.
+template <int FMT, int NP, int NO>
+__global__ void __launch_bounds__(kThreads, kCtas<FMT, NP>) shared_kernel(const __grid_constant__ SharedArgs a, int first) {
     // (the call's first kernel waits for what comes before the call, and only then lets the next one
     // begin, which does not wait for it)
     if (first) pdl_wait();
@@ -626,11 +628,12 @@ __global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const 
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ ScheduleScratch<kThreads> scratch;
     __shared__ Item s_items[kWarps][2];
-    __shared__ float s_unit[kWarps][8 * NT];       // pages in 8 bits: run_steps_q8's q_unit
+    static_assert(NP >= NO && kPages<FMT, NP> == kPages<FMT, NO>, "one line");
+    __shared__ float s_unit[kWarps][8 * NP];       // pages in 8 bits: run_steps_q8's q_unit
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c = lane & 3;
-    const Line& line = a.line[which];
-    uint4* qs = reinterpret_cast<uint4*>(smem) + (size_t)warp * (kQBytes<NT> / sizeof(uint4));
-    const Plan plan = build_plan<kThreads>(a, line.u0, line.u1, smem + kWarps * kQBytes<NT>, &scratch, t);
+    const Line& line = a.line[1];
+    uint4* qs = reinterpret_cast<uint4*>(smem) + (size_t)warp * (kQBytes<NP> / sizeof(uint4));
+    const Plan plan = build_plan<kThreads>(a, line.u0, line.u1, smem + kWarps * kQBytes<NP>, &scratch, t);
     const long long* const base = plan.base;
     const int n_units = line.u1 - line.u0;
     const long long total = base[n_units], share = share_of(line, total);
@@ -643,6 +646,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const 
         while (x < end) {
             while (base[u + 1] <= x) ++u;          // (units without rows have no places)
             const UnitShape s = unit_shape(a, plan.n, line.u0 + u);
+            const bool own = line.u0 + u >= a.n_group;
             const int places = unit_places(s, line);
             const long long in = x - base[u], item = quotient(in, places);
             const int off = (int)(in - item * places);
@@ -654,11 +658,10 @@ __global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const 
             const bool begins = first + 1 >= team * share, whole = begins && first + places <= (team + 1) * share;
             __syncwarp();
             if (lane == 0) {
-                const bool own = line.u0 + u >= a.n_group;
                 to->own = own;
                 to->row0 = s.row0;
                 to->rows = s.rows;
-                to->i0 = (int)item * 8 * NT;
+                to->i0 = (int)item * 8 * (own ? NO : NP);
                 to->ctx = s.ctx;
                 to->keys = s.keys;
                 to->b0 = max(off - 1, 0);
@@ -674,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const 
     };
     const int head = me - team * a.n_kv_head;
     int at = 0;                        // which of the warp's two items is this one
-    StepLoads<FMT, kPages<FMT, NT>> in;
+    StepLoads<FMT, kPages<FMT, NP>> in;
     bool here = find(&s_items[warp][0]);
     if (here) {
         ItemAt it = &s_items[warp][0];
@@ -683,7 +686,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const 
         in.keys();
         in.values();
     }
-    while (here) {
+    auto process = [&](auto height) {
+        constexpr int NT = decltype(height)::value;
         ItemAt it = &s_items[warp][at];
         // Q, scaled, as B operands: column g, this lane's 16 dims
         __syncwarp();
@@ -748,7 +752,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const 
         else run_steps<FMT, NT>(a, it, next, in, reinterpret_cast<const uint2*>(qs), lane, st);
         // where the result goes: out, the rows' own place, or a part of this warp's
         const int whole = it->whole, parts = it->parts, own = it->own, end_row0 = it->row0, end_rows = it->rows, end_i0 = it->i0;
-        const size_t slot = (2 * (size_t)me + (parts > 0)) * (8 * NT);
+        const size_t slot = (2 * (size_t)me + (parts > 0)) * line.per;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -780,6 +784,10 @@ __global__ void __launch_bounds__(kThreads, kCtas<FMT, NT>) shared_kernel(const 
             }
         at ^= 1;
         here = more;
+    };
+    while (here) {
+        if (NP == NO || s_items[warp][at].own) process(std::integral_constant<int, NO>{});
+        else process(std::integral_constant<int, NP>{});
     }
     // (nothing above needs another kernel's results, but what waits for this kernel waits
     // for the one before it too)
@@ -877,7 +885,7 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(const __grid_cons
             const int2 where = there ? __ldcg(a.place[w] + at) : make_int2(0, 0);
             const Line& l = a.line[w];
             z.n[w] = where.y;
-            z.per[w] = 8 * l.nt;
+            z.per[w] = l.per;
             z.apart[w] = l.heads == 1 ? a.n_kv_head : 1;
             z.o[w] = where.x < 0 ? a.whole_o[w] + at * kHeadDim : l.part_o + (size_t)where.x * kHeadDim;
             z.ml[w] = where.x < 0 ? a.whole_ml[w] + 2 * at : l.part_ml + 2 * (size_t)where.x;
@@ -914,11 +922,18 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(const __grid_cons
 }
 
 // --------------------------------------------------------------- the entry ----
-// Rows of a group and K/V head, on average, from which its prefix goes to k_shared_tc.cu.
-#ifndef TCFROM
-#define TCFROM 64
-#endif
-constexpr int kTcFrom = TCFROM;
+// Prefixes go to k_shared_tc.cu from this many rows of a group and K/V head, on average, and this
+// many scores (as the tables' width bounds them): its tiles have 128 rows, and it is a kernel
+// more, which nothing else runs beside. One group, 8 heads, a token each, without and with
+// it, us (fp32; bf16; 8 bits):
+//   128 sequences behind  700 (0.7 M scores)  22 and 24;  19 and 21;  17 and 22
+//    64 sequences behind 4000 (2.0 M)         32 and 32;  24 and 27;  22 and 27
+//   128 sequences behind 4000 (4.1 M)         46 and 36;  33 and 31;  29 and 31
+//   256 sequences behind 4000 (8.2 M)         75 and 55;  53 and 46;  48 and 47
+// (256 sequences behind 700, 12 heads, with 300 positions of their own, fp32, 2.2 M: 75 and 92; 640
+// rows a head behind 14336, 8 heads, bf16, 73 M: 271 and 135.)
+constexpr int kTcFrom = 64;
+constexpr long long tc_scores(int format) { return format == TIE_KV_F32 ? 3000000 : format == TIE_KV_BF16 ? 4000000 : 8000000; }
 int most_warps(int sms) { return sms * 16; }
 
 // floats of the workspace: parts of two lines, and the whole items of two sources
@@ -926,18 +941,20 @@ size_t part_floats(int sms) { return (size_t)2 * most_warps(sms) * 32 * (kHeadDi
 // (and their places)
 size_t workspace_floats(int sms, long long pairs) { return 2 * part_floats(sms) + (size_t)2 * pairs * (kHeadDim + 2 + 2); }
 
-using Kernel = void (*)(SharedArgs, int, int);
-template <int FMT>
-Kernel kernel_of(int nt) {
-    return nt == 1 ? shared_kernel<FMT, 1> : nt == 2 ? shared_kernel<FMT, 2> : shared_kernel<FMT, 4>;
+using Kernel = void (*)(SharedArgs, int);
+// What is launched for items of 8 np and 8 no rows: 1 1, 2 1, 2 2 or 4 4.
+struct Variant {
+    Kernel kernel;
+    int pages, ctas;                   // of a step; on an SM
+    size_t q_bytes;
+};
+template <int FMT, int NP, int NO>
+Variant variant() {
+    return Variant{shared_kernel<FMT, NP, NO>, kPages<FMT, NP>, kCtas<FMT, NP>, (size_t)kWarps * kQBytes<NP>};
 }
 template <int FMT>
-int ctas_of(int nt) {
-    return nt == 1 ? kCtas<FMT, 1> : nt == 2 ? kCtas<FMT, 2> : kCtas<FMT, 4>;
-}
-template <int FMT>
-int pages_of(int nt) {
-    return nt == 1 ? kPages<FMT, 1> : nt == 2 ? kPages<FMT, 2> : kPages<FMT, 4>;
+Variant variant_of(int np, int no) {
+    return np == 1 ? variant<FMT, 1, 1>() : np == 4 ? variant<FMT, 4, 4>() : no == 1 ? variant<FMT, 2, 1>() : variant<FMT, 2, 2>();
 }
 
 }  // namespace
@@ -1004,57 +1021,49 @@ extern "C" model_status tie_attention_shared(const float* q, int ldq, int n_head
         a.whole_ml[i] = f + 2 * pairs * kHeadDim + i * pairs * 2;
         a.place[i] = reinterpret_cast<int2*>(f + 2 * pairs * (kHeadDim + 2) + i * pairs * 2);
     }
-    // rows that share keys, at most of a sequence and on average of a group: the items' height
-    auto height = [](long long most) { return most <= 8 ? 1 : most <= 16 ? 2 : 4; };
+    // Rows that share keys, at most of a sequence and on average of a group, say how high the items are.
     const long long per_seq = (long long)max_new * a.group, per_group = n_group ? ((long long)rows * a.group - 1) / n_group + 1 : 0;
-    // (prefixes of many rows: tensor cores of their own)
-    const bool tc = per_group >= kTcFrom;
-    const int nt[2] = {n_group ? height(per_group) : 0, height(per_seq)};
-    const bool one_line = n_group && !tc && nt[0] == nt[1];
-    int ctas[2];
+    const bool tc = per_group >= kTcFrom && pairs * ((long long)pages_per_prefix * kPageRows) >= tc_scores(kv_format);
+    const int no = per_seq <= 8 ? 1 : per_seq <= 16 ? 2 : 4;
+    const int np = tc || no > 1 || per_group <= 8 ? no : 2;
+    const Variant v = q8 ? variant_of<TIE_KV_INT8>(np, no)
+                         : kv_format == TIE_KV_BF16 ? variant_of<TIE_KV_BF16>(np, no) : variant_of<TIE_KV_F32>(np, no);
     for (int i = 0; i < 2; ++i) {
         Line& l = a.line[i];
-        l.nt = nt[i] ? nt[i] : nt[1];
-        l.pages = q8 ? pages_of<TIE_KV_INT8>(l.nt) : kv_format == TIE_KV_BF16 ? pages_of<TIE_KV_BF16>(l.nt) : pages_of<TIE_KV_F32>(l.nt);
-        ctas[i] = sms * (q8 ? ctas_of<TIE_KV_INT8>(l.nt) : kv_format == TIE_KV_BF16 ? ctas_of<TIE_KV_BF16>(l.nt) : ctas_of<TIE_KV_F32>(l.nt));
-        l.u0 = i ? n_group : 0;
-        l.u1 = i ? n_group + n_seq : n_group;
-        l.teams = ctas[i] * kWarps / n_kv_head;
+        l.nt = i ? no : np;
+        l.per = 8 * np;
+        l.pages = v.pages;
         l.heads = 1;
+        l.u0 = 0;
+        l.u1 = n_group + n_seq;
+        l.teams = sms * v.ctas * kWarps / n_kv_head;
         if (l.teams == 0) return MODEL_ERR_CAPACITY;          // (the K/V heads that are taken fit the GPU's warps)
     }
-    if (tc) {
-        a.line[0].nt = kTcRows / 8;
-        a.line[0].pages = kTcPages;
-        a.line[0].heads = n_kv_head;
-        a.line[0].teams = shared_tc_ctas(sms);
-    }
-    if (one_line) {
-        a.line[0].u1 = n_group + n_seq;
-        a.line[1] = a.line[0];
-    }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    bool first = true;
-    for (int i = 0; i < 2; ++i) {
-        const Line& l = a.line[i];
-        if (l.u1 == l.u0 || (i == 1 && one_line)) continue;
-        if (i == 0 && tc) {
-            TIE_OP_CU(launch_shared_tc(a, kv_format, st));
-            ++op_launches;
-            first = false;
-            continue;
-        }
-        Kernel kernel = q8 ? kernel_of<TIE_KV_INT8>(l.nt) : kv_format == TIE_KV_BF16 ? kernel_of<TIE_KV_BF16>(l.nt) : kernel_of<TIE_KV_F32>(l.nt);
-        const size_t q_bytes = (size_t)kWarps * (l.nt == 1 ? kQBytes<1> : l.nt == 2 ? kQBytes<2> : kQBytes<4>);
-        const size_t smem = q_bytes + plan_bytes(l.u1 - l.u0, n_seq, n_group);
+    if (tc) {
+        Line& l = a.line[0];
+        l.nt = kTcRows / 8;
+        l.per = kTcRows;
+        l.pages = kTcPages;
+        l.heads = n_kv_head;
+        l.u1 = n_group;
+        l.teams = shared_tc_ctas(sms);
+        a.line[1].u0 = n_group;
+        TIE_OP_CU(launch_shared_tc(a, kv_format, st));
+        ++op_launches;
+    } else {
+        a.line[1].part_o = a.line[0].part_o;                  // one line
+        a.line[1].part_ml = a.line[0].part_ml;
+    }
+    {
+        const Line& l = a.line[1];
+        const size_t smem = v.q_bytes + plan_bytes(l.u1 - l.u0, n_seq, n_group);
         // (always the most that any call wants: calls on other threads set it too)
         if (smem > 32 * 1024)
-            TIE_OP_CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           (int)(q_bytes + plan_bytes(2 * kOpsMaxSeqs, kOpsMaxSeqs, kOpsMaxSeqs))));
-        TIE_OP_CU(launch_pdl(kernel, dim3((unsigned)ctas[i]), dim3(kThreads), smem, st, a, i, (int)first));
-        TIE_OP_CU(cudaGetLastError());
+            TIE_OP_CU(cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)(v.q_bytes + plan_bytes(2 * kOpsMaxSeqs, kOpsMaxSeqs, kOpsMaxSeqs))));
+        TIE_OP_CU(launch_pdl(v.kernel, dim3((unsigned)(sms * v.ctas)), dim3(kThreads), smem, st, a, (int)!tc));
         ++op_launches;
-        first = false;
     }
     const long long most_pairs = (long long)max_new * n_head;         // of a sequence
     const bool wide = pairs <= 8LL * sms;

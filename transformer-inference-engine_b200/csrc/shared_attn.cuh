@@ -19,8 +19,8 @@ constexpr int kMinShare = 2;
 // CTAs, to which an item's K/V heads are items side by side (heads: as many).
 struct Line {
     int u0, u1, nt, pages, teams;      // nt: an item has 8 nt rows; pages: of a step
-    int heads;
-    float* part_o;                     // [2 * warps or CTAs][8 nt][64]: its parts of the item it goes on with
+    int heads, per;                    // per: rows of a part
+    float* part_o;                     // [2 * warps or CTAs][per][64]: its parts of the item it goes on with
     float* part_ml;                    // and of the one that it begins; (maximum, sum)
 };
 
@@ -46,7 +46,7 @@ struct SharedArgs {
     float* whole_ml[2];                // (only where rows have two sources)
     int2* place[2];                    // [prefix, own][row][head]: the row of its first part in the line's parts,
                                        // or -1: whole; how many parts
-    Line line[2];                      // of the prefixes and of the sequences; line[1] may be line[0]
+    Line line[2];                      // for prefixes and for sequences; one line, or one each
     int* status;
 };
 
