@@ -13,11 +13,19 @@
 //         (maximum; weights), write P, three terms of two bf16 a column, into TMEM, and keep
 //         the row's O.
 //   8-11  loaders: a page of 16 keys each; K and V as terms into 128-byte-swizzled rows
-//         (K K-major; V as it lies, MN-major). The next step's rows are in registers by then.
+//         (K K-major; V as it lies, MN-major). The next step's rows are in registers by then;
+//         bf16 rows need no conversion and are copied to three stages, two steps ahead.
 //   12    allocates TMEM and issues the MMAs. 13-15 only complete the warpgroup.
 // TMEM (256 columns): P 96, S 64, O 64. Shared memory: Q 48 KB, K and V 8 KB a term each.
 // What a step waits for: K stored -> S -> P written -> O. S's completion also says that the step
 // before has read its V (the MMAs complete in order), so four barriers do.
+//
+// Measured (B200, the whole call: this kernel, the sequences' own positions, the join): 64
+// answers x 1-4 tokens over bf16 pages, 14336 shared positions, 12 heads: 133 us (the same on
+// mma.sync 240). A wait that reads the timer at every try takes 13 us of a skeleton without
+// softmax (84 -> 71 us) and 1 us of the whole; the scores held in registers instead of read from
+// TMEM twice spill and take 139. What bounds it is the softmax warps' instructions, 60 us of
+// them by themselves, then the way round the barriers.
 //
 // Every wait is bounded (2 s): on expiry it raises the abort flag, which ends every other wait;
 // the roles run out without storing, the MMAs issued are drained and TMEM is freed.
@@ -45,7 +53,7 @@ template <int FMT>
 constexpr int kRegsLoad = FMT == TIE_KV_F32 ? 80 : 64;
 template <int FMT>
 constexpr bool kRegsFit = 128 * (2 * kRegsSoftmax<FMT> + kRegsLoad<FMT> + kRegsMma) <= kThreads * kRegsLaunch;
-static_assert(kRegsFit<TIE_KV_F32> && kRegsFit<TIE_KV_BF16>, "register split");
+static_assert(kRegsFit<TIE_KV_F32> && kRegsFit<TIE_KV_BF16> && kRegsFit<TIE_KV_INT8>, "register split");
 
 constexpr uint32_t kQTerm = kTcRows * 128, kKvTerm = kKeys * 128;    // bytes of a term
 constexpr uint32_t kColP = 0, kColS = 96, kColO = 160, kTmemCols = 256;
@@ -53,10 +61,13 @@ constexpr uint32_t kColP = 0, kColS = 96, kColO = 160, kTmemCols = 256;
 template <int FMT>
 struct Tc {
     static constexpr int kTerms = FMT == TIE_KV_F32 ? 3 : 1;
-    static constexpr uint32_t kOffQ = 0, kOffK = 3 * kQTerm, kOffV = kOffK + kTerms * kKvTerm;
-    static constexpr uint32_t kOffScales = kOffV + kTerms * kKvTerm;     // [step % 2][key, value][64]
-    static constexpr uint32_t kOffThere = kOffScales + 4 * kKeys * 4;    // [step % 2][page]: its positions
-    static constexpr uint32_t kOffTop = kOffThere + 2 * kTcPages * 4;     // [step % 2][half][row]: maxima, at the end sums
+    // bf16 rows go from memory straight to their places, two steps ahead
+    static constexpr int kStages = FMT == TIE_KV_BF16 ? 3 : 1;
+    static constexpr uint32_t kStage = 2 * kTerms * kKvTerm, kValues = kTerms * kKvTerm;    // bytes of a stage; to its values
+    static constexpr uint32_t kOffQ = 0, kOffKv = 3 * kQTerm;
+    static constexpr uint32_t kOffScales = kOffKv + kStages * kStage;    // [step % 2][key, value][64]
+    static constexpr uint32_t kOffThere = kOffScales + 4 * kKeys * 4;    // [step % 4][page]: its positions
+    static constexpr uint32_t kOffTop = kOffThere + 4 * kTcPages * 4;     // [step % 2][half][row]: maxima, at the end sums
     static constexpr uint32_t kOffBars = kOffTop + 4 * kTcRows * 4;
     static constexpr uint32_t kBytes = kOffBars + 64;
 };
@@ -258,12 +269,16 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         return false;
     };
     auto wait = [&](const uint64_t* bar, uint32_t parity) -> bool {
-        const uint32_t b = smem_u32(bar), t0 = nanoseconds();
-        for (uint32_t i = 1; !mbar_try_wait(b, parity); ++i)
-            if ((i & 255u) == 0 && (s_abort || nanoseconds() - t0 > kWaitLimitNs)) {
+        const uint32_t b = smem_u32(bar);
+        uint32_t t0 = 0;                 // (the timer is not looked at before a wait has become long)
+        for (uint32_t i = 1; !mbar_try_wait(b, parity); ++i) {
+            if ((i & 255u) != 0) continue;
+            if (i == 256) t0 = nanoseconds();
+            if (s_abort || nanoseconds() - t0 > kWaitLimitNs) {
                 s_abort = 1;
                 return false;
             }
+        }
         return true;
     };
     auto wait_all = [&](const uint64_t* bar, uint32_t phase) -> bool { return __all_sync(kAll, wait(bar, phase & 1u)); };
@@ -301,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
             for (int b = job.b0; b < job.b1; ++b, ++f) {
                 if (!(ok = wait_all(s_full, f))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;");
-                const int* there = s_there + (f & 1u) * kTcPages + 2 * half;
+                const int* there = s_there + (f & 3u) * kTcPages + 2 * half;
                 const bool all = there[0] + there[1] == 2 * kPageRows;
                 const float4* ks = reinterpret_cast<const float4*>(s_scales + (f & 1u) * 2 * kKeys) + 8 * half;
                 const float4* vs = ks + kKeys / 4;
@@ -413,9 +428,11 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         constexpr int kBytes = FMT == TIE_KV_F32 ? 4 : FMT == TIE_KV_BF16 ? 2 : 1;
         const int lw = warp - kSoftmaxWarps, sub = lane >> 3, dl = lane & 7;
         const size_t w = (size_t)a.n_kv_head * kHeadDim * kBytes;     // bytes of a row
+        constexpr bool kCopied = FMT == TIE_KV_BF16;
         Row8<FMT> k[4], v[4];
         float ks = 0.f, vs = 0.f;
         int page = 0, there = 0;             // of the step that is loaded: this warp's page, its positions
+        int now_at = 0;                      // the step that f counts
         auto page_of = [&](int b) {
             const int p = b * kTcPages + lw, left = job.keys - p * kPageRows;
             const int e = left > 0 ? __ldg(job.table + p) : -1;
@@ -447,8 +464,34 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
         for (; ok && find(job); ++un) {
-            page_of(job.b0);
-            if constexpr (FMT != TIE_KV_F32) {
+            uint32_t stage = f % T::kStages;             // of the step that is copied next
+            // a step's rows, and zeros for what is not there, to the next stage
+            auto copy = [&](int b) {
+                if (b < job.b1) {
+                    page_of(b);
+                    if (lane == 0) s_there[((f + (uint32_t)(b - now_at)) & 3u) * kTcPages + lw] = there;
+                    const uint32_t to = smem_u32(smem + T::kOffKv + stage * T::kStage);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = lw * kPageRows + 4 * i + sub;
+                        const uint32_t at = to + row * 128 + ((dl ^ (row & 7)) << 4);
+                        const int bytes = 4 * i + sub < there ? 16 : 0;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(row_at(a.k, i)), "r"(bytes) : "memory");
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + T::kValues), "l"(row_at(a.v, i)), "r"(bytes)
+                                     : "memory");
+                    }
+                    stage = stage + 1 == T::kStages ? 0 : stage + 1;
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            now_at = job.b0;
+            if constexpr (kCopied) {
+                copy(job.b0);
+                copy(job.b0 + 1);
+            } else {
+                page_of(job.b0);
+            }
+            if constexpr (FMT == TIE_KV_INT8) {
                 load_k();
                 load_v();
             }
@@ -484,29 +527,42 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             arrive(q_full);
+            if constexpr (kCopied) {
 #pragma unroll 1
-            for (int b = job.b0; b < job.b1; ++b, ++f) {
-                // (the step before's S has been waited for: K is free)
-                const int now = there;
-                store(smem + T::kOffK, k, now);
-                if constexpr (FMT == TIE_KV_INT8) {
-                    if (lane < kPageRows) {
-                        float* to = s_scales + (f & 1u) * 2 * kKeys + lw * kPageRows + lane;
-                        to[0] = lane < now ? ks : 0.f;
-                        to[kKeys] = lane < now ? vs : 0.f;
+                for (int b = job.b0; b < job.b1; ++b, ++f) {
+                    now_at = b;
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    arrive(s_full);
+                    if (lane == 0) mbar_arrive(smem_u32(k_full));
+                    if (!(ok = wait_all(s_full, f))) break;      // the step before has left its stage
+                    copy(b + 2);
+                }
+            } else {
+#pragma unroll 1
+                for (int b = job.b0; b < job.b1; ++b, ++f) {
+                    // (the step before's S has been waited for: K is free)
+                    const int now = there;
+                    store(smem + T::kOffKv, k, now);
+                    if constexpr (FMT == TIE_KV_INT8) {
+                        if (lane < kPageRows) {
+                            float* to = s_scales + (f & 1u) * 2 * kKeys + lw * kPageRows + lane;
+                            to[0] = lane < now ? ks : 0.f;
+                            to[kKeys] = lane < now ? vs : 0.f;
+                        }
                     }
+                    if (lane == 0) s_there[(f & 3u) * kTcPages + lw] = now;
+                    arrive(s_full);
+                    if (lane == 0) mbar_arrive(smem_u32(k_full));
+                    if (b + 1 < job.b1) {
+                        page_of(b + 1);
+                        load_k();
+                    }
+                    if (!(ok = wait_all(s_full, f))) break;      // K has been read, and the step before's V
+                    store(smem + T::kOffKv + T::kValues, v, now);
+                    arrive(v_full);
+                    if (b + 1 < job.b1) load_v();
                 }
-                if (lane == 0) s_there[(f & 1u) * kTcPages + lw] = now;
-                arrive(s_full);
-                if (lane == 0) mbar_arrive(smem_u32(k_full));
-                if (b + 1 < job.b1) {
-                    page_of(b + 1);
-                    load_k();
-                }
-                if (!(ok = wait_all(s_full, f))) break;      // K has been read, and the step before's V
-                store(smem + T::kOffV, v, now);
-                arrive(v_full);
-                if (b + 1 < job.b1) load_v();
             }
         }
     } else {
@@ -528,18 +584,19 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
 #pragma unroll 1
                     for (int z = 0; z < kProducts; ++z) {
                         const uint32_t q = sb + T::kOffQ + (kA >> (4 * z) & 15u) * kQTerm;
-                        const uint32_t k = sb + T::kOffK + (kB >> (4 * z) & 15u) * kKvTerm;
+                        const uint32_t k = sb + T::kOffKv + (f % T::kStages) * T::kStage + (kB >> (4 * z) & 15u) * kKvTerm;
 #pragma unroll
                         for (int s = 0; s < 4; ++s)
                             mma_ss(tm + kColS, sw128_desc(q + 32u * s), sw128_desc(k + 32u * s), kIdesc, z || s ? 1u : 0u);
                     }
                     commit_elected(smem_u32(s_full));
-                    if (!(ok = wait_all(p_full, f) && wait_all(v_full, f))) break;
+                    // (copied rows: k_full was for both)
+                    if (!(ok = wait_all(p_full, f) && (FMT == TIE_KV_BF16 || wait_all(v_full, f)))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;");
 #pragma unroll 1
                     for (int z = 0; z < kProducts; ++z) {
                         const uint32_t p = tm + kColP + (kA >> (4 * z) & 15u) * 32u;
-                        const uint32_t v = sb + T::kOffV + (kB >> (4 * z) & 15u) * kKvTerm;
+                        const uint32_t v = sb + T::kOffKv + (f % T::kStages) * T::kStage + T::kValues + (kB >> (4 * z) & 15u) * kKvTerm;
 #pragma unroll
                         for (int s = 0; s < 4; ++s)
                             mma_ts(tm + kColO, p + 8u * s, sw128_desc(v + 2048u * s), kIdescO, z || s ? 1u : 0u);
