@@ -7,25 +7,25 @@
 // the small ones first, since the MMA cuts its sums off. Each step's O starts at zero and is
 // added, in fp32 registers, to what a row has: O = O 2^(m_before - m) + step's.
 //
-// A CTA has all roles, one step after another, and half of an SM: two CTAs fill each
-// other's waits, so no role needs a second buffer. 16 warps:
-//   0-7   softmax: two threads per row, 32 keys and 32 dims each. Read S from TMEM twice
-//         (maximum; weights), write P, three terms of two bf16 a column, into TMEM, and keep
-//         the row's O.
-//   8-11  loaders: a page of 16 keys each; K and V as terms into 128-byte-swizzled rows
+// A CTA has all roles and half of an SM: two CTAs fill each other's waits. 12 warps:
+//   0-3   softmax: a thread per row. Read S from TMEM, add the step before's O to the row's, write
+//         P, three terms of two bf16 a column, into TMEM. With bf16 pages a step's 64 scores stay in
+//         registers and the next step's S is computed meanwhile; the other formats' loaders need
+//         those registers, and S is read twice (maximum; weights).
+//   4-7   loaders: a page of 16 keys each; K and V as terms into 128-byte-swizzled rows
 //         (K K-major; V as it lies, MN-major). The next step's rows are in registers by then;
 //         bf16 rows need no conversion and are copied to three stages, two steps ahead.
-//   12    allocates TMEM and issues the MMAs. 13-15 only complete the warpgroup.
+//   8     allocates TMEM and issues the MMAs. 9-11 only complete the warpgroup.
 // TMEM (256 columns): P 96, S 64, O 64. Shared memory: Q 48 KB, K and V 8 KB a term each.
-// What a step waits for: K stored -> S -> P written -> O. S's completion also says that the step
-// before has read its V (the MMAs complete in order), so four barriers do.
+// The MMAs complete in order. A warp arrives at no barrier for a step before that
+// barrier's phase of the step before has completed (loaders wait for S, softmax warps for O).
 //
 // Measured (B200, the whole call: this kernel, the sequences' own positions, the join): 64
-// answers x 1-4 tokens over bf16 pages, 14336 shared positions, 12 heads: 133 us (the same on
-// mma.sync 240). A wait that reads the timer at every try takes 13 us of a skeleton without
-// softmax (84 -> 71 us) and 1 us of the whole; the scores held in registers instead of read from
-// TMEM twice spill and take 139. What bounds it is the softmax warps' instructions, 60 us of
-// them by themselves, then the way round the barriers.
+// answers x 1-4 tokens over bf16 pages, 14336 shared positions, 8 K/V heads: 118 us (on mma.sync
+// 240); this kernel by itself 96 under the profiler. Steps to it: a pair of threads per row, which exchange
+// their maxima, 133; a thread per row and pairs of fp32 numbers in an instruction, 120;
+// S of the next step ahead, 118. What bounds it is the way round a step (S, softmax, P, O): its issue
+// slots are 44 % used, the tensor pipe 28 %. A wait that reads the timer at every try takes 1 us.
 //
 // Every wait is bounded (2 s): on expiry it raises the abort flag, which ends every other wait;
 // the roles run out without storing, the MMAs issued are drained and TMEM is freed.
@@ -40,19 +40,19 @@ namespace {
 
 #include "tc_ptx.cuh"
 
-constexpr int kThreads = 512, kSoftmaxWarps = 8, kLoadWarps = 4, kMmaWarp = 12;
+constexpr int kThreads = 384, kSoftmaxWarps = 4, kLoadWarps = 4, kMmaWarp = 8;
 constexpr unsigned kAll = 0xffffffffu;
 constexpr uint32_t kWaitLimitNs = 2000000000u;
 constexpr int kKeys = kTcPages * kPageRows;            // of a step
-// registers a thread: at launch, and as the warpgroups share them out (fp32 rows take the
-// loaders more)
-constexpr int kRegsLaunch = 64, kRegsMma = 32;
+// registers a thread: at launch, and as the warpgroups share them out (rows that are converted
+// take the loaders more)
+constexpr int kRegsLaunch = 80, kRegsMma = 24;
 template <int FMT>
-constexpr int kRegsSoftmax = FMT == TIE_KV_F32 ? 72 : 80;
+constexpr int kRegsLoad = FMT == TIE_KV_F32 ? 80 : FMT == TIE_KV_BF16 ? 48 : 64;
 template <int FMT>
-constexpr int kRegsLoad = FMT == TIE_KV_F32 ? 80 : 64;
+constexpr int kRegsSoftmax = 3 * kRegsLaunch - kRegsMma - kRegsLoad<FMT>;
 template <int FMT>
-constexpr bool kRegsFit = 128 * (2 * kRegsSoftmax<FMT> + kRegsLoad<FMT> + kRegsMma) <= kThreads * kRegsLaunch;
+constexpr bool kRegsFit = 128 * (kRegsSoftmax<FMT> + kRegsLoad<FMT> + kRegsMma) <= kThreads * kRegsLaunch && kRegsSoftmax<FMT> % 8 == 0;
 static_assert(kRegsFit<TIE_KV_F32> && kRegsFit<TIE_KV_BF16> && kRegsFit<TIE_KV_INT8>, "register split");
 
 constexpr uint32_t kQTerm = kTcRows * 128, kKvTerm = kKeys * 128;    // bytes of a term
@@ -61,14 +61,15 @@ constexpr uint32_t kColP = 0, kColS = 96, kColO = 160, kTmemCols = 256;
 template <int FMT>
 struct Tc {
     static constexpr int kTerms = FMT == TIE_KV_F32 ? 3 : 1;
-    // bf16 rows go from memory straight to their places, two steps ahead
-    static constexpr int kStages = FMT == TIE_KV_BF16 ? 3 : 1;
+    // bf16 rows go from memory straight to their places, two steps ahead, and need few of the loaders'
+    // registers: a step's scores stay in the softmax warps', and the next one's are computed meanwhile
+    static constexpr bool kAhead = FMT == TIE_KV_BF16;
+    static constexpr int kStages = kAhead ? 3 : 1;
     static constexpr uint32_t kStage = 2 * kTerms * kKvTerm, kValues = kTerms * kKvTerm;    // bytes of a stage; to its values
     static constexpr uint32_t kOffQ = 0, kOffKv = 3 * kQTerm;
     static constexpr uint32_t kOffScales = kOffKv + kStages * kStage;    // [step % 2][key, value][64]
     static constexpr uint32_t kOffThere = kOffScales + 4 * kKeys * 4;    // [step % 4][page]: its positions
-    static constexpr uint32_t kOffTop = kOffThere + 4 * kTcPages * 4;     // [step % 2][half][row]: maxima, at the end sums
-    static constexpr uint32_t kOffBars = kOffTop + 4 * kTcRows * 4;
+    static constexpr uint32_t kOffBars = kOffThere + 4 * kTcPages * 4;
     static constexpr uint32_t kBytes = kOffBars + 64;
 };
 
@@ -107,22 +108,27 @@ __device__ __forceinline__ uint32_t nanoseconds() {
     asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
     return t;
 }
-// 16 columns of the warp's 32 lanes read, 8 written
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+// 32 columns of the warp's 32 lanes read, 16 written
+__device__ __forceinline__ void tmem_begin32(uint32_t taddr, uint32_t* r) {
     __syncwarp();
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     __syncwarp();
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
+}
+
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float m;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+    return m;
 }
 
 // Bytes 0 and 2 of a word, as signed levels, in a pair of bf16: 0x4300 | u is 128 + u for
@@ -196,16 +202,16 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float* s_scales = reinterpret_cast<float*>(smem + T::kOffScales);
     int* s_there = reinterpret_cast<int*>(smem + T::kOffThere);
-    float* s_top = reinterpret_cast<float*>(smem + T::kOffTop);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + T::kOffBars);
     uint64_t* q_full = bars;             // an item's Q written (loader warps)
     uint64_t* k_full = bars + 1;         // a step's keys written (loader warps)
     uint64_t* v_full = bars + 2;         // a step's values written (loader warps)
-    uint64_t* s_full = bars + 3;         // a step's S computed, and all MMAs before it (commit); its scales and
-                                         // what is there of it written (loader warps)
-    uint64_t* p_full = bars + 4;         // a step's P written, the O before it read (softmax warps)
-    uint64_t* o_last = bars + 5;         // an item's last O computed (commit)
-    uint64_t* drained = bars + 6;        // every MMA done (commit)
+    uint64_t* s_full = bars + 3;         // a step's S computed (commit); its scales and what is there of it
+                                         // written (loader warps)
+    uint64_t* s_free = bars + 4;         // a step's S read (softmax warps, kAhead)
+    uint64_t* p_full = bars + 5;         // a step's P written, the O before it read (softmax warps)
+    uint64_t* o_full = bars + 6;         // a step's O computed (commit)
+    uint64_t* drained = bars + 7;        // every MMA done (commit)
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
     __shared__ ScheduleScratch<kThreads> scratch;
@@ -218,7 +224,8 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         mbar_init(smem_u32(v_full), kLoadWarps);
         mbar_init(smem_u32(s_full), 1 + kLoadWarps);
         mbar_init(smem_u32(p_full), kSoftmaxWarps);
-        mbar_init(smem_u32(o_last), 1);
+        mbar_init(smem_u32(s_free), kSoftmaxWarps);
+        mbar_init(smem_u32(o_full), 1);
         mbar_init(smem_u32(drained), 1);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -294,39 +301,49 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         // ------------------------------------------------------------ softmax
         // (tcgen05.ld and .st are the warp's: so is every condition around them)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax<FMT>));
-        const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane;
-        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        // both threads of the quarter's rows
-        auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory"); };
+        // (a read of tensor memory is used only behind its wait: the registers are volatile asm's)
+        constexpr int kChunk = T::kAhead ? 64 : 32;       // scores in registers at a time
+        const int r = warp * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
         for (; ok && find(job); ++un) {
-            float m = -INFINITY, l = 0.f, alpha = 1.f, o[32];
+            float m = -INFINITY, alpha = 1.f;
+            Float2x l(0.f, 0.f), o[32];
 #pragma unroll
-            for (int d = 0; d < 32; ++d) o[d] = 0.f;
+            for (int d = 0; d < 32; ++d) o[d] = Float2x(0.f, 0.f);
             // the step before has left its O: it is relative to that step's maximum
             auto add_step = [&]() {
+                const Float2x by(alpha, alpha);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    uint32_t y[16];
-                    tmem_ld16(lanes + kColO + 32u * half + 16u * h, y);
+                    uint32_t y[32];
+                    tmem_begin32(lanes + kColO + 32u * h, y);
+                    tmem_wait_ld();
 #pragma unroll
-                    for (int d = 0; d < 16; ++d) o[16 * h + d] = fmaf(o[16 * h + d], alpha, __uint_as_float(y[d]));
+                    for (int d = 0; d < 16; ++d)
+                        o[16 * h + d] = fma2(o[16 * h + d], by, Float2x(__uint_as_float(y[2 * d]), __uint_as_float(y[2 * d + 1])));
                 }
             };
 #pragma unroll 1
             for (int b = job.b0; b < job.b1; ++b, ++f) {
                 if (!(ok = wait_all(s_full, f))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;");
-                const int* there = s_there + (f & 3u) * kTcPages + 2 * half;
-                const bool all = there[0] + there[1] == 2 * kPageRows;
-                const float4* ks = reinterpret_cast<const float4*>(s_scales + (f & 1u) * 2 * kKeys) + 8 * half;
+                const int4 there = *reinterpret_cast<const int4*>(s_there + (f & 3u) * kTcPages);
+                const bool all = there.x + there.y + there.z + there.w == kKeys;
+                const float4* ks = reinterpret_cast<const float4*>(s_scales + (f & 1u) * 2 * kKeys);
                 const float4* vs = ks + kKeys / 4;
-                // page h (of this thread's two) of S as scores
-                auto scores = [&](int h, uint32_t (&y)[16]) {
-                    tmem_ld16(lanes + kColS + 32u * half + 16u * h, y);
+                // the step's scores c0 ..
+                auto scores = [&](int c0, uint32_t (&y)[kChunk]) {
+#pragma unroll
+                    for (int i = 0; i < kChunk; i += 32) tmem_begin32(lanes + kColS + c0 + i, y + i);
+                    tmem_wait_ld();
+                    if constexpr (T::kAhead) {
+                        asm volatile("tcgen05.fence::before_thread_sync;");
+                        arrive(s_free);
+                    }
                     if constexpr (FMT == TIE_KV_INT8) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float4 z = ks[4 * h + i];
+                        for (int i = 0; i < kChunk / 4; ++i) {
+                            const float4 z = ks[c0 / 4 + i];
                             y[4 * i] = __float_as_uint(__uint_as_float(y[4 * i]) * z.x);
                             y[4 * i + 1] = __float_as_uint(__uint_as_float(y[4 * i + 1]) * z.y);
                             y[4 * i + 2] = __float_as_uint(__uint_as_float(y[4 * i + 2]) * z.z);
@@ -334,101 +351,106 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                         }
                     }
                     if (!all) {
-                        const int n = there[h];
+                        const int n0 = c0 ? there.z : there.x, n1 = c0 ? there.w : there.y;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (i >= n) y[i] = 0xff800000u;
+                        for (int i = 0; i < kChunk; ++i)
+                            if ((i & 15) >= (i < 16 ? n0 : i < 32 ? n1 : i < 48 ? there.z : there.w)) y[i] = 0xff800000u;
                     }
                 };
+                uint32_t y[kChunk];
                 float top = -INFINITY;
 #pragma unroll 1
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t y[16];
-                    scores(h, y);
+                for (int c0 = 0; c0 < kKeys; c0 += kChunk) {
+                    scores(c0, y);
+                    float a0 = max3(top, __uint_as_float(y[0]), __uint_as_float(y[1])), a1 = max3(-INFINITY, __uint_as_float(y[2]), __uint_as_float(y[3]));
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) top = fmaxf(top, __uint_as_float(y[i]));
+                    for (int i = 4; i < kChunk; i += 4) {
+                        a0 = max3(a0, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
+                        a1 = max3(a1, __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
+                    }
+                    top = fmaxf(a0, a1);
                 }
-                float* const tops = s_top + (f & 1u) * 2 * kTcRows;
-                tops[half * kTcRows + r] = top;
-                if (b > job.b0) add_step();
-                meet();
-                top = fmaxf(top, tops[(half ^ 1) * kTcRows + r]);
+                // (the step before's O is computed: so P may be written over its P)
+                if (b > job.b0) {
+                    if (!(ok = wait_all(o_full, f - 1))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+                    add_step();
+                }
                 const float m_new = fmaxf(m, top), from = m_new == -INFINITY ? 0.f : m_new;
                 alpha = ex2_ftz(m - from);
                 m = m_new;
-                l *= alpha;
+                l = l * Float2x(alpha, alpha);
+                const Float2x less(-from, -from), weight(kWeight, kWeight);
 #pragma unroll 1
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t y[16];
-                    scores(h, y);
+                for (int c0 = 0; c0 < kKeys; c0 += kChunk) {
+                    if constexpr (kChunk < kKeys) scores(c0, y);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float w = kWeight * ex2_ftz(__uint_as_float(y[i]) - from);
-                        l += w;
-                        y[i] = __float_as_uint(w);
-                    }
-                    if constexpr (FMT == TIE_KV_INT8) {
+                    for (int h = 0; h < kChunk / 32; ++h) {
+                        float w[32];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float4 z = vs[4 * h + i];
-                            y[4 * i] = __float_as_uint(__uint_as_float(y[4 * i]) * z.x);
-                            y[4 * i + 1] = __float_as_uint(__uint_as_float(y[4 * i + 1]) * z.y);
-                            y[4 * i + 2] = __float_as_uint(__uint_as_float(y[4 * i + 2]) * z.z);
-                            y[4 * i + 3] = __float_as_uint(__uint_as_float(y[4 * i + 3]) * z.w);
+                        for (int i = 0; i < 32; i += 2) {
+                            float x0, x1;
+                            (Float2x(__uint_as_float(y[32 * h + i]), __uint_as_float(y[32 * h + i + 1])) + less).get(x0, x1);
+                            const Float2x e = Float2x(ex2_ftz(x0), ex2_ftz(x1)) * weight;
+                            l = l + e;
+                            e.get(w[i], w[i + 1]);
                         }
-                    }
+                        if constexpr (FMT == TIE_KV_INT8) {
 #pragma unroll
-                    for (int e = 0; e < 3; ++e) {
-                        uint32_t p[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            p[i] = __byte_perm(y[2 * i], y[2 * i + 1], 0x7632);
-                            if (e < 2) {
-                                y[2 * i] = __float_as_uint(rest(__uint_as_float(y[2 * i])));
-                                y[2 * i + 1] = __float_as_uint(rest(__uint_as_float(y[2 * i + 1])));
+                            for (int i = 0; i < 8; ++i) {
+                                const float4 z = vs[c0 / 4 + 8 * h + i];
+                                w[4 * i] *= z.x;
+                                w[4 * i + 1] *= z.y;
+                                w[4 * i + 2] *= z.z;
+                                w[4 * i + 3] *= z.w;
                             }
                         }
-                        tmem_st8(lanes + kColP + 32u * e + 16u * half + 8u * h, p);
+#pragma unroll
+                        for (int e = 0; e < 3; ++e) {
+                            uint32_t p[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                p[i] = terms2(w[2 * i], w[2 * i + 1]);
+                                if (e < 2) rest2(w[2 * i], w[2 * i + 1]);
+                            }
+                            tmem_st16(lanes + kColP + 32u * e + c0 / 2 + 16u * h, p);
+                        }
                     }
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;");
                 arrive(p_full);
             }
-            if (!ok || !(ok = wait_all(o_last, un))) break;
+            if (!ok || !(ok = wait_all(o_full, f - 1))) break;
             asm volatile("tcgen05.fence::after_thread_sync;");
+            // (the next item's first P, which lets its O begin, is written after this)
             add_step();
-            // (the next item's first P, which lets its O begin, is written after this; the last
-            // step's maxima have been read, and the ones of the step before, whose place this is)
-            float* const sums = s_top + (f & 1u) * 2 * kTcRows;
-            sums[half * kTcRows + r] = l;
-            meet();
-            l += sums[(half ^ 1) * kTcRows + r];
-            meet();
             const int i = job.i0 + r;
             if (i < job.rows) {
                 const size_t slot = (2 * (size_t)me + (job.parts > 0)) * kTcRows + r;
                 const int tok = a.by_group(i), h = job.head * a.group + i - tok * a.group;
                 const size_t place = (size_t)(job.row0 + tok) * a.n_head + h;
-                float* to = (job.whole ? a.whole_o[0] + place * kHeadDim : line.part_o + slot * kHeadDim) + 32 * half;
-                if (half == 0) {
-                    if (job.parts) a.place[0][place] = make_int2(job.whole ? -1 : (int)slot, job.parts);
-                    *reinterpret_cast<float2*>(job.whole ? a.whole_ml[0] + 2 * place : line.part_ml + 2 * slot) = make_float2(m, l);
-                }
+                float* to = job.whole ? a.whole_o[0] + place * kHeadDim : line.part_o + slot * kHeadDim;
+                if (job.parts) a.place[0][place] = make_int2(job.whole ? -1 : (int)slot, job.parts);
+                float l0, l1;
+                l.get(l0, l1);
+                *reinterpret_cast<float2*>(job.whole ? a.whole_ml[0] + 2 * place : line.part_ml + 2 * slot) = make_float2(m, l0 + l1);
 #pragma unroll
-                for (int d = 0; d < 8; ++d)
-                    reinterpret_cast<float4*>(to)[d] = make_float4(o[4 * d], o[4 * d + 1], o[4 * d + 2], o[4 * d + 3]);
+                for (int d = 0; d < 16; ++d) {
+                    float4 v;
+                    o[2 * d].get(v.x, v.y);
+                    o[2 * d + 1].get(v.z, v.w);
+                    reinterpret_cast<float4*>(to)[d] = v;
+                }
             }
             __syncwarp();
         }
     } else if (warp < kSoftmaxWarps + kLoadWarps) {
         // ------------------------------------------------------------ loaders
-        // (.inc or .dec: more, or no fewer, than at launch)
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsLoad<FMT>));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad<FMT>));
         constexpr int kBytes = FMT == TIE_KV_F32 ? 4 : FMT == TIE_KV_BF16 ? 2 : 1;
         const int lw = warp - kSoftmaxWarps, sub = lane >> 3, dl = lane & 7;
         const size_t w = (size_t)a.n_kv_head * kHeadDim * kBytes;     // bytes of a row
-        constexpr bool kCopied = FMT == TIE_KV_BF16;
         Row8<FMT> k[4], v[4];
         float ks = 0.f, vs = 0.f;
         int page = 0, there = 0;             // of the step that is loaded: this warp's page, its positions
@@ -485,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
             now_at = job.b0;
-            if constexpr (kCopied) {
+            if constexpr (T::kAhead) {
                 copy(job.b0);
                 copy(job.b0 + 1);
             } else {
@@ -527,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             arrive(q_full);
-            if constexpr (kCopied) {
+            if constexpr (T::kAhead) {
 #pragma unroll 1
                 for (int b = job.b0; b < job.b1; ++b, ++f) {
                     now_at = b;
@@ -535,8 +557,10 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     arrive(s_full);
                     if (lane == 0) mbar_arrive(smem_u32(k_full));
-                    if (!(ok = wait_all(s_full, f))) break;      // the step before has left its stage
+                    if (f && !(ok = wait_all(o_full, f - 1))) break;       // the step before has left its stage
                     copy(b + 2);
+                    // (nor may this warp arrive for a step before the last one's barriers have completed)
+                    if (!(ok = wait_all(s_full, f))) break;
                 }
             } else {
 #pragma unroll 1
@@ -558,10 +582,11 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                         page_of(b + 1);
                         load_k();
                     }
-                    if (!(ok = wait_all(s_full, f))) break;      // K has been read, and the step before's V
+                    if (f && !(ok = wait_all(o_full, f - 1))) break;       // the step before's V has been read
                     store(smem + T::kOffKv + T::kValues, v, now);
                     arrive(v_full);
                     if (b + 1 < job.b1) load_v();
+                    if (!(ok = wait_all(s_full, f))) break;      // K has been read
                 }
             }
         }
@@ -577,31 +602,42 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
             for (; ok && find(job); ++un) {
                 if (!(ok = wait_all(q_full, un))) break;
                 const int steps = __shfl_sync(kAll, job.b1 - job.b0, 0);
-#pragma unroll 1
-                for (int b = 0; b < steps; ++b, ++f) {
-                    if (!(ok = wait_all(k_full, f))) break;
+                auto stage = [&](uint32_t step) { return sb + T::kOffKv + (step % T::kStages) * T::kStage; };
+                // S of a step whose keys are there, where the S before it has been read
+                auto scores = [&](uint32_t step) -> bool {
+                    if (!wait_all(k_full, step)) return false;
                     asm volatile("tcgen05.fence::after_thread_sync;");
 #pragma unroll 1
                     for (int z = 0; z < kProducts; ++z) {
                         const uint32_t q = sb + T::kOffQ + (kA >> (4 * z) & 15u) * kQTerm;
-                        const uint32_t k = sb + T::kOffKv + (f % T::kStages) * T::kStage + (kB >> (4 * z) & 15u) * kKvTerm;
+                        const uint32_t k = stage(step) + (kB >> (4 * z) & 15u) * kKvTerm;
 #pragma unroll
                         for (int s = 0; s < 4; ++s)
                             mma_ss(tm + kColS, sw128_desc(q + 32u * s), sw128_desc(k + 32u * s), kIdesc, z || s ? 1u : 0u);
                     }
                     commit_elected(smem_u32(s_full));
+                    return true;
+                };
+                if (T::kAhead && !(ok = scores(f))) break;
+#pragma unroll 1
+                for (int b = 0; b < steps; ++b, ++f) {
+                    if constexpr (T::kAhead) {
+                        if (b + 1 < steps && !(ok = wait_all(s_free, f) && scores(f + 1))) break;
+                    } else if (!(ok = scores(f))) {
+                        break;
+                    }
                     // (copied rows: k_full was for both)
-                    if (!(ok = wait_all(p_full, f) && (FMT == TIE_KV_BF16 || wait_all(v_full, f)))) break;
+                    if (!(ok = wait_all(p_full, f) && (T::kAhead || wait_all(v_full, f)))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;");
 #pragma unroll 1
                     for (int z = 0; z < kProducts; ++z) {
                         const uint32_t p = tm + kColP + (kA >> (4 * z) & 15u) * 32u;
-                        const uint32_t v = sb + T::kOffKv + (f % T::kStages) * T::kStage + T::kValues + (kB >> (4 * z) & 15u) * kKvTerm;
+                        const uint32_t v = stage(f) + T::kValues + (kB >> (4 * z) & 15u) * kKvTerm;
 #pragma unroll
                         for (int s = 0; s < 4; ++s)
                             mma_ts(tm + kColO, p + 8u * s, sw128_desc(v + 2048u * s), kIdescO, z || s ? 1u : 0u);
                     }
-                    if (b + 1 == steps) commit_elected(smem_u32(o_last));
+                    commit_elected(smem_u32(o_full));
                 }
             }
             // every MMA issued completes before TMEM is freed, also when cut short

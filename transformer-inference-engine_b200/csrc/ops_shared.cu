@@ -594,7 +594,7 @@ __device__ __forceinline__ void run_steps_q8(const SharedArgs& a, ItemAt it, Ite
                         vt[p][4 * h + 2] = __byte_perm(y, w, 0x5410);
                         vt[p][4 * h + 3] = __byte_perm(y, w, 0x7632);
                     }
-                            }
+            }
 #pragma unroll
             for (int p = 0; p < PG; p += 2)
 #pragma unroll
@@ -859,7 +859,10 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(const __grid_cons
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, q = blockIdx.x;
     const Lengths lengths{a.row_start, a.ctx, a.gstart, a.plen};
     const UnitShape s = unit_shape(a, lengths, a.n_group + q);
-    if (!s.rows) return;
+    if (!s.rows) {
+        pdl_wait();                    // (whoever waits for this kernel waits for the one before it too)
+        return;
+    }
     bool grouped = false;
     if (a.n_group) {
         if (t == 0) s_group = -1;

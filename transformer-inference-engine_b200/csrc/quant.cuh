@@ -107,6 +107,36 @@ __device__ __forceinline__ uint32_t terms2(float lo, float hi) {
     return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
 }
 
+// Two fp32 numbers in one instruction, rounded as each alone would be.
+struct Float2x {
+    unsigned long long v;
+    __device__ __forceinline__ Float2x() {}
+    __device__ __forceinline__ explicit Float2x(unsigned long long of) : v(of) {}
+    __device__ __forceinline__ Float2x(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+    __device__ __forceinline__ void get(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+};
+__device__ __forceinline__ Float2x operator+(Float2x a, Float2x b) {
+    Float2x c;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v));
+    return c;
+}
+__device__ __forceinline__ Float2x operator*(Float2x a, Float2x b) {
+    Float2x c;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v));
+    return c;
+}
+__device__ __forceinline__ Float2x fma2(Float2x a, Float2x b, Float2x c) {
+    Float2x d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+// rest() of two values
+__device__ __forceinline__ void rest2(float& lo, float& hi) {
+    const Float2x less(__uint_as_float((__float_as_uint(lo) & 0xffff0000u) ^ 0x80000000u),
+                       __uint_as_float((__float_as_uint(hi) & 0xffff0000u) ^ 0x80000000u));
+    (Float2x(lo, hi) + less).get(lo, hi);
+}
+
 // d = c + a b on bf16 (m16n8k16), fp32 sums
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "

@@ -158,10 +158,10 @@ __device__ __forceinline__ Plan build_plan(const SharedArgs& a, int u0, int u1, 
 // Terms of two numbers: [0] the largest.
 __device__ __forceinline__ void split3(float lo, float hi, uint32_t (&x)[3]) {
     x[0] = terms2(lo, hi);
-    lo = rest(lo);
-    hi = rest(hi);
+    rest2(lo, hi);
     x[1] = terms2(lo, hi);
-    x[2] = terms2(rest(lo), rest(hi));
+    rest2(lo, hi);
+    x[2] = terms2(lo, hi);
 }
 
 // Tensor-core kernel (k_shared_tc.cu) for prefixes of many rows: items of 128 rows, steps of 64 keys.
