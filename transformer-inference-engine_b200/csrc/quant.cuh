@@ -19,8 +19,41 @@ __device__ __forceinline__ float max_abs(float a, float b) {
     return r;
 }
 
-// 1 / s for level_of, 0 where s is so small that its reciprocal may be beyond fp32.
-__device__ __forceinline__ float reciprocal_of(float s) { return s < 0x1p-100f ? 0.f : __frcp_rn(s); }
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// Two fp32 numbers in one instruction, rounded as each alone would be.
+struct Float2x {
+    unsigned long long v;
+    __device__ __forceinline__ Float2x() {}
+    __device__ __forceinline__ explicit Float2x(unsigned long long of) : v(of) {}
+    __device__ __forceinline__ Float2x(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+    __device__ __forceinline__ void get(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+};
+__device__ __forceinline__ Float2x operator+(Float2x a, Float2x b) {
+    Float2x c;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v));
+    return c;
+}
+__device__ __forceinline__ Float2x operator*(Float2x a, Float2x b) {
+    Float2x c;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v));
+    return c;
+}
+__device__ __forceinline__ Float2x fma2(Float2x a, Float2x b, Float2x c) {
+    Float2x d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+// 1 / s to one place, 0 where s is so small that its reciprocal may be beyond fp32.
+__device__ __forceinline__ float reciprocal_of(float s) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+    return s < 0x1p-100f ? 0.f : r;
+}
 
 // The level of x at scale s > 0: the integer nearest to the exact quotient, ties to even,
 // within +-most. The approximate quotient's nearest integer q is off by one at most; the
@@ -41,13 +74,19 @@ __device__ __forceinline__ int level_of(float x, float s, float inv, float most)
 constexpr uint32_t kLevelBase = 0x4b400000u;
 template <int N>
 __device__ __forceinline__ void levels_of(const float (&x)[N], float s, float most, uint32_t (&level)[N]) {
+    static_assert(N % 2 == 0, "pairs");
     const float inv = reciprocal_of(s), base = __uint_as_float(kLevelBase);
+    const Float2x inv2(inv, inv), base2(base, base), less2(-base, -base), minus2(-1.f, -1.f);
     float far = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float t = x[i] * inv, y = t + base;
-        level[i] = __float_as_uint(y);
-        far = fmaxf(far, fabsf(t - (y - base)));
+    for (int i = 0; i < N; i += 2) {
+        const Float2x t = Float2x(x[i], x[i + 1]) * inv2, y = t + base2;
+        float y0, y1, e0, e1;
+        y.get(y0, y1);
+        fma2(y + less2, minus2, t).get(e0, e1);
+        level[i] = __float_as_uint(y0);
+        level[i + 1] = __float_as_uint(y1);
+        far = max_abs3(far, e0, e1);
     }
     if (far > 0.49996f || inv == 0.f) {
 #pragma unroll
@@ -107,29 +146,6 @@ __device__ __forceinline__ uint32_t terms2(float lo, float hi) {
     return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
 }
 
-// Two fp32 numbers in one instruction, rounded as each alone would be.
-struct Float2x {
-    unsigned long long v;
-    __device__ __forceinline__ Float2x() {}
-    __device__ __forceinline__ explicit Float2x(unsigned long long of) : v(of) {}
-    __device__ __forceinline__ Float2x(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
-    __device__ __forceinline__ void get(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-};
-__device__ __forceinline__ Float2x operator+(Float2x a, Float2x b) {
-    Float2x c;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v));
-    return c;
-}
-__device__ __forceinline__ Float2x operator*(Float2x a, Float2x b) {
-    Float2x c;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v));
-    return c;
-}
-__device__ __forceinline__ Float2x fma2(Float2x a, Float2x b, Float2x c) {
-    Float2x d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return d;
-}
 // rest() of two values
 __device__ __forceinline__ void rest2(float& lo, float& hi) {
     const Float2x less(__uint_as_float((__float_as_uint(lo) & 0xffff0000u) ^ 0x80000000u),
