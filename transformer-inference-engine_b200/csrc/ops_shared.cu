@@ -30,10 +30,12 @@
 // the sum, so it takes 16 in a row, and each lane's 8 dims of 4 values are packed in pairs of keys.
 //
 // Measured (B200, whole calls): 64 sequences of up to 4000 positions, 8-bit pages (127 MB), one token
-// each, 39 us: 27 of steps, the others the start (4) and the join; 12 warps an SM wait for memory
-// (4.7 TB/s). 256 answers of a token behind 700 positions, fp32, 75 us: 60-65 % of what their own
-// positions take to read; the fp32 split's instructions (with pairs of numbers per
-// instruction it took as long). 24 groups in 8 bits 55 us, 4 beams 12: the chain of two launches.
+// each, 39 us: 27 of steps (4.7 TB/s; two thirds of the issue slots, 600 instructions for 32 keys of a
+// head), the others the start (4) and the join. Steps copied to shared memory, with 16 warps an SM instead of
+// 12, reads with hints for the L2 and pairs of numbers per instruction in the 8-bit path each
+// took 39 too. 256 answers of a token behind 700 positions, fp32, 74 us: 60-65 % of what their own
+// positions take to read; the fp32 split's instructions (numbers in pairs: 76 -> 74). 24 groups in 8
+// bits 55 us, 4 beams 12: the chain of two launches.
 #include <cuda_bf16.h>
 
 #include <climits>
@@ -365,7 +367,8 @@ __device__ __forceinline__ void run_steps(const SharedArgs& a, ItemAt it, ItemAt
 #pragma unroll
         for (int r = 0; r < kAcc; ++r)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[r][e] += s_small[r][e];
+            for (int e = 0; e < 4; e += 2)
+                (Float2x(s[r][e], s[r][e + 1]) + Float2x(s_small[r][e], s_small[r][e + 1])).get(s[r][e], s[r][e + 1]);
         if (!whole) {
 #pragma unroll
             for (int r = 0; r < kAcc; ++r)
@@ -401,10 +404,12 @@ __device__ __forceinline__ void run_steps(const SharedArgs& a, ItemAt it, ItemAt
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float w[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        w[e] = kWeight * ex2_ftz(s[n * PG + p][2 * h + e] - from[n][e]);
-                        st.l[n][e] += w[e];
+                    {
+                        const float(&y)[4] = s[n * PG + p];
+                        (Float2x(y[2 * h], y[2 * h + 1]) + Float2x(-from[n][0], -from[n][1])).get(w[0], w[1]);
+                        const Float2x x = Float2x(ex2_ftz(w[0]), ex2_ftz(w[1])) * Float2x(kWeight, kWeight);
+                        (Float2x(st.l[n][0], st.l[n][1]) + x).get(st.l[n][0], st.l[n][1]);
+                        x.get(w[0], w[1]);
                     }
                     uint32_t x[3];
                     split3(w[0], w[1], x);
@@ -424,9 +429,10 @@ __device__ __forceinline__ void run_steps(const SharedArgs& a, ItemAt it, ItemAt
 #pragma unroll
                 for (int r = 0; r < kI * NT; ++r)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float& o = st.o[r % NT][i + r / NT][e];
-                        o = p == 0 ? fmaf(o, alpha[r % NT][e & 1], d[r][e]) : o + d[r][e];
+                    for (int e = 0; e < 4; e += 2) {
+                        float &o0 = st.o[r % NT][i + r / NT][e], &o1 = st.o[r % NT][i + r / NT][e + 1];
+                        const Float2x o(o0, o1), x(d[r][e], d[r][e + 1]);
+                        (p == 0 ? fma2(o, Float2x(alpha[r % NT][0], alpha[r % NT][1]), x) : o + x).get(o0, o1);
                     }
             }
         }
