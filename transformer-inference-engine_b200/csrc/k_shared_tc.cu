@@ -21,7 +21,7 @@
 // barrier's phase of the step before has completed (loaders wait for S, softmax warps for O).
 //
 // Measured (B200, the whole call: this kernel, the sequences' own positions, the join): 64
-// answers x 1-4 tokens over bf16 pages, 14336 shared positions, 8 K/V heads: 113 us (on mma.sync
+// answers x 1-4 tokens over bf16 pages, 14336 shared positions, 8 K/V heads: 112 us (on mma.sync
 // 271). Steps to it: a pair of threads per row, which exchange their maxima, 133; a thread per
 // row and pairs of fp32 numbers in an instruction, 120; S of the next step ahead, 118; its keys
 // told of before the next rows are asked for (a page's table entry a step sooner), 113. What bounds it
@@ -120,7 +120,13 @@ __device__ __forceinline__ void tmem_begin32(uint32_t taddr, uint32_t* r) {
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The reads are done. What a read is to return is an operand, so that no use of it comes before this.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     __syncwarp();
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -304,7 +310,6 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         // ------------------------------------------------------------ softmax
         // (tcgen05.ld and .st are the warp's: so is every condition around them)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax<FMT>));
-        // (a read of tensor memory is used only behind its wait: the registers are volatile asm's)
         constexpr int kChunk = T::kAhead ? 64 : 32;       // scores in registers at a time
         const int r = warp * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
@@ -320,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                 for (int h = 0; h < 2; ++h) {
                     uint32_t y[32];
                     tmem_begin32(lanes + kColO + 32u * h, y);
-                    tmem_wait_ld();
+                    tmem_wait_ld(y);
 #pragma unroll
                     for (int d = 0; d < 16; ++d)
                         o[16 * h + d] = fma2(o[16 * h + d], by, Float2x(__uint_as_float(y[2 * d]), __uint_as_float(y[2 * d + 1])));
@@ -338,7 +343,8 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                 auto scores = [&](int c0, uint32_t (&y)[kChunk]) {
 #pragma unroll
                     for (int i = 0; i < kChunk; i += 32) tmem_begin32(lanes + kColS + c0 + i, y + i);
-                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < kChunk; i += 32) tmem_wait_ld(y + i);
                     if constexpr (T::kAhead) {
                         asm volatile("tcgen05.fence::before_thread_sync;");
                         arrive(s_free);
