@@ -438,6 +438,16 @@ def test_long_prefixes_of_many_steps(kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_long_prefixes_of_as_many_sequences_as_there_may_be(kind):
+    """Lengths that leave shared memory for one CTA an SM, and groups of 64 to 192 rows."""
+    rng = np.random.default_rng(6)
+    cuts = np.sort(rng.choice(np.arange(1, 64), 31, replace=False)) * 64
+    b = _long(3, rng.integers(0, 3, 4096).tolist(), [1] * 4096, 1, 1, kind, tuple([0] + cuts.tolist() + [4096]),
+              tuple(rng.integers(0, 90, 32).tolist()))
+    b.check()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_long_prefixes_with_holes(kind):
     """Pages that are not mapped, all of them, and lengths without meaning."""
     b = _long(5, [5] * 90, [1] * 90, 4, 2, kind, (0, 50, 90), (400, 77), unmapped=0.4)
@@ -865,3 +875,39 @@ def test_a_captured_decode_step(rows):
         graph.replay()
         assert torch.equal(y, want[i])
     assert all(torch.equal(p, q) for p, q in zip(pools, kept))
+
+
+def test_calls_of_two_threads():
+    """Attention and products from two threads at once, each on a stream of its own, with one set of pages and weights."""
+    import threading
+    rng = np.random.default_rng(33)
+    b = [Batch(34, [400, 20], [1, 1], 4, 2, "q8", (0, 2), (500,)), _long(35, [9] * 70, [1] * 70, 4, 2, "f32", (0, 70), (300,))]
+    packed, scales, _ = _weights_of(rng, 500, 256, 64)
+    want = []
+    for x in b:
+        o = x.call()
+        y = torch.empty(x.rows, 500, device="cuda")
+        ops.matvec_q4(o, packed, scales, 64, y)
+        want.append(y)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(x, y0):
+        st = torch.cuda.Stream()
+        try:
+            with torch.cuda.stream(st):
+                for _ in range(20):
+                    o, y = x.call(), torch.empty(x.rows, 500, device="cuda")
+                    ops.matvec_q4(o, packed, scales, 64, y)
+                    st.synchronize()
+                    if not torch.equal(y, y0):
+                        wrong.append(x.kind)
+        except Exception as e:                 # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(b, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]
