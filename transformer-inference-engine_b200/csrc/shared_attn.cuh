@@ -11,8 +11,10 @@ namespace tie {
 // Weights are 2^(s - max) times this, so that the sum of as many of them as there are
 // positions (2^30) times any finite value stays finite.
 constexpr float kWeight = 0x1p-30f;
-// fewest steps worth a warp's stretch
-constexpr int kMinShare = 2;
+// Fewest pages worth a warp's stretch: two steps over fp32 pages (16 keys), one over others (32). With one
+// and with two steps, us: one sequence of 1000, fp32, 11.6 and 10.8; 16 sequences behind 700, fp32, 14.1 and
+// 14.1, 8 bits 12.2 and 13.7; 32 behind 700, bf16, 13.8 and 14.8. (Three: 1 to 2 more than two.)
+constexpr int kMinPages = 2;
 
 // A line: units [u0, u1) (a unit below n_group is a group's prefix, the others are
 // sequences), cut into stretches for `teams` teams: of a warp per K/V head (heads 1), or
@@ -101,7 +103,8 @@ __device__ __forceinline__ long long quotient(long long x, long long y) {
 
 __device__ __forceinline__ long long share_of(const Line& l, long long total) {
     const long long even = quotient(total + l.teams - 1, l.teams);
-    return even > kMinShare ? even : kMinShare;
+    const int least = l.pages < kMinPages ? kMinPages / l.pages : 1;
+    return even > least ? even : least;
 }
 
 // A CTA's copy of the lengths and the line in shared memory: base[u - u0] places before unit u, all
