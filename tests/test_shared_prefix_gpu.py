@@ -1,0 +1,61 @@
+"""Attention over shared positions where its tensor-core kernel has the most to do: CTAs with several parts of several
+steps each. Against the 64-bit definitions (serving_oracle.py)."""
+import os
+import sys
+
+import numpy as np
+import pytest
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import ops_oracle as paged  # noqa: E402
+import serving_oracle as ref  # noqa: E402
+from test_serving_ops_gpu import KINDS, Batch, _np  # noqa: E402
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def _parts(shared, tiles_heads, ctas):
+    """Steps of the parts that each CTA has of groups of `shared` positions with that many items each: a line of
+    items, a place for each step of 64 positions and one before them, in equal stretches."""
+    line = [(n - 1) // 64 + 2 for n in shared for _ in range(tiles_heads)]
+    share = -(-sum(line) // ctas)
+    out, x = [[] for _ in range(ctas)], 0
+    for places in line:
+        for c in range(x // share, (x + places - 1) // share + 1):
+            lo, hi = max(x, c * share) - x, min(x + places, (c + 1) * share) - x
+            if hi - 1 > max(lo - 1, 0):
+                out[c].append(hi - 1 - max(lo - 1, 0))
+        x += places
+    return out
+
+
+def _some(b, chosen):
+    """The definition's rows of the chosen sequences (new tokens: one each), and how far fp32 may be from them."""
+    rows = b.start[chosen]
+    starts = np.searchsorted(chosen, b.groups)
+    o, vmax, smax = ref.attention(b.q[rows], b.kn, b.vn, b.table[chosen], np.arange(len(chosen) + 1), b.ctx[chosen], b.heads,
+                                  b.scale, np.zeros((len(chosen), b.q.shape[1])), 1, b.ksn, b.vsn, prefix_table=b.ptable,
+                                  prefix_lens=b.shared, group_start=starts)
+    return rows, o, paged.attention_bound(vmax, smax, int(b.shared.max() + b.ctx.max()) + 1)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_ctas_with_several_parts_of_several_steps(kind):
+    """32 prompts of a few hundred positions with 128 answers each: some answers of each are as the definition has them,
+    all of them the same whenever they are computed."""
+    rng = np.random.default_rng(31)
+    n, groups, heads, kv_heads = 4096, 32, 12, 4
+    shared = rng.integers(270, 400, groups)
+    ctas = 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    many = [p for p in _parts(shared, n // groups * (heads // kv_heads) // 128 * kv_heads, ctas) if sum(m >= 2 for m in p) >= 2]
+    assert len(many) > ctas // 2
+    b = Batch(4, rng.integers(0, 9, n).tolist(), [1] * n, heads, kv_heads, kind, tuple(range(0, n + 1, n // groups)), tuple(shared))
+    assert b.rows * heads * b.ptable.shape[1] * 16 >= 8_000_000          # the tensor-core kernel's, over every format
+    first = b.call()
+    got = _np(first).astype(np.float64)
+    chosen = np.sort(np.concatenate([np.arange(groups) * (n // groups) + at for at in (0, 77)]))
+    rows, o, bound = _some(b, chosen)
+    assert (np.abs(got[rows] - o) <= bound).all()
+    for _ in range(6):
+        assert torch.equal(b.call(), first)

@@ -37,6 +37,7 @@
 #include <cuda_bf16.h>
 
 #include "shared_attn.cuh"
+#include "shared_stages.h"
 
 namespace tie {
 namespace {
@@ -67,13 +68,14 @@ struct Tc {
     // bf16 rows go from memory straight to their places, two steps ahead, and need few of the loaders'
     // registers: a step's scores stay in the softmax warps', and the next one's are computed meanwhile
     static constexpr bool kAhead = FMT == TIE_KV_BF16;
-    static constexpr int kStages = kAhead ? 3 : 1;
+    static constexpr uint32_t kStages = kAhead ? 3 : 1;
+    using Stage = Stages<kStages>;
     static constexpr uint32_t kStage = 2 * kTerms * kKvTerm, kValues = kTerms * kKvTerm;    // bytes of a stage; to its values
     static constexpr uint32_t kOffQ = 0, kOffKv = 3 * kQTerm;
     static constexpr uint32_t kOffScales = kOffKv + kStages * kStage;    // [step % 2][key, value][64]
     static constexpr uint32_t kOffThere = kOffScales + 4 * kKeys * 4;    // [step % 4][page]: its positions
     static constexpr uint32_t kOffBars = kOffThere + 4 * kTcPages * 4;
-    static constexpr uint32_t kBytes = kOffBars + 64;
+    static constexpr uint32_t kBytes = kOffBars + (7 + kStages + 1) / 2 * 16;
 };
 
 // kind::f16 with bf16 operands, fp32 accumulation, M = 128, N = 64
@@ -219,8 +221,8 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                                          // written (loader warps)
     uint64_t* s_free = bars + 4;         // a step's S read (softmax warps, kAhead)
     uint64_t* p_full = bars + 5;         // a step's P written, the O before it read (softmax warps)
-    uint64_t* o_full = bars + 6;         // a step's O computed (commit)
-    uint64_t* drained = bars + 7;        // every MMA done (commit)
+    uint64_t* drained = bars + 6;        // every MMA done (commit)
+    uint64_t* o_full = bars + 7;         // [stage] a step's O computed, its stage read (commit): shared_stages.h
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
     __shared__ ScheduleScratch<kThreads> scratch;
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         mbar_init(smem_u32(s_full), 1 + kLoadWarps);
         mbar_init(smem_u32(p_full), kSoftmaxWarps);
         mbar_init(smem_u32(s_free), kSoftmaxWarps);
-        mbar_init(smem_u32(o_full), 1);
+        for (uint32_t i = 0; i < T::kStages; ++i) mbar_init(smem_u32(o_full + i), 1);
         mbar_init(smem_u32(drained), 1);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -298,6 +300,8 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         return true;
     };
     auto wait_all = [&](const uint64_t* bar, uint32_t phase) -> bool { return __all_sync(kAll, wait(bar, phase & 1u)); };
+    // the O of a step is computed
+    auto wait_o = [&](uint32_t step) -> bool { return wait_all(o_full + T::Stage::of(step), T::Stage::phase(step)); };
     auto arrive = [&](const uint64_t* bar) {
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(bar));
@@ -381,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                 }
                 // (the step before's O is computed: so P may be written over its P)
                 if (b > job.b0) {
-                    if (!(ok = wait_all(o_full, f - 1))) break;
+                    if (!(ok = wait_o(f - 1))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;");
                     add_step();
                 }
@@ -430,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                 asm volatile("tcgen05.fence::before_thread_sync;");
                 arrive(p_full);
             }
-            if (!ok || !(ok = wait_all(o_full, f - 1))) break;
+            if (!ok || !(ok = wait_o(f - 1))) break;
             asm volatile("tcgen05.fence::after_thread_sync;");
             // (the next item's first P, which lets its O begin, is written after this)
             add_step();
@@ -500,13 +504,14 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
         for (; ok && find(job); ++un) {
-            uint32_t stage = f % T::kStages;             // of the step that is copied next
-            // a step's rows, and zeros for what is not there, to the next stage
-            auto copy = [&](int b) {
+            // a step's rows, and zeros for what is not there, to its stage, once that has been read
+            auto copy = [&](int b) -> bool {
                 if (b < job.b1) {
+                    const uint32_t step = f + (uint32_t)(b - now_at);
+                    if (T::Stage::used(step) && !wait_o(T::Stage::before(step))) return false;
                     page_of(b);
-                    if (lane == 0) s_there[((f + (uint32_t)(b - now_at)) & 3u) * kTcPages + lw] = there;
-                    const uint32_t to = smem_u32(smem + T::kOffKv + stage * T::kStage);
+                    if (lane == 0) s_there[(step & 3u) * kTcPages + lw] = there;
+                    const uint32_t to = smem_u32(smem + T::kOffKv + T::Stage::of(step) * T::kStage);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int row = lw * kPageRows + 4 * i + sub;
@@ -516,15 +521,14 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + T::kValues), "l"(row_at(a.v, i)), "r"(bytes)
                                      : "memory");
                     }
-                    stage = stage + 1 == T::kStages ? 0 : stage + 1;
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
+                return true;
             };
             now_at = job.b0;
             entry = entry_of(job.b0);
             if constexpr (T::kAhead) {
-                copy(job.b0);
-                copy(job.b0 + 1);
+                if (!(ok = copy(job.b0) && copy(job.b0 + 1))) break;
             } else {
                 page_of(job.b0);
             }
@@ -580,14 +584,8 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                         asm volatile("cp.async.wait_group 0;" ::: "memory");
                         arrive_copied();
                     }
-                    if (b + 2 < job.b1) {
-                        // the step before has left its stage (o_full may be at the step after this one, where
-                        // this warp is late: then that step's end is waited for, which needs no more of this warp)
-                        if (f && !(ok = wait_all(o_full, f - 1))) break;
-                        copy(b + 2);
-                    }
+                    if (b + 2 < job.b1 && !(ok = copy(b + 2))) break;
                 }
-                if (!ok || !(ok = wait_all(o_full, f - 1))) break;       // the stages are free
             } else {
 #pragma unroll 1
                 for (int b = job.b0; b < job.b1; ++b, ++f) {
@@ -608,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                         page_of(b + 1);
                         load_k();
                     }
-                    if (f && !(ok = wait_all(o_full, f - 1))) break;       // the step before's V has been read
+                    if (f && !(ok = wait_o(f - 1))) break;       // the step before's V has been read
                     store(smem + T::kOffKv + T::kValues, v, now);
                     arrive(v_full);
                     if (b + 1 < job.b1) load_v();
@@ -628,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
             for (; ok && find(job); ++un) {
                 if (!(ok = wait_all(q_full, un))) break;
                 const int steps = __shfl_sync(kAll, job.b1 - job.b0, 0);
-                auto stage = [&](uint32_t step) { return sb + T::kOffKv + (step % T::kStages) * T::kStage; };
+                auto stage = [&](uint32_t step) { return sb + T::kOffKv + T::Stage::of(step) * T::kStage; };
                 // S of a step whose keys are there, where the S before it has been read
                 auto scores = [&](uint32_t step) -> bool {
                     if (!wait_all(k_full, step)) return false;
@@ -663,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                         for (int s = 0; s < 4; ++s)
                             mma_ts(tm + kColO, p + 8u * s, sw128_desc(v + 2048u * s), kIdescO, z || s ? 1u : 0u);
                     }
-                    commit_elected(smem_u32(o_full));
+                    commit_elected(smem_u32(o_full + T::Stage::of(f)));
                 }
             }
             // every MMA issued completes before TMEM is freed, also when cut short
