@@ -445,8 +445,8 @@ model_status tie_kv_load(const int32_t *slots, int rows, const void *k_pages, co
  * no groups (prefix_table, prefix_lens and group_start NULL). kv_format may be
  * TIE_KV_INT8, with the pool's scales (NULL for the others).
  * All else is as for tie_attention_paged: rows, limits, what is left out, what is
- * not finite, and status (set where a wait of a long prefix's kernel ran out; may be
- * NULL). Sums and softmax statistics are fp32. Over fp32 and bf16 pages products are
+ * not finite, and status. It is set where a wait of a long prefix's kernel ran out (2 s) and may
+ * be NULL; rows whose shared positions were not finished then are NaN, the others as always. Sums and softmax statistics are fp32. Over fp32 and bf16 pages products are
  * of all of their operands' 24 bits. Over pages in 8 bits a row's scaled query is held
  * in 24 bits relative to its largest element (to 2^-126), and the products of a step
  * of 32 keys' weights (at most 1) with their values' scales in 23 bits relative to the
@@ -456,6 +456,11 @@ model_status tie_kv_load(const int32_t *slots, int rows, const void *k_pages, co
  * workspace: tie_attention_shared_workspace(rows, n_head) bytes (on the current
  * device) or more. */
 size_t tie_attention_shared_workspace(int rows, int n_head);
+
+/* The failure drill of it: in the calling thread's next tie_attention_shared with a prefix long enough for
+ * the tensor cores, waits last limit_ns (1 to 2,000,000,000) at most, and half of that kernel's CTAs
+ * wait for what does not come. So a test sees NaN, MODEL_ERR_DEVICE in status, and then a clean next call. */
+model_status tie_attention_shared_wait_drill(uint64_t limit_ns);
 model_status tie_attention_shared(const float *q, int ldq, int n_head, const void *k_pages,
                                   const void *v_pages, const float *k_scales,
                                   const float *v_scales, int kv_format, int n_pages, int n_kv_head,

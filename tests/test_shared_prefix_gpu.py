@@ -6,10 +6,13 @@ import sys
 import numpy as np
 import pytest
 
+import tie_b200
+from tie_b200 import ops
+
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 import ops_oracle as paged  # noqa: E402
 import serving_oracle as ref  # noqa: E402
-from test_serving_ops_gpu import KINDS, Batch, _np  # noqa: E402
+from test_serving_ops_gpu import KINDS, Batch, _i, _f, _long, _np  # noqa: E402
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -59,3 +62,38 @@ def test_ctas_with_several_parts_of_several_steps(kind):
     assert (np.abs(got[rows] - o) <= bound).all()
     for _ in range(6):
         assert torch.equal(b.call(), first)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("held", [0x00, 0x3f, 0x7f, 0xff])
+def test_a_wait_that_runs_out(kind, held):
+    """Whatever the workspace held: rows that were not finished are NaN as a whole head, the others are right, the status
+    says so, and the next call is as if nothing had been."""
+    rng = np.random.default_rng(2)
+    n, groups, heads = 4096, 32, 12
+    b = _long(2, rng.integers(0, 9, n).tolist(), [1] * n, heads, 4, kind, tuple(range(0, n + 1, n // groups)),
+              tuple(rng.integers(20, 190, groups)))
+    rows, o, bound = _some(b, np.sort(rng.choice(n, 150, replace=False)))
+    want = b.call()
+    out, ws = torch.full_like(want, -3.0), torch.empty(ops.attention_shared_workspace(b.rows, b.heads), dtype=torch.uint8, device="cuda")
+    ws.fill_(held)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def call():
+        ops.attention_shared(_f(b.q), b.k, b.v, _i(b.table), _i(b.start), _i(b.ctx), 1, out, ws, k_scales=b.ks, v_scales=b.vs,
+                             prefix_table=_i(b.ptable), prefix_lens=_i(b.shared), group_start=_i(b.groups), status=status)
+
+    ops.attention_shared_wait_drill(5_000_000)
+    call()
+    assert status.item() == tie_b200.MODEL_STATUS.index("MODEL_ERR_DEVICE")
+    got = _np(out).reshape(n, heads, 64)
+    lost = np.isnan(got)
+    assert np.array_equal(lost.any(-1), lost.all(-1)) and lost.any() and not lost.all()
+    kept = ~lost.any(-1)
+    assert np.array_equal(got[kept], _np(want).reshape(got.shape)[kept])
+    kept = kept[rows]
+    assert kept.any() and not kept.all()
+    assert (np.abs(got[rows] - o.reshape(-1, heads, 64)) <= bound.reshape(-1, heads, 64))[kept].all()
+    status.zero_()
+    call()
+    assert status.item() == 0 and torch.equal(out, want)

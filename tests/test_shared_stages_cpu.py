@@ -29,3 +29,10 @@ def test_the_kernel_takes_its_stages_from_there():
     bars = [line for line in source.splitlines() if "o_full" in line and ("wait_all(" in line or "commit_elected(" in line)]
     assert len(bars) == 2 and all("Stage::of(" in line for line in bars), bars
     assert re.search(r"Stage::used\(step\) && !wait_o\(T::Stage::before\(step\)\)", source)
+
+
+def test_the_drill_refuses_limits_without_meaning():
+    from tie_b200 import MODEL_STATUS, library
+    drill = library().tie_attention_shared_wait_drill
+    for limit in (0, 2_000_000_001, 1 << 40):
+        assert drill(limit) == MODEL_STATUS.index("MODEL_ERR_ARG")

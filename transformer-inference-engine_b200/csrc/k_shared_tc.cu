@@ -31,7 +31,9 @@
 // are 44 % used, the tensor pipe 28 %. A wait that reads the timer at every try takes 1 us.
 //
 // Every wait is bounded (2 s): on expiry it raises the abort flag, which ends every other wait;
-// the roles run out without storing, the MMAs issued are drained and TMEM is freed.
+// the roles run out without storing, the copies and MMAs issued are drained and TMEM is freed. The join finds
+// places and parts of this call all the same, since they are written before anything is waited for: a part
+// that was not finished has a maximum and a sum that are NaN, and so has the row.
 #include <cuda.h>
 
 #include <cuda_bf16.h>
@@ -46,7 +48,7 @@ namespace {
 
 constexpr int kThreads = 384, kSoftmaxWarps = 4, kLoadWarps = 4, kMmaWarp = 8;
 constexpr unsigned kAll = 0xffffffffu;
-constexpr uint32_t kWaitLimitNs = 2000000000u;
+constexpr uint32_t kDrainLimitNs = 2000000000u;
 constexpr int kKeys = kTcPages * kPageRows;            // of a step
 // registers a thread: at launch, and as the warpgroups share them out (rows that are converted
 // take the loaders more)
@@ -258,8 +260,8 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
     long long x = me * share;
     const long long end = min(x + share, total);
     int u = x < end ? owner_of<long long>(base, n_units, x) : 0;
-    // the next part of this CTA's stretch that has steps
-    auto find = [&](Job& job) -> bool {
+    // the next part from place x of unit u on that has steps, in this CTA's stretch
+    auto find_at = [&](long long& x, int& u, Job& job) -> bool {
         while (x < end) {
             while (base[u + 1] <= x) ++u;          // (units without rows have no places)
             const UnitShape s = unit_shape(a, plan.n, line.u0 + u);
@@ -286,13 +288,14 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         }
         return false;
     };
+    auto find = [&](Job& job) -> bool { return find_at(x, u, job); };
     auto wait = [&](const uint64_t* bar, uint32_t parity) -> bool {
         const uint32_t b = smem_u32(bar);
         uint32_t t0 = 0;                 // (the timer is not looked at before a wait has become long)
         for (uint32_t i = 1; !mbar_try_wait(b, parity); ++i) {
             if ((i & 255u) != 0) continue;
             if (i == 256) t0 = nanoseconds();
-            if (s_abort || nanoseconds() - t0 > kWaitLimitNs) {
+            if (s_abort || nanoseconds() - t0 > a.wait_ns) {
                 s_abort = 1;
                 return false;
             }
@@ -317,6 +320,29 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         constexpr int kChunk = T::kAhead ? 64 : 32;       // scores in registers at a time
         const int r = warp * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+        // where this thread's row of a part goes (-1: it has none): of the whole items' rows, or of the parts'
+        auto place_of = [&](const Job& job) -> long long {
+            const int i = job.i0 + r;
+            if (i >= job.rows) return -1;
+            const int tok = a.by_group(i), h = job.head * a.group + i - tok * a.group;
+            return (long long)(job.row0 + tok) * a.n_head + h;
+        };
+        auto slot_of = [&](const Job& job) { return (2 * (size_t)me + (job.parts > 0)) * kTcRows + r; };
+        auto ml_of = [&](const Job& job, long long place) {
+            return reinterpret_cast<float2*>(job.whole ? a.whole_ml[0] + 2 * place : line.part_ml + 2 * slot_of(job));
+        };
+        {
+            // what the join reads, as it is if nothing more comes of it (the first S is on its way meanwhile)
+            long long ahead = x;
+            int unit = u;
+            Job part;
+            while (find_at(ahead, unit, part)) {
+                const long long place = place_of(part);
+                if (place < 0) continue;
+                if (part.parts) a.place[0][place] = make_int2(part.whole ? -1 : (int)slot_of(part), part.parts);
+                *ml_of(part, place) = make_float2(NAN, NAN);
+            }
+        }
         for (; ok && find(job); ++un) {
             float m = -INFINITY, alpha = 1.f;
             Float2x l(0.f, 0.f), o[32];
@@ -438,16 +464,12 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
             asm volatile("tcgen05.fence::after_thread_sync;");
             // (the next item's first P, which lets its O begin, is written after this)
             add_step();
-            const int i = job.i0 + r;
-            if (i < job.rows) {
-                const size_t slot = (2 * (size_t)me + (job.parts > 0)) * kTcRows + r;
-                const int tok = a.by_group(i), h = job.head * a.group + i - tok * a.group;
-                const size_t place = (size_t)(job.row0 + tok) * a.n_head + h;
-                float* to = job.whole ? a.whole_o[0] + place * kHeadDim : line.part_o + slot * kHeadDim;
-                if (job.parts) a.place[0][place] = make_int2(job.whole ? -1 : (int)slot, job.parts);
+            const long long place = place_of(job);
+            if (place >= 0) {
+                float* to = job.whole ? a.whole_o[0] + place * kHeadDim : line.part_o + slot_of(job) * kHeadDim;
                 float l0, l1;
                 l.get(l0, l1);
-                *reinterpret_cast<float2*>(job.whole ? a.whole_ml[0] + 2 * place : line.part_ml + 2 * slot) = make_float2(m, l0 + l1);
+                *ml_of(job, place) = make_float2(m, l0 + l1);
 #pragma unroll
                 for (int d = 0; d < 16; ++d) {
                     float4 v;
@@ -614,6 +636,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                 }
             }
         }
+        if constexpr (T::kAhead) asm volatile("cp.async.wait_all;" ::: "memory");      // (cut short: copies are on their way)
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
         if (warp == kMmaWarp) {
@@ -623,6 +646,8 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
             constexpr int kProducts = kTerms == 3 ? 6 : 3;
             constexpr uint32_t kA = kTerms == 3 ? 0x001102u : 0x012u;      // a digit each, the first lowest
             constexpr uint32_t kB = kTerms == 3 ? 0x010120u : 0x000u;
+            // (a drill: a wait for what does not come)
+            if (a.stall && (blockIdx.x & 1)) ok = wait_all(drained, 0);
             for (; ok && find(job); ++un) {
                 if (!(ok = wait_all(q_full, un))) break;
                 const int steps = __shfl_sync(kAll, job.b1 - job.b0, 0);
@@ -668,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
             commit_elected(smem_u32(drained));
             const uint32_t t0 = nanoseconds();
             while (!mbar_try_wait(smem_u32(drained), 0))
-                if (nanoseconds() - t0 > kWaitLimitNs) {
+                if (nanoseconds() - t0 > kDrainLimitNs) {
                     s_abort = 1;
                     break;
                 }

@@ -973,10 +973,19 @@ Variant variant_of(int np, int no) {
     return np == 1 ? variant<FMT, 1, 1>() : np == 4 ? variant<FMT, 4, 4>() : no == 1 ? variant<FMT, 2, 1>() : variant<FMT, 2, 2>();
 }
 
+constexpr uint32_t kWaitLimitNs = 2000000000u;         // of a wait in k_shared_tc.cu
+thread_local uint32_t drill_ns = 0;                    // of the next one's, by tie_attention_shared_wait_drill
+
 }  // namespace
 }  // namespace tie
 
 using namespace tie;
+
+extern "C" model_status tie_attention_shared_wait_drill(uint64_t limit_ns) {
+    if (limit_ns == 0 || limit_ns > kWaitLimitNs) return MODEL_ERR_ARG;
+    drill_ns = (uint32_t)limit_ns;
+    return MODEL_OK;
+}
 
 extern "C" size_t tie_attention_shared_workspace(int rows, int n_head) {
     int dev = 0;
@@ -1065,6 +1074,9 @@ extern "C" model_status tie_attention_shared(const float* q, int ldq, int n_head
         l.u1 = n_group;
         l.teams = shared_tc_ctas(sms);
         a.line[1].u0 = n_group;
+        a.wait_ns = drill_ns ? drill_ns : kWaitLimitNs;
+        a.stall = drill_ns != 0;
+        drill_ns = 0;
         TIE_OP_CU(launch_shared_tc(a, kv_format, st));
         ++op_launches;
     } else {

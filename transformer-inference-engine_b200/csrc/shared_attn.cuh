@@ -50,6 +50,8 @@ struct SharedArgs {
                                        // or -1: whole; how many parts
     Line line[2];                      // for prefixes and for sequences; one line, or one each
     int* status;
+    uint32_t wait_ns;                  // how long k_shared_tc.cu waits for anything; stall: every other CTA of it
+    int stall;                         // waits for what does not come
 };
 
 // What a unit's rows are, and its keys. rows == 0: nothing to do.

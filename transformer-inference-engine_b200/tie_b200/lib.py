@@ -151,6 +151,7 @@ def library():
         "tie_kv_store_q8": (C.c_int, [_vp, _vp, C.c_int, _vp, C.c_int, _vp, _vp, _vp, _vp, C.c_int, C.c_int, _vp]),
         "tie_kv_load": (C.c_int, [_vp, C.c_int, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp]),
         "tie_attention_shared_workspace": (C.c_size_t, [C.c_int, C.c_int]),
+        "tie_attention_shared_wait_drill": (C.c_int, [C.c_uint64]),
         "tie_attention_shared": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp,
                                            C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp,
                                            C.c_int, C.c_float, _vp, C.c_int, _vp, C.c_size_t, _vp, _vp]),

@@ -125,12 +125,20 @@ def attention_shared(q, k_pages, v_pages, page_table, row_start, ctx_lens, max_n
     """Attention of the new rows q over their sequences' own pages and over the pages that groups of sequences
     share (tie_attention_shared). prefix_table: [n_group, pages_per_prefix]; prefix_lens: the positions that each
     group shares; group_start: the groups' first sequences, and the end of the last. All three, or none.
-    scale: 1 / sqrt(64) by default. status: as for attention_paged."""
+    scale: 1 / sqrt(64) by default. status: as for attention_paged; rows that were not finished are NaN."""
     rc = (_module or _ops()).attention_shared(q, k_pages, v_pages, page_table, row_start, ctx_lens, max_new, out, workspace,
                                               k_scales, v_scales, prefix_table, prefix_lens, group_start,
                                               0.125 if scale is None else scale, status, stream)
     if rc:
         raise ModelError(rc, "tie_attention_shared")
+
+
+def attention_shared_wait_drill(limit_ns):
+    """Makes this thread's next attention_shared over a long prefix run out of a wait of limit_ns
+    (tie_attention_shared_wait_drill)."""
+    rc = library().tie_attention_shared_wait_drill(limit_ns)
+    if rc:
+        raise ModelError(rc, "tie_attention_shared_wait_drill")
 
 
 def q4_shapes(n, k, group):
