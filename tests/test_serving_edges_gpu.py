@@ -1,0 +1,105 @@
+"""Products with 4-bit weights at the ends of fp32 and of the sizes that one kernel takes, against their definition in
+64 bits."""
+import os
+import sys
+
+import numpy as np
+import pytest
+
+from tie_b200 import ops
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import serving_oracle as ref  # noqa: E402
+from test_serving_ops_gpu import _f, _np  # noqa: E402
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+EPS = 2.0 ** -24
+
+
+def _bound(x, w, group):
+    """How far a product may be from x w^T.
+
+    An element is an integer of a unit that is 2^-29 of the largest of its 128 columns at most (and 2^-127 at least),
+    rounded to the nearest: off by half of that, and by nothing where it is zero or, having 24 bits, within 2^-6 of the
+    largest. Sums of digits over a group are exact; joining them rounds five times, a group's product with its scale and
+    its addition once, 16 warps' parts of a row and the digits of one or two rows add 16 and 4 more. Nothing below 2^-149
+    is held of an fp32 sum."""
+    k = x.shape[1]
+    wide = np.zeros((len(x), -(-k // 128) * 128))
+    wide[:, :k] = np.abs(x)
+    top = np.repeat(wide.reshape(len(x), -1, 128).max(-1), 128, 1)[:, :k]
+    near = (x == 0) | ((np.abs(x) >= top * 2.0 ** -6) & (top >= 2.0 ** -97))
+    held = np.where(near, 0.0, np.maximum(top * 2.0 ** -30, 2.0 ** -128))
+    adds = -(-k // group) + 5 + 16 + 4
+    return (np.abs(x) @ np.abs(w).T) * adds * EPS + held @ np.abs(w).T + adds * 2.0 ** -149
+
+
+def _weights(rng, n, k, group, scale, zero=()):
+    """packed and scales on the device, and the weights in 64 bits; the columns `zero` have level 0."""
+    q = rng.integers(-7, 8, (n, k))
+    q[:, list(zero)] = 0
+    s = ref.bf16((scale * (1.0 + rng.random((n, -(-k // group))))).astype(np.float32))
+    return torch.tensor(ref.pack_q4(q), device="cuda"), torch.tensor(s, device="cuda").to(torch.bfloat16), ref.weights(q, s, group)
+
+
+def _product(x, packed, scales, group):
+    y = torch.empty(len(x), packed.shape[0], device="cuda")
+    ops.matvec_q4(_f(x.astype(np.float32)), packed, scales, group, y)
+    return _np(y).astype(np.float64)
+
+
+GROUPS = pytest.mark.parametrize("group", [32, 64, 128])
+ROWS = pytest.mark.parametrize("rows", [1, 2, 3, 8])
+
+
+@GROUPS
+@ROWS
+@pytest.mark.parametrize("size,scale", [(1e-30, 1.375 * 2.0 ** -20), (1e-36, 1e-3), (1e-20, 1e-22), (1e-37, 1e30), (1e-38, 2.0 ** 120),
+                                        (1.0, 2.0 ** -125), (1e30, 2.0 ** -130), (1e-25, 2.0 ** -60)])
+def test_small_products_keep_their_bits(group, rows, size, scale):
+    """Activations and scales whose product with the smallest unit is no normal number, though the result may be."""
+    rng = np.random.default_rng(rows)
+    packed, scales, w = _weights(rng, 37, 256, group, scale)
+    x = (size * rng.standard_normal((rows, 256))).astype(np.float32).astype(np.float64)
+    want = x @ w.T
+    assert (np.abs(_product(x, packed, scales, group) - want) <= _bound(x, w, group)).all()
+
+
+@GROUPS
+@ROWS
+@pytest.mark.parametrize("scale", [64.0, 2.0 ** 40, 2.0 ** 100, 2.0 ** 126])
+def test_a_large_activation_that_meets_nothing(group, rows, scale):
+    """3e38 in a column whose levels are 0: the result is the other columns', whatever the scales are."""
+    rng = np.random.default_rng(rows)
+    packed, scales, w = _weights(rng, 37, 256, group, scale, zero=[5])
+    x = np.zeros((rows, 256))
+    x[:, 5] = np.float32(3e38)
+    x[:, 128:] = (rng.standard_normal((rows, 128)) * min(1.0, 2.0 ** 100 / scale)).astype(np.float32)
+    want = x @ w.T
+    got = _product(x, packed, scales, group)
+    assert np.isfinite(got).all() and (np.abs(got - want) <= _bound(x, w, group)).all()
+
+
+@GROUPS
+@ROWS
+def test_large_activations(group, rows):
+    """Sums of levels times activations beyond fp32, with scales that bring them back."""
+    rng = np.random.default_rng(rows)
+    packed, scales, w = _weights(rng, 37, 256, group, 1e-4)
+    x = (1e38 * (2.0 * rng.random((rows, 256)) + 1.0)).astype(np.float32).astype(np.float64)
+    want = x @ w.T
+    assert (np.abs(_product(x, packed, scales, group) - want) <= _bound(x, w, group)).all()
+
+
+@GROUPS
+@pytest.mark.parametrize("rows", [2, 3])
+def test_a_large_row_leaves_the_rows_beside_it(group, rows):
+    rng = np.random.default_rng(rows)
+    packed, scales, w = _weights(rng, 37, 256, group, 2.0 ** -20)
+    x = 1e-30 * rng.standard_normal((rows, 256))
+    before = _product(x, packed, scales, group)
+    x[1] = 3e38
+    got = _product(x, packed, scales, group)
+    keep = np.arange(rows) != 1
+    assert np.array_equal(got[keep], before[keep])

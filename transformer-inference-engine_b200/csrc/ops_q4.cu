@@ -12,6 +12,7 @@
 #include <cuda_bf16.h>
 
 #include <climits>
+#include <type_traits>
 
 #include "ops.h"
 #include "quant.cuh"
@@ -173,6 +174,18 @@ struct XBlock {
 };
 constexpr int kSumBytes = 16 * 8 * 4;              // a warp's sums of a strip
 
+// acc + y s unit, rounded once, for a group's sum y (an integer below 2^40, of one digit below 2^17), its scale s and
+// a unit, which is a power of two. y times the unit is exact (it is a multiple of 2^-127) and fits in fp32 below
+// kFarUnit, whatever s is; s times the unit need not: with s first, small products lost bits and
+// 0 times infinity was NaN. From kFarUnit on, s (a bf16 number) times the unit is exact or infinite, and infinite only
+// where the product with any y but 0 is.
+constexpr float kFarUnit = 0x1p80f;
+template <bool FAR>
+__device__ __forceinline__ float add_group(float y, float s, float unit, float acc) {
+    if (FAR && unit >= kFarUnit) return fmaf(y, y == 0.f ? s : s * unit, acc);
+    return fmaf(y * unit, s, acc);
+}
+
 // y of row r0 + r, output j, from the sum of its products
 __device__ __forceinline__ void put(const MatvecArgs& a, int r, int j, float sum) {
     if (j >= a.n) return;
@@ -236,6 +249,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) matvec_q4_kernel(const __grid_
     const int xr = FEW ? g >> 2 : g;
     const bool real = xr < rows;
     const float* x = a.x + (long long)(r0 + min(xr, rows - 1)) * a.ldx;
+    bool far = false;                              // a unit of x is above kFarUnit
     // block kb of x, by one warp
     auto x_of = [&](int kb) {
         uint8_t* const to = smem + (size_t)kb * X::kBytes;
@@ -254,6 +268,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) matvec_q4_kernel(const __grid_
         // (2^-127 is the smallest unit; a row with an element that is not finite gets NaN)
         float one = e >= 255 ? top * 0.f : __uint_as_float(e == 29 ? 0x00400000u : (uint32_t)(e - 29) << 23);
         if constexpr (FEW) one *= (float)(1 << (8 * (g & 3)));
+        far |= one >= kFarUnit;
         int sum[kDigits][kGroups] = {};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -297,12 +312,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1) matvec_q4_kernel(const __grid_
         if (c == 0) reinterpret_cast<float*>(to + X::kDigitBytes + X::kStartBytes)[g] = one;
     };
     for (int kb = warp; kb < a.blocks; kb += kWarps) x_of(kb);
-    __syncthreads();
+    far = __syncthreads_or(far);                   // (a row's sums are the same either way, if its own units are below)
 
     float acc[4] = {}, ended[4];                   // ended: of the strip that the warp goes on with
     bool went_on = false;
     int strip = strip0 + q0 / a.blocks, kb = q0 % a.blocks, first = kb;
-    auto add = [&](uint4 (&wd)[2], unsigned short (&sd)[2]) {
+    auto add = [&](auto far_units, uint4 (&wd)[2], unsigned short (&sd)[2]) {
+        constexpr bool kFar = decltype(far_units)::value;
         const uint32_t w0[4] = {wd[0].x, wd[0].y, wd[0].z, wd[0].w}, w1[4] = {wd[1].x, wd[1].y, wd[1].z, wd[1].w};
         const float s[2] = {__uint_as_float((uint32_t)sd[0] << 16), __uint_as_float((uint32_t)sd[1] << 16)};
         load(wd, sd);
@@ -337,7 +353,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1) matvec_q4_kernel(const __grid_
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const float f = kGroups == 1 ? s[h] : __shfl_sync(kAll, s[h], (lane & ~3) | i);
-                const float f2[2] = {f * unit.x, f * unit.y};
 #pragma unroll
                 for (int e = 2 * h; e < 2 * h + 2; ++e) {
                     float y;
@@ -349,7 +364,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) matvec_q4_kernel(const __grid_
                         const float low = __int_as_float(d[1 % kDigits][e]) - (__int_as_float(start_of(1)) + __int_as_float(start_of(0)));
                         y = high + (low + __int_as_float(d[0][e]));
                     }
-                    acc[e] = fmaf(y, f2[e & 1], acc[e]);
+                    acc[e] = add_group<kFar>(y, f, e & 1 ? unit.y : unit.x, acc[e]);
                 }
             }
         }
@@ -378,11 +393,16 @@ __global__ void __launch_bounds__(kWarps * 32, 1) matvec_q4_kernel(const __grid_
         kb = first = 0;
         ++strip;
     };
-    for (int q = q0; q < q1; q += kAhead) {
+    // (two loops: with the choice inside, five rows of 6400 x 1600 in groups of 32 took 8.4 us instead of 7.9)
+    auto run = [&](auto far_units) {
+        for (int q = q0; q < q1; q += kAhead) {
 #pragma unroll
-        for (int d = 0; d < kAhead; ++d)
-            if (q + d < q1) add(w[d], sc[d]);
-    }
+            for (int d = 0; d < kAhead; ++d)
+                if (q + d < q1) add(far_units, w[d], sc[d]);
+        }
+    };
+    if (far) run(std::true_type{});
+    else run(std::false_type{});
     // (a strip that is not at its end here: begun by this warp, or, within the stretch, gone on with)
     const bool open = q0 < q1 && kb > 0, begun = open && first == 0;
     // Sums of a warp's cut strips, where x was: of the one that it goes on with, of the one that it begins.
