@@ -500,7 +500,7 @@ model_status tie_dequantize_q4(const void *packed, const void *scales, int n, in
  * ldr, ldy floats apart): the matmul of a decode step with its epilogue (the
  * bias, GELU and residual forms of model.c:735-752). bias [n] and residual may be
  * NULL; gelu 1: act is GELU (model.c:615-623), 0: none. residual may be y itself, x
- * must not overlap y. An activation is held to 2^-32 of the largest of its 128
+ * must not overlap y. An activation is held to 2^-30 of the largest of its 128
  * columns (and to 2^-128), its products with levels and their sums over a group are
  * exact, sums over groups fp32. A row's result does not depend on the rows beside
  * it, except by their number being above 2; a row with an element that is not finite

@@ -103,3 +103,24 @@ def test_a_large_row_leaves_the_rows_beside_it(group, rows):
     got = _product(x, packed, scales, group)
     keep = np.arange(rows) != 1
     assert np.array_equal(got[keep], before[keep])
+
+
+@ROWS
+def test_what_is_held_of_small_elements(rows):
+    """Beside a largest element of 1, others are held to 2^-30: half of a unit of 2^-29."""
+    rng = np.random.default_rng(rows)
+    packed, scales, w = _weights(rng, 37, 128, 128, 0.01)
+    x = np.zeros((rows, 128))
+    x[:, 3] = 1.0
+    x[:, 70] = [np.float32(2.0 ** -30 * f) for f in (0.999, 1.001, 2.9, 0.5, 1.5, 0.999, 4.1, 1000.5)][:rows]
+    want = x @ w.T
+    # (the sum of two products is rounded to 2^-24 of it, which hides the second: so without the first as well)
+    off = np.abs(_product(x, packed, scales, 128) - want)
+    assert (off <= _bound(x, w, 128)).all()
+    held = np.rint(x[:, 70] * 2.0 ** 29) * 2.0 ** -29
+    q = np.zeros((37, 128), np.int64)
+    q[:, 70] = 1
+    packed = torch.tensor(ref.pack_q4(q), device="cuda")
+    one = torch.ones(37, 1, dtype=torch.bfloat16, device="cuda")
+    got = _product(x, packed, one, 128)
+    assert np.array_equal(got, np.repeat(held[:, None], 37, 1)) and (np.abs(got[:, 0] - x[:, 70]) <= 2.0 ** -30).all()

@@ -123,10 +123,10 @@ dequantize_q4_kernel(const uint32_t* __restrict__ packed, const __nv_bfloat16* _
 // y[r] = act(x[r] W^T + bias) + residual[r] for up to 8 rows of x a CTA, on integer MMAs
 // (m16n8k32): 16 rows of W are the A operand, as the nibbles level + 8 lie in a word (a mask, a
 // shift and a mask for eight of them), the columns of B are rows of x. The elements of 128
-// columns of x become integers of 31 bits, relative to their largest, in four signed 8-bit
-// digits. A group's sum of each digit is exact; it starts at -8 times the digits' own sum, which takes the
-// 8 out of the levels, and at the bits of an fp32 number (quant.cuh), so that it ends as fp32 and needs no
-// conversion. Then come the group's scale and the sum over groups, in fp32. One or
+// columns of x become integers of 31 bits in four signed 8-bit digits: the largest of them is 2^29 to 2^30
+// units, so that a rounding is at most 2^-30 of it. A group's sum of each digit is exact; it starts at
+// -8 times the digits' own sum, which takes the 8 out of the levels, and at the bits of an fp32 number
+// (quant.cuh), so that it ends as fp32 and needs no conversion. Then come the group's scale and the sum over groups, in fp32. One or
 // two rows of x put their digits into B's eight columns, one MMA for 32 weights of each
 // row; up to 8 rows take four. (On bf16 terms of x the levels had to be converted, 11 instructions for eight
 // weights instead of 3: 50257 x 1600 took 24.7 us for 2 rows and 28.8 for 8.)
