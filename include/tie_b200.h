@@ -505,7 +505,7 @@ model_status tie_dequantize_q4(const void *packed, const void *scales, int n, in
  * exact, sums over groups fp32. A row's result does not depend on the rows beside
  * it, except by their number being above 2; a row with an element that is not finite
  * is not finite. The weights are read once for every 8 rows (every 2, where k is
- * above about 6,000). rows == 0 is allowed (x and y may be NULL then); at most 16,384
+ * above 6,400, 6,784 or 6,912 for groups of 32, 64 or 128). rows == 0 is allowed (x and y may be NULL then); at most 16,384
  * columns and 131,070 rows (MODEL_ERR_CAPACITY). */
 model_status tie_matvec_q4(const float *x, long long ldx, int rows, const void *packed,
                            const void *scales, int n, int k, int group, const float *bias,

@@ -124,3 +124,17 @@ def test_what_is_held_of_small_elements(rows):
     one = torch.ones(37, 1, dtype=torch.bfloat16, device="cuda")
     got = _product(x, packed, one, 128)
     assert np.array_equal(got, np.repeat(held[:, None], 37, 1)) and (np.abs(got[:, 0] - x[:, 70]) <= 2.0 ** -30).all()
+
+
+@pytest.mark.parametrize("group,k", [(32, 6400), (32, 6401), (64, 6784), (64, 6785), (128, 6912), (128, 6913)])
+def test_the_longest_rows_that_are_taken_by_eight(group, k):
+    """The length where eight rows' digits fill shared memory, and one column more: two rows at a time."""
+    rng = np.random.default_rng(k)
+    packed, scales, w = _weights(rng, 37, k, group, 0.01)
+    x = rng.standard_normal((8, k)).astype(np.float32).astype(np.float64)
+    got = _product(x, packed, scales, group)
+    assert (np.abs(got - x @ w.T) <= _bound(x, w, group)).all()
+    # by two, a row does not depend on the rows beside it, nor on how many there are
+    for lo in (0, 6):
+        alone = _product(x[lo:lo + 2], packed, scales, group)
+        assert np.array_equal(alone, got[lo:lo + 2]) == (k % 128 == 1)
