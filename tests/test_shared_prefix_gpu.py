@@ -1,5 +1,5 @@
-"""Attention over shared positions where its tensor-core kernel has the most to do: CTAs with several parts of several
-steps each. Against the 64-bit definitions (serving_oracle.py)."""
+"""Attention over shared positions where its tensor-core kernel has the most to do (CTAs with several parts of several
+steps each) or gives up, and how near to their 64-bit definitions (serving_oracle.py) all its kernels come."""
 import os
 import sys
 
@@ -10,6 +10,7 @@ import tie_b200
 from tie_b200 import ops
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import attention_precision as precision  # noqa: E402
 import ops_oracle as paged  # noqa: E402
 import serving_oracle as ref  # noqa: E402
 from test_serving_ops_gpu import KINDS, Batch, _i, _f, _long, _np  # noqa: E402
@@ -97,3 +98,27 @@ def test_a_wait_that_runs_out(kind, held):
     status.zero_()
     call()
     assert status.item() == 0 and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv_heads", [(3, 3), (8, 2), (16, 1)])
+@pytest.mark.parametrize("ctx,new,groups,shared", [
+    ([15], [1], (), ()), ([700], [1], (), ()), ([3000, 40, 333], [1, 1, 1], (), ()), ([500, 90], [9, 40], (), ()),
+    ([20, 100, 3, 60], [1, 2, 1, 5], (0, 4), (900,)), ([30] * 24, [1] * 24, (0, 10, 24), (200, 77)),
+])
+def test_rows_are_near_the_definition(kind, heads, kv_heads, ctx, new, groups, shared):
+    b = Batch(41, ctx, new, heads, kv_heads, kind, groups, shared)
+    got, want = _np(b.call()), b.want()[0]
+    shape = (b.rows * heads, 64)
+    assert precision.near(got.reshape(shape), want.reshape(shape)), precision.off(got.reshape(shape), want.reshape(shape))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,new,heads,kv_heads,groups,shared", [
+    (130, 1, 2, 2, (0, 130), (70,)), (64, 2, 8, 2, (0, 64), (1000,)), (100, 1, 12, 1, (0, 40, 100), (333, 2000)),
+])
+def test_rows_of_long_prefixes_are_near_the_definition(kind, n, new, heads, kv_heads, groups, shared):
+    b = _long(43, np.random.default_rng(n).integers(0, 50, n).tolist(), [new] * n, heads, kv_heads, kind, groups, shared)
+    got, want = _np(b.call()), b.want()[0]
+    shape = (b.rows * heads, 64)
+    assert precision.near(got.reshape(shape), want.reshape(shape)), precision.off(got.reshape(shape), want.reshape(shape))
