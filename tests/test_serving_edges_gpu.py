@@ -1,5 +1,5 @@
 """Products with 4-bit weights at the ends of fp32 and of the sizes that one kernel takes, against their definition in
-64 bits."""
+64 bits; rows that are alone."""
 import os
 import sys
 
@@ -138,3 +138,40 @@ def test_the_longest_rows_that_are_taken_by_eight(group, k):
     for lo in (0, 6):
         alone = _product(x[lo:lo + 2], packed, scales, group)
         assert np.array_equal(alone, got[lo:lo + 2]) == (k % 128 == 1)
+
+
+@pytest.mark.parametrize("kind", ["f32", "q8"])
+def test_a_row_alone_may_have_any_stride(kind):
+    """There is no next row, so strides that two tensors do not share, or that are not whole groups of 4, mean nothing."""
+    rng = np.random.default_rng(1)
+    w = 2 * 64
+    k, v, q = (rng.standard_normal((1, w)).astype(np.float32) for _ in range(3))
+
+    def wide(x, extra):
+        t = torch.zeros(1, w + extra, device="cuda")
+        if x is not None:
+            t[:, :w] = _f(x)
+        return t[:, :w]
+
+    def i(*x):
+        return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+    dtype = torch.int8 if kind == "q8" else torch.float32
+    pages = [torch.zeros(3, 16, w, dtype=dtype, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(3, 2, 16, device="cuda") for _ in range(2)] if kind == "q8" else [None, None]
+    if kind == "q8":
+        ops.kv_store_q8(wide(k, 64), wide(v, 3), i(17), *pages, *scales)
+    else:
+        ops.kv_store(wide(k, 64), wide(v, 3), i(17), *pages)
+    out = [wide(None, 7), wide(None, 128)]
+    ops.kv_load(i(17), *pages, *out, *scales)
+    for x, o in zip((k, v), out):
+        # (levels are within half of a step of 1 / 127 of the largest)
+        assert np.abs(_np(o) - x).max() <= (np.abs(x).max() / 253 if kind == "q8" else 0.0)
+    # a sequence of one position: the row of values
+    got = wide(None, 5)
+    ws = torch.empty(ops.attention_shared_workspace(1, 2), dtype=torch.uint8, device="cuda")
+    table, start, ctx = i(1).view(1, 1), i(0, 1), i(0)
+    ops.kv_store_q8(wide(k, 1), wide(v, 2), i(16), *pages, *scales) if kind == "q8" else ops.kv_store(wide(k, 1), wide(v, 2), i(16), *pages)
+    ops.attention_shared(wide(q, 3), *pages, table, start, ctx, 1, got, ws, *scales)
+    assert np.abs(_np(got) - _np(out[1])).max() <= 4 * EPS * np.abs(v).max()

@@ -120,7 +120,9 @@ struct Rows {
         const int64_t w = x.t.shape[1], one = x.t.strides ? x.t.strides[1] : 1;
         int64_t step = x.t.strides ? x.t.strides[0] : w;
         if (w != width || (one != 1 && w > 1)) wrong(name, "one width with contiguous rows is");
-        if (rows <= 1 && step < w) step = w;
+        // (a row alone has no next one, so its stride means nothing, and two of them need not agree; one of a width that is
+        // not whole groups of 4 keeps a stride that may be)
+        if (rows <= 1 && (step < w || w % 4 == 0)) step = w;
         p = static_cast<float*>(x.data());
         ld = as_int(name, step);
         as_int(name, rows);
