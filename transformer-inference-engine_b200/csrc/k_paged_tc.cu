@@ -154,36 +154,6 @@ constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kTileKeys >> 3) << 17) | ((
 constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) /* B is MN-major */ | ((uint32_t)(kHeadDim >> 3) << 17) |
                              ((uint32_t)(kHalfRows >> 4) << 24);
 
-// D += A . B with A in tensor memory (two fp16 of consecutive k per 32-bit
-// column), or in shared memory. Called by a whole, converged warp, of which one
-// lane issues: with one lane in a branch of its own every operand of every MMA
-// would be moved to a uniform register there and then, and the MMAs would wait
-// for the moves.
-__device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, one;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "elect.sync _|one, 0xffffffff;\n\t"
-        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
-}
-
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, one;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "elect.sync _|one, 0xffffffff;\n\t"
-        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
-}
-
-// wraps after 4.3 s; differences of less are right
-__device__ __forceinline__ uint32_t nanoseconds() {
-    uint32_t t;
-    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
-    return t;
-}
-
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -198,15 +168,6 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
 
 __device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t n) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory");
-}
-
-__device__ __forceinline__ void commit_elected(uint32_t bar) {
-    asm volatile(
-        "{\n\t.reg .pred one;\n\t"
-        "elect.sync _|one, 0xffffffff;\n\t"
-        "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
-        ::"r"(bar)
-        : "memory");
 }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {

@@ -84,37 +84,6 @@ struct Tc {
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (64u >> 3 << 17) | ((uint32_t)(kTcRows >> 4) << 24);
 constexpr uint32_t kIdescO = kIdesc | (1u << 16);      // B is MN-major
 
-// D += A . B, A in shared memory or in tensor memory; a whole, converged warp calls, one lane
-// issues (as in k_paged_tc.cu).
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, one;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "elect.sync _|one, 0xffffffff;\n\t"
-        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, one;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "elect.sync _|one, 0xffffffff;\n\t"
-        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
-}
-__device__ __forceinline__ void commit_elected(uint32_t bar) {
-    asm volatile(
-        "{\n\t.reg .pred one;\n\t"
-        "elect.sync _|one, 0xffffffff;\n\t"
-        "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
-        ::"r"(bar)
-        : "memory");
-}
-__device__ __forceinline__ uint32_t nanoseconds() {
-    uint32_t t;
-    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
-    return t;
-}
 // 32 columns of the warp's 32 lanes read, 16 written
 __device__ __forceinline__ void tmem_begin32(uint32_t taddr, uint32_t* r) {
     __syncwarp();
@@ -662,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                         const uint32_t k = stage(step) + (kB >> (4 * z) & 15u) * kKvTerm;
 #pragma unroll
                         for (int s = 0; s < 4; ++s)
-                            mma_ss(tm + kColS, sw128_desc(q + 32u * s), sw128_desc(k + 32u * s), kIdesc, z || s ? 1u : 0u);
+                            mma_f16(tm + kColS, sw128_desc(q + 32u * s), sw128_desc(k + 32u * s), kIdesc, z || s ? 1u : 0u);
                     }
                     commit_elected(smem_u32(s_full));
                     return true;
@@ -684,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                         const uint32_t v = stage(f) + T::kValues + (kB >> (4 * z) & 15u) * kKvTerm;
 #pragma unroll
                         for (int s = 0; s < 4; ++s)
-                            mma_ts(tm + kColO, p + 8u * s, sw128_desc(v + 2048u * s), kIdescO, z || s ? 1u : 0u);
+                            mma_f16_ta(tm + kColO, p + 8u * s, sw128_desc(v + 2048u * s), kIdescO, z || s ? 1u : 0u);
                     }
                     commit_elected(smem_u32(o_full + T::Stage::of(f)));
                 }

@@ -34,6 +34,13 @@ __device__ __forceinline__ unsigned long long globaltimer_ns() {
     return t;
 }
 
+// wraps after 4.3 s; differences of less are right
+__device__ __forceinline__ uint32_t nanoseconds() {
+    uint32_t t;
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+    return t;
+}
+
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
                                             int y) {
     asm volatile(
@@ -89,9 +96,41 @@ __device__ __forceinline__ void mma_tf32_ta(uint32_t tmem_d, uint32_t a_tmem, ui
         ::"r"(tmem_d), "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate));
 }
 
+// D += A . B on fp16 or bf16 (as idesc says) with A in tensor memory (two of consecutive k
+// per 32-bit column), or in shared memory. Called by a whole, converged warp, of which one
+// lane issues: with one lane in a branch of its own every operand of every MMA
+// would be moved to a uniform register there and then, and the MMAs would wait
+// for the moves.
+__device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, one;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, one;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
                  : "memory");
+}
+
+__device__ __forceinline__ void commit_elected(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred one;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(bar)
+        : "memory");
 }
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
