@@ -433,9 +433,12 @@ model_status tie_kv_load(const int32_t *slots, int rows, const void *k_pages, co
  * groups of sequences share: beams and answers of one prompt, requests behind one
  * instruction. Group g is sequences group_start[g] .. group_start[g + 1] - 1
  * (group_start[n_group + 1], ascending); its first prefix_lens[g] positions lie in
- * the pages of prefix_table (n_group rows of pages_per_prefix entries) and are read
- * once for all its rows. A sequence's own pages (page_table, ctx_lens) hold what
- * comes behind them, from a page's first row on. For row r of sequence s, its new
+ * the pages of prefix_table (n_group rows of pages_per_prefix entries). They are read for 8 to 32 of
+ * its rows (tokens times query heads of a K/V head) together, or, where a group has 64 rows and more in the
+ * mean and the products of rows and pages_per_prefix are many, by the tensor cores for 128. (The arguments
+ * decide, not the lengths on the device: a table far wider than its prefixes, or one large group among many
+ * small ones, may be better served by a table or a call of its own.) A sequence's own pages
+ * (page_table, ctx_lens) hold what comes behind them, from a page's first row on. For row r of sequence s, its new
  * token i, and query head h,
  *   out[r][h] = sum_j softmax_j(scale * q[r][h] . k[j]) v[j]
  * over the group's shared positions and the sequence's own positions 0 ..
@@ -446,8 +449,9 @@ model_status tie_kv_load(const int32_t *slots, int rows, const void *k_pages, co
  * TIE_KV_INT8, with the pool's scales (NULL for the others).
  * All else is as for tie_attention_paged: rows, limits, what is left out, what is
  * not finite, and status. It is set where a wait of a long prefix's kernel ran out (2 s) and may
- * be NULL; rows whose shared positions were not finished then are NaN, the others as always. Sums and softmax statistics are fp32. Over fp32 and bf16 pages products are
- * of all of their operands' 24 bits. Over pages in 8 bits a row's scaled query is held
+ * be NULL; rows whose shared positions were not finished then are NaN, the others as always. Sums
+ * and softmax statistics are fp32. Over fp32 and bf16 pages products are of all of their operands' 24
+ * bits. Over pages in 8 bits a row's scaled query is held
  * in 24 bits relative to its largest element (to 2^-126), and the products of a step
  * of 32 keys' weights (at most 1) with their values' scales in 23 bits relative to the
  * largest of the step (to 2^-95). The result of a row depends, in its rounding, on how

@@ -21,14 +21,15 @@
 // barrier's phase of the step before has completed (loaders wait for S, softmax warps for O).
 //
 // Measured (B200, the whole call: this kernel, the sequences' own positions, the join): 64
-// answers x 1-4 tokens over bf16 pages, 14336 shared positions, 8 K/V heads: 112 us (on mma.sync
-// 271). Steps to it: a pair of threads per row, which exchange their maxima, 133; a thread per
-// row and pairs of fp32 numbers in an instruction, 120; S of the next step ahead, 118; its keys
-// told of before the next rows are asked for (a page's table entry a step sooner), 113. What bounds it
-// is the way round a step: of about 5000 cycles (two CTAs side by side) a softmax warp takes 700 for
-// S and the maximum, 800 to add O, 1600 for weights and terms (512 of them exponentials, at the
-// rate of the SM), 700 to write and report P; P V and the waits take the others. Issue slots
-// are 44 % used, the tensor pipe 28 %. A wait that reads the timer at every try takes 1 us.
+// answers x 1-4 tokens over bf16 pages, 14336 shared positions, 8 K/V heads: 116 us (on mma.sync
+// 271), about 80 of them this kernel's. Steps to it: a pair of threads per row, which exchange their
+// maxima, 133; a thread per row and pairs of fp32 numbers in an instruction, 120; S of the next step
+// ahead, 118; its keys told of before the next rows are asked for (a page's table entry a step sooner), 113;
+// a barrier for each stage, and places and sums that are there before any wait, 116. What bounds it is the way
+// round a step: of about 5000 cycles (two CTAs side by side) a softmax warp takes 700 for S and the
+// maximum, 800 to add O, 1600 for weights and terms (512 of them exponentials, at the rate of the SM), 700 to
+// write and report P; P V and the waits take the others. Issue slots are 48 % used, the tensor pipe
+// 33 %. A wait that reads the timer at every try takes 1 us.
 //
 // Every wait is bounded (2 s): on expiry it raises the abort flag, which ends every other wait;
 // the roles run out without storing, the copies and MMAs issued are drained and TMEM is freed. The join finds

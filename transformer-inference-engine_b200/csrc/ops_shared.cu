@@ -30,12 +30,13 @@
 // the sum, so it takes 16 in a row, and each lane's 8 dims of 4 values are packed in pairs of keys.
 //
 // Measured (B200, whole calls): 64 sequences of up to 4000 positions, 8-bit pages (127 MB), one token
-// each, 39 us: 27 of steps (4.7 TB/s; two thirds of the issue slots, 600 instructions for 32 keys of a
-// head), the others the start (4) and the join. Steps copied to shared memory, with 16 warps an SM instead of
+// each, 39 us: 27 of steps (4.7 TB/s; 600 instructions for 32 keys of a head), the others the start (4)
+// and the join; 40 % of DRAM's rate and 47 % of issue slots over all. Steps copied to shared memory, with 16 warps an SM instead of
 // 12, reads with hints for the L2 and pairs of numbers per instruction in the 8-bit path each
-// took 39 too. 256 answers of a token behind 700 positions, fp32, 74 us: 60-65 % of what their own
-// positions take to read; the fp32 split's instructions (numbers in pairs: 76 -> 74). 24 groups in 8
-// bits 55 us, 4 beams 12: the chain of two launches.
+// took 39 too (the same 64 bytes of a row a warp, all of them: pages as a whole were not tried). 256 answers of a
+// token behind 700 positions, fp32, 74 us, 42 % of DRAM's rate and 41 % of issue slots: neither is full, 12
+// warps an SM with a step ahead each wait for it. (Numbers in pairs in the fp32 split: 76 -> 74.) 24 groups in
+// 8 bits 55 us, 4 beams 11.4: two launches in turn.
 #include <cuda_bf16.h>
 
 #include <climits>
@@ -947,7 +948,8 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(const __grid_cons
 //   128 sequences behind 4000 (4.1 M)         46 and 36;  33 and 32;  29 and 31
 //   256 sequences behind 4000 (8.2 M)         75 and 53;  53 and 46;  48 and 46
 // (256 sequences behind 700, 12 heads, with 300 positions of their own, fp32, 2.2 M: 75 and 92; 640
-// rows a head behind 14336, 8 heads, bf16, 73 M: 271 and 113.)
+// rows a head behind 14336, 8 heads, bf16, 73 M: 271 and 116.) The lengths are on the device, so a table much wider than
+// its prefixes takes the slower one of these.
 constexpr int kTcFrom = 64;
 constexpr long long tc_scores(int format) { return format == TIE_KV_F32 ? 3000000 : format == TIE_KV_BF16 ? 4000000 : 8000000; }
 int most_warps(int sms) { return sms * 16; }
