@@ -292,7 +292,7 @@ model_status tie_head_argmax_noalloc(const float *x, int ldx, const float *w, in
  * Pointers are DEVICE pointers of one device (made current for the call) and
  * `stream` a cudaStream_t of it (NULL: the legacy default stream); work is
  * enqueued and not waited for. Activations, workspaces and pages are 16-byte aligned
- * (pages that tie_attention_paged reads 32-byte), leading dimensions multiples of 4 floats. A workspace holds nothing
+ * (pages that attention reads 32-byte), leading dimensions multiples of 4 floats. A workspace holds nothing
  * from one call to the next, but two calls that overlap on the GPU (streams,
  * replayed graphs) need one each. Nothing is allocated, and every call may be
  * captured into a graph. MODEL_ERR_ARG for a null or misaligned pointer, a
@@ -454,7 +454,8 @@ model_status tie_kv_load(const int32_t *slots, int rows, const void *k_pages, co
  * bits. Over pages in 8 bits a row's scaled query is held
  * in 24 bits relative to its largest element (to 2^-126), and the products of a step
  * of 32 keys' weights (at most 1) with their values' scales in 23 bits relative to the
- * largest of the step (to 2^-95). The result of a row depends, in its rounding, on how
+ * largest of the step (to 2^-95); its products with a key's levels are summed before the key's scale, so
+ * such a sum has to be finite in fp32 too. The result of a row depends, in its rounding, on how
  * the batch splits its keys, and is the same for the same call. Where group_start does
  * not ascend, rows of a sequence in two groups' ranges hold no particular result.
  * workspace: tie_attention_shared_workspace(rows, n_head) bytes (on the current

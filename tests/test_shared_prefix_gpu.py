@@ -122,3 +122,31 @@ def test_rows_of_long_prefixes_are_near_the_definition(kind, n, new, heads, kv_h
     got, want = _np(b.call()), b.want()[0]
     shape = (b.rows * heads, 64)
     assert precision.near(got.reshape(shape), want.reshape(shape)), precision.off(got.reshape(shape), want.reshape(shape))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv_heads,new", [(1024, 1024, 1), (8192, 1024, 1), (1024, 1024, 5)])
+def test_as_many_heads_as_there_may_be(kind, heads, kv_heads, new):
+    """One team of warps, or not even a second one, on the GPU."""
+    b = Batch(47, [20, 3], [new, 1], heads, kv_heads, kind, (0, 2), (18,))
+    b.check()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_long_prefixes_of_many_heads(kind):
+    b = _long(49, [2] * 64, [1] * 64, 256, 256, kind, (0, 64), (130,))
+    got = _np(b.call()).astype(np.float64)
+    rows, o, bound = _some(b, np.array([0, 33, 63]))
+    assert (np.abs(got[rows] - o) <= bound).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_as_many_groups_as_sequences_and_any_bound_of_new_tokens(kind):
+    """4096 groups of a sequence each; max_new is a bound, however far off."""
+    rng = np.random.default_rng(51)
+    n = 4096
+    b = Batch(51, rng.integers(0, 9, n).tolist(), rng.integers(0, 2, n).tolist(), 1, 1, kind, tuple(range(n + 1)),
+              tuple(rng.integers(1, 40, n).tolist()))
+    b.check()
+    b.max_new = 2 ** 31 - 1
+    b.check()
